@@ -449,6 +449,93 @@ LATENT_API int latent_router_route(const float *scores, int32_t n_tokens, int32_
                                    double threshold, uint32_t flags, int32_t *ids, float *weights, int32_t *n_kept,
                                    int32_t *expert_counts, struct CUstream_st *stream);
 
+/* Gradient of the router's weights with respect to its scores (no
+ * counterpart in the reference, which has no training code).  ids and the
+ * flags as latent_router_route made and took them; d_weights[n_tokens][top_k]
+ * fp32, read for kept slots only.  scores and d_scores have one type (F32,
+ * F16 or BF16), [n_tokens][n_expert].  The kept set is held fixed.  With
+ * LATENT_ROUTER_SOFTMAX the scores are logits and so is the gradient's
+ * argument; LATENT_ROUTER_ACCUMULATE adds into d_scores instead of writing
+ * it.  A row without a kept slot has a zero gradient.  An id that several
+ * slots of a row hold counts once per slot; ids outside [0, n_expert) are
+ * dropped slots.  LATENT_ERR_UNSUPPORTED beyond 1024 experts or top_k 32.
+ * Stream-ordered, allocates nothing; repeated calls agree bit for bit. */
+enum { LATENT_ROUTER_ACCUMULATE = 1u << 2 };
+LATENT_API int latent_router_grad(const void *scores, int32_t type, const int32_t *ids, const float *d_weights,
+                                  int32_t n_tokens, int32_t n_expert, int32_t top_k, uint32_t flags, void *d_scores,
+                                  struct CUstream_st *stream);
+
+/* Load-balance and z losses of a router over packed sequences, the expert
+ * counts, and the loss's gradient (no counterpart in the reference).
+ * logits[n_tokens][n_expert] of `type`, p their softmax; ids[n_tokens][top_k]
+ * (outside [0, n_expert): no slot).  cu_seqlens[n_sequences + 1] (device,
+ * ascending; NULL with n_sequences 1: all rows): rows outside the sequences,
+ * and rows whose valid[] byte is 0 (valid NULL: none), take no part and have
+ * a zero gradient, whatever they hold.  With counted rows n_s, kept slots
+ * counts[n_sequences][n_expert], f = counts / max(1, their sum per sequence),
+ * P_se the mean of p over the counted rows and S' the sequences that have one:
+ *   losses[1] = (1/S') sum_s n_expert sum_e f_se P_se
+ *   losses[2] = mean over counted rows of logsumexp(logits)^2
+ *   losses[0] = balance_coef losses[1] + z_coef losses[2]
+ * and grad (optional) = *d_loss dlosses[0]/dlogits in the logits' type, with f
+ * held fixed (d_loss: the device scalar that comes from behind, NULL: 1).  A row whose logits are all -inf has no distribution: it counts as a
+ * row, adds nothing and has a zero gradient.  Workspace: 256-byte aligned,
+ * latent_balance_workspace_size() bytes.  LATENT_ERR_UNSUPPORTED beyond 1024
+ * experts.  Stream-ordered; repeated calls agree bit for bit. */
+LATENT_API int latent_balance_workspace_size(int32_t n_sequences, size_t *bytes);
+LATENT_API int latent_balance_loss(const void *logits, int32_t type, const int32_t *ids, const uint8_t *valid,
+                                   const int32_t *cu_seqlens, int32_t n_tokens, int32_t n_expert, int32_t top_k,
+                                   int32_t n_sequences, float balance_coef, float z_coef, const float *d_loss,
+                                   float *losses, int32_t *counts, void *grad, void *workspace,
+                                   size_t workspace_bytes, struct CUstream_st *stream);
+
+/* Low-rank adapters of many requests beside one shared projection (no
+ * counterpart in the reference; its low-rank pair is loader/latent_runtime.py
+ * :35-36).  Per row t with a = ids[t]:
+ *   y[t] = x[t].W + scale[a] (x[t].A_a).B_a        (a < 0: x[t].W alone)
+ * x, w, a and b have one type, F16 or BF16; y has that type or F32; every sum
+ * is fp32 and y is rounded once.  The adapters are stored at one padded rank
+ * (16, 32, 64 or 128; zero rows change nothing): a holds A_a transposed,
+ * [n_adapter][rank][lda], b holds B_a, [n_adapter][rank][ldb].  w is
+ * [n_in][ldw], or [n_out][ldw] with LATENT_ADAPTER_W_TRANSPOSED; w == NULL:
+ * y += the adapters' part.  An id >= n_adapter counts as none and is recorded
+ * in *err (latent_adapter_check).  Adapter factors must be finite: a
+ * tile of rows multiplies by the factors of every adapter that one of them
+ * uses, zero times the others' (0 x inf would not stay out).  Workspace:
+ * 256-byte aligned, latent_adapter_workspace_size() bytes. */
+enum { LATENT_ADAPTER_W_TRANSPOSED = 1u << 0 };
+typedef struct latent_adapter_desc {
+    int32_t n_adapter;
+    int32_t rank;            /* padded rank: 16, 32, 64 or 128 */
+    int32_t n_in;            /* K */
+    int32_t n_out;           /* N */
+    int32_t n_tokens;        /* T */
+    int32_t type;            /* latent_type of x, w, a, b (F16 or BF16) */
+    int32_t y_type;          /* the same, or LATENT_TYPE_F32 */
+    uint32_t flags;          /* LATENT_ADAPTER_* */
+    const void *x;           /* [T][ldx] */
+    int64_t ldx;             /* elements between rows, as all ld* */
+    const void *w;
+    int64_t ldw;
+    const void *a;
+    int64_t lda;             /* >= n_in */
+    const void *b;
+    int64_t ldb;             /* >= n_out */
+    const float *scale;      /* [n_adapter] */
+    const int32_t *ids;      /* [T] */
+    void *y;                 /* [T][ldy] */
+    int64_t ldy;
+    uint32_t *err;           /* one device word, error bits are or-ed into it */
+    void *workspace;
+    size_t workspace_bytes;
+} latent_adapter_desc;
+
+LATENT_API int latent_adapter_workspace_size(const latent_adapter_desc *desc, size_t *bytes);
+LATENT_API int latent_adapter_project(const latent_adapter_desc *desc, struct CUstream_st *stream);
+/* Synchronises `stream`, reports the error bits in *err (LATENT_ERR_EXPERT_ID:
+ * an id >= n_adapter; LATENT_ERR_TIMEOUT) and clears them. */
+LATENT_API int latent_adapter_check(uint32_t *err, struct CUstream_st *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,8 @@ FLAG_WEIGHT_BEFORE_DOWN = 1 << 0
 FLAG_OUT_PER_SLOT = 1 << 1
 ROUTER_RENORMALIZE = 1 << 0
 ROUTER_SOFTMAX = 1 << 1
+ROUTER_ACCUMULATE = 1 << 2
+ADAPTER_W_TRANSPOSED = 1 << 0
 PATH_AUTO, PATH_DECODE, PATH_PREFILL = 0, 1, 2
 
 # Every entry point the header declares, with (restype, argtypes).
@@ -140,7 +142,44 @@ class EpDesc(C.Structure):
     ]
 
 
+class AdapterDesc(C.Structure):
+    _fields_ = [
+        ("n_adapter", C.c_int32),
+        ("rank", C.c_int32),
+        ("n_in", C.c_int32),
+        ("n_out", C.c_int32),
+        ("n_tokens", C.c_int32),
+        ("type", C.c_int32),
+        ("y_type", C.c_int32),
+        ("flags", C.c_uint32),
+        ("x", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("w", C.c_void_p),
+        ("ldw", C.c_int64),
+        ("a", C.c_void_p),
+        ("lda", C.c_int64),
+        ("b", C.c_void_p),
+        ("ldb", C.c_int64),
+        ("scale", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("y", C.c_void_p),
+        ("ldy", C.c_int64),
+        ("err", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 EXPORTS.update({
+    "latent_adapter_workspace_size": (C.c_int, [C.POINTER(AdapterDesc), C.POINTER(C.c_size_t)]),
+    "latent_adapter_project": (C.c_int, [C.POINTER(AdapterDesc), C.c_void_p]),
+    "latent_adapter_check": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "latent_balance_workspace_size": (C.c_int, [C.c_int32, C.POINTER(C.c_size_t)]),
+    "latent_balance_loss": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                      C.c_int32, C.c_int32, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "latent_router_grad": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                     C.c_uint32, C.c_void_p, C.c_void_p]),
     "latent_ep_workspace_size": (C.c_int, [C.POINTER(EpDesc), C.POINTER(C.c_size_t)]),
     "latent_ep_dispatch": (C.c_int, [C.POINTER(EpDesc), C.c_void_p]),
     "latent_ep_combine": (C.c_int, [C.POINTER(EpDesc), C.c_void_p]),

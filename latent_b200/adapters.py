@@ -1,0 +1,170 @@
+"""Low-rank adapters of many requests beside one shared projection.
+
+``AdapterSet`` lays the adapters out once on the device; ``adapter_project``
+multiplies a batch by the shared weight and adds, row by row, the product of
+that row's own adapter:
+
+    y[t] = x[t] . W + scale_a (x[t] . A_a) . B_a,   a = ids[t]  (< 0: W alone)
+
+The shared projection is a dense fp16/bf16 matrix (either memory order) or a
+packed ``FactorPair``.  The rows of a batch may be single tokens of many
+requests or packed prompts, in any order.  An inference operator: inputs that
+require a gradient are refused.  The reference has no adapters; its low-rank
+projection is loader/latent_runtime.py:35-36.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .router_train import _on
+from .runtime import FactorPair, _stream_ptr, project
+
+__all__ = ["AdapterSet", "adapter_project"]
+
+_TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+_Y_TYPES = {**_TYPES, torch.float32: _lib.TYPE_F32}
+
+
+def _tensor(a, device) -> torch.Tensor:
+    return (a if torch.is_tensor(a) else torch.from_numpy(np.ascontiguousarray(a))).to(device)
+
+
+class AdapterSet:
+    """Device-resident adapters (A [K, r], B [r, N], scale) of one projection.
+
+    ``adapters``: one triple per adapter (scale may be left out: 1.0), ranks
+    may differ.  They are stored at one padded rank (16, 32, 64 or 128, zero
+    rows change no result) in ``dtype``: A transposed, so that a rank column
+    is contiguous, B as given.  Factors that are not finite in ``dtype`` are
+    refused: rows of several adapters share tiles in which a foreign factor
+    is multiplied by zero.
+    """
+
+    def __init__(self, adapters: Sequence[Tuple], device="cuda", dtype: Optional[torch.dtype] = None):
+        if not adapters:
+            raise ValueError("an AdapterSet needs at least one adapter")
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        if dtype is None:
+            first = adapters[0][0]
+            dtype = first.dtype if torch.is_tensor(first) and first.dtype in _TYPES else torch.bfloat16
+        if dtype not in _TYPES:
+            raise ValueError(f"adapter dtype {dtype} unsupported (float16 or bfloat16)")
+        K, N = int(adapters[0][0].shape[0]), int(adapters[0][1].shape[1])
+        rmax = 0
+        for ad in adapters:
+            a, b = ad[0], ad[1]
+            if a.ndim != 2 or b.ndim != 2 or a.shape[0] != K or b.shape[1] != N or a.shape[1] != b.shape[0] or \
+                    a.shape[1] < 1:
+                raise ValueError(f"adapter factors {tuple(a.shape)}, {tuple(b.shape)} do not match [{K}, r], [r, {N}]")
+            rmax = max(rmax, int(a.shape[1]))
+        rank = 16
+        while rank < rmax:
+            rank *= 2
+        if rank > 128:
+            raise ValueError(f"adapter rank {rmax} unsupported (at most 128)")
+        n = len(adapters)
+        self.device, self.dtype, self.rank = dev, dtype, rank
+        self.n_adapter, self.n_in, self.n_out = n, K, N
+        self.ranks = [int(ad[0].shape[1]) for ad in adapters]
+        # rows padded to 16 bytes
+        self.a = torch.zeros((n, rank, (K + 7) // 8 * 8), dtype=dtype, device=dev)
+        self.b = torch.zeros((n, rank, (N + 7) // 8 * 8), dtype=dtype, device=dev)
+        for i, ad in enumerate(adapters):
+            self.a[i, :self.ranks[i], :K] = _tensor(ad[0], dev).detach().t()
+            self.b[i, :self.ranks[i], :N] = _tensor(ad[1], dev).detach()
+        scales = [float(ad[2]) if len(ad) > 2 else 1.0 for ad in adapters]
+        self.scale = torch.tensor(scales, dtype=torch.float32, device=dev)
+        if not np.isfinite(scales).all() or not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
+            raise ValueError(f"adapter factors and scales must be finite in {dtype}")
+        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def check(self) -> None:
+        """Synchronises and raises if a call since the last check recorded a device-side error
+        (an id >= n_adapter, which counts as no adapter, or a bounded wait that ran out)."""
+        _lib.check(_on(self.device, _lib.lib().latent_adapter_check, self.err.data_ptr(), _stream_ptr(self.device)),
+                   "device check")
+
+
+def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Tensor,
+                    out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x . W plus each row's own adapter (latent_adapter_project).
+
+    x [T, K] in the set's dtype (rows may be strided); ``weight`` [K, N] of
+    the same dtype, row-major or the transposed view of a linear layer's
+    [N, K] weight, or a ``FactorPair`` (its fp32 ``project`` is then summed
+    with the adapters' part in fp32); ids int32 [T], negative: no adapter,
+    >= n_adapter: none either, and ``adapters.check()`` reports it.  Returns
+    [T, N] in ``out_dtype`` (x's dtype or float32; x's by default), fp32 sums
+    rounded once, or fills ``out`` (rows may be strided).
+    """
+    s = adapters
+    if x.dim() != 2 or x.shape[1] != s.n_in:
+        raise ValueError(f"x must be [T, {s.n_in}], got {tuple(x.shape)}")
+    if x.dtype != s.dtype:
+        raise ValueError(f"x must be {s.dtype} like the adapters, got {x.dtype}")
+    T, K = x.shape
+    N = s.n_out
+    if ids.dim() != 1 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise ValueError(f"ids must be contiguous int32 [{T}]")
+    pair = isinstance(weight, FactorPair)
+    if not pair:
+        if weight.dim() != 2 or tuple(weight.shape) != (K, N) or weight.dtype != x.dtype:
+            raise ValueError(f"weight must be {x.dtype} [{K}, {N}]")
+        if weight.device != s.device:
+            raise ValueError("x, weight, ids and out must be on the adapters' device")
+    if x.device != s.device or ids.device != s.device or (out is not None and out.device != s.device):
+        raise ValueError("x, weight, ids and out must be on the adapters' device")
+    if torch.is_grad_enabled() and (x.requires_grad or (not pair and weight.requires_grad) or
+                                    (out is not None and out.requires_grad)):
+        raise ValueError("adapter_project computes no gradients: call it under torch.no_grad() or on detached tensors")
+    if out is not None:
+        if out_dtype not in (None, out.dtype):
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        out_dtype = out.dtype
+        if tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be [{T}, {N}] with contiguous rows")
+    elif out_dtype is None:
+        out_dtype = x.dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"out_dtype {out_dtype} unsupported ({x.dtype} or float32)")
+    if x.stride(1) != 1 and K > 1 or T > 1 and x.stride(0) < K:
+        x = x.contiguous()
+    if T == 0:
+        return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=s.device)
+    flags, w_ptr, ldw = 0, None, 0
+    if pair:
+        y = project(x, weight)
+        if y.shape[1] != N:
+            raise ValueError(f"the factor pair has {y.shape[1]} columns, the adapters {N}")
+    else:
+        ws0, ws1 = weight.stride()
+        if (ws1 == 1 or N == 1) and (ws0 >= N or K == 1):
+            ldw = max(ws0, N)
+        elif (ws0 == 1 or K == 1) and (ws1 >= K or N == 1):
+            flags, ldw = _lib.ADAPTER_W_TRANSPOSED, max(ws1, K)
+        else:
+            raise ValueError("weight must be row-major or the transposed view of a row-major matrix")
+        w_ptr = weight.data_ptr()
+        y = out if out is not None else torch.empty((T, N), dtype=out_dtype, device=s.device)
+    ldx = x.stride(0) if T > 1 else K
+    ldy = y.stride(0) if T > 1 else N
+    L = _lib.lib()
+    d = _lib.AdapterDesc(s.n_adapter, s.rank, K, N, T, _TYPES[x.dtype], _Y_TYPES[y.dtype], flags, x.data_ptr(), ldx,
+                         w_ptr, ldw, s.a.data_ptr(), s.a.shape[2], s.b.data_ptr(), s.b.shape[2], s.scale.data_ptr(),
+                         ids.data_ptr(), y.data_ptr(), ldy, s.err.data_ptr(), None, 0)
+    n = C.c_size_t(0)
+    _lib.check(L.latent_adapter_workspace_size(C.byref(d), C.byref(n)), "latent_adapter_workspace_size")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=s.device)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), n.value
+    _lib.check(_on(s.device, L.latent_adapter_project, C.byref(d), _stream_ptr(s.device)), "latent_adapter_project")
+    if pair:
+        return y.to(out_dtype) if out is None else out.copy_(y)
+    return y

@@ -1,0 +1,178 @@
+// Low-rank adapters of many requests beside one shared projection
+// (latent_adapter_project): y[t] = x[t].W + s_a (x[t].A_a).B_a, a = ids[t].
+//
+// Two steps: k_ad_shrink makes t[t] = s_a x[t].A_a (fp32, [T][rank]) and a
+// product kernel adds t.B_a to x.W.  This file has the shrink and the product
+// on the CUDA cores, for any size, stride and alignment.
+#include "internal.h"
+
+namespace latent {
+
+namespace {
+
+template <typename T> __device__ __forceinline__ float ad_f32(T v);
+template <> __device__ __forceinline__ float ad_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float ad_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ __forceinline__ void ad_store(void *y, int y_type, int64_t i, float v) {
+    if (y_type == LATENT_TYPE_F32) static_cast<float *>(y)[i] = v;
+    else if (y_type == LATENT_TYPE_F16) static_cast<__half *>(y)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(y)[i] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ float ad_load(const void *y, int y_type, int64_t i) {
+    if (y_type == LATENT_TYPE_F32) return static_cast<const float *>(y)[i];
+    if (y_type == LATENT_TYPE_F16) return __half2float(static_cast<const __half *>(y)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(y)[i]);
+}
+
+constexpr int kShrinkWarps = 8;
+
+// One warp per (row, rank column): block (t, j0 / 8).
+template <typename T>
+__global__ void __launch_bounds__(kShrinkWarps * 32) k_ad_shrink(latent_adapter_desc d, float *tt) {
+    const int t = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int j = blockIdx.y * kShrinkWarps + warp;
+    const int a = __ldg(d.ids + t);
+    if (a >= d.n_adapter && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(d.err, kErrExpertId);
+    if (a < 0 || a >= d.n_adapter) return;
+    const T *x = static_cast<const T *>(d.x) + (int64_t)t * d.ldx;
+    const T *w = static_cast<const T *>(d.a) + ((int64_t)a * d.rank + j) * d.lda;
+    float s = 0.f;
+    for (int k = lane; k < d.n_in; k += 32) s = fmaf(ad_f32(x[k]), ad_f32(w[k]), s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) tt[(int64_t)t * d.rank + j] = s * __ldg(d.scale + a);
+}
+
+// 64 x 64 outputs per block, 4 x 4 per thread, K in steps of 16 through shared memory.
+constexpr int kSB = 64, kSK = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_ad_simple(latent_adapter_desc d, const float *tt) {
+    __shared__ float xs[kSK][kSB + 4], ws[kSK][kSB + 4];
+    const int row0 = blockIdx.y * kSB, col0 = blockIdx.x * kSB;
+    const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
+    const T *x = static_cast<const T *>(d.x), *w = static_cast<const T *>(d.w), *b = static_cast<const T *>(d.b);
+    const bool tn = d.flags & LATENT_ADAPTER_W_TRANSPOSED;
+    const int64_t sk = tn ? 1 : d.ldw, sn = tn ? d.ldw : 1;
+    float acc[4][4] = {};
+    for (int k0 = 0; w && k0 < d.n_in; k0 += kSK) {
+        for (int i = threadIdx.x; i < kSB * kSK; i += 256) {
+            const int r = i / kSK, k = i % kSK;
+            xs[k][r] = row0 + r < d.n_tokens && k0 + k < d.n_in ? ad_f32(x[(int64_t)(row0 + r) * d.ldx + k0 + k]) : 0.f;
+            const int wk = tn ? i % kSK : i / kSB, wn = tn ? i / kSK : i % kSB;
+            ws[wk][wn] = col0 + wn < d.n_out && k0 + wk < d.n_in ? ad_f32(w[(k0 + wk) * sk + (col0 + wn) * sn]) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSK; ++k) {
+            float xv[4], wv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xv[i] = xs[k][tr * 4 + i];
+                wv[i] = ws[k][tc + 16 * i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int t = row0 + tr * 4 + i;
+        if (t >= d.n_tokens) continue;
+        const int a = __ldg(d.ids + t);
+        if (a >= 0 && a < d.n_adapter) {
+            const float *tv = tt + (int64_t)t * d.rank;
+            const T *bv = b + (int64_t)a * d.rank * d.ldb;
+            for (int r = 0; r < d.rank; ++r) {
+                const float s = tv[r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = col0 + tc + 16 * j;
+                    if (n < d.n_out) acc[i][j] = fmaf(s, ad_f32(bv[(int64_t)r * d.ldb + n]), acc[i][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = col0 + tc + 16 * j;
+            if (n >= d.n_out) continue;
+            const int64_t at = (int64_t)t * d.ldy + n;
+            ad_store(d.y, d.y_type, at, w ? acc[i][j] : ad_load(d.y, d.y_type, at) + acc[i][j]);
+        }
+    }
+}
+
+bool ad_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
+
+int ad_validate(const latent_adapter_desc *d) {
+    if (!d) return LATENT_ERR_INVALID;
+    if (d->n_adapter < 0 || d->n_in < 1 || d->n_out < 1 || d->n_tokens < 0) return LATENT_ERR_SHAPE;
+    if (d->rank != 16 && d->rank != 32 && d->rank != 64 && d->rank != 128) return LATENT_ERR_UNSUPPORTED;
+    if (d->type != LATENT_TYPE_F16 && d->type != LATENT_TYPE_BF16) return LATENT_ERR_DTYPE;
+    if (d->y_type != d->type && d->y_type != LATENT_TYPE_F32) return LATENT_ERR_DTYPE;
+    if (d->flags & ~(uint32_t)LATENT_ADAPTER_W_TRANSPOSED) return LATENT_ERR_INVALID;
+    return LATENT_OK;
+}
+
+}  // namespace
+
+}  // namespace latent
+
+extern "C" LATENT_API int latent_adapter_workspace_size(const latent_adapter_desc *d, size_t *bytes) {
+    const int st = latent::ad_validate(d);
+    if (st) return st;
+    if (!bytes) return LATENT_ERR_INVALID;
+    *bytes = ((size_t)d->n_tokens * d->rank * 4 + 511) / 256 * 256;
+    return LATENT_OK;
+}
+
+extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, CUstream_st *stream) {
+    using namespace latent;
+    const int st = ad_validate(d);
+    if (st) return st;
+    if (d->n_tokens == 0) return LATENT_OK;
+    const bool tn = d->flags & LATENT_ADAPTER_W_TRANSPOSED;
+    if (!d->x || !d->ids || !d->y || !d->err || !d->workspace || (d->n_adapter > 0 && (!d->a || !d->b || !d->scale)))
+        return LATENT_ERR_INVALID;
+    if (d->ldx < d->n_in || d->ldy < d->n_out || (d->w && d->ldw < (tn ? d->n_in : d->n_out)) ||
+        (d->n_adapter > 0 && (d->lda < d->n_in || d->ldb < d->n_out)))
+        return LATENT_ERR_SHAPE;
+    if (!ad_aligned(d->x, 2) || !ad_aligned(d->w, 2) || !ad_aligned(d->a, 2) || !ad_aligned(d->b, 2) ||
+        !ad_aligned(d->scale, 4) || !ad_aligned(d->ids, 4) || !ad_aligned(d->y, d->y_type == LATENT_TYPE_F32 ? 4 : 2) ||
+        !ad_aligned(d->err, 4) || !ad_aligned(d->workspace, 256))
+        return LATENT_ERR_ALIGN;
+    size_t need = 0;
+    latent_adapter_workspace_size(d, &need);
+    if (d->workspace_bytes < need) return LATENT_ERR_WORKSPACE;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    float *tt = static_cast<float *>(d->workspace);
+    const dim3 gs((unsigned)d->n_tokens, (unsigned)d->rank / kShrinkWarps);
+    const dim3 gp((unsigned)((d->n_out + kSB - 1) / kSB), (unsigned)((d->n_tokens + kSB - 1) / kSB));
+    if (gp.y > 65535u) return LATENT_ERR_SHAPE;
+    if (d->type == LATENT_TYPE_F16) {
+        k_ad_shrink<__half><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
+        k_ad_simple<__half><<<gp, 256, 0, s>>>(*d, tt);
+    } else {
+        k_ad_shrink<__nv_bfloat16><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
+        k_ad_simple<__nv_bfloat16><<<gp, 256, 0, s>>>(*d, tt);
+    }
+    return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+}
+
+extern "C" LATENT_API int latent_adapter_check(uint32_t *err, CUstream_st *stream) {
+    using namespace latent;
+    if (!err) return LATENT_ERR_INVALID;
+    uint32_t bits = 0;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (cudaMemcpyAsync(&bits, err, 4, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+        cudaMemsetAsync(err, 0, 4, s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
+        return LATENT_ERR_CUDA;
+    if (bits & kErrTimeout) return LATENT_ERR_TIMEOUT;
+    if (bits & kErrExpertId) return LATENT_ERR_EXPERT_ID;
+    return LATENT_OK;
+}

@@ -1,0 +1,565 @@
+// Training side of the router (csrc/router.cu): the load-balance and z losses
+// with the per-expert counts and their gradient (latent_balance_loss), and the
+// gradient of the routing weights (latent_router_grad).  The reference has no
+// training code; the routing rule differentiated here is
+// loader/adaptive_topk.py:29-90 with its kept set held fixed.
+//
+// Balance loss over packed sequences s (rows [cu[s], cu[s+1]), counted rows
+// n_s, kept slots c_se, f_se = c_se / max(1, sum_e c_se), S' sequences with a
+// counted row, n = sum n_s):
+//   L_bal = (1/S') sum_s E sum_e f_se P_se,  P_se = (1/n_s) sum_t p_te
+//   L_z   = (1/n) sum_t lse_t^2,             loss = b L_bal + z L_z
+// With C_se = E f_se / (S' n_s), a number per sequence and expert that the ids
+// alone give, L_bal = sum_t D_t with D_t = sum_e C_se p_te, and
+//   dloss/dl_ti = p_ti (b (C_si - D_t) + 2 z lse_t / n):
+// value and gradient need the counts first and then ONE pass over the logits,
+// and no per-expert probability sums.
+//
+// k_balance_count: one cluster of 8 blocks per sequence; each block counts its
+// rows' ids in a shared-memory histogram, the blocks add theirs up through
+// distributed shared memory: integers, no global atomics, nothing to zero.
+// k_balance_main: one warp per row, the row in registers; every block leaves
+// its two partial sums (64 bits) and the last one adds them up in block order,
+// so that a call's results do not depend on the order of execution.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "internal.h"
+
+namespace latent {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kMaxTrainExperts = 1024;  // 32 logits per lane in registers
+constexpr int kMaxTrainTopK = 32;       // one lane per slot
+constexpr int kCountCluster = 8;
+constexpr int kCountThreads = 512;
+constexpr int kRowWarps = 8;
+constexpr unsigned kFull = 0xffffffffu;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <int BYTES> struct Raw;
+template <> struct Raw<2> { using type = uint16_t; };
+template <> struct Raw<4> { using type = uint32_t; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<16> { using type = uint4; };
+
+// A row of E values held by one warp: lane l has, of each run of 32 * VEC
+// columns, the VEC adjacent ones from l * VEC (one load or store of
+// VEC * sizeof(T) bytes).  E is a multiple of VEC and rows are aligned to it.
+template <typename T, int PL, int VEC>
+struct Row {
+    static constexpr int NV = PL / VEC;
+    using R = typename Raw<VEC * sizeof(T)>::type;
+    static __device__ __forceinline__ int col(int lane, int v) { return (v * 32 + lane) * VEC; }
+    static __device__ __forceinline__ void load(const T *row, int E, int lane, float pad, float (&x)[PL]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = col(lane, v);
+            if (c < E) {
+                const R raw = __ldg(reinterpret_cast<const R *>(row + c));
+                const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[v * VEC + i] = to_f32(e[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[v * VEC + i] = pad;
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T *row, int E, int lane, const float (&x)[PL]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = col(lane, v);
+            if (c < E) {
+                R raw;
+                T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(x[v * VEC + i]);
+                *reinterpret_cast<R *>(row + c) = raw;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+// Rows [lo, hi) of sequence s; cu == NULL: one sequence of all T rows.  The
+// borders are device data: whatever they hold, no row outside [0, T) is touched.
+__device__ __forceinline__ void sequence_rows(const int32_t *cu, int s, int T, int &lo, int &hi) {
+    if (!cu) {
+        lo = 0;
+        hi = T;
+        return;
+    }
+    lo = min(max(__ldg(cu + s), 0), T);
+    hi = min(max(__ldg(cu + s + 1), lo), T);
+}
+
+// Sequence of row t, -1 for a row before the first or behind the last.
+__device__ __forceinline__ int sequence_of(const int32_t *cu, int S, int t) {
+    if (!cu) return 0;
+    if (t < __ldg(cu) || t >= __ldg(cu + S)) return -1;
+    int lo = 0, hi = S;  // the last s with cu[s] <= t: empty sequences before it are passed over
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+struct BalanceArgs {
+    const void *logits;
+    const int32_t *ids;
+    const uint8_t *valid;
+    const int32_t *cu;
+    int T, E, k, S;
+    float b, z;
+    const float *d_loss;  // gradient with respect to losses[0]; NULL: 1
+    float *losses;
+    int32_t *counts;    // [S][E]
+    void *grad;
+    int32_t *seq;       // [S][2] counted rows, kept slots
+    double *partial;    // [blocks][2]
+    uint32_t *ticket;
+};
+
+__global__ void __cluster_dims__(kCountCluster, 1, 1) __launch_bounds__(kCountThreads)
+k_balance_count(BalanceArgs a) {
+    __shared__ int hist[kMaxTrainExperts];
+    __shared__ int tot[2];  // counted rows, kept slots of this block
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank();
+    const int s = blockIdx.x / kCountCluster;
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
+    if (threadIdx.x < 2) tot[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
+    __syncthreads();
+    int lo, hi;
+    sequence_rows(a.cu, s, a.T, lo, hi);
+    const int per = (hi - lo + kCountCluster - 1) / kCountCluster;
+    const int r0 = min(hi, lo + rank * per), r1 = min(hi, r0 + per);
+    int rows = 0, slots = 0;
+    for (int i = r0 * a.k + threadIdx.x; i < r1 * a.k; i += blockDim.x) {
+        if (a.valid && !__ldg(a.valid + i / a.k)) continue;
+        const int e = __ldg(a.ids + i);
+        if (e >= 0 && e < a.E) {
+            atomicAdd(&hist[e], 1);
+            ++slots;
+        }
+    }
+    if (a.valid) {
+        for (int t = r0 + threadIdx.x; t < r1; t += blockDim.x) rows += __ldg(a.valid + t) != 0;
+    } else if (threadIdx.x == 0) {
+        rows = r1 - r0;
+    }
+    rows = __reduce_add_sync(kFull, rows);
+    slots = __reduce_add_sync(kFull, slots);
+    if ((threadIdx.x & 31) == 0) {
+        if (rows) atomicAdd(&tot[0], rows);
+        if (slots) atomicAdd(&tot[1], slots);
+    }
+    cluster.sync();
+    const int step = (a.E + kCountCluster - 1) / kCountCluster;
+    const int e0 = rank * step, e1 = min(a.E, e0 + step);
+    for (int e = e0 + threadIdx.x; e < e1; e += blockDim.x) {
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < kCountCluster; ++q) c += *cluster.map_shared_rank(&hist[e], q);
+        a.counts[(int64_t)s * a.E + e] = c;
+    }
+    if (rank == 0 && threadIdx.x < 2) {
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < kCountCluster; ++q) c += *cluster.map_shared_rank(&tot[threadIdx.x], q);
+        a.seq[2 * s + threadIdx.x] = c;
+    }
+    cluster.sync();  // the others' shared memory stays until every block has read it
+}
+
+template <typename T, int PL, int VEC>
+__global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) {
+    using RW = Row<T, PL, VEC>;
+    __shared__ double part[kRowWarps][2];
+    __shared__ bool last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t n = 0;   // counted rows
+    int used = 0;    // sequences that have one
+    for (int s = lane; s < a.S; s += 32) {
+        const int c = a.seq[2 * s];
+        n += c;
+        used += c > 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(kFull, n, o);
+    used = __reduce_add_sync(kFull, used);
+    const float up = a.d_loss ? __ldg(a.d_loss) : 1.f;
+    const float gb = up * a.b, gz = n > 0 ? up * (2.f * a.z / (float)n) : 0.f;
+    const T *logits = static_cast<const T *>(a.logits);
+    T *grad = static_cast<T *>(a.grad);
+    double sb = 0.0, sz = 0.0;
+    for (int t = blockIdx.x * kRowWarps + warp; t < a.T; t += gridDim.x * kRowWarps) {
+        const int s = a.valid && !__ldg(a.valid + t) ? -1 : sequence_of(a.cu, a.S, t);
+        float g[PL];
+        if (s < 0) {  // a padded row, whatever it holds, gives nothing and gets a zero gradient
+#pragma unroll
+            for (int j = 0; j < PL; ++j) g[j] = 0.f;
+        } else {
+            float x[PL];
+            RW::load(logits + (int64_t)t * a.E, a.E, lane, -INFINITY, x);
+            float m = -INFINITY;
+            bool nan = false;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) {
+                m = fmaxf(m, x[j]);
+                nan |= x[j] != x[j];
+            }
+            m = warp_max(m);
+            const bool none = m == -INFINITY && !__any_sync(kFull, nan);  // every expert masked: no distribution
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) {
+                x[j] = none ? 0.f : expf(x[j] - m);
+                sum += x[j];
+            }
+            sum = warp_sum(sum);
+            const float inv = none ? 0.f : 1.f / sum;
+            const float lse = none ? 0.f : m + logf(sum);
+            const int ns = a.seq[2 * s], cs = max(1, a.seq[2 * s + 1]);
+            const float scale = (float)a.E / ((float)used * (float)ns) / (float)cs;
+            const int32_t *cnt = a.counts + (int64_t)s * a.E;
+            float c[PL], d = 0.f;
+#pragma unroll
+            for (int v = 0; v < RW::NV; ++v) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int j = v * VEC + i, col = RW::col(lane, v) + i;
+                    c[j] = col < a.E ? (float)cnt[col] * scale : 0.f;
+                    x[j] *= inv;
+                    d = fmaf(c[j], x[j], d);
+                }
+            }
+            d = warp_sum(d);
+            sb += d;
+            sz += (double)lse * lse;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) g[j] = x[j] * fmaf(gb, c[j] - d, gz * lse);
+        }
+        if (grad) RW::store(grad + (int64_t)t * a.E, a.E, lane, g);
+    }
+    if (lane == 0) {
+        part[warp][0] = sb;
+        part[warp][1] = sz;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double b = 0.0, z = 0.0;
+        for (int w = 0; w < kRowWarps; ++w) {
+            b += part[w][0];
+            z += part[w][1];
+        }
+        a.partial[2 * blockIdx.x] = b;
+        a.partial[2 * blockIdx.x + 1] = z;
+        __threadfence();
+        last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last || warp != 0) return;
+    __threadfence();
+    double b = 0.0, z = 0.0;  // lane l adds blocks l, l + 32, ... in order, then the lanes are added by a fixed tree
+    for (int i = lane; i < (int)gridDim.x; i += 32) {
+        b += __ldcg(a.partial + 2 * i);
+        z += __ldcg(a.partial + 2 * i + 1);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        b += __shfl_xor_sync(kFull, b, o);
+        z += __shfl_xor_sync(kFull, z, o);
+    }
+    if (lane == 0) {
+        z = n > 0 ? z / (double)n : 0.0;
+        a.losses[0] = (float)(a.b * b + a.z * z);
+        a.losses[1] = (float)b;
+        a.losses[2] = (float)z;
+    }
+}
+
+// Gradient of the routing weights.  Slot j of row t (id i_j, kept when
+// 0 <= i_j < E) has the weight w_j = s_j, or s_j / sum_kept s with RENORM; the
+// scores s are given (SOFTMAX: as logits).  With c = sum_kept dw_j w_j:
+//   scores: ds_j = (dw_j - c) / sum_kept s with RENORM, else dw_j;
+//   logits, RENORM: the softmax's own sum cancels, w is the softmax over the
+//     kept logits alone and dl_j = w_j (dw_j - c), zero elsewhere;
+//   logits, raw: dl_i = p_i (dw_i - c) over the whole row.
+// One warp per row, lane j has slot j.  Only the raw logits form reads the
+// row; the others gather the kept scores.  A row is written as zeros (or
+// -c p_i) and then its kept columns, after a __syncwarp, by their slots' lanes
+// (an id held by several slots: the lowest of those lanes, with their sum).
+// ACCUM adds to what dscores holds and touches nothing else of the row
+// (raw logits: the whole row).
+template <typename T, int PL, int VEC, bool SOFTMAX, bool RENORM, bool ACCUM>
+__global__ void __launch_bounds__(kRowWarps * 32) k_router_grad(const T *__restrict__ scores,
+                                                                const int32_t *__restrict__ ids,
+                                                                const float *__restrict__ dw, int T_, int E, int k,
+                                                                T *__restrict__ out) {
+    using RW = Row<T, PL, VEC>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int t = blockIdx.x * kRowWarps + warp; t < T_; t += gridDim.x * kRowWarps) {
+        const T *row = scores + (int64_t)t * E;
+        T *o = out + (int64_t)t * E;
+        int id = lane < k ? __ldg(ids + (int64_t)t * k + lane) : -1;
+        const bool kept = id >= 0 && id < E;
+        if (!kept) id = -1 - lane;  // no other lane's id
+        const float d = kept ? __ldg(dw + (int64_t)t * k + lane) : 0.f;
+        const bool any = __any_sync(kFull, kept);
+        float old = 0.f;
+        if (ACCUM && kept) old = to_f32(o[id]);
+        float v = kept ? to_f32(__ldg(row + id)) : 0.f, g = 0.f;
+        float x[PL];
+        if (SOFTMAX && !RENORM) {
+            RW::load(row, E, lane, -INFINITY, x);
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) m = fmaxf(m, x[j]);
+            m = warp_max(m);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) {
+                x[j] = expf(x[j] - m);
+                sum += x[j];
+            }
+            sum = warp_sum(sum);
+            const float p = kept ? expf(v - m) / sum : 0.f;
+            const float c = warp_sum(d * p);
+            const float cn = any ? -c / sum : 0.f;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) x[j] = any ? x[j] * cn : 0.f;
+            // a kept column is p (sum of its slots' dw - c): the lanes of one id share p
+            g = p * d;
+            v = -c * p;
+        } else if (SOFTMAX) {
+            const float m = warp_max(kept ? v : -INFINITY);
+            const float e = kept ? expf(v - m) : 0.f;
+            const float w = any ? e / warp_sum(e) : 0.f;
+            g = w * (d - warp_sum(w * d));
+            v = 0.f;
+        } else if (RENORM) {
+            const float sum = warp_sum(v);
+            const float c = warp_sum(kept ? v / sum * d : 0.f);
+            g = kept ? (d - c) / sum : 0.f;
+            v = 0.f;
+        } else {
+            g = d;
+            v = 0.f;
+        }
+        if (!(SOFTMAX && !RENORM)) {
+#pragma unroll
+            for (int j = 0; j < PL; ++j) x[j] = 0.f;
+        }
+        if (ACCUM) {
+            if (SOFTMAX && !RENORM) {
+                float y[PL];
+                RW::load(o, E, lane, 0.f, y);
+#pragma unroll
+                for (int j = 0; j < PL; ++j) x[j] += y[j];
+                __syncwarp();
+                RW::store(o, E, lane, x);
+            }
+        } else {
+            RW::store(o, E, lane, x);
+        }
+        const unsigned same = __match_any_sync(kFull, id);
+        float total = 0.f;
+        for (unsigned rest = kept ? same : 0u; __any_sync(kFull, rest != 0u);) {
+            const int src = rest ? __ffs(rest) - 1 : lane;
+            const float add = __shfl_sync(kFull, g, src);
+            if (rest) total += add;
+            rest &= rest - 1;
+        }
+        __syncwarp();
+        if (kept && lane == __ffs(same) - 1) o[id] = from_f32<T>(old + (v + total));
+    }
+}
+
+bool is_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+int sm_count(int *sms) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return LATENT_ERR_CUDA;
+    return LATENT_OK;
+}
+
+constexpr int kBalanceBlocksPerSm = 8;
+constexpr int kMaxBalanceBlocks = 4096;  // partial sums in the workspace
+
+struct BalanceLayout {
+    size_t seq, partial, ticket, total;
+};
+BalanceLayout balance_layout(int S) {
+    BalanceLayout L;
+    L.seq = 0;
+    L.partial = round256((size_t)S * 8);
+    L.ticket = L.partial + (size_t)kMaxBalanceBlocks * 16;
+    L.total = L.ticket + 256;
+    return L;
+}
+
+// Elements per lane, and whether rows can be moved in vectors of them.
+template <typename T, typename F>
+int with_row(int E, bool vec_ok, F f) {
+    constexpr int MAXV = 16 / (int)sizeof(T);
+    auto pick = [&](auto pl) {
+        constexpr int PL = decltype(pl)::value;
+        constexpr int V = PL < MAXV ? PL : MAXV;
+        if (V > 1 && E % V == 0 && vec_ok)
+            f(std::integral_constant<int, PL>{}, std::integral_constant<int, V>{});
+        else
+            f(std::integral_constant<int, PL>{}, std::integral_constant<int, 1>{});
+    };
+    if (E <= 32) pick(std::integral_constant<int, 1>{});
+    else if (E <= 64) pick(std::integral_constant<int, 2>{});
+    else if (E <= 128) pick(std::integral_constant<int, 4>{});
+    else if (E <= 256) pick(std::integral_constant<int, 8>{});
+    else if (E <= 512) pick(std::integral_constant<int, 16>{});
+    else pick(std::integral_constant<int, 32>{});
+    return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+}
+
+template <typename T>
+int launch_balance(const BalanceArgs &a, int blocks, cudaStream_t s) {
+    const bool vec = is_aligned(a.logits, 16) && is_aligned(a.grad, 16);
+    return with_row<T>(a.E, vec, [&](auto pl, auto v) {
+        k_balance_main<T, decltype(pl)::value, decltype(v)::value><<<blocks, kRowWarps * 32, 0, s>>>(a);
+    });
+}
+
+template <typename T>
+int launch_router_grad(const void *scores, const int32_t *ids, const float *dw, int n, int E, int k, uint32_t flags,
+                       void *out, cudaStream_t s) {
+    const bool vec = is_aligned(scores, 16) && is_aligned(out, 16);
+    const int64_t blocks = ((int64_t)n + kRowWarps - 1) / kRowWarps;
+    return with_row<T>(E, vec, [&](auto pl, auto v) {
+        constexpr int PL = decltype(pl)::value, V = decltype(v)::value;
+        const T *sc = static_cast<const T *>(scores);
+        T *o = static_cast<T *>(out);
+        const unsigned g = (unsigned)blocks;
+        const int mode = ((flags & LATENT_ROUTER_SOFTMAX) ? 4 : 0) | ((flags & LATENT_ROUTER_RENORMALIZE) ? 2 : 0) |
+                         ((flags & LATENT_ROUTER_ACCUMULATE) ? 1 : 0);
+#define LATENT_RG(S_, R_, A_) k_router_grad<T, PL, V, S_, R_, A_><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o)
+        switch (mode) {
+            case 0: LATENT_RG(false, false, false); break;
+            case 1: LATENT_RG(false, false, true); break;
+            case 2: LATENT_RG(false, true, false); break;
+            case 3: LATENT_RG(false, true, true); break;
+            case 4: LATENT_RG(true, false, false); break;
+            case 5: LATENT_RG(true, false, true); break;
+            case 6: LATENT_RG(true, true, false); break;
+            default: LATENT_RG(true, true, true); break;
+        }
+#undef LATENT_RG
+    });
+}
+
+bool float_type(int t) { return t == LATENT_TYPE_F32 || t == LATENT_TYPE_F16 || t == LATENT_TYPE_BF16; }
+size_t type_size(int t) { return t == LATENT_TYPE_F32 ? 4 : 2; }
+
+int train_shape(int32_t T, int32_t E, int32_t k) {
+    if (T < 0 || E < 1 || k < 1) return LATENT_ERR_SHAPE;
+    if ((int64_t)T * k > (int64_t)1 << 30) return LATENT_ERR_SHAPE;
+    if (E > kMaxTrainExperts) return LATENT_ERR_UNSUPPORTED;
+    return LATENT_OK;
+}
+
+}  // namespace
+
+}  // namespace latent
+
+extern "C" LATENT_API int latent_balance_workspace_size(int32_t n_sequences, size_t *bytes) {
+    if (!bytes) return LATENT_ERR_INVALID;
+    if (n_sequences < 1) return LATENT_ERR_SHAPE;
+    *bytes = latent::balance_layout(n_sequences).total;
+    return LATENT_OK;
+}
+
+extern "C" LATENT_API int latent_balance_loss(const void *logits, int32_t type, const int32_t *ids,
+                                              const uint8_t *valid, const int32_t *cu_seqlens, int32_t n_tokens,
+                                              int32_t n_expert, int32_t top_k, int32_t n_sequences,
+                                              float balance_coef, float z_coef, const float *d_loss, float *losses,
+                                              int32_t *counts, void *grad, void *workspace, size_t workspace_bytes,
+                                              CUstream_st *stream) {
+    using namespace latent;
+    int st = train_shape(n_tokens, n_expert, top_k);
+    if (st) return st;
+    if (n_sequences < 1 || (n_sequences > 1 && !cu_seqlens)) return LATENT_ERR_SHAPE;
+    if ((int64_t)n_sequences * kCountCluster > 0x7fffffff) return LATENT_ERR_SHAPE;
+    if (!float_type(type)) return LATENT_ERR_DTYPE;
+    if (!losses || !counts || !workspace || (n_tokens > 0 && (!logits || !ids))) return LATENT_ERR_INVALID;
+    const size_t es = type_size(type);
+    if (!is_aligned(logits, es) || !is_aligned(grad, es) || !is_aligned(ids, 4) || !is_aligned(cu_seqlens, 4) ||
+        !is_aligned(d_loss, 4) || !is_aligned(losses, 4) || !is_aligned(counts, 4) || !is_aligned(workspace, 256))
+        return LATENT_ERR_ALIGN;
+    const BalanceLayout L = balance_layout(n_sequences);
+    if (workspace_bytes < L.total) return LATENT_ERR_WORKSPACE;
+    int sms = 0;
+    if ((st = sm_count(&sms))) return st;
+    char *ws = static_cast<char *>(workspace);
+    BalanceArgs a{logits, ids, valid, cu_seqlens, n_tokens, n_expert, top_k, n_sequences, balance_coef, z_coef, d_loss, losses,
+                  counts, grad, reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<double *>(ws + L.partial),
+                  reinterpret_cast<uint32_t *>(ws + L.ticket)};
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    k_balance_count<<<(unsigned)n_sequences * kCountCluster, kCountThreads, 0, s>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return LATENT_ERR_CUDA;
+    int blocks = (n_tokens + kRowWarps - 1) / kRowWarps;
+    const int most = sms * kBalanceBlocksPerSm < kMaxBalanceBlocks ? sms * kBalanceBlocksPerSm : kMaxBalanceBlocks;
+    blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
+    switch (type) {
+        case LATENT_TYPE_F32: return launch_balance<float>(a, blocks, s);
+        case LATENT_TYPE_F16: return launch_balance<__half>(a, blocks, s);
+        default: return launch_balance<__nv_bfloat16>(a, blocks, s);
+    }
+}
+
+extern "C" LATENT_API int latent_router_grad(const void *scores, int32_t type, const int32_t *ids,
+                                             const float *d_weights, int32_t n_tokens, int32_t n_expert, int32_t top_k,
+                                             uint32_t flags, void *d_scores, CUstream_st *stream) {
+    using namespace latent;
+    const int st = train_shape(n_tokens, n_expert, top_k);
+    if (st) return st;
+    if (flags & ~(uint32_t)(LATENT_ROUTER_RENORMALIZE | LATENT_ROUTER_SOFTMAX | LATENT_ROUTER_ACCUMULATE))
+        return LATENT_ERR_INVALID;
+    if (!float_type(type)) return LATENT_ERR_DTYPE;
+    if (top_k > kMaxTrainTopK) return LATENT_ERR_UNSUPPORTED;
+    if (n_tokens == 0) return LATENT_OK;
+    if (!scores || !ids || !d_weights || !d_scores) return LATENT_ERR_INVALID;
+    const size_t es = type_size(type);
+    if (!is_aligned(scores, es) || !is_aligned(d_scores, es) || !is_aligned(ids, 4) || !is_aligned(d_weights, 4))
+        return LATENT_ERR_ALIGN;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    switch (type) {
+        case LATENT_TYPE_F32: return launch_router_grad<float>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
+        case LATENT_TYPE_F16: return launch_router_grad<__half>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
+        default: return launch_router_grad<__nv_bfloat16>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
+    }
+}

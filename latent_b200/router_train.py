@@ -1,0 +1,207 @@
+"""Training side of the router: the balance loss with its gradient, and the gradient of the routing weights.
+
+For recalibrating the router of a compressed layer (the experts stay packed
+and frozen): ``router_topk`` routes the logits, ``ExpertFFN`` runs the
+experts (its per-slot rows give d_weights = <d_out, y_slot>),
+``router_topk_grad`` carries that back to the logits and ``balance_loss``
+adds the load-balance and z losses.  The reference has no training code.
+Both kernels return explicit gradients, which add up in one buffer
+(``out=``) and can be captured into a CUDA graph; where autograd is on and
+the logits require a gradient, ``balance_loss`` and ``router_topk`` are
+differentiable through it as well (outside graph capture).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .runtime import _X_TYPES, _stream_ptr
+
+__all__ = ["BalanceLoss", "balance_loss", "router_topk_grad"]
+
+
+class BalanceLoss(NamedTuple):
+    """What ``balance_loss`` returns."""
+
+    loss: torch.Tensor             # balance_coef * balance + z_coef * z, 0-dim fp32
+    balance: torch.Tensor          # 0-dim fp32
+    z: torch.Tensor                # 0-dim fp32
+    counts: torch.Tensor           # kept slots per expert, int32 [S, E] ([E] without cu_seqlens)
+    grad: Optional[torch.Tensor]   # d loss / d logits in the logits' dtype, with gradient=True
+
+
+def _on(device: torch.device, fn, *args) -> int:
+    """Calls a C entry point with ``device`` current (kernels launch on the current device)."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _router_inputs(logits: torch.Tensor, ids: torch.Tensor, name: str):
+    if not torch.is_tensor(logits) or logits.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{name} must be [T, E], got {tuple(logits.shape)}")
+    if logits.dtype not in _X_TYPES:
+        raise ValueError(f"{name} dtype {logits.dtype} unsupported")
+    if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or ids.shape[1] < 1 or ids.dtype != torch.int32:
+        raise ValueError("ids must be int32 [T, k]")
+    if ids.device != logits.device:
+        raise ValueError(f"ids must be on {logits.device}")
+    return logits.detach().contiguous(), ids.contiguous()
+
+
+def _no_capture(what: str) -> None:
+    # Autograd ties a leaf's gradient to the stream that first used it: a
+    # captured backward pass beside an eager one of the same leaves would end
+    # the process.  The explicit gradients capture.
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} is not differentiated by autograd during graph capture: pass detached logits and "
+                           "use the explicit gradient")
+
+
+def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradient):
+    T, E = logits.shape
+    dev = logits.device
+    L = _lib.lib()
+    n = C.c_size_t(0)
+    _lib.check(L.latent_balance_workspace_size(n_seq, C.byref(n)), "latent_balance_workspace_size")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    losses = torch.empty(3, dtype=torch.float32, device=dev)
+    counts = torch.empty((n_seq, E), dtype=torch.int32, device=dev)
+    grad = torch.empty_like(logits) if gradient else None
+    _lib.check(_on(dev, L.latent_balance_loss, logits.data_ptr(), _X_TYPES[logits.dtype], ids.data_ptr(),
+                   None if valid is None else valid.data_ptr(), None if cu is None else cu.data_ptr(), T, E,
+                   ids.shape[1], n_seq, balance_coef, z_coef, None if d_loss is None else d_loss.data_ptr(),
+                   losses.data_ptr(), counts.data_ptr(), None if grad is None else grad.data_ptr(), ws.data_ptr(),
+                   n.value, _stream_ptr(dev)), "latent_balance_loss")
+    return losses, counts, grad
+
+
+class _BalanceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, balance_coef, z_coef, valid, cu, n_seq):
+        _no_capture("balance_loss")
+        flat = logits.detach().contiguous()
+        losses, counts, _ = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, None, False)
+        ctx.save_for_backward(flat, ids, valid, cu)
+        ctx.args = (balance_coef, z_coef, n_seq)
+        loss, balance, z = losses.unbind()
+        loss, balance, z = loss.clone(), balance.clone(), z.clone()
+        ctx.mark_non_differentiable(balance, z, counts)
+        return loss, balance, z, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, *_):
+        _no_capture("balance_loss")
+        flat, ids, valid, cu = ctx.saved_tensors
+        balance_coef, z_coef, n_seq = ctx.args
+        d = d_loss.to(torch.float32).contiguous()
+        grad = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, d, True)[2]
+        return grad, None, None, None, None, None, None
+
+
+def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 0.01, z_coef: float = 0.0,
+                 valid: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                 gradient: bool = False) -> BalanceLoss:
+    """Load-balance and z losses of a router, the expert counts and the gradient (latent_balance_loss).
+
+    logits [T, E] fp32, bf16 or fp16 on a CUDA device, ids int32 [T, k] as
+    ``router_topk`` returns them (negative: dropped slot).  ``cu_seqlens``
+    int32 [S + 1]: the balance loss is taken per packed sequence and averaged
+    over the sequences that have a row; rows behind the last one take no
+    part.  ``valid`` bool [T]: False marks padded rows, which take no part
+    whatever they hold.  The loss is
+    ``balance_coef * mean_s E sum_e f_se P_se + z_coef * mean_t logsumexp^2``
+    with f the share of the kept slots and P the mean softmax probability.
+
+    With ``gradient`` the result carries d loss / d logits (the logits'
+    dtype), made in the same pass.  An fp16 gradient of a mean over many rows
+    underflows: scale the two coefficients up.  Without it, logits that
+    require a gradient make ``loss`` differentiable by autograd.
+    """
+    flat, ids = _router_inputs(logits, ids, "logits")
+    T = flat.shape[0]
+    n_seq = 1
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2 or cu_seqlens.dtype != torch.int32 or \
+                cu_seqlens.device != flat.device:
+            raise ValueError(f"cu_seqlens must be int32 [S + 1] on {flat.device}")
+        cu_seqlens = cu_seqlens.contiguous()
+        n_seq = cu_seqlens.shape[0] - 1
+    if valid is not None:
+        if tuple(valid.shape) != (T,) or valid.dtype != torch.bool or valid.device != flat.device:
+            raise ValueError(f"valid must be bool [{T}] on {flat.device}")
+        valid = valid.contiguous()
+    balance_coef, z_coef = float(balance_coef), float(z_coef)
+    if logits.requires_grad and torch.is_grad_enabled() and not gradient:
+        loss, balance, z, counts = _BalanceLossFn.apply(logits, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq)
+        grad = None
+    else:
+        losses, counts, grad = _balance(flat, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq, None, gradient)
+        loss, balance, z = losses.unbind()
+    return BalanceLoss(loss, balance, z, counts if cu_seqlens is not None else counts[0], grad)
+
+
+def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.Tensor, renormalize: bool = True,
+                     logits: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``router_topk``'s weights with respect to its scores (latent_router_grad).
+
+    ``scores`` [T, E], ``renormalize`` and ``logits`` as given to
+    ``router_topk``, ``ids`` int32 [T, k] as it returned them, ``d_weights``
+    fp32 [T, k].  Returns [T, E] in the scores' dtype; the kept set is held
+    fixed.  ``out``: a contiguous tensor of the scores' shape and dtype that
+    the gradient is added into (for instance ``balance_loss(...).grad``).
+    """
+    flat, ids = _router_inputs(scores, ids, "scores")
+    if d_weights.shape != ids.shape or d_weights.dtype != torch.float32 or d_weights.device != flat.device:
+        raise ValueError(f"d_weights must be float32 {tuple(ids.shape)} on {flat.device}")
+    flags = (_lib.ROUTER_RENORMALIZE if renormalize else 0) | (_lib.ROUTER_SOFTMAX if logits else 0)
+    if out is None:
+        g = torch.empty_like(flat)
+    else:
+        if out.shape != flat.shape or out.dtype != flat.dtype or out.device != flat.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {flat.dtype} {tuple(flat.shape)} tensor on {flat.device}")
+        if out.data_ptr() == flat.data_ptr() and flat.numel():
+            raise ValueError("out must not be the scores")
+        flags |= _lib.ROUTER_ACCUMULATE
+        g = out
+    d_weights = d_weights.detach().contiguous()
+    T, E = flat.shape
+    _lib.check(_on(flat.device, _lib.lib().latent_router_grad, flat.data_ptr(), _X_TYPES[flat.dtype], ids.data_ptr(),
+                   d_weights.data_ptr(), T, E, ids.shape[1], flags, g.data_ptr(), _stream_ptr(flat.device)),
+               "latent_router_grad")
+    return g
+
+
+class RouterTopK(torch.autograd.Function):
+    """``router_topk`` with weights that autograd can differentiate."""
+
+    @staticmethod
+    def forward(ctx, scores, top_k, threshold, renormalize, logits, expert_counts):
+        from .runtime import router_topk
+        _no_capture("router_topk")
+        flat = scores.detach().contiguous()
+        out = router_topk(flat, top_k, threshold, renormalize, logits, expert_counts)
+        ids, w, n_kept = out[:3]
+        counts = out[3] if expert_counts else None
+        ctx.save_for_backward(flat, ids)
+        ctx.args = (renormalize, logits)
+        ctx.mark_non_differentiable(ids, n_kept, *([counts] if expert_counts else []))
+        return ids, w, n_kept, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_ids, d_w, *_):
+        _no_capture("router_topk")
+        flat, ids = ctx.saved_tensors
+        renormalize, logits = ctx.args
+        exact = flat if flat.dtype in _X_TYPES else flat.to(torch.float32)
+        g = router_topk_grad(exact, ids, d_w.to(torch.float32), renormalize, logits)
+        return g.to(flat.dtype), None, None, None, None, None

@@ -1,0 +1,100 @@
+"""Host-side validation of the adapter and router-training entry points: bad descriptors are rejected
+before anything touches the device (this file needs no GPU)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from latent_b200 import AdapterSet, _lib, balance_loss, router_topk_grad
+from latent_b200.build import build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build()
+    return _lib.lib()
+
+
+def test_router_grad_validates_on_the_host(lib):
+    f = lib.latent_router_grad
+    assert f(None, 0, None, None, 4, 0, 2, 0, None, None) == 2            # no experts
+    assert f(None, 0, None, None, -1, 8, 2, 0, None, None) == 2
+    assert f(None, 0, None, None, 4, 8, 0, 0, None, None) == 2
+    assert f(None, 0, None, None, 1 << 28, 8, 32, 0, None, None) == 2     # too many slots
+    assert f(None, 0, None, None, 4, 8, 2, 8, None, None) == 1            # unknown flag
+    assert f(None, 7, None, None, 4, 8, 2, 0, None, None) == 3
+    assert f(None, 0, None, None, 4, 2048, 2, 0, None, None) == 9
+    assert f(None, 0, None, None, 4, 64, 33, 0, None, None) == 9
+    assert f(None, 0, None, None, 0, 8, 2, 0, None, None) == 0            # empty batch
+    assert f(None, 0, None, None, 4, 8, 2, 0, None, None) == 1            # missing buffers
+    assert f(64, 0, 64, 64, 4, 8, 2, 0, 66, None) == 4                    # unaligned gradient
+
+
+def test_balance_loss_validates_on_the_host(lib):
+    n = C.c_size_t()
+    assert lib.latent_balance_workspace_size(0, C.byref(n)) == 2
+    assert lib.latent_balance_workspace_size(1, None) == 1
+    assert lib.latent_balance_workspace_size(3, C.byref(n)) == 0 and n.value % 256 == 0
+
+    def f(logits=256, typ=0, ids=256, cu=None, T=4, E=8, k=2, S=1, losses=256, counts=256, ws=256, nbytes=n.value):
+        return lib.latent_balance_loss(logits, typ, ids, None, cu, T, E, k, S, 0.1, 0.0, None, losses, counts, None, ws,
+                                       nbytes, None)
+
+    assert f(E=0) == 2 and f(T=-1) == 2 and f(k=0) == 2 and f(S=0) == 2
+    assert f(S=2) == 2                                                    # sequences without borders
+    assert f(typ=5) == 3 and f(E=1025) == 9
+    assert f(logits=None) == 1 and f(ids=None) == 1 and f(losses=None) == 1 and f(counts=None) == 1 and f(ws=None) == 1
+    assert f(logits=258) == 4 and f(ids=258) == 4 and f(ws=128) == 4
+    assert f(nbytes=n.value - 1) == 6
+
+
+def _desc(**kw):
+    d = _lib.AdapterDesc(2, 16, 64, 32, 4, _lib.TYPE_BF16, _lib.TYPE_BF16, 0, 256, 64, 256, 32, 256, 64, 256, 32, 256,
+                         256, 256, 32, 256, 256, 1 << 20)
+    for name, v in kw.items():
+        setattr(d, name, v)
+    return C.byref(d)
+
+
+def test_adapter_project_validates_on_the_host(lib):
+    f = lib.latent_adapter_project
+    assert f(None, None) == 1
+    for bad in ({"n_adapter": -1}, {"n_in": 0}, {"n_out": 0}, {"n_tokens": -1}, {"ldx": 63}, {"ldw": 31}, {"lda": 63},
+                {"ldb": 31}, {"ldy": 31}, {"flags": 1, "ldw": 63}):
+        assert f(_desc(**bad), None) == 2, bad
+    for bad in ({"rank": 8}, {"rank": 48}, {"rank": 256}):
+        assert f(_desc(**bad), None) == 9, bad
+    for bad in ({"type": 0}, {"type": 9}, {"y_type": 1}):
+        assert f(_desc(**bad), None) == 3, bad
+    assert f(_desc(flags=2), None) == 1
+    for name in ("x", "a", "b", "scale", "ids", "y", "err", "workspace"):
+        assert f(_desc(**{name: None}), None) == 1, name
+    for bad in ({"x": 257}, {"w": 257}, {"ids": 258}, {"y": 257}, {"y": 258, "y_type": 0}, {"workspace": 272}):
+        assert f(_desc(**bad), None) == 4, bad
+    assert f(_desc(workspace_bytes=16), None) == 6
+    assert f(_desc(n_tokens=0, x=None), None) == 0                        # empty batch
+    n = C.c_size_t()
+    assert lib.latent_adapter_workspace_size(_desc(), None) == 1
+    assert lib.latent_adapter_workspace_size(_desc(), C.byref(n)) == 0 and n.value % 256 == 0
+    assert lib.latent_adapter_check(None, None) == 1
+
+
+def test_python_refusals_without_a_device():
+    l, ids = torch.zeros((4, 8)), torch.zeros((4, 2), dtype=torch.int32)
+    for bad in (lambda: balance_loss(l, ids), lambda: router_topk_grad(l, ids, torch.zeros((4, 2))),
+                lambda: AdapterSet([], device="cpu"),
+                lambda: AdapterSet([(torch.zeros(8, 2), torch.zeros(3, 8))], device="cpu"),
+                lambda: AdapterSet([(torch.full((8, 2), float("inf")), torch.zeros(2, 8))], device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_adapter_set_layout():
+    """Padding: ranks to one of 16, 32, 64, 128, rows to 16 bytes, zeros everywhere else."""
+    a, b = torch.randn(10, 17), torch.randn(17, 13)
+    s = AdapterSet([(a, b, 0.5), (a[:, :3], b[:3])], device="cpu", dtype=torch.float16)
+    assert s.rank == 32 and s.a.shape == (2, 32, 16) and s.b.shape == (2, 32, 16) and s.ranks == [17, 3]
+    assert torch.equal(s.a[0, :17, :10], a.t().half()) and torch.equal(s.b[1, :3, :13], b[:3].half())
+    assert float(s.a.float().abs().sum()) == float(s.a[0, :17, :10].float().abs().sum() + s.a[1, :3, :10].float().abs().sum())
+    assert s.scale.tolist() == [0.5, 1.0]
