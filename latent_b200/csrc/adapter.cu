@@ -1,10 +1,12 @@
 // Low-rank adapters of many requests beside one shared projection
 // (latent_adapter_project): y[t] = x[t].W + s_a (x[t].A_a).B_a, a = ids[t].
 //
-// Two steps: k_ad_shrink makes t[t] = s_a x[t].A_a (fp32, [T][rank]) and a
-// product kernel adds t.B_a to x.W.  This file has the shrink and the product
-// on the CUDA cores, for any size, stride and alignment.
-#include "internal.h"
+// Two steps: t[t] = s_a x[t].A_a (fp32, [T][rank] in the workspace), then a
+// product kernel that adds t.B_a to x.W.  This file has the entry points and
+// both steps on the CUDA cores (k_ad_shrink_any, k_ad_any), for what the
+// tensor-core kernels cannot read: sizes or strides that are not multiples of
+// 8, unaligned rows, and the adapters' part alone (no dense W).
+#include "adapter_mma.cuh"
 
 namespace latent {
 
@@ -29,7 +31,7 @@ constexpr int kShrinkWarps = 8;
 
 // One warp per (row, rank column): block (t, j0 / 8).
 template <typename T>
-__global__ void __launch_bounds__(kShrinkWarps * 32) k_ad_shrink(latent_adapter_desc d, float *tt) {
+__global__ void __launch_bounds__(kShrinkWarps * 32) k_ad_shrink_any(latent_adapter_desc d, float *tt) {
     const int t = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int j = blockIdx.y * kShrinkWarps + warp;
@@ -49,7 +51,7 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) k_ad_shrink(latent_adapter_
 constexpr int kSB = 64, kSK = 16;
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_ad_simple(latent_adapter_desc d, const float *tt) {
+__global__ void __launch_bounds__(256) k_ad_any(latent_adapter_desc d, const float *tt) {
     __shared__ float xs[kSK][kSB + 4], ws[kSK][kSB + 4];
     const int row0 = blockIdx.y * kSB, col0 = blockIdx.x * kSB;
     const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
@@ -119,6 +121,13 @@ int ad_validate(const latent_adapter_desc *d) {
     return LATENT_OK;
 }
 
+// What TMA and 16-byte stores need: rows of multiples of 16 bytes from 16-byte boundaries.
+bool ad_tensor_cores(const latent_adapter_desc *d) {
+    return d->w && d->n_adapter > 0 && (d->n_in | d->n_out) % 8 == 0 &&
+           (d->ldx | d->ldw | d->lda | d->ldb | d->ldy) % 8 == 0 && ad_aligned(d->x, 16) && ad_aligned(d->w, 16) &&
+           ad_aligned(d->a, 16) && ad_aligned(d->b, 16) && ad_aligned(d->y, 16);
+}
+
 }  // namespace
 
 }  // namespace latent
@@ -149,17 +158,27 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
     size_t need = 0;
     latent_adapter_workspace_size(d, &need);
     if (d->workspace_bytes < need) return LATENT_ERR_WORKSPACE;
+    if (d->n_tokens > 65535 * kSB) return LATENT_ERR_SHAPE;  // row tiles of the CUDA-core grid
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     float *tt = static_cast<float *>(d->workspace);
+    if (ad_tensor_cores(d)) {
+        int dev = 0, sms = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            return LATENT_ERR_CUDA;
+        const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows};
+        if (launch_adapter_shrink(a, sms, s) != cudaSuccess || launch_adapter_skinny(a, sms, s) != cudaSuccess)
+            return LATENT_ERR_CUDA;
+        return LATENT_OK;
+    }
     const dim3 gs((unsigned)d->n_tokens, (unsigned)d->rank / kShrinkWarps);
     const dim3 gp((unsigned)((d->n_out + kSB - 1) / kSB), (unsigned)((d->n_tokens + kSB - 1) / kSB));
-    if (gp.y > 65535u) return LATENT_ERR_SHAPE;
     if (d->type == LATENT_TYPE_F16) {
-        k_ad_shrink<__half><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
-        k_ad_simple<__half><<<gp, 256, 0, s>>>(*d, tt);
+        k_ad_shrink_any<__half><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
+        k_ad_any<__half><<<gp, 256, 0, s>>>(*d, tt);
     } else {
-        k_ad_shrink<__nv_bfloat16><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
-        k_ad_simple<__nv_bfloat16><<<gp, 256, 0, s>>>(*d, tt);
+        k_ad_shrink_any<__nv_bfloat16><<<gs, kShrinkWarps * 32, 0, s>>>(*d, tt);
+        k_ad_any<__nv_bfloat16><<<gp, 256, 0, s>>>(*d, tt);
     }
     return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
