@@ -167,7 +167,9 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return LATENT_ERR_CUDA;
         const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows};
-        if (launch_adapter_shrink(a, sms, s) != cudaSuccess || launch_adapter_skinny(a, sms, s) != cudaSuccess)
+        const bool wide = d->y_type == d->type && d->n_tokens > 256;
+        if (launch_adapter_shrink(a, sms, s) != cudaSuccess ||
+            (wide ? launch_adapter_wide(a, sms, s) : launch_adapter_skinny(a, sms, s)) != cudaSuccess)
             return LATENT_ERR_CUDA;
         return LATENT_OK;
     }

@@ -25,6 +25,7 @@ struct AdapterArgs {
 
 cudaError_t launch_adapter_shrink(const AdapterArgs &a, int sms, cudaStream_t s);
 cudaError_t launch_adapter_skinny(const AdapterArgs &a, int sms, cudaStream_t s);
+cudaError_t launch_adapter_wide(const AdapterArgs &a, int sms, cudaStream_t s);
 
 namespace adapter {
 
@@ -58,6 +59,19 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ bool bar_all(int id, int threads, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "barrier.red.and.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(threads), "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
 }
 
 // Distinct adapters of a tile's rows, in order of first use.
@@ -125,38 +139,45 @@ template <bool BF> __device__ __forceinline__ float load16(const void *p, int64_
     else return __half2float(__ldg(static_cast<const __half *>(p) + i));
 }
 
-// One row of block e (contraction rows 64 e .. 64 e + 63 of the stacked B's) in
-// the K-major 128B-swizzled tile of each part: t where the row's own segment
-// lies, zeros elsewhere.  A part that would not be finite is left to zero.
+// Eight values of t as PARTS 16-byte runs of the operand type that add up to
+// them; what a part that is not finite leaves is zero.
 template <bool BF, int PARTS>
+__device__ __forceinline__ void split_t(const float *t, uint4 (&out)[PARTS]) {
+    const float4 u = __ldcg(reinterpret_cast<const float4 *>(t)), w = __ldcg(reinterpret_cast<const float4 *>(t) + 1);
+    float2 v[4] = {{u.x, u.y}, {u.z, u.w}, {w.x, w.y}, {w.z, w.w}};
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[i] = pack2<BF>(v[i].x, v[i].y);
+            const float2 back = unpack2<BF>(q[i]);
+            v[i].x = isfinite(back.x) ? v[i].x - back.x : 0.f;
+            v[i].y = isfinite(back.y) ? v[i].y - back.y : 0.f;
+        }
+        out[p] = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+}
+
+// One row of an extension block (stacked B rows r0 .. r0 + 8 CHUNKS - 1) in a
+// K-major 128B-swizzled tile: t where the row's own segment lies, zeros
+// elsewhere.  Part p of chunk c goes to 16-byte run c of tile p (CHUNKS 8), or
+// to run 4 p + c of one tile (CHUNKS 4).
+template <bool BF, int PARTS, int CHUNKS>
 __device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t part_bytes, int row, int seg, int rank,
-                                            const float *t, int e) {
+                                            const float *t, int r0) {
 #pragma unroll 2
-    for (int c = 0; c < 8; ++c) {
-        const int r = 64 * e + 8 * c;
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int r = r0 + 8 * c;
         uint4 out[PARTS];
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) out[p] = make_uint4(0u, 0u, 0u, 0u);
-        if (seg >= 0 && r / rank == seg) {
-            const float4 u = __ldcg(reinterpret_cast<const float4 *>(t + r % rank));
-            const float4 w = __ldcg(reinterpret_cast<const float4 *>(t + r % rank) + 1);
-            float2 v[4] = {{u.x, u.y}, {u.z, u.w}, {w.x, w.y}, {w.z, w.w}};
+        if (seg >= 0 && r / rank == seg) split_t<BF, PARTS>(t + r % rank, out);
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                uint32_t q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    q[i] = pack2<BF>(v[i].x, v[i].y);
-                    const float2 back = unpack2<BF>(q[i]);
-                    v[i].x = isfinite(back.x) ? v[i].x - back.x : 0.f;
-                    v[i].y = isfinite(back.y) ? v[i].y - back.y : 0.f;
-                }
-                out[p] = make_uint4(q[0], q[1], q[2], q[3]);
-            }
+        for (int p = 0; p < PARTS; ++p) {
+            const int run = CHUNKS == 8 ? c : CHUNKS * p + c;
+            *reinterpret_cast<uint4 *>(tile + (CHUNKS == 8 ? p * part_bytes : 0u) + row * 128 + ((run ^ (row & 7)) * 16)) = out[p];
         }
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-            *reinterpret_cast<uint4 *>(tile + p * part_bytes + row * 128 + ((c ^ (row & 7)) * 16)) = out[p];
     }
 }
 

@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             const int b = (e - e0) & 1;
             if (e - e0 >= 2 && !mbar_wait(sh.t_empty + b, (uint32_t)((e - e0) / 2 - 1) & 1u)) { ok = false; break; }
             if (sh.abort) { ok = false; break; }
-            if (r < p.rows) build_t_row<BF, PARTS>(tbuf + (uint32_t)(b * PARTS) * xbytes, xbytes, r, wide ? -1 : seg, rank, t, e);
+            if (r < p.rows) build_t_row<BF, PARTS, 8>(tbuf + (uint32_t)(b * PARTS) * xbytes, xbytes, r, wide ? -1 : seg, rank, t, e * kBK);
             fence_async_shared();
             mbar_arrive(sh.t_full + b);
         }
