@@ -166,7 +166,8 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         if (cudaGetDevice(&dev) != cudaSuccess ||
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return LATENT_ERR_CUDA;
-        const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows};
+        const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows,
+                            d->rank == 16 ? 4 : d->rank == 32 ? 5 : d->rank == 64 ? 6 : 7};
         const bool wide = d->y_type == d->type && d->n_tokens > 256;
         if (launch_adapter_shrink(a, sms, s) != cudaSuccess ||
             (wide ? launch_adapter_wide(a, sms, s) : launch_adapter_skinny(a, sms, s)) != cudaSuccess)

@@ -21,6 +21,7 @@ struct AdapterArgs {
     latent_adapter_desc d;
     float *t;        // [T][rank] scale * x.A (fp32)
     int tile_rows;   // rows per tile: 128, fewer rounded up to 16
+    int log2r;       // rank = 1 << log2r
 };
 
 cudaError_t launch_adapter_shrink(const AdapterArgs &a, int sms, cudaStream_t s);
@@ -54,6 +55,36 @@ __device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t saddr) {
     return d;
 }
 
+// Bounded wait for the phase with parity `parity`; CLUSTER: acquires what
+// threads of the other blocks wrote before they arrived.  Each try suspends for
+// a while; the clock is read after every 32.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_addr(bar);
+    unsigned long long t0 = 0;
+    for (unsigned i = 1;; ++i) {
+        uint32_t done;
+        if constexpr (CLUSTER)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(done) : "r"(a), "r"(parity) : "memory");
+        else
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(done) : "r"(a), "r"(parity) : "memory");
+        if (done) return true;
+        if ((i & 31u) == 0) {
+            const unsigned long long now = global_ns();
+            if (i == 32) t0 = now;
+            else if (now - t0 > kWaitNs) return false;
+        }
+    }
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -84,20 +115,24 @@ struct Segments {
     int n;                       // distinct adapters
 };
 
-// By 128 threads (tid 0..127, named barrier `bar`): thread i finds the first
-// row with row i's adapter; the rows that are their own first are numbered.
-__device__ __forceinline__ void build_segments(Segments &s, const latent_adapter_desc &d, int t0, int nt, int tid,
-                                               int bar, bool report) {
-    int a = tid < nt ? __ldg(d.ids + t0 + tid) : -1;
-    if (a >= d.n_adapter) {
-        if (report) atomicOr(d.err, kErrExpertId);
-        a = -1;
-    }
+// A row's adapter, -1 for none (ids that no adapter has are reported and count as none).
+__device__ __forceinline__ int row_adapter(const latent_adapter_desc &d, int t, bool live, bool report) {
+    const int a = live ? __ldg(d.ids + t) : -1;
+    if (a < d.n_adapter) return a;
+    if (report) atomicOr(d.err, kErrExpertId);
+    return -1;
+}
+
+// By 128 threads (tid 0..127, named barrier `bar`), a: the adapter of row tid
+// (-1 behind row nt): thread i finds the first row with row i's adapter; the
+// rows that are their own first are numbered.  The other warps see the result
+// behind a barrier of the caller's.
+__device__ __forceinline__ void build_segments(Segments &s, int a, int nt, int tid, int bar) {
     s.ids[tid] = a;
     bar_sync(bar, kRows);
     int lead = tid;
 #pragma unroll 4
-    for (int j = kRows - 4; j >= 0; j -= 4) {
+    for (int j = (nt - 1) & ~3; j >= 0; j -= 4) {
         const int4 v = *reinterpret_cast<const int4 *>(s.ids + j);
         if (v.w == a) lead = j + 3;
         if (v.z == a) lead = j + 2;
@@ -118,7 +153,6 @@ __device__ __forceinline__ void build_segments(Segments &s, const latent_adapter
     if (tid == 0) s.n = s.warp_n[0] + s.warp_n[1] + s.warp_n[2] + s.warp_n[3];
     bar_sync(bar, kRows);
     s.row[tid] = a >= 0 ? s.first[lead] : -1;
-    bar_sync(bar, kRows);
 }
 
 template <bool BF> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -139,46 +173,49 @@ template <bool BF> __device__ __forceinline__ float load16(const void *p, int64_
     else return __half2float(__ldg(static_cast<const __half *>(p) + i));
 }
 
-// Eight values of t as PARTS 16-byte runs of the operand type that add up to
-// them; what a part that is not finite leaves is zero.
-template <bool BF, int PARTS>
-__device__ __forceinline__ void split_t(const float *t, uint4 (&out)[PARTS]) {
-    const float4 u = __ldcg(reinterpret_cast<const float4 *>(t)), w = __ldcg(reinterpret_cast<const float4 *>(t) + 1);
-    float2 v[4] = {{u.x, u.y}, {u.z, u.w}, {w.x, w.y}, {w.z, w.w}};
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-        uint32_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q[i] = pack2<BF>(v[i].x, v[i].y);
-            const float2 back = unpack2<BF>(q[i]);
-            v[i].x = isfinite(back.x) ? v[i].x - back.x : 0.f;
-            v[i].y = isfinite(back.y) ? v[i].y - back.y : 0.f;
-        }
-        out[p] = make_uint4(q[0], q[1], q[2], q[3]);
-    }
-}
+// The contraction of an extension block: 32 stacked B rows.
+constexpr int kExt = 32;
 
-// One row of an extension block (stacked B rows r0 .. r0 + 8 CHUNKS - 1) in a
-// K-major 128B-swizzled tile: t where the row's own segment lies, zeros
-// elsewhere.  Part p of chunk c goes to 16-byte run c of tile p (CHUNKS 8), or
-// to run 4 p + c of one tile (CHUNKS 4).
-template <bool BF, int PARTS, int CHUNKS>
-__device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t part_bytes, int row, int seg, int rank,
+// One row of an extension block (stacked rows r0 .. r0 + 31) in K-major
+// 128B-swizzled tiles: t where the row's own segment lies, zeros elsewhere.  A
+// 128-byte row holds two parts of the 32 values (a third goes to a second
+// tile, tile_bytes further); what a part that is not finite leaves is zero.
+template <bool BF, int PARTS>
+__device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t tile_bytes, int row, int seg, int rank, int log2r,
                                             const float *t, int r0) {
-#pragma unroll 2
-    for (int c = 0; c < CHUNKS; ++c) {
+    float4 v[8];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {  // all loads first: one trip to L2
         const int r = r0 + 8 * c;
-        uint4 out[PARTS];
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) out[p] = make_uint4(0u, 0u, 0u, 0u);
-        if (seg >= 0 && r / rank == seg) split_t<BF, PARTS>(t + r % rank, out);
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            const int run = CHUNKS == 8 ? c : CHUNKS * p + c;
-            *reinterpret_cast<uint4 *>(tile + (CHUNKS == 8 ? p * part_bytes : 0u) + row * 128 + ((run ^ (row & 7)) * 16)) = out[p];
-        }
+        const bool mine = seg >= 0 && (r >> log2r) == seg;
+        const float4 *p = reinterpret_cast<const float4 *>(t + (r & (rank - 1)));
+        v[2 * c] = mine ? __ldcg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[2 * c + 1] = mine ? __ldcg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float &x = i & 1 ? v[2 * c + i / 2].z : v[2 * c + i / 2].x;
+                float &y = i & 1 ? v[2 * c + i / 2].w : v[2 * c + i / 2].y;
+                q[i] = pack2<BF>(x, y);
+                if (p + 1 < PARTS) {
+                    const float2 back = unpack2<BF>(q[i]);
+                    x = isfinite(back.x) ? x - back.x : 0.f;
+                    y = isfinite(back.y) ? y - back.y : 0.f;
+                }
+            }
+            const int run = 4 * (p & 1) + c;
+            *reinterpret_cast<uint4 *>(tile + (p >> 1) * tile_bytes + row * 128 + ((run ^ (row & 7)) * 16)) =
+                make_uint4(q[0], q[1], q[2], q[3]);
+        }
+}
+// Byte offset of part p, contraction step kk (16 values) in those tiles.
+__device__ __forceinline__ uint32_t t_offset(int p, int kk, uint32_t tile_bytes) {
+    return (uint32_t)(p >> 1) * tile_bytes + (uint32_t)(p & 1) * 64u + (uint32_t)kk * 32u;
 }
 
 // fp16 parts reach 65504.  A row whose t goes further (or is not a number)

@@ -13,7 +13,6 @@
 // k_ad_skinny is launched as a programmatic dependent of k_ad_shrink: it
 // streams W while x.A is still being made and waits for it (griddepcontrol)
 // only before the extension blocks.
-#include <cooperative_groups.h>
 #include <cuda.h>
 
 #include <mutex>
@@ -24,29 +23,40 @@ namespace latent {
 
 namespace {
 
-namespace cg = cooperative_groups;
 using namespace adapter;
 
 constexpr int kThreads = 256;  // warp 0: TMA, 1: MMA, 2: TMEM, 4..7: rows (segments, x.A parts, epilogue)
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 12;
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc, t_full[2], t_empty[2];
+    uint64_t acc_full[2], acc_empty[2], t_full[2], t_empty[2], seg;
     uint32_t tmem;
     volatile int abort;
     uint8_t wide[kRows];   // fp16: rows finished in fp32
-    Segments seg;
+    Segments segs;
 };
 
 struct Plan {
     int rows;       // N of the MMA: rows of x per tile, a multiple of 16
     int stages;
-    int cluster;
-    int parts;
-    int chunk;      // blocks per accumulator
+    int chunk;      // blocks per accumulator (k_ad_skinny)
     uint32_t cols;  // TMEM columns
     size_t smem;
+};
+
+// Position in the ring of stages: slot and the parity of its current phase.
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    bool wrapped = false;
+    __device__ __forceinline__ void next(int stages) {
+        if (++s == stages) {
+            s = 0;
+            phase ^= 1u;
+            wrapped = true;
+        }
+    }
 };
 
 __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
@@ -58,53 +68,53 @@ __device__ __forceinline__ void give_up(Shared &sh, uint32_t *err) {
     sh.abort = 1;
 }
 
-// The loads of the last stages issued must land before the block exits.
-__device__ __forceinline__ void drain(Shared &sh, int issued, int stages) {
-    for (int j = 0; j < stages && j < issued; ++j) {
-        const int i = issued - 1 - j;
-        mbar_wait(sh.full + i % stages, (uint32_t)(i / stages) & 1u);
-    }
+// After a failure: the loads in flight land well within 20 ms.
+__device__ __forceinline__ void drain() {
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 20000000ull) __nanosleep(1000);
 }
 
-__device__ __forceinline__ void setup(Shared &sh, int stages, uint32_t cols, int builders) {
+__device__ __forceinline__ void setup(Shared &sh, const Plan &p) {
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < p.stages; ++s) {
             mbar_init(sh.full + s, 1);
             mbar_init(sh.empty + s, 1);
         }
-        mbar_init(&sh.acc, 1);
         for (int b = 0; b < 2; ++b) {
-            mbar_init(sh.t_full + b, builders);
+            mbar_init(sh.acc_full + b, 1);
+            mbar_init(sh.acc_empty + b, 128);
+            mbar_init(sh.t_full + b, 128);
             mbar_init(sh.t_empty + b, 1);
         }
+        mbar_init(&sh.seg, 128);
         sh.abort = 0;
         fence_barrier_init();
     }
     if (threadIdx.x / 32 == 2) {
-        tmem_alloc(&sh.tmem, cols);
+        tmem_alloc(&sh.tmem, p.cols);
         tmem_relinquish();
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
 }
 
-// This block's accumulator (lane = M row, column = row of x) as part[row][128].
-__device__ __forceinline__ void store_partial(float *part, uint32_t tmem, int rows, int groups, int tid) {
-    for (int c = 0; c < rows; c += 32) {  // columns behind `rows` inside the last 32 are allocated and dropped
-        float s[32];
-        for (int g = 0; g < groups; ++g) {
-            uint32_t v[32];
-            tmem_ld32(tmem + ((uint32_t)(tid & ~31) << 16) + (uint32_t)(g * rows + c), v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] = g ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (c + j < rows) part[(c + j) * 128 + tid] = s[j];
-    }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // x.A.  Block (cluster rank, slot, row tile); the stacked rank columns of the
-// tile's adapters in tiles of 128, slot, slot + gridDim.y, ...
+// tile's adapters in tiles of 128: slot, slot + gridDim.y, ...  Rank q of the
+// cluster sums K blocks of its share; every block sends the t of a row to the
+// row's owner (rows are dealt to the cluster in runs), which adds them up in
+// rank order.
 template <bool BF>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant__ CUtensorMap mA,
                                                            const __grid_constant__ CUtensorMap mX, AdapterArgs g,
@@ -112,84 +122,127 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     extern __shared__ uint8_t raw[];
     uint8_t *ring = align1024(raw);
     const uint32_t stage = 16384u + (uint32_t)p.rows * 128u;
-    float *part = reinterpret_cast<float *>(ring + p.stages * stage);
+    float *recv = reinterpret_cast<float *>(ring + p.stages * stage);  // [cluster][rows of a rank][rank]
     __shared__ Shared sh;
-    cg::cluster_group cluster = cg::this_cluster();
     const int q = blockIdx.x, CS = gridDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
-    const int rank = d.rank;
+    const int rank = d.rank, log2r = g.log2r;
     launch_dependents();
-    setup(sh, p.stages, p.cols, 1);
-    if (warp >= 4) build_segments(sh.seg, d, t0, nt, threadIdx.x - 128, 1, q == 0 && blockIdx.y == 0);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    cluster_arrive();  // the others may send once every block has started
+    int a = -1;
+    if (warp == 0 && lane == 0) {
+        prefetch_tensormap(&mA);
+        prefetch_tensormap(&mX);
+    } else if (warp >= 4) {
+        const int r = threadIdx.x - 128;
+        a = row_adapter(d, t0 + r, r < nt, q == 0 && blockIdx.y == 0);
+    }
+    setup(sh, p);
     const uint32_t tmem = sh.tmem;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
-    const int total = sh.seg.n * rank;  // stacked rank columns
-    int it = 0;                         // stages issued or used by this role
-    uint32_t tile = 0;
-    for (int m = blockIdx.y * 128; m < total; m += gridDim.y * 128, ++tile) {
-        if (warp == 0 && lane == 0 && !sh.abort) {
-            const int boxes = min(8, (total - m) / 16);
-            bool ok = true;
-            for (int k = k0; k < k1; ++k, ++it) {
-                const int s = it % p.stages;
-                if (it >= p.stages && !mbar_wait(sh.empty + s, (uint32_t)(it / p.stages - 1) & 1u)) { ok = false; break; }
-                if (sh.abort) { ok = false; break; }
-                uint8_t *st = ring + s * stage;
-                mbar_arrive_expect_tx(sh.full + s, (uint32_t)boxes * 2048u + (uint32_t)p.rows * 128u);
-                for (int i = 0; i < boxes; ++i) {
-                    const int r = m + 16 * i;
-                    tma_load_2d(st + i * 2048, &mA, k * kBK, sh.seg.id[r / rank] * rank + r % rank, sh.full + s);
+    const int per = (nt + CS - 1) / CS;  // rows of an owner
+    bool ok = true;
+    if (warp >= 4) {
+        build_segments(sh.segs, a, nt, threadIdx.x - 128, 1);
+        mbar_arrive(&sh.seg);
+    }
+    ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
+    const int total = ok ? sh.segs.n * rank : 0;  // stacked rank columns
+    if (warp == 0) {
+        // lane i loads the i-th run of stacked columns of a stage; the last one loads x
+        Ring at;
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128) {
+            const int cols = min(128, total - m), boxes = cols >> log2r;
+            int row = 0;
+            if (lane < boxes) row = sh.segs.id[(m >> log2r) + lane] << log2r;
+            for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+                if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
+                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+                uint8_t *st = ring + at.s * stage;
+                if (lane == 31) {
+                    mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(cols + p.rows) * 128u);
+                    tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
                 }
-                tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + s);
+                if (lane < boxes) tma_load_2d(st + ((uint32_t)lane << log2r) * 128u, &mA, k * kBK, row, sh.full + at.s);
             }
-            if (!ok) {
-                give_up(sh, d.err);
-                drain(sh, it, p.stages);
-            }
-        } else if (warp == 1 && lane == 0 && !sh.abort) {
-            const uint32_t id = idesc(BF, p.rows, false, false);
-            bool ok = true;
-            for (int k = k0; k < k1; ++k, ++it) {
-                const int s = it % p.stages;
-                if (!mbar_wait(sh.full + s, (uint32_t)(it / p.stages) & 1u) || sh.abort) { ok = false; break; }
+        }
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t id = idesc(BF, p.rows, false, false);
+        Ring at;
+        uint32_t n = 0;
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128, ++n) {
+            const uint32_t b = n & 1u;
+            if (n >= 2 && !wait(sh.acc_empty + b, ((n >> 1) - 1u) & 1u)) { ok = false; break; }
+            tc_fence_after();
+            for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+                if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t a = smem_addr(ring + s * stage), x = a + 16384u;
+                const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    mma_f16(tmem, desc_kmajor_sw128(a + kk * 32), desc_kmajor_sw128(x + kk * 32), id, (k > k0) | kk);
-                mma_commit(sh.empty + s);
+                    mma_f16(tmem + b * 128u, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), id,
+                            (k > k0) | kk);
+                mma_commit(sh.empty + at.s);
             }
-            if (!ok) give_up(sh, d.err);
-            mma_commit(&sh.acc);
-        } else if (warp >= 4 && !sh.abort) {
-            if (!mbar_wait(&sh.acc, tile & 1u)) give_up(sh, d.err);
+            if (ok) mma_commit(sh.acc_full + b);
+        }
+        if (!ok) {
+            mma_commit(sh.acc_full);
+            mma_commit(sh.acc_full + 1);
+        }
+    } else if (warp >= 4) {
+        const int tid = threadIdx.x - 128;
+        cluster_wait();
+        uint32_t n = 0;
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128, ++n) {
+            const uint32_t b = n & 1u;
+            if (!wait(sh.acc_full + b, (n >> 1) & 1u) || sh.abort) ok = false;
+            if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
             tc_fence_after();
-            store_partial(part, tmem, p.rows, 1, threadIdx.x - 128);
+            const int seg = (m + tid) >> log2r, j = (m + tid) & (rank - 1);
+            int owner = 0, r_own = 0;  // of row c + i below
+            for (int c = 0; c < p.rows; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(tmem + b * 128u + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (c + i < nt) {
+                        if (sh.segs.row[c + i] == seg)
+                            st_cluster(map_rank(smem_addr(recv + ((q * per + r_own) << log2r) + j), owner),
+                                       __uint_as_float(v[i]));
+                        if (++r_own == per) {
+                            r_own = 0;
+                            ++owner;
+                        }
+                    }
+                }
+                __syncwarp();
+            }
             tc_fence_before();
+            mbar_arrive(sh.acc_empty + b);
         }
-        __syncwarp();
-        cluster.sync();
-        // this block's share of the rows: t[row][j] = scale * sum over the cluster, in rank order
-        const int per = (nt + CS - 1) / CS;
-        const int r0 = q * per, r1 = min(nt, r0 + per);
-        for (int i = threadIdx.x; i < (r1 - r0) * rank; i += kThreads) {
-            const int r = r0 + i / rank, j = i % rank;
-            const int s = sh.seg.row[r];
-            const int at = s * rank + j - m;
-            if (s < 0 || at < 0 || at >= 128) continue;
-            float v = 0.f;
-            for (int c = 0; c < CS; ++c) v += cluster.map_shared_rank(part, c)[r * 128 + at];
-            g.t[(int64_t)(t0 + r) * rank + j] = v * __ldg(d.scale + sh.seg.id[s]);
-        }
-        __syncwarp();
-        cluster.sync();
-        tc_fence_after();
+    }
+    if (!ok) {
+        give_up(sh, d.err);
+        drain();
+    }
+    __syncwarp();
+    if (warp < 4) cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+    // this block's rows: t[row][j] = scale * sum over the cluster, in rank order
+    const int r0 = q * per, r1 = min(nt, r0 + per);
+    for (int i = threadIdx.x; i < (r1 - r0) << log2r; i += kThreads) {
+        const int r = i >> log2r, s = sh.segs.row[r0 + r];
+        // rows without an adapter, and rows of another slot's tiles
+        if (s < 0 || ((uint32_t)(s << log2r) / 128u) % gridDim.y != blockIdx.y) continue;
+        float v = 0.f;
+        for (int c = 0; c < CS; ++c) v += recv[((c * per) << log2r) + i];
+        g.t[((int64_t)(t0 + r0) << log2r) + i] = v * __ldg(d.scale + sh.segs.id[s]);
     }
     tc_fence_before();
     __syncthreads();
@@ -203,141 +256,195 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                                                            const __grid_constant__ CUtensorMap mB,
                                                            const __grid_constant__ CUtensorMap mX, AdapterArgs g,
                                                            Plan p) {
+    constexpr uint32_t kTiles = (PARTS + 1) / 2;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = align1024(raw);
     const uint32_t xbytes = (uint32_t)p.rows * 128u, stage = 16384u + xbytes;
-    uint8_t *tbuf = ring + p.stages * stage;              // 2 x PARTS x [rows][128 bytes]
-    float *part = reinterpret_cast<float *>(ring);        // after the last MMA
+    uint8_t *tbuf = ring + p.stages * stage;                                      // 2 x kTiles x [rows][128 bytes]
+    float *recv = reinterpret_cast<float *>(tbuf + 2 * kTiles * xbytes);          // [cluster][rows of a rank][128]
     __shared__ Shared sh;
-    cg::cluster_group cluster = cg::this_cluster();
     const int q = blockIdx.x, CS = gridDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int n0 = blockIdx.y * 128, t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
-    const int rank = d.rank;
-    setup(sh, p.stages, p.cols, 128);
-    if (warp >= 4) build_segments(sh.seg, d, t0, nt, threadIdx.x - 128, 1, false);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    const int rank = d.rank, log2r = g.log2r;
+    cluster_arrive();
+    int a = -1;
+    if (warp == 0 && lane == 0) {
+        prefetch_tensormap(&mW);
+        prefetch_tensormap(&mX);
+        prefetch_tensormap(&mB);
+    } else if (warp >= 4) {
+        const int r = threadIdx.x - 128;
+        a = row_adapter(d, t0 + r, r < nt, false);
+    }
+    setup(sh, p);
     const uint32_t tmem = sh.tmem;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
-    const int ext = sh.seg.n * rank, ne = (ext + kBK - 1) / kBK;
-    const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
-    const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators; the extension goes to the last
-    if (warp == 0 && lane == 0) {
-        int it = 0;
-        bool ok = true;
-        for (int k = k0; k < k1 + (e1 - e0); ++k, ++it) {
-            const int s = it % p.stages;
-            if (it >= p.stages && !mbar_wait(sh.empty + s, (uint32_t)(it / p.stages - 1) & 1u)) { ok = false; break; }
-            if (sh.abort) { ok = false; break; }
-            uint8_t *st = ring + s * stage;
-            if (k < k1) {
-                mbar_arrive_expect_tx(sh.full + s, stage);
-                if (KN) {
-                    tma_load_2d(st, &mW, n0, k * kBK, sh.full + s);
-                    tma_load_2d(st + 8192, &mW, n0 + 64, k * kBK, sh.full + s);
-                } else {
-                    tma_load_2d(st, &mW, k * kBK, n0, sh.full + s);
-                }
-                tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + s);
-            } else {
-                const int r0 = (e0 + k - k1) * kBK, boxes = min(4, (ext - r0) / 16);
-                mbar_arrive_expect_tx(sh.full + s, (uint32_t)boxes * 4096u);
-                for (int i = 0; i < boxes; ++i) {
-                    const int r = r0 + 16 * i, row = sh.seg.id[r / rank] * rank + r % rank;
-                    tma_load_2d(st + i * 2048, &mB, n0, row, sh.full + s);
-                    tma_load_2d(st + 8192 + i * 2048, &mB, n0 + 64, row, sh.full + s);
+    const int per = (nt + CS - 1) / CS;  // rows of an owner
+    bool ok = true;
+    if (warp == 0) {
+        Ring at;
+        for (int k = k0; k < k1 && ok; ++k, at.next(p.stages)) {
+            if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
+            if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+            uint8_t *st = ring + at.s * stage;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(sh.full + at.s, stage);
+                if (KN) tma_load_2d(st, &mW, n0, k * kBK, sh.full + at.s);
+                else tma_load_2d(st, &mW, k * kBK, n0, sh.full + at.s);
+            } else if (lane == 1) {
+                if (KN) tma_load_2d(st + 8192, &mW, n0 + 64, k * kBK, sh.full + at.s);
+            } else if (lane == 2) {
+                tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
+            }
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
+        if (ok) {
+            const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
+            const int e1 = (int)((int64_t)ne * (q + 1) / CS), box = min(rank, kExt);
+            for (int e = (int)((int64_t)ne * q / CS); e < e1; ++e, at.next(p.stages)) {
+                if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
+                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+                uint8_t *st = ring + at.s * stage;
+                const int rows = min(kExt, ext - e * kExt), j = (lane >> 1) * box;
+                if (lane == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 256u);
+                __syncwarp();
+                if (j < rows) {
+                    const int r = e * kExt + j;
+                    tma_load_2d(st + (lane & 1) * 8192 + j * 128, &mB, n0 + (lane & 1) * 64,
+                                (sh.segs.id[r >> log2r] << log2r) + (r & (rank - 1)), sh.full + at.s);
                 }
             }
         }
-        if (!ok) {
-            give_up(sh, d.err);
-            drain(sh, it, p.stages);
-        }
     } else if (warp == 1 && lane == 0) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
-        int it = 0;
-        bool ok = true;
-        for (int k = k0; k < k1; ++k, ++it) {
-            const int s = it % p.stages;
-            if (!mbar_wait(sh.full + s, (uint32_t)(it / p.stages) & 1u) || sh.abort) { ok = false; break; }
+        Ring at;
+        int in_chunk = 0;
+        uint32_t acc = tmem;
+        for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+            if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
             tc_fence_after();
-            const uint32_t a = smem_addr(ring + s * stage), x = a + 16384u;
-            const int grp = (k - k0) / p.chunk, first = grp * p.chunk + k0;
+            const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
+            if (in_chunk == p.chunk) {
+                in_chunk = 0;
+                acc += (uint32_t)p.rows;
+            }
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-                mma_f16(tmem + (uint32_t)(grp * p.rows), KN ? desc_mnmajor_sw128(a + kk * 2048) : desc_kmajor_sw128(a + kk * 32),
-                        desc_kmajor_sw128(x + kk * 32), id, (k > first) | kk);
-            mma_commit(sh.empty + s);
+                mma_f16(acc, KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32),
+                        desc_kmajor_sw128(x + kk * 32), id, in_chunk | kk);
+            ++in_chunk;
+            mma_commit(sh.empty + at.s);
         }
-        for (int e = e0; ok && e < e1; ++e, ++it) {
-            const int s = it % p.stages, b = (e - e0) & 1;
-            if (!mbar_wait(sh.full + s, (uint32_t)(it / p.stages) & 1u) ||
-                !mbar_wait(sh.t_full + b, (uint32_t)((e - e0) >> 1) & 1u) || sh.abort) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t a = smem_addr(ring + s * stage), t = smem_addr(tbuf) + (uint32_t)(b * PARTS) * xbytes;
-            const int steps = min(4, (ext - e * kBK) / 16);
-            for (int kk = 0; kk < steps; ++kk)
+        if (ok) ok = wait(&sh.seg, 0u);
+        if (ok) {
+            const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
+            const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
+            for (int e = e0; e < e1; ++e, at.next(p.stages)) {
+                const int b = (e - e0) & 1;
+                if (!wait(sh.full + at.s, at.phase) || !wait(sh.t_full + b, (uint32_t)((e - e0) >> 1) & 1u) || sh.abort) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t w = smem_addr(ring + at.s * stage), t = smem_addr(tbuf) + (uint32_t)b * kTiles * xbytes;
+                const int steps = min(kExt / 16, (ext - e * kExt) / 16);
+                for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
-                for (int w = 0; w < PARTS; ++w)
-                    mma_f16(tmem + (uint32_t)((groups - 1) * p.rows), desc_mnmajor_sw128(a + kk * 2048),
-                            desc_kmajor_sw128(t + w * xbytes + kk * 32), idx, 1);
-            mma_commit(sh.empty + s);
-            mma_commit(sh.t_empty + b);
+                    for (int w2 = 0; w2 < PARTS; ++w2)
+                        mma_f16(acc, desc_mnmajor_sw128(w + kk * 2048), desc_kmajor_sw128(t + t_offset(w2, kk, xbytes)),
+                                idx, 1);
+                mma_commit(sh.empty + at.s);
+                mma_commit(sh.t_empty + b);
+            }
         }
-        if (!ok) give_up(sh, d.err);
-        mma_commit(&sh.acc);
+        mma_commit(sh.acc_full);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
-        const int seg = sh.seg.row[r];
-        const float *t = g.t + (int64_t)(t0 + r) * rank;
+        build_segments(sh.segs, a, nt, r, 1);
+        mbar_arrive(&sh.seg);
+        ok = wait(&sh.seg, 0u);
+        const int seg = sh.segs.row[r];
+        const int ext = ok ? sh.segs.n * rank : 0, ne = (ext + kExt - 1) / kExt;
+        const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
+        const float *t = g.t + ((int64_t)(t0 + r) << log2r);
         dependency_wait();
         const bool wide = !BF && seg >= 0 && beyond_f16(t, rank);
         sh.wide[r] = wide;
-        bool ok = true;
         for (int e = e0; e < e1; ++e) {
             const int b = (e - e0) & 1;
-            if (e - e0 >= 2 && !mbar_wait(sh.t_empty + b, (uint32_t)((e - e0) / 2 - 1) & 1u)) { ok = false; break; }
+            if (e - e0 >= 2 && !wait(sh.t_empty + b, (uint32_t)((e - e0) / 2 - 1) & 1u)) { ok = false; break; }
             if (sh.abort) { ok = false; break; }
-            if (r < p.rows) build_t_row<BF, PARTS, 8>(tbuf + (uint32_t)(b * PARTS) * xbytes, xbytes, r, wide ? -1 : seg, rank, t, e * kBK);
+            if (r < p.rows)
+                build_t_row<BF, PARTS>(tbuf + (uint32_t)b * kTiles * xbytes, xbytes, r, wide ? -1 : seg, rank, log2r, t,
+                                       e * kExt);
             fence_async_shared();
             mbar_arrive(sh.t_full + b);
         }
-        if (!ok || !mbar_wait(&sh.acc, 0u)) give_up(sh, d.err);
+        __syncwarp();
+        if (!wait(sh.acc_full, 0u)) ok = false;
+        __syncwarp();
         tc_fence_after();
-        store_partial(part, tmem, p.rows, groups, r);
+        cluster_wait();
+        // column c of the accumulator = row c of x, to its owner
+        const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
+        const uint32_t base = smem_addr(recv) + (uint32_t)r * 4u;
+        int owner = 0, r_own = 0;
+        for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
+            float s[32];
+            for (int gr = 0; gr < groups; ++gr) {
+                uint32_t v[32];
+                tmem_ld32(tmem + ((uint32_t)(r & ~31) << 16) + (uint32_t)(gr * p.rows + c), v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) s[j] = gr ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                if (c + j < nt) {
+                    st_cluster(map_rank(base + (uint32_t)(q * per + r_own) * 512u, owner), s[j]);
+                    if (++r_own == per) {
+                        r_own = 0;
+                        ++owner;
+                    }
+                }
+            }
+        }
         tc_fence_before();
     }
+    if (!ok) {
+        give_up(sh, d.err);
+        drain();
+    }
     __syncwarp();
-    cluster.sync();
-    // this block's share of the rows, two columns per thread: the cluster's partial tiles in rank order
-    const int per = (nt + CS - 1) / CS;
+    if (warp < 4) cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+    // this block's rows, two columns per thread: the cluster's parts in rank order
     const int r0 = q * per, r1 = min(nt, r0 + per);
     const int n = n0 + 2 * (threadIdx.x & 63);
-    for (int r = r0 + (threadIdx.x >> 6); r < r1; r += kThreads / 64) {
+    for (int r = r0 + (threadIdx.x >> 6); r < r1 && n < d.n_out; r += kThreads / 64) {
         float2 v = make_float2(0.f, 0.f);
         for (int c = 0; c < CS; ++c) {
-            const float2 u = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(part, c) + r * 128 + 2 * (threadIdx.x & 63));
+            const float2 u = *reinterpret_cast<const float2 *>(recv + (c * per + r - r0) * 128 + 2 * (threadIdx.x & 63));
             v.x += u.x;
             v.y += u.y;
         }
-        if (n >= d.n_out) continue;
         if (!BF && sh.wide[r]) {
-            const float *t = g.t + (int64_t)(t0 + r) * rank;
-            const int a = sh.seg.id[sh.seg.row[r]];
-            v.x += adapter_dot<BF>(d, t, a, n);
-            v.y += adapter_dot<BF>(d, t, a, n + 1);
+            const float *t = g.t + ((int64_t)(t0 + r) << log2r);
+            const int ad = sh.segs.id[sh.segs.row[r]];
+            v.x += adapter_dot<BF>(d, t, ad, n);
+            v.y += adapter_dot<BF>(d, t, ad, n + 1);
         }
         if constexpr (sizeof(Y) == 4)
             *reinterpret_cast<float2 *>(static_cast<float *>(d.y) + (int64_t)(t0 + r) * d.ldy + n) = v;
         else
             *reinterpret_cast<uint32_t *>(static_cast<Y *>(d.y) + (int64_t)(t0 + r) * d.ldy + n) = pack2<BF>(v.x, v.y);
     }
-    __syncwarp();
-    cluster.sync();  // the others' partial tiles stay until every block has read them
+    tc_fence_before();
+    __syncthreads();
     tc_fence_after();
     if (warp == 2) tmem_dealloc(tmem, p.cols);
 }
@@ -396,6 +503,18 @@ int pick_cluster(int64_t others, int blocks, int sms) {
     return c;
 }
 
+// What the cluster sends to one block: a row of `row` bytes per rank and owned row.
+size_t recv_bytes(int tile_rows, int cluster, int row) {
+    return (size_t)cluster * ((tile_rows + cluster - 1) / cluster) * row;
+}
+
+// Stages beside `other` bytes of shared memory, no more than the block has loads for.
+int pick_stages(size_t stage, size_t other, int loads) {
+    int n = (int)((kSmemLimit - 1024 - other) / stage);
+    if (n > kMaxStages) n = kMaxStages;
+    return n < loads ? n : loads;
+}
+
 template <typename Y>
 const void *skinny_fn(bool bf, bool kn, int parts) {
     if (bf) {
@@ -428,24 +547,21 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, int sms, cudaStream_t s)
     const int nk = (d.n_in + kBK - 1) / kBK;
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
-    const size_t part = (size_t)p.rows * 512, stage = 16384 + (size_t)p.rows * 128;
-    p.cluster = pick_cluster(tiles, nk, sms);
-    int slots = sms / (tiles * p.cluster);  // tiles of stacked rank columns side by side
+    const int cluster = pick_cluster(tiles, nk, sms);
+    int slots = sms / (tiles * cluster);  // tiles of stacked rank columns side by side
     slots = slots < 1 ? 1 : slots > most ? most : slots;
-    const int per = (nk + p.cluster - 1) / p.cluster;
-    p.stages = (int)((kSmemLimit - 1024 - part) / stage);
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    if (p.stages > per) p.stages = per;
-    p.cols = tmem_cols(p.rows);
-    p.smem = 1024 + p.stages * stage + part;
+    const size_t recv = recv_bytes(g.tile_rows, cluster, d.rank * 4), stage = 16384 + (size_t)p.rows * 128;
+    p.stages = pick_stages(stage, recv, (nk + cluster - 1) / cluster * ((most + slots - 1) / slots));
+    p.cols = 256;  // two accumulators of 128
+    p.smem = 1024 + p.stages * stage + recv;
     CUtensorMap mA, mX;
-    if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, 16) ||
+    if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank) ||
         !adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, p.rows))
         return cudaErrorInvalidValue;
     AdapterArgs a = g;
     void *args[] = {&mA, &mX, &a, &p};
     return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
-                          dim3(p.cluster, slots, tiles), p.smem, p.cluster, false, args, s);
+                          dim3(cluster, slots, tiles), p.smem, cluster, false, args, s);
 }
 
 cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s) {
@@ -456,8 +572,8 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s)
     const int nk = (d.n_in + kBK - 1) / kBK;
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
-    p.parts = bf && f32 ? 3 : 2;
-    p.cluster = pick_cluster((int64_t)tiles * ntn, nk, sms);
+    const int parts = bf && f32 ? 3 : 2;
+    int cluster = pick_cluster((int64_t)tiles * ntn, nk, sms);
     // The tensor cores cut a sum off instead of rounding it: a chain over K
     // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
     // fp32 results therefore use an accumulator per 512 of K, added up in
@@ -465,29 +581,26 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s)
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
     const int groups = (512 - read) / p.rows + 1;
     if (f32)
-        while (p.cluster < 8 && p.cluster < nk && (nk + p.cluster - 1) / p.cluster > 8 * groups) p.cluster *= 2;
-    const int per = (nk + p.cluster - 1) / p.cluster;
+        while (cluster < 8 && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) cluster *= 2;
+    const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
-    const int used = (per + p.chunk - 1) / p.chunk;
-    p.cols = tmem_cols((used - 1) * p.rows + read);
-    const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)p.parts * p.rows * 128;
-    p.stages = (int)((kSmemLimit - 1024 - tb) / stage);
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    const int least = (int)(((size_t)p.rows * 512 + stage - 1) / stage);  // the partial tile lies in the ring
-    if (p.stages > per + 4) p.stages = per + 4;
-    if (p.stages < least) p.stages = least;
-    p.smem = 1024 + p.stages * stage + tb;
+    p.cols = tmem_cols(((per + p.chunk - 1) / p.chunk - 1) * p.rows + read);
+    const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)((parts + 1) / 2) * p.rows * 128;
+    const size_t recv = recv_bytes(g.tile_rows, cluster, 512);
+    p.stages = pick_stages(stage, tb + recv, per + 4);
+    p.smem = 1024 + p.stages * stage + tb + recv;
     CUtensorMap mW, mB, mX;
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
-        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, 16) ||
+        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
+                     d.rank < kExt ? d.rank : kExt) ||
         !adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, p.rows))
         return cudaErrorInvalidValue;
-    const void *fn = f32 ? skinny_fn<float>(bf, kn, p.parts)
-                         : bf ? skinny_fn<__nv_bfloat16>(bf, kn, p.parts) : skinny_fn<__half>(bf, kn, p.parts);
+    const void *fn = f32 ? skinny_fn<float>(bf, kn, parts)
+                         : bf ? skinny_fn<__nv_bfloat16>(bf, kn, parts) : skinny_fn<__half>(bf, kn, parts);
     AdapterArgs a = g;
     void *args[] = {&mW, &mB, &mX, &a, &p};
-    return launch_cluster(fn, dim3(p.cluster, ntn, tiles), p.smem, p.cluster, true, args, s);
+    return launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, cluster, true, args, s);
 }
 
 }  // namespace latent

@@ -30,7 +30,6 @@ constexpr int kStages = 5;
 constexpr int kPairRows = 256, kPairCols = 256;
 constexpr uint32_t kStage = 32768;             // 16 KB of x, 16 KB of W
 constexpr uint32_t kTTile = 16384;             // 128 rows x (2 parts x 32) of x.A
-constexpr int kExt = 32;                       // stacked B rows per extension block
 constexpr int kParts = 2;
 constexpr int kGroupM = 8;                     // row tiles that share a sweep over the columns (L2 reuse)
 constexpr size_t kSmem = 1024 + kStages * kStage + 2 * kTTile;
@@ -60,27 +59,6 @@ __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bounded wait that also acquires what the other block's threads wrote before they arrived.
-__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity) {
-    const uint32_t a = smem_addr(bar);
-    unsigned long long t0 = 0;
-    for (unsigned i = 0;; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 255u) == 0) {
-            const unsigned long long now = global_ns();
-            if (i == 0) t0 = now;
-            else if (now - t0 > kWaitNs) return false;
-        }
-    }
 }
 __device__ __forceinline__ void load_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(
@@ -178,12 +156,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const PairSegments &seg = sh.seg[tl & 1];
             for (int k = 0;; ++k, ++it) {
                 if (k == nk) {
-                    if (!mbar_wait(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
+                    if (!wait(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
                     ext = seg.n * rank;
                 }
                 if (k >= nk && (k - nk) * kExt >= ext) break;
                 const int s = it % kStages;
-                if (it >= kStages && !mbar_wait(sh.empty + s, (uint32_t)(it / kStages - 1) & 1u)) { ok = false; break; }
+                if (it >= kStages && !wait(sh.empty + s, (uint32_t)(it / kStages - 1) & 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
                 uint8_t *st = ring + s * kStage;
                 const uint32_t bar = peer_addr(sh.full + s, 0);
@@ -197,12 +175,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                         load_pair(st + 16384, &mW, k * kBK, col, bar);
                     }
                 } else {
-                    const int r0 = (k - nk) * kExt, boxes = min(kExt / 16, (ext - r0) / 16);
-                    if (cta == 0) mbar_arrive_expect_tx(sh.full + s, (uint32_t)boxes * 8192u);
-                    for (int j = 0; j < boxes; ++j) {
-                        const int r = r0 + 16 * j, src = seg.id[r / rank] * rank + r % rank;
-                        load_pair(st + 16384 + j * 2048, &mB, col, src, bar);
-                        load_pair(st + 16384 + 8192 + j * 2048, &mB, col + 64, src, bar);
+                    const int r0 = (k - nk) * kExt, box = min(rank, kExt), rows = min(kExt, ext - r0);
+                    if (cta == 0) mbar_arrive_expect_tx(sh.full + s, (uint32_t)rows * 512u);
+                    for (int j = 0; j < rows; j += box) {
+                        const int src = (seg.id[(r0 + j) >> g.log2r] << g.log2r) + ((r0 + j) & (rank - 1));
+                        load_pair(st + 16384 + j * 128, &mB, col, src, bar);
+                        load_pair(st + 16384 + 8192 + j * 128, &mB, col + 64, src, bar);
                     }
                 }
             }
@@ -215,12 +193,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         for (int i = pair; i < tiles && ok; i += pairs, ++tl) {
             const int b = tl & 1;
             if (cta == 0) {
-                if (tl >= 2 && !wait_cluster(sh.acc_empty + b, (uint32_t)((tl >> 1) - 1) & 1u)) { ok = false; break; }
+                if (tl >= 2 && !wait<true>(sh.acc_empty + b, (uint32_t)((tl >> 1) - 1) & 1u)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t acc = tmem + (uint32_t)b * 256u;
                 for (int k = 0; k < nk; ++k, ++it) {
                     const int s = it % kStages;
-                    if (!mbar_wait(sh.full + s, (uint32_t)(it / kStages) & 1u) || sh.abort) { ok = false; break; }
+                    if (!wait(sh.full + s, (uint32_t)(it / kStages) & 1u) || sh.abort) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t x = smem_addr(ring + s * kStage), w = x + 16384u;
 #pragma unroll
@@ -231,21 +209,21 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                 }
                 if (!ok) break;
             }
-            if (!mbar_wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
+            if (!wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
             const int ext = sh.seg[b].n * rank;
             if (cta == 0) {
                 const uint32_t acc = tmem + (uint32_t)b * 256u;
                 for (int r0 = 0; r0 < ext; r0 += kExt, ++it, ++eb) {
                     const int s = it % kStages;
-                    if (!mbar_wait(sh.full + s, (uint32_t)(it / kStages) & 1u) ||
-                        !wait_cluster(sh.t_full + (eb & 1), (uint32_t)(eb >> 1) & 1u) || sh.abort) { ok = false; break; }
+                    if (!wait(sh.full + s, (uint32_t)(it / kStages) & 1u) ||
+                        !wait<true>(sh.t_full + (eb & 1), (uint32_t)(eb >> 1) & 1u) || sh.abort) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t w = smem_addr(ring + s * kStage) + 16384u, t = smem_addr(tbuf + (eb & 1) * kTTile);
                     const int steps = min(kExt / 16, (ext - r0) / 16);
                     for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
                         for (int q = 0; q < kParts; ++q)
-                            mma_pair(acc, desc_kmajor_sw128(t + (uint32_t)(q * kExt * 2 + kk * 32)),
+                            mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 0u)),
                                      desc_mnmajor_sw128(w + kk * 2048), idx, 1);
                     commit_pair(sh.empty + s);
                     commit_pair(sh.t_empty + (eb & 1));
@@ -266,8 +244,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         for (int i = pair; i < tiles; i += pairs, ++tl) {
             const int b = tl & 1;
             const Tile tile = tile_at(i, tm, tn);
-            if (!mbar_wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u) ||
-                !mbar_wait(sh.acc_full + b, (uint32_t)(tl >> 1) & 1u) || sh.abort) { ok = false; break; }
+            if (!wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u) ||
+                !wait(sh.acc_full + b, (uint32_t)(tl >> 1) & 1u) || sh.abort) { ok = false; break; }
             tc_fence_after();
             const int t = tile.t0 + (int)cta * 128 + r;
             const bool live = t < d.n_tokens;
@@ -311,7 +289,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         dependency_wait();
         for (int i = pair; i < tiles; i += pairs, ++tl) {
             const Tile tile = tile_at(i, tm, tn);
-            if (tl >= 2 && ok) ok = mbar_wait(sh.seg_empty + (tl & 1), (uint32_t)((tl >> 1) - 1) & 1u);
+            if (tl >= 2 && ok) ok = wait(sh.seg_empty + (tl & 1), (uint32_t)((tl >> 1) - 1) & 1u);
             // all 128 go on or none: the named barriers below have no limit of their own
             if (!bar_all(2, 128, ok && !sh.abort)) { ok = false; break; }
             PairSegments &seg = sh.seg[tl & 1];
@@ -370,9 +348,9 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const int ext = seg.n * rank;
             mbar_arrive(sh.seg_full + (tl & 1));
             for (int r0 = 0; r0 < ext; r0 += kExt, ++eb) {  // a thread that gives up here is heard at the next tile
-                if (eb >= 2 && !mbar_wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
+                if (eb >= 2 && !wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
-                build_t_row<BF, kParts, kExt / 8>(tbuf + (eb & 1) * kTTile, 0u, tid, wide ? -1 : my, rank, tp, r0);
+                build_t_row<BF, kParts>(tbuf + (eb & 1) * kTTile, 0u, tid, wide ? -1 : my, rank, g.log2r, tp, r0);
                 fence_async_shared();
                 arrive_cluster(peer_addr(sh.t_full + (eb & 1), 0));
             }
@@ -401,7 +379,8 @@ cudaError_t launch_adapter_wide(const AdapterArgs &g, int sms, cudaStream_t s) {
     CUtensorMap mX, mW, mB;
     if (!adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, 128) ||
         !(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
-        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, 16))
+        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
+                     d.rank < kExt ? d.rank : kExt))
         return cudaErrorInvalidValue;
     const void *fn = bf ? kn ? (const void *)k_ad_wide<true, true> : (const void *)k_ad_wide<true, false>
                         : kn ? (const void *)k_ad_wide<false, true> : (const void *)k_ad_wide<false, false>;
