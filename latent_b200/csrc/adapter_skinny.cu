@@ -35,7 +35,9 @@ struct Shared {
     volatile int abort;
     uint8_t wide[kRows];   // fp16: rows finished in fp32
     Segments segs;
+    alignas(16) uint32_t dest[kRows];  // where a row's sums go: its owner's shared memory, kNoRow behind the last row
 };
+constexpr uint32_t kNoRow = 0xffffffffu;
 
 struct Plan {
     int rows;       // N of the MMA: rows of x per tile, a multiple of 16
@@ -74,28 +76,37 @@ __device__ __forceinline__ void drain() {
     while (global_ns() - t0 < 20000000ull) __nanosleep(1000);
 }
 
-__device__ __forceinline__ void setup(Shared &sh, const Plan &p) {
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(sh.full + s, 1);
-            mbar_init(sh.empty + s, 1);
+// Barriers by warp 0, which goes on at once (its first loads wait for nobody),
+// TMEM by warp 2, which then lets a dependent kernel start.
+template <bool DEPENDENTS>
+__device__ __forceinline__ void setup(Shared &sh, const Plan &p, int warp, int lane) {
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < p.stages; ++s) {
+                mbar_init(sh.full + s, 1);
+                mbar_init(sh.empty + s, 1);
+            }
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(sh.acc_full + b, 1);
+                mbar_init(sh.acc_empty + b, 128);
+                mbar_init(sh.t_full + b, 128);
+                mbar_init(sh.t_empty + b, 1);
+            }
+            mbar_init(&sh.seg, 128);
+            sh.abort = 0;
+            fence_barrier_init();
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(sh.acc_full + b, 1);
-            mbar_init(sh.acc_empty + b, 128);
-            mbar_init(sh.t_full + b, 128);
-            mbar_init(sh.t_empty + b, 1);
-        }
-        mbar_init(&sh.seg, 128);
-        sh.abort = 0;
-        fence_barrier_init();
+        __syncwarp();
+        asm volatile("bar.arrive 3, 256;" ::: "memory");
+        return;
     }
-    if (threadIdx.x / 32 == 2) {
+    if (warp == 2) {
         tmem_alloc(&sh.tmem, p.cols);
         tmem_relinquish();
+        if (DEPENDENTS) launch_dependents();
     }
     tc_fence_before();
-    __syncthreads();
+    bar_sync(3, kThreads);
     tc_fence_after();
 }
 
@@ -103,11 +114,28 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void load32(const void *p, uint32_t (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        const uint4 u = reinterpret_cast<const uint4 *>(p)[i / 4];
+        v[i] = u.x;
+        v[i + 1] = u.y;
+        v[i + 2] = u.z;
+        v[i + 3] = u.w;
+    }
+}
+
+// By the thread of row r: rows are dealt to the cluster in runs of `per`; rank
+// q's sums of a row (row_bytes) lie at place q * per + r % per of its owner.
+__device__ __forceinline__ void set_dest(Shared &sh, const float *recv, int r, int nt, int per, int q, uint32_t row_bytes) {
+    sh.dest[r] = r < nt ? map_rank(smem_addr(recv) + (uint32_t)(q * per + r % per) * row_bytes, r / per) : kNoRow;
 }
 
 // x.A.  Block (cluster rank, slot, row tile); the stacked rank columns of the
@@ -129,7 +157,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     const latent_adapter_desc &d = g.d;
     const int t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
     const int rank = d.rank, log2r = g.log2r;
-    launch_dependents();
     cluster_arrive();  // the others may send once every block has started
     int a = -1;
     if (warp == 0 && lane == 0) {
@@ -139,14 +166,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         const int r = threadIdx.x - 128;
         a = row_adapter(d, t0 + r, r < nt, q == 0 && blockIdx.y == 0);
     }
-    setup(sh, p);
-    const uint32_t tmem = sh.tmem;
+    setup<true>(sh, p, warp, lane);
+    const uint32_t tmem = warp ? sh.tmem : 0u, read = (uint32_t)(p.rows + 31) & ~31u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
     bool ok = true;
     if (warp >= 4) {
         build_segments(sh.segs, a, nt, threadIdx.x - 128, 1);
+        set_dest(sh, recv, threadIdx.x - 128, nt, per, q, (uint32_t)rank * 4u);
         mbar_arrive(&sh.seg);
     }
     ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
@@ -183,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
                 const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    mma_f16(tmem + b * 128u, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), id,
+                    mma_f16(tmem + b * read, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), id,
                             (k > k0) | kk);
                 mma_commit(sh.empty + at.s);
             }
@@ -203,24 +231,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
             if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
             tc_fence_after();
             const int seg = (m + tid) >> log2r, j = (m + tid) & (rank - 1);
-            int owner = 0, r_own = 0;  // of row c + i below
             for (int c = 0; c < p.rows; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(tmem + b * 128u + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
+                uint32_t v[32], to[32], of[32];
+                __syncwarp();
+                tmem_ld32(tmem + b * read + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
+                load32(sh.dest + c, to);
+                load32(sh.segs.row + c, of);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (c + i < nt) {
-                        if (sh.segs.row[c + i] == seg)
-                            st_cluster(map_rank(smem_addr(recv + ((q * per + r_own) << log2r) + j), owner),
-                                       __uint_as_float(v[i]));
-                        if (++r_own == per) {
-                            r_own = 0;
-                            ++owner;
-                        }
-                    }
-                }
-                __syncwarp();
+                for (int i = 0; i < 32; ++i)
+                    if ((int)of[i] == seg) st_cluster(to[i] + (uint32_t)j * 4u, __uint_as_float(v[i]));
             }
             tc_fence_before();
             mbar_arrive(sh.acc_empty + b);
@@ -278,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         const int r = threadIdx.x - 128;
         a = row_adapter(d, t0 + r, r < nt, false);
     }
-    setup(sh, p);
-    const uint32_t tmem = sh.tmem;
+    setup<false>(sh, p, warp, lane);
+    const uint32_t tmem = warp ? sh.tmem : 0u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
@@ -364,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
         build_segments(sh.segs, a, nt, r, 1);
+        set_dest(sh, recv, r, nt, per, q, 512u);
         mbar_arrive(&sh.seg);
         ok = wait(&sh.seg, 0u);
         const int seg = sh.segs.row[r];
@@ -390,27 +411,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         cluster_wait();
         // column c of the accumulator = row c of x, to its owner
         const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
-        const uint32_t base = smem_addr(recv) + (uint32_t)r * 4u;
-        int owner = 0, r_own = 0;
         for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
             float s[32];
+            uint32_t to[32];
+            load32(sh.dest + c, to);
             for (int gr = 0; gr < groups; ++gr) {
                 uint32_t v[32];
+                __syncwarp();
                 tmem_ld32(tmem + ((uint32_t)(r & ~31) << 16) + (uint32_t)(gr * p.rows + c), v);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) s[j] = gr ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
             }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                if (c + j < nt) {
-                    st_cluster(map_rank(base + (uint32_t)(q * per + r_own) * 512u, owner), s[j]);
-                    if (++r_own == per) {
-                        r_own = 0;
-                        ++owner;
-                    }
-                }
-            }
+            for (int j = 0; j < 32; ++j)
+                if (to[j] != kNoRow) st_cluster(to[j] + (uint32_t)r * 4u, s[j]);
         }
         tc_fence_before();
     }
@@ -472,7 +487,16 @@ uint32_t tmem_cols(int n) {
     return c;
 }
 
-constexpr size_t kSmemLimit = 220 * 1024;  // dynamic; the static part holds Shared
+// Dynamic shared memory of a block beside the static: all of an SM's, or half.  A block's share of the shared memory is at least its share of
+// the 512 TMEM columns, so that whatever blocks an SM holds, of whichever calls
+// and streams, no TMEM allocation waits: blocks of two clusters that wait for
+// each other's columns would never end.
+constexpr size_t kSmemWhole = 227 * 1024 - sizeof(Shared);
+constexpr size_t kSmemHalf = 113 * 1024 - sizeof(Shared);
+size_t smem_of(size_t used, uint32_t cols) {
+    const size_t share = (size_t)cols * 228 * 1024 / 512 - 1024 - sizeof(Shared);  // of 228 KB; 1 KB goes to the system
+    return used < share ? share : used;
+}
 
 cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, int cluster, bool dependent, void **args,
                            cudaStream_t s) {
@@ -495,11 +519,45 @@ cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, int cluster, 
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-// Blocks of a cluster: as many of 8, 4, 2, 1 as the contraction has blocks for
-// and the SMs have room for beside the other clusters.
-int pick_cluster(int64_t others, int blocks, int sms) {
-    int c = 8;
-    while (c > 1 && (c > blocks || others * c > sms)) c /= 2;
+// Clusters of 1..8 blocks that the device holds at once with one block per SM
+// (a cluster stays within a GPC: 15 of 8, 22 of 6, 33 of 4 on the 148 SMs).
+const int *cluster_room() {
+    struct Table {
+        bool set = false;
+        int n[9];
+    };
+    static std::mutex mu;
+    static Table tables[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    Table &t = tables[dev];
+    if (!t.set) {
+        const void *fn = (const void *)k_ad_shrink<true>;
+        if (ensure_smem(fn, kSmemWhole) != cudaSuccess) return nullptr;
+        for (int c = 1; c <= 8; ++c) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(c, 256);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = kSmemWhole;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = (unsigned)c;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&t.n[c], fn, &cfg) != cudaSuccess) return nullptr;
+        }
+        t.set = true;
+    }
+    return t.n;
+}
+
+// Blocks of a cluster for `others` clusters: as many as the contraction has
+// blocks for and as run at once (half: two blocks may share an SM).
+int pick_cluster(int64_t others, int blocks, int sms, const int *room, bool half) {
+    int c = blocks < 8 ? blocks : 8;
+    while (c > 1 && (others * c > sms || others > (half ? 2 : 1) * room[c])) --c;
     return c;
 }
 
@@ -508,11 +566,11 @@ size_t recv_bytes(int tile_rows, int cluster, int row) {
     return (size_t)cluster * ((tile_rows + cluster - 1) / cluster) * row;
 }
 
-// Stages beside `other` bytes of shared memory, no more than the block has loads for.
-int pick_stages(size_t stage, size_t other, int loads) {
-    int n = (int)((kSmemLimit - 1024 - other) / stage);
-    if (n > kMaxStages) n = kMaxStages;
-    return n < loads ? n : loads;
+// Stages beside `other` bytes of shared memory.
+int pick_stages(size_t limit, size_t stage, size_t other) {
+    if (limit < 1024 + other + stage) return 0;
+    const int n = (int)((limit - 1024 - other) / stage);
+    return n < kMaxStages ? n : kMaxStages;
 }
 
 template <typename Y>
@@ -547,13 +605,22 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, int sms, cudaStream_t s)
     const int nk = (d.n_in + kBK - 1) / kBK;
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
-    const int cluster = pick_cluster(tiles, nk, sms);
+    const int *room = cluster_room();
+    if (!room) return cudaErrorInvalidConfiguration;
+    // two blocks per SM where two stages fit into half of its shared memory
+    const size_t stage = 16384 + (size_t)p.rows * 128;
+    size_t recv = recv_bytes(g.tile_rows, 8, d.rank * 4);
+    const bool half = pick_stages(kSmemHalf, stage, recv) >= 2;
+    const int cluster = pick_cluster(tiles, nk, sms, room, half);
+    recv = recv_bytes(g.tile_rows, cluster, d.rank * 4);
     int slots = sms / (tiles * cluster);  // tiles of stacked rank columns side by side
     slots = slots < 1 ? 1 : slots > most ? most : slots;
-    const size_t recv = recv_bytes(g.tile_rows, cluster, d.rank * 4), stage = 16384 + (size_t)p.rows * 128;
-    p.stages = pick_stages(stage, recv, (nk + cluster - 1) / cluster * ((most + slots - 1) / slots));
-    p.cols = 256;  // two accumulators of 128
-    p.smem = 1024 + p.stages * stage + recv;
+    const int loads = (nk + cluster - 1) / cluster * ((most + slots - 1) / slots);
+    p.stages = pick_stages(half ? kSmemHalf : kSmemWhole, stage, recv);
+    if (p.stages > loads) p.stages = loads;
+    if (p.stages < 1) return cudaErrorInvalidConfiguration;
+    p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
+    p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
     CUtensorMap mA, mX;
     if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank) ||
         !adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, p.rows))
@@ -573,23 +640,28 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s)
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
     const int parts = bf && f32 ? 3 : 2;
-    int cluster = pick_cluster((int64_t)tiles * ntn, nk, sms);
+    const int *room = cluster_room();
+    if (!room) return cudaErrorInvalidConfiguration;
+    const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)((parts + 1) / 2) * p.rows * 128;
+    const bool half = pick_stages(kSmemHalf, stage, tb + recv_bytes(g.tile_rows, 8, 512)) >= 2;
+    int cluster = pick_cluster((int64_t)tiles * ntn, nk, sms, room, half);
     // The tensor cores cut a sum off instead of rounding it: a chain over K
     // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
     // fp32 results therefore use an accumulator per 512 of K, added up in
     // fp32, as far as the 512 TMEM columns go, and clusters long enough.
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    const int groups = (512 - read) / p.rows + 1;
+    const int groups = ((half ? 256 : 512) - read) / p.rows + 1;
     if (f32)
-        while (cluster < 8 && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) cluster *= 2;
+        while (cluster < 8 && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
     p.cols = tmem_cols(((per + p.chunk - 1) / p.chunk - 1) * p.rows + read);
-    const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)((parts + 1) / 2) * p.rows * 128;
     const size_t recv = recv_bytes(g.tile_rows, cluster, 512);
-    p.stages = pick_stages(stage, tb + recv, per + 4);
-    p.smem = 1024 + p.stages * stage + tb + recv;
+    p.stages = pick_stages(half ? kSmemHalf : kSmemWhole, stage, tb + recv);
+    if (p.stages > per + 4) p.stages = per + 4;
+    if (p.stages < 1) return cudaErrorInvalidConfiguration;
+    p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
     CUtensorMap mW, mB, mX;
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,

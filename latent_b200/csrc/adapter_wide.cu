@@ -32,7 +32,11 @@ constexpr uint32_t kStage = 32768;             // 16 KB of x, 16 KB of W
 constexpr uint32_t kTTile = 16384;             // 128 rows x (2 parts x 32) of x.A
 constexpr int kParts = 2;
 constexpr int kGroupM = 8;                     // row tiles that share a sweep over the columns (L2 reuse)
-constexpr size_t kSmem = 1024 + kStages * kStage + 2 * kTTile;
+// All of an SM's shared memory, more than the ring needs: the block takes all
+// TMEM columns, and no other block that wants some may start beside it.
+constexpr size_t kStatic = 6144;
+constexpr size_t kSmem = 227 * 1024 - kStatic;
+static_assert(1024 + kStages * kStage + 2 * kTTile <= kSmem, "ring and x.A tiles");
 
 struct PairSegments {
     int n;
@@ -51,6 +55,8 @@ struct Shared {
     int warp_n[8];
     PairSegments seg[2];
 };
+
+static_assert(sizeof(Shared) <= kStatic, "static shared memory");
 
 __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     uint32_t r;
