@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .router_train import _on
-from .runtime import FactorPair, _stream_ptr, project
+from .runtime import FactorPair, project
 
 __all__ = ["AdapterSet", "adapter_project"]
 
@@ -31,8 +31,8 @@ _TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _Y_TYPES = {**_TYPES, torch.float32: _lib.TYPE_F32}
 
 
-def _tensor(a, device) -> torch.Tensor:
-    return (a if torch.is_tensor(a) else torch.from_numpy(np.ascontiguousarray(a))).to(device)
+def _tensor(a, device, dtype) -> torch.Tensor:
+    return (a.detach() if torch.is_tensor(a) else torch.from_numpy(np.ascontiguousarray(a))).to(device, dtype)
 
 
 class AdapterSet:
@@ -77,20 +77,38 @@ class AdapterSet:
         # rows padded to 16 bytes
         self.a = torch.zeros((n, rank, (K + 7) // 8 * 8), dtype=dtype, device=dev)
         self.b = torch.zeros((n, rank, (N + 7) // 8 * 8), dtype=dtype, device=dev)
-        for i, ad in enumerate(adapters):
-            self.a[i, :self.ranks[i], :K] = _tensor(ad[0], dev).detach().t()
-            self.b[i, :self.ranks[i], :N] = _tensor(ad[1], dev).detach()
+        # one copy per factor kind: A's columns and B's rows side by side, then to their padded places
+        live = torch.tensor([i * rank + j for i in range(n) for j in range(self.ranks[i])], device=dev)
+        self.a.view(n * rank, -1)[live, :K] = torch.cat([_tensor(ad[0], dev, dtype) for ad in adapters], 1).t()
+        self.b.view(n * rank, -1)[live, :N] = torch.cat([_tensor(ad[1], dev, dtype) for ad in adapters], 0)
         scales = [float(ad[2]) if len(ad) > 2 else 1.0 for ad in adapters]
         self.scale = torch.tensor(scales, dtype=torch.float32, device=dev)
         if not np.isfinite(scales).all() or not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
             raise ValueError(f"adapter factors and scales must be finite in {dtype}")
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+        # a, lda, b, ldb, scale as a call's descriptor takes them
+        self._factors = (self.a.data_ptr(), self.a.shape[2], self.b.data_ptr(), self.b.shape[2], self.scale.data_ptr())
+        self._err_ptr = self.err.data_ptr()
+        self._ws = {}
+
+    def workspace_bytes(self, n_tokens: int) -> int:
+        """Workspace a call on this many rows needs (latent_adapter_workspace_size)."""
+        n = self._ws.get(n_tokens)
+        if n is None:
+            d = _lib.AdapterDesc(self.n_adapter, self.rank, self.n_in, self.n_out, n_tokens, _TYPES[self.dtype],
+                                 _TYPES[self.dtype])
+            size = C.c_size_t(0)
+            _lib.check(_lib.lib().latent_adapter_workspace_size(C.byref(d), C.byref(size)),
+                       "latent_adapter_workspace_size")
+            n = size.value
+            if len(self._ws) < 4096:
+                self._ws[n_tokens] = n
+        return n
 
     def check(self) -> None:
         """Synchronises and raises if a call since the last check recorded a device-side error
         (an id >= n_adapter, which counts as no adapter, or a bounded wait that ran out)."""
-        _lib.check(_on(self.device, _lib.lib().latent_adapter_check, self.err.data_ptr(), _stream_ptr(self.device)),
-                   "device check")
+        _lib.check(_on(self.device, _lib.lib().latent_adapter_check, self.err.data_ptr()), "device check")
 
 
 def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Tensor,
@@ -106,24 +124,22 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     rounded once, or fills ``out`` (rows may be strided).
     """
     s = adapters
-    if x.dim() != 2 or x.shape[1] != s.n_in:
-        raise ValueError(f"x must be [T, {s.n_in}], got {tuple(x.shape)}")
-    if x.dtype != s.dtype:
-        raise ValueError(f"x must be {s.dtype} like the adapters, got {x.dtype}")
-    T, K = x.shape
-    N = s.n_out
+    dev, dt, K, N = s.device, s.dtype, s.n_in, s.n_out
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be [T, {K}], got {tuple(x.shape)}")
+    if x.dtype != dt:
+        raise ValueError(f"x must be {dt} like the adapters, got {x.dtype}")
+    T = x.shape[0]
     if ids.dim() != 1 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"ids must be contiguous int32 [{T}]")
     pair = isinstance(weight, FactorPair)
-    if not pair:
-        if weight.dim() != 2 or tuple(weight.shape) != (K, N) or weight.dtype != x.dtype:
-            raise ValueError(f"weight must be {x.dtype} [{K}, {N}]")
-        if weight.device != s.device:
-            raise ValueError("x, weight, ids and out must be on the adapters' device")
-    if x.device != s.device or ids.device != s.device or (out is not None and out.device != s.device):
+    if not pair and (weight.dim() != 2 or weight.shape[0] != K or weight.shape[1] != N or weight.dtype != dt):
+        raise ValueError(f"weight must be {dt} [{K}, {N}]")
+    if x.device != dev or ids.device != dev or (not pair and weight.device != dev) or \
+            (out is not None and out.device != dev):
         raise ValueError("x, weight, ids and out must be on the adapters' device")
-    if torch.is_grad_enabled() and (x.requires_grad or (not pair and weight.requires_grad) or
-                                    (out is not None and out.requires_grad)):
+    if (x.requires_grad or (not pair and weight.requires_grad) or (out is not None and out.requires_grad)) and \
+            torch.is_grad_enabled():
         raise ValueError("adapter_project computes no gradients: call it under torch.no_grad() or on detached tensors")
     if out is not None:
         if out_dtype not in (None, out.dtype):
@@ -132,14 +148,18 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
         if tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{T}, {N}] with contiguous rows")
     elif out_dtype is None:
-        out_dtype = x.dtype
-    if out_dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"out_dtype {out_dtype} unsupported ({x.dtype} or float32)")
-    if x.stride(1) != 1 and K > 1 or T > 1 and x.stride(0) < K:
-        x = x.contiguous()
+        out_dtype = dt
+    if out_dtype != dt and out_dtype != torch.float32:
+        raise ValueError(f"out_dtype {out_dtype} unsupported ({dt} or float32)")
     if T == 0:
-        return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=s.device)
-    flags, w_ptr, ldw = 0, None, 0
+        return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=dev)
+    ldx, inner = x.stride()
+    if (inner != 1 and K > 1) or (T > 1 and ldx < K):
+        x = x.contiguous()
+        ldx = K
+    if T == 1:
+        ldx = K
+    flags, w_ptr, ldw = 0, 0, 0
     if pair:
         y = project(x, weight)
         if y.shape[1] != N:
@@ -153,18 +173,13 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
         else:
             raise ValueError("weight must be row-major or the transposed view of a row-major matrix")
         w_ptr = weight.data_ptr()
-        y = out if out is not None else torch.empty((T, N), dtype=out_dtype, device=s.device)
-    ldx = x.stride(0) if T > 1 else K
-    ldy = y.stride(0) if T > 1 else N
-    L = _lib.lib()
-    d = _lib.AdapterDesc(s.n_adapter, s.rank, K, N, T, _TYPES[x.dtype], _Y_TYPES[y.dtype], flags, x.data_ptr(), ldx,
-                         w_ptr, ldw, s.a.data_ptr(), s.a.shape[2], s.b.data_ptr(), s.b.shape[2], s.scale.data_ptr(),
-                         ids.data_ptr(), y.data_ptr(), ldy, s.err.data_ptr(), None, 0)
-    n = C.c_size_t(0)
-    _lib.check(L.latent_adapter_workspace_size(C.byref(d), C.byref(n)), "latent_adapter_workspace_size")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=s.device)
-    d.workspace, d.workspace_bytes = ws.data_ptr(), n.value
-    _lib.check(_on(s.device, L.latent_adapter_project, C.byref(d), _stream_ptr(s.device)), "latent_adapter_project")
+        y = out if out is not None else torch.empty(T, N, dtype=out_dtype, device=dev)
+    n = s.workspace_bytes(T)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    d = _lib.ADAPTER_DESC.pack(s.n_adapter, s.rank, K, N, T, _TYPES[dt], _Y_TYPES[y.dtype], flags, x.data_ptr(), ldx,
+                               w_ptr, ldw, *s._factors, ids.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
+                               s._err_ptr, ws.data_ptr(), n)
+    _lib.check(_on(dev, _lib.lib().latent_adapter_project, d), "latent_adapter_project")
     if pair:
         return y.to(out_dtype) if out is None else out.copy_(y)
     return y

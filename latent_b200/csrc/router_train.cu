@@ -18,9 +18,11 @@
 // k_balance_count: one cluster of 8 blocks per sequence; each block counts its
 // rows' ids in a shared-memory histogram, the blocks add theirs up through
 // distributed shared memory: integers, no global atomics, nothing to zero.
-// k_balance_main: one warp per row, the row in registers; every block leaves
-// its two partial sums (64 bits) and the last one adds them up in block order,
-// so that a call's results do not depend on the order of execution.
+// k_balance_main, its programmatic dependent, takes the softmax of its first
+// rows before it waits for the counts: one warp per row, two rows at once in
+// registers; every block leaves its two partial sums (64 bits) and the last one
+// adds them up in block order, so that a call's results do not depend on the
+// order of execution.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -77,6 +79,35 @@ struct Row {
             }
         }
     }
+    // A row that this kernel also writes.
+    static __device__ __forceinline__ void load_rw(const T *row, int E, int lane, float (&x)[PL]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = col(lane, v);
+            R raw = R();
+            if (c < E) raw = *reinterpret_cast<const R *>(row + c);
+            const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[v * VEC + i] = to_f32(e[i]);
+        }
+    }
+    // Integers laid out like the row, scaled.
+    static __device__ __forceinline__ void counts(const int32_t *row, int E, int lane, float scale, float (&x)[PL]) {
+        constexpr int W = VEC < 4 ? VEC : 4;
+        using R4 = typename Raw<W * 4>::type;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = col(lane, v);
+#pragma unroll
+            for (int i = 0; i < VEC; i += W) {
+                R4 raw = R4();
+                if (c < E) raw = __ldcg(reinterpret_cast<const R4 *>(row + c + i));
+                const int32_t *e = reinterpret_cast<const int32_t *>(&raw);
+#pragma unroll
+                for (int u = 0; u < W; ++u) x[v * VEC + i + u] = (float)e[u] * scale;
+            }
+        }
+    }
     static __device__ __forceinline__ void store(T *row, int E, int lane, const float (&x)[PL]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -91,6 +122,9 @@ struct Row {
         }
     }
 };
+
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -150,6 +184,7 @@ k_balance_count(BalanceArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank();
     const int s = blockIdx.x / kCountCluster;
+    launch_dependents();
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
     if (threadIdx.x < 2) tot[threadIdx.x] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
@@ -196,75 +231,94 @@ k_balance_count(BalanceArgs a) {
     cluster.sync();  // the others' shared memory stays until every block has read it
 }
 
+// Rows a warp works on at once: two while they fit into registers (16 floats a lane).
+template <int PL> constexpr int kRowsAtOnce = PL <= 8 ? 2 : 1;
+
 template <typename T, int PL, int VEC>
 __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) {
     using RW = Row<T, PL, VEC>;
+    constexpr int R = kRowsAtOnce<PL>;
     __shared__ double part[kRowWarps][2];
     __shared__ bool last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t n = 0;   // counted rows
-    int used = 0;    // sequences that have one
-    for (int s = lane; s < a.S; s += 32) {
-        const int c = a.seq[2 * s];
-        n += c;
-        used += c > 0;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(kFull, n, o);
-    used = __reduce_add_sync(kFull, used);
-    const float up = a.d_loss ? __ldg(a.d_loss) : 1.f;
-    const float gb = up * a.b, gz = n > 0 ? up * (2.f * a.z / (float)n) : 0.f;
     const T *logits = static_cast<const T *>(a.logits);
     T *grad = static_cast<T *>(a.grad);
+    bool first = true;
+    int used = 0;    // sequences that have a counted row
+    int64_t n = 0;   // counted rows
+    float gb = 0.f, gz = 0.f;
     double sb = 0.0, sz = 0.0;
-    for (int t = blockIdx.x * kRowWarps + warp; t < a.T; t += gridDim.x * kRowWarps) {
-        const int s = a.valid && !__ldg(a.valid + t) ? -1 : sequence_of(a.cu, a.S, t);
-        float g[PL];
-        if (s < 0) {  // a padded row, whatever it holds, gives nothing and gets a zero gradient
+    for (int t0 = (blockIdx.x * kRowWarps + warp) * R; first || t0 < a.T; t0 += gridDim.x * kRowWarps * R) {
+        float x[R][PL], lse[R];
+        int seq[R];
 #pragma unroll
-            for (int j = 0; j < PL; ++j) g[j] = 0.f;
-        } else {
-            float x[PL];
-            RW::load(logits + (int64_t)t * a.E, a.E, lane, -INFINITY, x);
+        for (int r = 0; r < R; ++r) {
+            const int t = t0 + r;
+            seq[r] = t >= a.T || (a.valid && !__ldg(a.valid + t)) ? -1 : sequence_of(a.cu, a.S, t);
+            // a padded row, whatever it holds, gives nothing and gets a zero gradient
+            RW::load(logits + (int64_t)t * a.E, seq[r] >= 0 ? a.E : 0, lane, -INFINITY, x[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
             float m = -INFINITY;
             bool nan = false;
 #pragma unroll
             for (int j = 0; j < PL; ++j) {
-                m = fmaxf(m, x[j]);
-                nan |= x[j] != x[j];
+                m = fmaxf(m, x[r][j]);
+                nan |= x[r][j] != x[r][j];
             }
             m = warp_max(m);
-            const bool none = m == -INFINITY && !__any_sync(kFull, nan);  // every expert masked: no distribution
+            const bool none = m == -INFINITY && !__any_sync(kFull, nan);  // padded, or every expert masked
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < PL; ++j) {
-                x[j] = none ? 0.f : expf(x[j] - m);
-                sum += x[j];
+                x[r][j] = none ? 0.f : expf(x[r][j] - m);
+                sum += x[r][j];
             }
             sum = warp_sum(sum);
             const float inv = none ? 0.f : 1.f / sum;
-            const float lse = none ? 0.f : m + logf(sum);
-            const int ns = a.seq[2 * s], cs = max(1, a.seq[2 * s + 1]);
-            const float scale = (float)a.E / ((float)used * (float)ns) / (float)cs;
-            const int32_t *cnt = a.counts + (int64_t)s * a.E;
+            lse[r] = none ? 0.f : m + logf(sum);
+#pragma unroll
+            for (int j = 0; j < PL; ++j) x[r][j] *= inv;
+        }
+        if (first) {  // the counts are needed only now
+            first = false;
+            dependency_wait();
+            for (int s = lane; s < a.S; s += 32) {
+                const int c = __ldcg(a.seq + 2 * s);
+                n += c;
+                used += c > 0;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(kFull, n, o);
+            used = __reduce_add_sync(kFull, used);
+            const float up = a.d_loss ? __ldg(a.d_loss) : 1.f;
+            gb = up * a.b;
+            gz = n > 0 ? up * (2.f * a.z / (float)n) : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = t0 + r;
             float c[PL], d = 0.f;
+            if (seq[r] >= 0) {
+                const int2 nc = __ldcg(reinterpret_cast<const int2 *>(a.seq) + seq[r]);
+                const float scale = (float)a.E / ((float)used * (float)nc.x) / (float)max(1, nc.y);
+                RW::counts(a.counts + (int64_t)seq[r] * a.E, a.E, lane, scale, c);
 #pragma unroll
-            for (int v = 0; v < RW::NV; ++v) {
+                for (int j = 0; j < PL; ++j) d = fmaf(c[j], x[r][j], d);
+            } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int j = v * VEC + i, col = RW::col(lane, v) + i;
-                    c[j] = col < a.E ? (float)cnt[col] * scale : 0.f;
-                    x[j] *= inv;
-                    d = fmaf(c[j], x[j], d);
-                }
+                for (int j = 0; j < PL; ++j) c[j] = 0.f;
             }
             d = warp_sum(d);
             sb += d;
-            sz += (double)lse * lse;
+            sz += (double)lse[r] * lse[r];
+            if (grad && t < a.T) {
 #pragma unroll
-            for (int j = 0; j < PL; ++j) g[j] = x[j] * fmaf(gb, c[j] - d, gz * lse);
+                for (int j = 0; j < PL; ++j) x[r][j] *= fmaf(gb, c[j] - d, gz * lse[r]);
+                RW::store(grad + (int64_t)t * a.E, a.E, lane, x[r]);
+            }
         }
-        if (grad) RW::store(grad + (int64_t)t * a.E, a.E, lane, g);
     }
     if (lane == 0) {
         part[warp][0] = sb;
@@ -277,18 +331,20 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
             b += part[w][0];
             z += part[w][1];
         }
-        a.partial[2 * blockIdx.x] = b;
-        a.partial[2 * blockIdx.x + 1] = z;
+        reinterpret_cast<double2 *>(a.partial)[blockIdx.x] = make_double2(b, z);
         __threadfence();
         last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
     }
     __syncthreads();
-    if (!last || warp != 0) return;
+    if (!last) return;
     __threadfence();
-    double b = 0.0, z = 0.0;  // lane l adds blocks l, l + 32, ... in order, then the lanes are added by a fixed tree
-    for (int i = lane; i < (int)gridDim.x; i += 32) {
-        b += __ldcg(a.partial + 2 * i);
-        z += __ldcg(a.partial + 2 * i + 1);
+    // thread i adds blocks i, i + 256, ... in order, then lanes and warps by a fixed tree
+    double b = 0.0, z = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += kRowWarps * 32) {
+        const double2 v = __ldcg(reinterpret_cast<const double2 *>(a.partial) + i);
+        b += v.x;
+        z += v.y;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -296,6 +352,16 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
         z += __shfl_xor_sync(kFull, z, o);
     }
     if (lane == 0) {
+        part[warp][0] = b;
+        part[warp][1] = z;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        b = z = 0.0;
+        for (int w = 0; w < kRowWarps; ++w) {
+            b += part[w][0];
+            z += part[w][1];
+        }
         z = n > 0 ? z / (double)n : 0.0;
         a.losses[0] = (float)(a.b * b + a.z * z);
         a.losses[1] = (float)b;
@@ -310,94 +376,120 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
 //   logits, RENORM: the softmax's own sum cancels, w is the softmax over the
 //     kept logits alone and dl_j = w_j (dw_j - c), zero elsewhere;
 //   logits, raw: dl_i = p_i (dw_i - c) over the whole row.
-// One warp per row, lane j has slot j.  Only the raw logits form reads the
-// row; the others gather the kept scores.  A row is written as zeros (or
-// -c p_i) and then its kept columns, after a __syncwarp, by their slots' lanes
-// (an id held by several slots: the lowest of those lanes, with their sum).
-// ACCUM adds to what dscores holds and touches nothing else of the row
-// (raw logits: the whole row).
-template <typename T, int PL, int VEC, bool SOFTMAX, bool RENORM, bool ACCUM>
-__global__ void __launch_bounds__(kRowWarps * 32) k_router_grad(const T *__restrict__ scores,
-                                                                const int32_t *__restrict__ ids,
-                                                                const float *__restrict__ dw, int T_, int E, int k,
-                                                                T *__restrict__ out) {
+// An id held by several slots of a row gets the sum of their parts.  ACCUM adds
+// to what dscores holds.
+__device__ __forceinline__ float same_id_sum(int key, float g, unsigned &same) {
+    same = __match_any_sync(kFull, key);
+    if (!__any_sync(kFull, (same & (same - 1)) != 0u)) return g;
+    float total = 0.f;  // in slot order
+    for (unsigned rest = same; __any_sync(kFull, rest != 0u);) {
+        const int src = rest ? __ffs(rest) - 1 : 0;
+        const float add = __shfl_sync(kFull, g, src);
+        if (rest) total += add;
+        rest &= rest - 1;
+    }
+    return total;
+}
+
+// All forms but the raw logits: the kept scores alone decide, the rest of a row
+// is zero (ACCUM: left alone).  A warp has 32 / kw rows side by side, kw = the
+// power of two that holds top_k: lane = slot.  The rows' zeros are stored first
+// (they wait for nothing), the kept columns after a __syncwarp.
+template <typename T, bool WIDE, bool SOFTMAX, bool RENORM, bool ACCUM>
+__global__ void __launch_bounds__(kRowWarps * 32) k_router_grad_kept(const T *__restrict__ scores,
+                                                                     const int32_t *__restrict__ ids,
+                                                                     const float *__restrict__ dw, int T_, int E,
+                                                                     int k, int log2kw, T *__restrict__ out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kw = 1 << log2kw, rows = 32 >> log2kw;
+    const int64_t t0 = ((int64_t)blockIdx.x * kRowWarps + warp) * rows;
+    if (t0 >= T_) return;
+    const int group = lane >> log2kw, slot = lane & (kw - 1);
+    const int64_t t = t0 + group;
+    const bool have = t < T_ && slot < k;
+    int id = have ? __ldg(ids + t * k + slot) : -1;
+    const bool kept = id >= 0 && id < E;
+    const float d = kept ? __ldg(dw + t * k + slot) : 0.f;
+    if (!ACCUM) {
+        T *o = out + t0 * E;
+        const int64_t n = (T_ - t0 < rows ? T_ - t0 : rows) * E;
+        if (WIDE) {
+            constexpr int W = 16 / (int)sizeof(T);
+            for (int64_t i = (int64_t)lane * W; i < n; i += 32 * W)
+                *reinterpret_cast<uint4 *>(o + i) = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            for (int64_t i = lane; i < n; i += 32) o[i] = from_f32<T>(0.f);
+        }
+    }
+    const float v = kept && (SOFTMAX || RENORM) ? to_f32(__ldg(scores + t * E + id)) : 0.f;
+    const float old = ACCUM && kept ? to_f32(out[t * E + id]) : 0.f;
+    auto sum = [&](float x) {
+        for (int o = kw >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+        return x;
+    };
+    float g = d;
+    if (SOFTMAX) {  // w: the softmax over the kept logits
+        float m = kept ? v : -INFINITY;
+        for (int o = kw >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+        const float e = kept ? expf(v - m) : 0.f;
+        const float total = sum(e);
+        const float w = kept ? e / total : 0.f;
+        g = w * (d - sum(w * d));
+    } else if (RENORM) {
+        const float total = sum(v);
+        const float c = sum(kept ? v / total * d : 0.f);
+        g = kept ? (d - c) / total : 0.f;
+    }
+    unsigned same;
+    g = same_id_sum(kept ? group * kMaxTrainExperts + id : -1 - lane, g, same);  // (also orders the zeros before the rest)
+    __syncwarp();
+    if (kept && lane == __ffs(same) - 1) out[t * E + id] = from_f32<T>(old + g);
+}
+
+// Raw weights of logits: dl_i = p_i (dw_i - c) over the whole row.  One warp
+// per row, lane = slot; the row is written as -c p_i, then the kept columns.
+template <typename T, int PL, int VEC, bool ACCUM>
+__global__ void __launch_bounds__(kRowWarps * 32) k_router_grad_raw(const T *__restrict__ scores,
+                                                                    const int32_t *__restrict__ ids,
+                                                                    const float *__restrict__ dw, int T_, int E, int k,
+                                                                    T *__restrict__ out) {
     using RW = Row<T, PL, VEC>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int t = blockIdx.x * kRowWarps + warp; t < T_; t += gridDim.x * kRowWarps) {
-        const T *row = scores + (int64_t)t * E;
-        T *o = out + (int64_t)t * E;
-        int id = lane < k ? __ldg(ids + (int64_t)t * k + lane) : -1;
-        const bool kept = id >= 0 && id < E;
-        if (!kept) id = -1 - lane;  // no other lane's id
-        const float d = kept ? __ldg(dw + (int64_t)t * k + lane) : 0.f;
-        const bool any = __any_sync(kFull, kept);
-        float old = 0.f;
-        if (ACCUM && kept) old = to_f32(o[id]);
-        float v = kept ? to_f32(__ldg(row + id)) : 0.f, g = 0.f;
-        float x[PL];
-        if (SOFTMAX && !RENORM) {
-            RW::load(row, E, lane, -INFINITY, x);
-            float m = -INFINITY;
+    const int t = blockIdx.x * kRowWarps + warp;
+    if (t >= T_) return;
+    const T *row = scores + (int64_t)t * E;
+    T *o = out + (int64_t)t * E;
+    const int id = lane < k ? __ldg(ids + (int64_t)t * k + lane) : -1;
+    const bool kept = id >= 0 && id < E;
+    const float d = kept ? __ldg(dw + (int64_t)t * k + lane) : 0.f;
+    const bool any = __any_sync(kFull, kept);
+    const float v = kept ? to_f32(__ldg(row + id)) : 0.f, old = ACCUM && kept ? to_f32(o[id]) : 0.f;
+    float x[PL];
+    RW::load(row, E, lane, -INFINITY, x);
+    float m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < PL; ++j) m = fmaxf(m, x[j]);
-            m = warp_max(m);
-            float sum = 0.f;
+    for (int j = 0; j < PL; ++j) m = fmaxf(m, x[j]);
+    m = warp_max(m);
+    float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < PL; ++j) {
-                x[j] = expf(x[j] - m);
-                sum += x[j];
-            }
-            sum = warp_sum(sum);
-            const float p = kept ? expf(v - m) / sum : 0.f;
-            const float c = warp_sum(d * p);
-            const float cn = any ? -c / sum : 0.f;
-#pragma unroll
-            for (int j = 0; j < PL; ++j) x[j] = any ? x[j] * cn : 0.f;
-            // a kept column is p (sum of its slots' dw - c): the lanes of one id share p
-            g = p * d;
-            v = -c * p;
-        } else if (SOFTMAX) {
-            const float m = warp_max(kept ? v : -INFINITY);
-            const float e = kept ? expf(v - m) : 0.f;
-            const float w = any ? e / warp_sum(e) : 0.f;
-            g = w * (d - warp_sum(w * d));
-            v = 0.f;
-        } else if (RENORM) {
-            const float sum = warp_sum(v);
-            const float c = warp_sum(kept ? v / sum * d : 0.f);
-            g = kept ? (d - c) / sum : 0.f;
-            v = 0.f;
-        } else {
-            g = d;
-            v = 0.f;
-        }
-        if (!(SOFTMAX && !RENORM)) {
-#pragma unroll
-            for (int j = 0; j < PL; ++j) x[j] = 0.f;
-        }
-        if (ACCUM) {
-            if (SOFTMAX && !RENORM) {
-                float y[PL];
-                RW::load(o, E, lane, 0.f, y);
-#pragma unroll
-                for (int j = 0; j < PL; ++j) x[j] += y[j];
-                __syncwarp();
-                RW::store(o, E, lane, x);
-            }
-        } else {
-            RW::store(o, E, lane, x);
-        }
-        const unsigned same = __match_any_sync(kFull, id);
-        float total = 0.f;
-        for (unsigned rest = kept ? same : 0u; __any_sync(kFull, rest != 0u);) {
-            const int src = rest ? __ffs(rest) - 1 : lane;
-            const float add = __shfl_sync(kFull, g, src);
-            if (rest) total += add;
-            rest &= rest - 1;
-        }
-        __syncwarp();
-        if (kept && lane == __ffs(same) - 1) o[id] = from_f32<T>(old + (v + total));
+    for (int j = 0; j < PL; ++j) {
+        x[j] = expf(x[j] - m);
+        sum += x[j];
     }
+    sum = warp_sum(sum);
+    const float p = kept ? expf(v - m) / sum : 0.f;
+    const float c = warp_sum(d * p);
+    const float cn = -c / sum;
+    float y[PL];
+    if (ACCUM) RW::load_rw(o, E, lane, y);
+#pragma unroll
+    for (int j = 0; j < PL; ++j) x[j] = (any ? x[j] * cn : 0.f) + (ACCUM ? y[j] : 0.f);
+    unsigned same;
+    const float g = same_id_sum(kept ? id : -1 - lane, p * d, same);
+    __syncwarp();
+    RW::store(o, E, lane, x);
+    __syncwarp();
+    if (kept && lane == __ffs(same) - 1) o[id] = from_f32<T>(old + (g - c * p));  // p (sum of its slots' dw - c)
 }
 
 bool is_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
@@ -448,37 +540,61 @@ int with_row(int E, bool vec_ok, F f) {
 }
 
 template <typename T>
-int launch_balance(const BalanceArgs &a, int blocks, cudaStream_t s) {
-    const bool vec = is_aligned(a.logits, 16) && is_aligned(a.grad, 16);
-    return with_row<T>(a.E, vec, [&](auto pl, auto v) {
-        k_balance_main<T, decltype(pl)::value, decltype(v)::value><<<blocks, kRowWarps * 32, 0, s>>>(a);
+int launch_balance(const BalanceArgs &a, int sms, cudaStream_t s) {
+    const bool vec = is_aligned(a.logits, 16) && is_aligned(a.grad, 16) && is_aligned(a.counts, 16);
+    cudaError_t err = cudaSuccess;
+    const int st = with_row<T>(a.E, vec, [&](auto pl, auto v) {
+        constexpr int PL = decltype(pl)::value;
+        constexpr int rows = kRowWarps * kRowsAtOnce<PL>;
+        int blocks = (a.T + rows - 1) / rows;
+        const int most = sms * kBalanceBlocksPerSm < kMaxBalanceBlocks ? sms * kBalanceBlocksPerSm : kMaxBalanceBlocks;
+        blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(kRowWarps * 32);
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        err = cudaLaunchKernelEx(&cfg, k_balance_main<T, PL, decltype(v)::value>, a);
     });
+    return err == cudaSuccess ? st : LATENT_ERR_CUDA;
+}
+
+template <typename T, bool SOFTMAX, bool RENORM>
+int launch_kept(const T *scores, const int32_t *ids, const float *dw, int n, int E, int k, bool accum, T *out,
+                cudaStream_t s) {
+    int log2kw = 0;
+    while ((1 << log2kw) < k) ++log2kw;
+    const int rows = kRowWarps * (32 >> log2kw);
+    const unsigned g = (unsigned)((n + rows - 1) / rows);
+    const bool wide = E * sizeof(T) % 16 == 0 && is_aligned(out, 16);
+    if (accum)
+        k_router_grad_kept<T, false, SOFTMAX, RENORM, true><<<g, kRowWarps * 32, 0, s>>>(scores, ids, dw, n, E, k, log2kw, out);
+    else if (wide)
+        k_router_grad_kept<T, true, SOFTMAX, RENORM, false><<<g, kRowWarps * 32, 0, s>>>(scores, ids, dw, n, E, k, log2kw, out);
+    else
+        k_router_grad_kept<T, false, SOFTMAX, RENORM, false><<<g, kRowWarps * 32, 0, s>>>(scores, ids, dw, n, E, k, log2kw, out);
+    return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
 
 template <typename T>
 int launch_router_grad(const void *scores, const int32_t *ids, const float *dw, int n, int E, int k, uint32_t flags,
                        void *out, cudaStream_t s) {
-    const bool vec = is_aligned(scores, 16) && is_aligned(out, 16);
-    const int64_t blocks = ((int64_t)n + kRowWarps - 1) / kRowWarps;
-    return with_row<T>(E, vec, [&](auto pl, auto v) {
+    const T *sc = static_cast<const T *>(scores);
+    T *o = static_cast<T *>(out);
+    const bool softmax = flags & LATENT_ROUTER_SOFTMAX, renorm = flags & LATENT_ROUTER_RENORMALIZE;
+    const bool accum = flags & LATENT_ROUTER_ACCUMULATE;
+    if (softmax && renorm) return launch_kept<T, true, true>(sc, ids, dw, n, E, k, accum, o, s);
+    if (renorm) return launch_kept<T, false, true>(sc, ids, dw, n, E, k, accum, o, s);
+    if (!softmax) return launch_kept<T, false, false>(sc, ids, dw, n, E, k, accum, o, s);
+    const unsigned g = (unsigned)((n + kRowWarps - 1) / kRowWarps);
+    return with_row<T>(E, is_aligned(scores, 16) && is_aligned(out, 16), [&](auto pl, auto v) {
         constexpr int PL = decltype(pl)::value, V = decltype(v)::value;
-        const T *sc = static_cast<const T *>(scores);
-        T *o = static_cast<T *>(out);
-        const unsigned g = (unsigned)blocks;
-        const int mode = ((flags & LATENT_ROUTER_SOFTMAX) ? 4 : 0) | ((flags & LATENT_ROUTER_RENORMALIZE) ? 2 : 0) |
-                         ((flags & LATENT_ROUTER_ACCUMULATE) ? 1 : 0);
-#define LATENT_RG(S_, R_, A_) k_router_grad<T, PL, V, S_, R_, A_><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o)
-        switch (mode) {
-            case 0: LATENT_RG(false, false, false); break;
-            case 1: LATENT_RG(false, false, true); break;
-            case 2: LATENT_RG(false, true, false); break;
-            case 3: LATENT_RG(false, true, true); break;
-            case 4: LATENT_RG(true, false, false); break;
-            case 5: LATENT_RG(true, false, true); break;
-            case 6: LATENT_RG(true, true, false); break;
-            default: LATENT_RG(true, true, true); break;
-        }
-#undef LATENT_RG
+        if (accum) k_router_grad_raw<T, PL, V, true><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
+        else k_router_grad_raw<T, PL, V, false><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
     });
 }
 
@@ -531,13 +647,10 @@ extern "C" LATENT_API int latent_balance_loss(const void *logits, int32_t type, 
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     k_balance_count<<<(unsigned)n_sequences * kCountCluster, kCountThreads, 0, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return LATENT_ERR_CUDA;
-    int blocks = (n_tokens + kRowWarps - 1) / kRowWarps;
-    const int most = sms * kBalanceBlocksPerSm < kMaxBalanceBlocks ? sms * kBalanceBlocksPerSm : kMaxBalanceBlocks;
-    blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
     switch (type) {
-        case LATENT_TYPE_F32: return launch_balance<float>(a, blocks, s);
-        case LATENT_TYPE_F16: return launch_balance<__half>(a, blocks, s);
-        default: return launch_balance<__nv_bfloat16>(a, blocks, s);
+        case LATENT_TYPE_F32: return launch_balance<float>(a, sms, s);
+        case LATENT_TYPE_F16: return launch_balance<__half>(a, sms, s);
+        default: return launch_balance<__nv_bfloat16>(a, sms, s);
     }
 }
 

@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .runtime import _X_TYPES, _stream_ptr
+from .runtime import _X_TYPES
 
 __all__ = ["BalanceLoss", "balance_loss", "router_topk_grad"]
 
@@ -35,15 +35,34 @@ class BalanceLoss(NamedTuple):
 
 
 def _on(device: torch.device, fn, *args) -> int:
-    """Calls a C entry point with ``device`` current (kernels launch on the current device)."""
-    if torch.cuda.current_device() == device.index:
-        return fn(*args)
+    """Calls a C entry point with ``device`` current (kernels launch on the current device), on its current stream."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return fn(*args, _raw_stream(index))
     with torch.cuda.device(device):
-        return fn(*args)
+        return fn(*args, _raw_stream(index))
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_WS_BYTES = {}    # workspace size by the number of sequences
+
+
+def _workspace_bytes(n_seq: int) -> int:
+    n = _WS_BYTES.get(n_seq)
+    if n is None:
+        size = C.c_size_t(0)
+        _lib.check(_lib.lib().latent_balance_workspace_size(n_seq, C.byref(size)), "latent_balance_workspace_size")
+        n = size.value
+        if len(_WS_BYTES) < 4096:
+            _WS_BYTES[n_seq] = n
+    return n
 
 
 def _router_inputs(logits: torch.Tensor, ids: torch.Tensor, name: str):
-    if not torch.is_tensor(logits) or logits.device.type != "cuda":
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{name} must be [T, E], got {tuple(logits.shape)}")
@@ -53,7 +72,7 @@ def _router_inputs(logits: torch.Tensor, ids: torch.Tensor, name: str):
         raise ValueError("ids must be int32 [T, k]")
     if ids.device != logits.device:
         raise ValueError(f"ids must be on {logits.device}")
-    return logits.detach().contiguous(), ids.contiguous()
+    return logits.contiguous(), ids.contiguous()
 
 
 def _no_capture(what: str) -> None:
@@ -68,18 +87,18 @@ def _no_capture(what: str) -> None:
 def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradient):
     T, E = logits.shape
     dev = logits.device
-    L = _lib.lib()
-    n = C.c_size_t(0)
-    _lib.check(L.latent_balance_workspace_size(n_seq, C.byref(n)), "latent_balance_workspace_size")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    n = _workspace_bytes(n_seq)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     losses = torch.empty(3, dtype=torch.float32, device=dev)
-    counts = torch.empty((n_seq, E), dtype=torch.int32, device=dev)
+    # [E] when the rows are one sequence without borders
+    counts = torch.empty(E, dtype=torch.int32, device=dev) if cu is None else \
+        torch.empty(n_seq, E, dtype=torch.int32, device=dev)
     grad = torch.empty_like(logits) if gradient else None
-    _lib.check(_on(dev, L.latent_balance_loss, logits.data_ptr(), _X_TYPES[logits.dtype], ids.data_ptr(),
+    _lib.check(_on(dev, _lib.lib().latent_balance_loss, logits.data_ptr(), _X_TYPES[logits.dtype], ids.data_ptr(),
                    None if valid is None else valid.data_ptr(), None if cu is None else cu.data_ptr(), T, E,
                    ids.shape[1], n_seq, balance_coef, z_coef, None if d_loss is None else d_loss.data_ptr(),
-                   losses.data_ptr(), counts.data_ptr(), None if grad is None else grad.data_ptr(), ws.data_ptr(),
-                   n.value, _stream_ptr(dev)), "latent_balance_loss")
+                   losses.data_ptr(), counts.data_ptr(), None if grad is None else grad.data_ptr(), ws.data_ptr(), n),
+               "latent_balance_loss")
     return losses, counts, grad
 
 
@@ -140,13 +159,13 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 
             raise ValueError(f"valid must be bool [{T}] on {flat.device}")
         valid = valid.contiguous()
     balance_coef, z_coef = float(balance_coef), float(z_coef)
-    if logits.requires_grad and torch.is_grad_enabled() and not gradient:
+    if not gradient and logits.requires_grad and torch.is_grad_enabled():
         loss, balance, z, counts = _BalanceLossFn.apply(logits, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq)
         grad = None
     else:
         losses, counts, grad = _balance(flat, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq, None, gradient)
         loss, balance, z = losses.unbind()
-    return BalanceLoss(loss, balance, z, counts if cu_seqlens is not None else counts[0], grad)
+    return BalanceLoss(loss, balance, z, counts, grad)
 
 
 def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.Tensor, renormalize: bool = True,
@@ -164,18 +183,20 @@ def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.T
         raise ValueError(f"d_weights must be float32 {tuple(ids.shape)} on {flat.device}")
     flags = (_lib.ROUTER_RENORMALIZE if renormalize else 0) | (_lib.ROUTER_SOFTMAX if logits else 0)
     if out is None:
-        g = torch.empty_like(flat)
+        g = torch.empty_like(flat)   # (never carries requires_grad)
     else:
         if out.shape != flat.shape or out.dtype != flat.dtype or out.device != flat.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {flat.dtype} {tuple(flat.shape)} tensor on {flat.device}")
         if out.data_ptr() == flat.data_ptr() and flat.numel():
             raise ValueError("out must not be the scores")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out must not require a gradient")
         flags |= _lib.ROUTER_ACCUMULATE
         g = out
-    d_weights = d_weights.detach().contiguous()
+    d_weights = d_weights.contiguous()
     T, E = flat.shape
     _lib.check(_on(flat.device, _lib.lib().latent_router_grad, flat.data_ptr(), _X_TYPES[flat.dtype], ids.data_ptr(),
-                   d_weights.data_ptr(), T, E, ids.shape[1], flags, g.data_ptr(), _stream_ptr(flat.device)),
+                   d_weights.data_ptr(), T, E, ids.shape[1], flags, g.data_ptr()),
                "latent_router_grad")
     return g
 
