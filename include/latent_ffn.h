@@ -482,12 +482,29 @@ LATENT_API int latent_router_grad(const void *scores, int32_t type, const int32_
  * row, adds nothing and has a zero gradient.  Workspace: 256-byte aligned,
  * latent_balance_workspace_size() bytes.  LATENT_ERR_UNSUPPORTED beyond 1024
  * experts.  Stream-ordered; repeated calls agree bit for bit. */
-LATENT_API int latent_balance_workspace_size(int32_t n_sequences, size_t *bytes);
-LATENT_API int latent_balance_loss(const void *logits, int32_t type, const int32_t *ids, const uint8_t *valid,
-                                   const int32_t *cu_seqlens, int32_t n_tokens, int32_t n_expert, int32_t top_k,
-                                   int32_t n_sequences, float balance_coef, float z_coef, const float *d_loss,
-                                   float *losses, int32_t *counts, void *grad, void *workspace,
-                                   size_t workspace_bytes, struct CUstream_st *stream);
+typedef struct latent_balance_desc {
+    int32_t n_tokens;          /* T */
+    int32_t n_expert;          /* E */
+    int32_t top_k;             /* k */
+    int32_t n_sequences;       /* S */
+    int32_t type;              /* latent_type of logits and grad */
+    uint32_t flags;            /* 0 */
+    float balance_coef;
+    float z_coef;
+    const void *logits;        /* [T][E] */
+    const int32_t *ids;        /* [T][k] */
+    const uint8_t *valid;      /* [T] or NULL */
+    const int32_t *cu_seqlens; /* [S + 1], or NULL with S = 1 */
+    const float *d_loss;       /* one device float, or NULL */
+    float *losses;             /* [3] */
+    int32_t *counts;           /* [S][E] */
+    void *grad;                /* [T][E] or NULL */
+    void *workspace;
+    size_t workspace_bytes;
+} latent_balance_desc;
+
+LATENT_API int latent_balance_workspace_size(const latent_balance_desc *desc, size_t *bytes);
+LATENT_API int latent_balance_loss(const latent_balance_desc *desc, struct CUstream_st *stream);
 
 /* Low-rank adapters of many requests beside one shared projection (no
  * counterpart in the reference; its low-rank pair is loader/latent_runtime.py

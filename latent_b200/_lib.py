@@ -171,18 +171,40 @@ class AdapterDesc(C.Structure):
     ]
 
 
-# AdapterDesc's fields in order, for callers that pack a descriptor per call (a third of the Structure's time).
+class BalanceDesc(C.Structure):
+    _fields_ = [
+        ("n_tokens", C.c_int32),
+        ("n_expert", C.c_int32),
+        ("top_k", C.c_int32),
+        ("n_sequences", C.c_int32),
+        ("type", C.c_int32),
+        ("flags", C.c_uint32),
+        ("balance_coef", C.c_float),
+        ("z_coef", C.c_float),
+        ("logits", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("valid", C.c_void_p),
+        ("cu_seqlens", C.c_void_p),
+        ("d_loss", C.c_void_p),
+        ("losses", C.c_void_p),
+        ("counts", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+# The two descriptors' fields in order, for callers that pack one per call (a third of the Structure's time).
 ADAPTER_DESC = struct.Struct("=8i15q")
-assert ADAPTER_DESC.size == C.sizeof(AdapterDesc)
+BALANCE_DESC = struct.Struct("=6i2f10q")
+assert ADAPTER_DESC.size == C.sizeof(AdapterDesc) and BALANCE_DESC.size == C.sizeof(BalanceDesc)
 
 EXPORTS.update({
     "latent_adapter_workspace_size": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
     "latent_adapter_project": (C.c_int, [C.c_void_p, C.c_void_p]),
     "latent_adapter_check": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "latent_balance_workspace_size": (C.c_int, [C.c_int32, C.POINTER(C.c_size_t)]),
-    "latent_balance_loss": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
-                                      C.c_int32, C.c_int32, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p,
-                                      C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "latent_balance_workspace_size": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
+    "latent_balance_loss": (C.c_int, [C.c_void_p, C.c_void_p]),
     "latent_router_grad": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
                                      C.c_uint32, C.c_void_p, C.c_void_p]),
     "latent_ep_workspace_size": (C.c_int, [C.POINTER(EpDesc), C.POINTER(C.c_size_t)]),

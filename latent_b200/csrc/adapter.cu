@@ -169,8 +169,10 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows,
                             d->rank == 16 ? 4 : d->rank == 32 ? 5 : d->rank == 64 ? 6 : 7};
         const bool wide = d->y_type == d->type && d->n_tokens > 256;
-        if (launch_adapter_shrink(a, sms, s) != cudaSuccess ||
-            (wide ? launch_adapter_wide(a, sms, s) : launch_adapter_skinny(a, sms, s)) != cudaSuccess)
+        CUtensorMap x;
+        if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows) ||
+            launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
+            (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, s)) != cudaSuccess)
             return LATENT_ERR_CUDA;
         return LATENT_OK;
     }

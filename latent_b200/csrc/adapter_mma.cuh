@@ -24,9 +24,10 @@ struct AdapterArgs {
     int log2r;       // rank = 1 << log2r
 };
 
-cudaError_t launch_adapter_shrink(const AdapterArgs &a, int sms, cudaStream_t s);
-cudaError_t launch_adapter_skinny(const AdapterArgs &a, int sms, cudaStream_t s);
-cudaError_t launch_adapter_wide(const AdapterArgs &a, int sms, cudaStream_t s);
+// x_map: the CUtensorMap of x with a box of tile_rows rows.
+cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
+cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
+cudaError_t launch_adapter_wide(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
 
 namespace adapter {
 

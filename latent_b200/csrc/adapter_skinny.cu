@@ -597,7 +597,7 @@ bool adapter_map(void *map, bool bf16, const void *base, uint64_t rows, uint64_t
            CUDA_SUCCESS;
 }
 
-cudaError_t launch_adapter_shrink(const AdapterArgs &g, int sms, cudaStream_t s) {
+cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16;
     const int tiles = (d.n_tokens + g.tile_rows - 1) / g.tile_rows;
@@ -621,17 +621,15 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, int sms, cudaStream_t s)
     if (p.stages < 1) return cudaErrorInvalidConfiguration;
     p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
     p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
-    CUtensorMap mA, mX;
-    if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank) ||
-        !adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, p.rows))
-        return cudaErrorInvalidValue;
+    CUtensorMap mA;
+    if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank)) return cudaErrorInvalidValue;
     AdapterArgs a = g;
-    void *args[] = {&mA, &mX, &a, &p};
+    void *args[] = {&mA, const_cast<void *>(x_map), &a, &p};
     return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
                           dim3(cluster, slots, tiles), p.smem, cluster, false, args, s);
 }
 
-cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s) {
+cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
     const bool f32 = d.y_type == LATENT_TYPE_F32;
@@ -662,16 +660,15 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, int sms, cudaStream_t s)
     if (p.stages > per + 4) p.stages = per + 4;
     if (p.stages < 1) return cudaErrorInvalidConfiguration;
     p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
-    CUtensorMap mW, mB, mX;
+    CUtensorMap mW, mB;
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
-                     d.rank < kExt ? d.rank : kExt) ||
-        !adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, p.rows))
+                     d.rank < kExt ? d.rank : kExt))
         return cudaErrorInvalidValue;
     const void *fn = f32 ? skinny_fn<float>(bf, kn, parts)
                          : bf ? skinny_fn<__nv_bfloat16>(bf, kn, parts) : skinny_fn<__half>(bf, kn, parts);
     AdapterArgs a = g;
-    void *args[] = {&mW, &mB, &mX, &a, &p};
+    void *args[] = {&mW, &mB, const_cast<void *>(x_map), &a, &p};
     return launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, cluster, true, args, s);
 }
 

@@ -379,12 +379,11 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
 
 }  // namespace
 
-cudaError_t launch_adapter_wide(const AdapterArgs &g, int sms, cudaStream_t s) {
+cudaError_t launch_adapter_wide(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
-    CUtensorMap mX, mW, mB;
-    if (!adapter_map(&mX, bf, d.x, d.n_tokens, d.n_in, d.ldx, 128) ||
-        !(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
+    CUtensorMap mW, mB;
+    if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
                      d.rank < kExt ? d.rank : kExt))
         return cudaErrorInvalidValue;
@@ -405,7 +404,7 @@ cudaError_t launch_adapter_wide(const AdapterArgs &g, int sms, cudaStream_t s) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     AdapterArgs a = g;
-    void *args[] = {&mX, &mW, &mB, &a};
+    void *args[] = {const_cast<void *>(x_map), &mW, &mB, &a};
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 

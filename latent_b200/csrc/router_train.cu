@@ -9,7 +9,7 @@
 // counted row, n = sum n_s):
 //   L_bal = (1/S') sum_s E sum_e f_se P_se,  P_se = (1/n_s) sum_t p_te
 //   L_z   = (1/n) sum_t lse_t^2,             loss = b L_bal + z L_z
-// With C_se = E f_se / (S' n_s), a number per sequence and expert that the ids
+// With C_se = E f_se / (S' n_s), numbers per sequence and expert that the ids
 // alone give, L_bal = sum_t D_t with D_t = sum_e C_se p_te, and
 //   dloss/dl_ti = p_ti (b (C_si - D_t) + 2 z lse_t / n):
 // value and gradient need the counts first and then ONE pass over the logits,
@@ -17,9 +17,11 @@
 //
 // k_balance_count: one cluster of 8 blocks per sequence; each block counts its
 // rows' ids in a shared-memory histogram, the blocks add theirs up through
-// distributed shared memory: integers, no global atomics, nothing to zero.
+// distributed shared memory: integers, no global atomics, nothing to zero.  It
+// leaves f as well, in fp32: an integer to float conversion per column and row
+// runs at a quarter of the rate.
 // k_balance_main, its programmatic dependent, takes the softmax of its first
-// rows before it waits for the counts: one warp per row, two rows at once in
+// rows before it waits for the counts: 4 to 32 lanes per row, the row in
 // registers; every block leaves its two partial sums (64 bits) and the last one
 // adds them up in block order, so that a call's results do not depend on the
 // order of execution.
@@ -56,14 +58,14 @@ template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<16> { using type = uint4; };
 
-// A row of E values held by one warp: lane l has, of each run of 32 * VEC
-// columns, the VEC adjacent ones from l * VEC (one load or store of
+// A row of E values held by LPR lanes, PL values each: lane l has, of each run
+// of LPR * VEC columns, the VEC adjacent ones from l * VEC (one load or store of
 // VEC * sizeof(T) bytes).  E is a multiple of VEC and rows are aligned to it.
-template <typename T, int PL, int VEC>
+template <typename T, int PL, int VEC, int LPR = 32>
 struct Row {
     static constexpr int NV = PL / VEC;
     using R = typename Raw<VEC * sizeof(T)>::type;
-    static __device__ __forceinline__ int col(int lane, int v) { return (v * 32 + lane) * VEC; }
+    static __device__ __forceinline__ int col(int lane, int v) { return (v * LPR + lane) * VEC; }
     static __device__ __forceinline__ void load(const T *row, int E, int lane, float pad, float (&x)[PL]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -91,8 +93,9 @@ struct Row {
             for (int i = 0; i < VEC; ++i) x[v * VEC + i] = to_f32(e[i]);
         }
     }
-    // Integers laid out like the row, scaled.
-    static __device__ __forceinline__ void counts(const int32_t *row, int E, int lane, float scale, float (&x)[PL]) {
+    // f(j, value) for fp32 values laid out like the row (0 behind column E).
+    template <typename F>
+    static __device__ __forceinline__ void floats(const float *row, int E, int lane, F f) {
         constexpr int W = VEC < 4 ? VEC : 4;
         using R4 = typename Raw<W * 4>::type;
 #pragma unroll
@@ -101,10 +104,10 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < VEC; i += W) {
                 R4 raw = R4();
-                if (c < E) raw = __ldcg(reinterpret_cast<const R4 *>(row + c + i));
-                const int32_t *e = reinterpret_cast<const int32_t *>(&raw);
+                if (c < E) raw = __ldca(reinterpret_cast<const R4 *>(row + c + i));
+                const float *e = reinterpret_cast<const float *>(&raw);
 #pragma unroll
-                for (int u = 0; u < W; ++u) x[v * VEC + i + u] = (float)e[u] * scale;
+                for (int u = 0; u < W; ++u) f(v * VEC + i + u, e[u]);
             }
         }
     }
@@ -123,17 +126,29 @@ struct Row {
     }
 };
 
+// exp(x) for x <= 0: 2^(x log2 e), the product rounded once more than expf's
+// (|x| 2^-24 of the result) and two steps of the approximation, at a third of
+// its instructions.
+__device__ __forceinline__ float exp_neg(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Over the LANES lanes that share a row.
+template <int LANES = 32>
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
+template <int LANES = 32>
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
 
@@ -172,7 +187,9 @@ struct BalanceArgs {
     float *losses;
     int32_t *counts;    // [S][E]
     void *grad;
-    int32_t *seq;       // [S][2] counted rows, kept slots
+    int32_t *seq;       // [S] counted rows
+    float *share;       // [S][row pitch] each expert's share of the sequence's kept slots
+    int share_ld;
     double *partial;    // [blocks][2]
     uint32_t *ticket;
 };
@@ -194,12 +211,20 @@ k_balance_count(BalanceArgs a) {
     const int per = (hi - lo + kCountCluster - 1) / kCountCluster;
     const int r0 = min(hi, lo + rank * per), r1 = min(hi, r0 + per);
     int rows = 0, slots = 0;
-    for (int i = r0 * a.k + threadIdx.x; i < r1 * a.k; i += blockDim.x) {
-        if (a.valid && !__ldg(a.valid + i / a.k)) continue;
-        const int e = __ldg(a.ids + i);
-        if (e >= 0 && e < a.E) {
-            atomicAdd(&hist[e], 1);
-            ++slots;
+    const int end = r1 * a.k;
+    for (int i = r0 * a.k + threadIdx.x; i < end; i += 4 * blockDim.x) {
+        int e[4];  // four loads on the way at once
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int at = i + u * blockDim.x;
+            e[u] = at < end && (!a.valid || __ldg(a.valid + at / a.k)) ? __ldg(a.ids + at) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (e[u] >= 0 && e[u] < a.E) {
+                atomicAdd(&hist[e[u]], 1);
+                ++slots;
+            }
         }
     }
     if (a.valid) {
@@ -214,6 +239,12 @@ k_balance_count(BalanceArgs a) {
         if (slots) atomicAdd(&tot[1], slots);
     }
     cluster.sync();
+    // lanes 2q and 2q + 1 have block q's rows and slots: sums over even and over odd lanes
+    int all = (threadIdx.x & 31) < 2 * kCountCluster ? cluster.map_shared_rank(tot, (threadIdx.x & 31) >> 1)[threadIdx.x & 1] : 0;
+#pragma unroll
+    for (int o = 16; o > 1; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
+    const int counted = __shfl_sync(kFull, all, 0), kept = __shfl_sync(kFull, all, 1);
+    const float inv = 1.f / (float)max(1, kept);
     const int step = (a.E + kCountCluster - 1) / kCountCluster;
     const int e0 = rank * step, e1 = min(a.E, e0 + step);
     for (int e = e0 + threadIdx.x; e < e1; e += blockDim.x) {
@@ -221,26 +252,24 @@ k_balance_count(BalanceArgs a) {
 #pragma unroll
         for (int q = 0; q < kCountCluster; ++q) c += *cluster.map_shared_rank(&hist[e], q);
         a.counts[(int64_t)s * a.E + e] = c;
+        a.share[(int64_t)s * a.share_ld + e] = (float)c * inv;
     }
-    if (rank == 0 && threadIdx.x < 2) {
-        int c = 0;
-#pragma unroll
-        for (int q = 0; q < kCountCluster; ++q) c += *cluster.map_shared_rank(&tot[threadIdx.x], q);
-        a.seq[2 * s + threadIdx.x] = c;
-    }
+    if (rank == 0 && threadIdx.x == 0) a.seq[s] = counted;
     cluster.sync();  // the others' shared memory stays until every block has read it
 }
 
-// Rows a warp works on at once: two while they fit into registers (16 floats a lane).
-template <int PL> constexpr int kRowsAtOnce = PL <= 8 ? 2 : 1;
+constexpr int kBalanceWarps = 4;
 
-template <typename T, int PL, int VEC>
-__global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) {
-    using RW = Row<T, PL, VEC>;
-    constexpr int R = kRowsAtOnce<PL>;
-    __shared__ double part[kRowWarps][2];
+// LPR lanes per row: the sums over a row, its logarithm, its divisions and its
+// place among the sequences cost instructions per group of lanes, so few lanes
+// with up to 32 values each take fewer of them per row than a whole warp.
+template <typename T, int PL, int VEC, int LPR>
+__global__ void __launch_bounds__(kBalanceWarps * 32, 7) k_balance_main(BalanceArgs a) {
+    using RW = Row<T, PL, VEC, LPR>;
+    constexpr int kRows = 32 / LPR;  // rows of a warp
+    __shared__ double part[kBalanceWarps][2];
     __shared__ bool last;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPR;
     const T *logits = static_cast<const T *>(a.logits);
     T *grad = static_cast<T *>(a.grad);
     bool first = true;
@@ -248,44 +277,42 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
     int64_t n = 0;   // counted rows
     float gb = 0.f, gz = 0.f;
     double sb = 0.0, sz = 0.0;
-    for (int t0 = (blockIdx.x * kRowWarps + warp) * R; first || t0 < a.T; t0 += gridDim.x * kRowWarps * R) {
-        float x[R][PL], lse[R];
-        int seq[R];
+    for (int t0 = (blockIdx.x * kBalanceWarps + warp) * kRows; first || t0 < a.T; t0 += gridDim.x * kBalanceWarps * kRows) {
+        const int t = t0 + lane / LPR;
+        float x[PL];
+        RW::load(logits + (int64_t)t * a.E, t < a.T ? a.E : 0, sub, -INFINITY, x);
+        const int seq = t >= a.T || (a.valid && !__ldg(a.valid + t)) ? -1 : sequence_of(a.cu, a.S, t);
+        float m = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int t = t0 + r;
-            seq[r] = t >= a.T || (a.valid && !__ldg(a.valid + t)) ? -1 : sequence_of(a.cu, a.S, t);
-            // a padded row, whatever it holds, gives nothing and gets a zero gradient
-            RW::load(logits + (int64_t)t * a.E, seq[r] >= 0 ? a.E : 0, lane, -INFINITY, x[r]);
+        for (int j = 0; j < PL; ++j) m = fmaxf(m, x[j]);
+        m = warp_max<LPR>(m);
+        bool nan = false;
+        if (m == -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < PL; ++j) nan |= x[j] != x[j];
         }
+        nan = warp_max<LPR>(nan ? 1.f : 0.f) != 0.f;
+        // a padded row, whatever it holds, gives nothing and gets a zero gradient; so does one with every expert masked
+        const bool none = seq < 0 || (m == -INFINITY && !nan);
+        if (none) {
+            m = 0.f;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float m = -INFINITY;
-            bool nan = false;
-#pragma unroll
-            for (int j = 0; j < PL; ++j) {
-                m = fmaxf(m, x[r][j]);
-                nan |= x[r][j] != x[r][j];
-            }
-            m = warp_max(m);
-            const bool none = m == -INFINITY && !__any_sync(kFull, nan);  // padded, or every expert masked
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < PL; ++j) {
-                x[r][j] = none ? 0.f : expf(x[r][j] - m);
-                sum += x[r][j];
-            }
-            sum = warp_sum(sum);
-            const float inv = none ? 0.f : 1.f / sum;
-            lse[r] = none ? 0.f : m + logf(sum);
-#pragma unroll
-            for (int j = 0; j < PL; ++j) x[r][j] *= inv;
+            for (int j = 0; j < PL; ++j) x[j] = -INFINITY;
         }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < PL; ++j) {
+            x[j] = exp_neg(x[j] - m);
+            sum += x[j];
+        }
+        sum = warp_sum<LPR>(sum);
+        const float inv = none ? 0.f : 1.f / sum;
+        const float lse = none ? 0.f : m + logf(sum);
         if (first) {  // the counts are needed only now
             first = false;
             dependency_wait();
             for (int s = lane; s < a.S; s += 32) {
-                const int c = __ldcg(a.seq + 2 * s);
+                const int c = __ldcg(a.seq + s);
                 n += c;
                 used += c > 0;
             }
@@ -296,29 +323,27 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
             gb = up * a.b;
             gz = n > 0 ? up * (2.f * a.z / (float)n) : 0.f;
         }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int t = t0 + r;
-            float c[PL], d = 0.f;
-            if (seq[r] >= 0) {
-                const int2 nc = __ldcg(reinterpret_cast<const int2 *>(a.seq) + seq[r]);
-                const float scale = (float)a.E / ((float)used * (float)nc.x) / (float)max(1, nc.y);
-                RW::counts(a.counts + (int64_t)seq[r] * a.E, a.E, lane, scale, c);
-#pragma unroll
-                for (int j = 0; j < PL; ++j) d = fmaf(c[j], x[r][j], d);
-            } else {
-#pragma unroll
-                for (int j = 0; j < PL; ++j) c[j] = 0.f;
-            }
-            d = warp_sum(d);
+        const int rows = __ldcg(a.seq + max(seq, 0));
+        const float scale = seq >= 0 ? (float)a.E / ((float)used * (float)rows) : 0.f;  // C = scale * share
+        const float *share = a.share + (int64_t)max(seq, 0) * a.share_ld;
+        const int cols = seq >= 0 ? a.E : 0;
+        float d = 0.f;
+        RW::floats(share, cols, sub, [&](int j, float c) { d = fmaf(c, x[j], d); });
+        d = warp_sum<LPR>(d) * (inv * scale);
+        if (sub == 0) {
             sb += d;
-            sz += (double)lse[r] * lse[r];
-            if (grad && t < a.T) {
-#pragma unroll
-                for (int j = 0; j < PL; ++j) x[r][j] *= fmaf(gb, c[j] - d, gz * lse[r]);
-                RW::store(grad + (int64_t)t * a.E, a.E, lane, x[r]);
-            }
+            sz += (double)lse * lse;
         }
+        if (grad && t < a.T) {  // the shares once more, from L1: kept, they would cost a register per column
+            const float ca = gb * scale * inv, cb = inv * (gz * lse - gb * d);
+            RW::floats(share, cols, sub, [&](int j, float c) { x[j] *= fmaf(ca, c, cb); });
+            RW::store(grad + (int64_t)t * a.E, a.E, sub, x);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o >= LPR; o >>= 1) {
+        sb += __shfl_xor_sync(kFull, sb, o);
+        sz += __shfl_xor_sync(kFull, sz, o);
     }
     if (lane == 0) {
         part[warp][0] = sb;
@@ -327,21 +352,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
     __syncthreads();
     if (threadIdx.x == 0) {
         double b = 0.0, z = 0.0;
-        for (int w = 0; w < kRowWarps; ++w) {
+        for (int w = 0; w < kBalanceWarps; ++w) {
             b += part[w][0];
             z += part[w][1];
         }
         reinterpret_cast<double2 *>(a.partial)[blockIdx.x] = make_double2(b, z);
-        __threadfence();
-        last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+        uint32_t done;  // releases the partial sums, acquires the others'
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(done) : "l"(a.ticket) : "memory");
+        last = done == gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
-    __threadfence();
-    // thread i adds blocks i, i + 256, ... in order, then lanes and warps by a fixed tree
+    // thread i adds blocks i, i + 128, ... in order, then lanes and warps by a fixed tree
     double b = 0.0, z = 0.0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += kRowWarps * 32) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += kBalanceWarps * 32) {
         const double2 v = __ldcg(reinterpret_cast<const double2 *>(a.partial) + i);
         b += v.x;
         z += v.y;
@@ -358,7 +383,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_balance_main(BalanceArgs a) 
     __syncthreads();
     if (threadIdx.x == 0) {
         b = z = 0.0;
-        for (int w = 0; w < kRowWarps; ++w) {
+        for (int w = 0; w < kBalanceWarps; ++w) {
             b += part[w][0];
             z += part[w][1];
         }
@@ -503,16 +528,19 @@ int sm_count(int *sms) {
     return LATENT_OK;
 }
 
-constexpr int kBalanceBlocksPerSm = 8;
+constexpr int kBalanceBlocksPerSm = 16;
 constexpr int kMaxBalanceBlocks = 4096;  // partial sums in the workspace
 
 struct BalanceLayout {
-    size_t seq, partial, ticket, total;
+    size_t seq, share, partial, ticket, total;
+    int share_ld;
 };
-BalanceLayout balance_layout(int S) {
+BalanceLayout balance_layout(int S, int E) {
     BalanceLayout L;
+    L.share_ld = (E + 3) / 4 * 4;  // rows of 16 bytes' multiples
     L.seq = 0;
-    L.partial = round256((size_t)S * 8);
+    L.share = round256((size_t)S * 4);
+    L.partial = L.share + round256((size_t)S * L.share_ld * 4);
     L.ticket = L.partial + (size_t)kMaxBalanceBlocks * 16;
     L.total = L.ticket + 256;
     return L;
@@ -539,28 +567,38 @@ int with_row(int E, bool vec_ok, F f) {
     return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
 
+template <typename T, int PL, int LPR>
+cudaError_t launch_balance_rows(const BalanceArgs &a, bool vec, int sms, cudaStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T);
+    constexpr int rows = kBalanceWarps * (32 / LPR);
+    int blocks = (a.T + rows - 1) / rows;
+    const int most = sms * kBalanceBlocksPerSm < kMaxBalanceBlocks ? sms * kBalanceBlocksPerSm : kMaxBalanceBlocks;
+    blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kBalanceWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return vec && a.E % V == 0 ? cudaLaunchKernelEx(&cfg, k_balance_main<T, PL, V, LPR>, a)
+                               : cudaLaunchKernelEx(&cfg, k_balance_main<T, PL, 1, LPR>, a);
+}
+
 template <typename T>
 int launch_balance(const BalanceArgs &a, int sms, cudaStream_t s) {
-    const bool vec = is_aligned(a.logits, 16) && is_aligned(a.grad, 16) && is_aligned(a.counts, 16);
-    cudaError_t err = cudaSuccess;
-    const int st = with_row<T>(a.E, vec, [&](auto pl, auto v) {
-        constexpr int PL = decltype(pl)::value;
-        constexpr int rows = kRowWarps * kRowsAtOnce<PL>;
-        int blocks = (a.T + rows - 1) / rows;
-        const int most = sms * kBalanceBlocksPerSm < kMaxBalanceBlocks ? sms * kBalanceBlocksPerSm : kMaxBalanceBlocks;
-        blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(blocks);
-        cfg.blockDim = dim3(kRowWarps * 32);
-        cfg.stream = s;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        err = cudaLaunchKernelEx(&cfg, k_balance_main<T, PL, decltype(v)::value>, a);
-    });
-    return err == cudaSuccess ? st : LATENT_ERR_CUDA;
+    const bool vec = is_aligned(a.logits, 16) && is_aligned(a.grad, 16);
+    cudaError_t err;
+    if (a.E <= 32) err = launch_balance_rows<T, 8, 4>(a, vec, sms, s);
+    else if (a.E <= 64) err = launch_balance_rows<T, 8, 8>(a, vec, sms, s);
+    else if (a.E <= 128) err = launch_balance_rows<T, 16, 8>(a, vec, sms, s);
+    else if (a.E <= 192) err = launch_balance_rows<T, 24, 8>(a, vec, sms, s);
+    else if (a.E <= 256) err = launch_balance_rows<T, 32, 8>(a, vec, sms, s);
+    else if (a.E <= 512) err = launch_balance_rows<T, 32, 16>(a, vec, sms, s);
+    else err = launch_balance_rows<T, 32, 32>(a, vec, sms, s);
+    return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
 
 template <typename T, bool SOFTMAX, bool RENORM>
@@ -612,42 +650,41 @@ int train_shape(int32_t T, int32_t E, int32_t k) {
 
 }  // namespace latent
 
-extern "C" LATENT_API int latent_balance_workspace_size(int32_t n_sequences, size_t *bytes) {
-    if (!bytes) return LATENT_ERR_INVALID;
-    if (n_sequences < 1) return LATENT_ERR_SHAPE;
-    *bytes = latent::balance_layout(n_sequences).total;
+extern "C" LATENT_API int latent_balance_workspace_size(const latent_balance_desc *d, size_t *bytes) {
+    if (!d || !bytes) return LATENT_ERR_INVALID;
+    if (d->n_sequences < 1 || d->n_expert < 1) return LATENT_ERR_SHAPE;
+    *bytes = latent::balance_layout(d->n_sequences, d->n_expert).total;
     return LATENT_OK;
 }
 
-extern "C" LATENT_API int latent_balance_loss(const void *logits, int32_t type, const int32_t *ids,
-                                              const uint8_t *valid, const int32_t *cu_seqlens, int32_t n_tokens,
-                                              int32_t n_expert, int32_t top_k, int32_t n_sequences,
-                                              float balance_coef, float z_coef, const float *d_loss, float *losses,
-                                              int32_t *counts, void *grad, void *workspace, size_t workspace_bytes,
-                                              CUstream_st *stream) {
+extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUstream_st *stream) {
     using namespace latent;
-    int st = train_shape(n_tokens, n_expert, top_k);
+    if (!d) return LATENT_ERR_INVALID;
+    int st = train_shape(d->n_tokens, d->n_expert, d->top_k);
     if (st) return st;
-    if (n_sequences < 1 || (n_sequences > 1 && !cu_seqlens)) return LATENT_ERR_SHAPE;
-    if ((int64_t)n_sequences * kCountCluster > 0x7fffffff) return LATENT_ERR_SHAPE;
-    if (!float_type(type)) return LATENT_ERR_DTYPE;
-    if (!losses || !counts || !workspace || (n_tokens > 0 && (!logits || !ids))) return LATENT_ERR_INVALID;
-    const size_t es = type_size(type);
-    if (!is_aligned(logits, es) || !is_aligned(grad, es) || !is_aligned(ids, 4) || !is_aligned(cu_seqlens, 4) ||
-        !is_aligned(d_loss, 4) || !is_aligned(losses, 4) || !is_aligned(counts, 4) || !is_aligned(workspace, 256))
+    if (d->n_sequences < 1 || (d->n_sequences > 1 && !d->cu_seqlens)) return LATENT_ERR_SHAPE;
+    if ((int64_t)d->n_sequences * kCountCluster > 0x7fffffff) return LATENT_ERR_SHAPE;
+    if (!float_type(d->type)) return LATENT_ERR_DTYPE;
+    if (d->flags || !d->losses || !d->counts || !d->workspace || (d->n_tokens > 0 && (!d->logits || !d->ids)))
+        return LATENT_ERR_INVALID;
+    const size_t es = type_size(d->type);
+    if (!is_aligned(d->logits, es) || !is_aligned(d->grad, es) || !is_aligned(d->ids, 4) ||
+        !is_aligned(d->cu_seqlens, 4) || !is_aligned(d->d_loss, 4) || !is_aligned(d->losses, 4) ||
+        !is_aligned(d->counts, 4) || !is_aligned(d->workspace, 256))
         return LATENT_ERR_ALIGN;
-    const BalanceLayout L = balance_layout(n_sequences);
-    if (workspace_bytes < L.total) return LATENT_ERR_WORKSPACE;
+    const BalanceLayout L = balance_layout(d->n_sequences, d->n_expert);
+    if (d->workspace_bytes < L.total) return LATENT_ERR_WORKSPACE;
     int sms = 0;
     if ((st = sm_count(&sms))) return st;
-    char *ws = static_cast<char *>(workspace);
-    BalanceArgs a{logits, ids, valid, cu_seqlens, n_tokens, n_expert, top_k, n_sequences, balance_coef, z_coef, d_loss, losses,
-                  counts, grad, reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<double *>(ws + L.partial),
-                  reinterpret_cast<uint32_t *>(ws + L.ticket)};
+    char *ws = static_cast<char *>(d->workspace);
+    const BalanceArgs a{d->logits, d->ids, d->valid, d->cu_seqlens, d->n_tokens, d->n_expert, d->top_k, d->n_sequences,
+                        d->balance_coef, d->z_coef, d->d_loss, d->losses, d->counts, d->grad,
+                        reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<float *>(ws + L.share), L.share_ld,
+                        reinterpret_cast<double *>(ws + L.partial), reinterpret_cast<uint32_t *>(ws + L.ticket)};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    k_balance_count<<<(unsigned)n_sequences * kCountCluster, kCountThreads, 0, s>>>(a);
+    k_balance_count<<<(unsigned)d->n_sequences * kCountCluster, kCountThreads, 0, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return LATENT_ERR_CUDA;
-    switch (type) {
+    switch (d->type) {
         case LATENT_TYPE_F32: return launch_balance<float>(a, sms, s);
         case LATENT_TYPE_F16: return launch_balance<__half>(a, sms, s);
         default: return launch_balance<__nv_bfloat16>(a, sms, s);

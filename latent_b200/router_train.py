@@ -47,17 +47,18 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_WS_BYTES = {}    # workspace size by the number of sequences
+_WS_BYTES = {}    # workspace size by (sequences, experts)
 
 
-def _workspace_bytes(n_seq: int) -> int:
-    n = _WS_BYTES.get(n_seq)
+def _workspace_bytes(n_seq: int, n_expert: int) -> int:
+    n = _WS_BYTES.get((n_seq, n_expert))
     if n is None:
         size = C.c_size_t(0)
-        _lib.check(_lib.lib().latent_balance_workspace_size(n_seq, C.byref(size)), "latent_balance_workspace_size")
+        d = _lib.BalanceDesc(n_sequences=n_seq, n_expert=n_expert)
+        _lib.check(_lib.lib().latent_balance_workspace_size(C.byref(d), C.byref(size)), "latent_balance_workspace_size")
         n = size.value
         if len(_WS_BYTES) < 4096:
-            _WS_BYTES[n_seq] = n
+            _WS_BYTES[n_seq, n_expert] = n
     return n
 
 
@@ -87,18 +88,19 @@ def _no_capture(what: str) -> None:
 def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradient):
     T, E = logits.shape
     dev = logits.device
-    n = _workspace_bytes(n_seq)
+    n = _workspace_bytes(n_seq, E)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     losses = torch.empty(3, dtype=torch.float32, device=dev)
     # [E] when the rows are one sequence without borders
     counts = torch.empty(E, dtype=torch.int32, device=dev) if cu is None else \
         torch.empty(n_seq, E, dtype=torch.int32, device=dev)
     grad = torch.empty_like(logits) if gradient else None
-    _lib.check(_on(dev, _lib.lib().latent_balance_loss, logits.data_ptr(), _X_TYPES[logits.dtype], ids.data_ptr(),
-                   None if valid is None else valid.data_ptr(), None if cu is None else cu.data_ptr(), T, E,
-                   ids.shape[1], n_seq, balance_coef, z_coef, None if d_loss is None else d_loss.data_ptr(),
-                   losses.data_ptr(), counts.data_ptr(), None if grad is None else grad.data_ptr(), ws.data_ptr(), n),
-               "latent_balance_loss")
+    d = _lib.BALANCE_DESC.pack(T, E, ids.shape[1], n_seq, _X_TYPES[logits.dtype], 0, balance_coef, z_coef,
+                               logits.data_ptr(), ids.data_ptr(), 0 if valid is None else valid.data_ptr(),
+                               0 if cu is None else cu.data_ptr(), 0 if d_loss is None else d_loss.data_ptr(),
+                               losses.data_ptr(), counts.data_ptr(), 0 if grad is None else grad.data_ptr(),
+                               ws.data_ptr(), n)
+    _lib.check(_on(dev, _lib.lib().latent_balance_loss, d), "latent_balance_loss")
     return losses, counts, grad
 
 

@@ -33,20 +33,28 @@ def test_router_grad_validates_on_the_host(lib):
 
 def test_balance_loss_validates_on_the_host(lib):
     n = C.c_size_t()
-    assert lib.latent_balance_workspace_size(0, C.byref(n)) == 2
-    assert lib.latent_balance_workspace_size(1, None) == 1
-    assert lib.latent_balance_workspace_size(3, C.byref(n)) == 0 and n.value % 256 == 0
 
-    def f(logits=256, typ=0, ids=256, cu=None, T=4, E=8, k=2, S=1, losses=256, counts=256, ws=256, nbytes=n.value):
-        return lib.latent_balance_loss(logits, typ, ids, None, cu, T, E, k, S, 0.1, 0.0, None, losses, counts, None, ws,
-                                       nbytes, None)
+    def size(**kw):
+        return lib.latent_balance_workspace_size(C.byref(_lib.BalanceDesc(**kw)), C.byref(n))
 
-    assert f(E=0) == 2 and f(T=-1) == 2 and f(k=0) == 2 and f(S=0) == 2
-    assert f(S=2) == 2                                                    # sequences without borders
-    assert f(typ=5) == 3 and f(E=1025) == 9
-    assert f(logits=None) == 1 and f(ids=None) == 1 and f(losses=None) == 1 and f(counts=None) == 1 and f(ws=None) == 1
-    assert f(logits=258) == 4 and f(ids=258) == 4 and f(ws=128) == 4
-    assert f(nbytes=n.value - 1) == 6
+    assert size(n_sequences=0, n_expert=8) == 2 and size(n_sequences=1, n_expert=0) == 2
+    assert lib.latent_balance_workspace_size(None, C.byref(n)) == 1
+    assert lib.latent_balance_workspace_size(C.byref(_lib.BalanceDesc(n_sequences=1, n_expert=8)), None) == 1
+    assert size(n_sequences=1, n_expert=8) == 0 and n.value % 256 == 0
+
+    def f(**kw):
+        d = dict(n_tokens=4, n_expert=8, top_k=2, n_sequences=1, type=0, balance_coef=0.1, logits=256, ids=256, losses=256,
+                 counts=256, workspace=256, workspace_bytes=n.value)
+        return lib.latent_balance_loss(C.byref(_lib.BalanceDesc(**{**d, **kw})), None)
+
+    assert lib.latent_balance_loss(None, None) == 1
+    assert f(n_expert=0) == 2 and f(n_tokens=-1) == 2 and f(top_k=0) == 2 and f(n_sequences=0) == 2
+    assert f(n_sequences=2) == 2                                          # sequences without borders
+    assert f(type=5) == 3 and f(n_expert=1025) == 9 and f(flags=1) == 1
+    for name in ("logits", "ids", "losses", "counts", "workspace"):
+        assert f(**{name: None}) == 1, name
+    assert f(logits=258) == 4 and f(ids=258) == 4 and f(grad=257) == 4 and f(d_loss=2) == 4 and f(workspace=128) == 4
+    assert f(workspace_bytes=n.value - 1) == 6
 
 
 def _desc(**kw):
