@@ -136,7 +136,7 @@ extern "C" LATENT_API int latent_adapter_workspace_size(const latent_adapter_des
     const int st = latent::ad_validate(d);
     if (st) return st;
     if (!bytes) return LATENT_ERR_INVALID;
-    *bytes = ((size_t)d->n_tokens * d->rank * 4 + 511) / 256 * 256;
+    *bytes = latent::adapter_t_bytes(d->n_tokens, d->rank) + latent::adapter_flag_bytes(d->n_tokens, d->n_adapter, d->rank) + 256;
     return LATENT_OK;
 }
 
@@ -166,12 +166,21 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         if (cudaGetDevice(&dev) != cudaSuccess ||
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return LATENT_ERR_CUDA;
-        const AdapterArgs a{*d, tt, d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows,
-                            d->rank == 16 ? 4 : d->rank == 32 ? 5 : d->rank == 64 ? 6 : 7};
-        const bool wide = d->y_type == d->type && d->n_tokens > 256;
+        AdapterArgs a{};
+        a.d = *d;
+        a.t = tt;
+        a.tile_rows = d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows;
+        a.log2r = d->rank == 16 ? 4 : d->rank == 32 ? 5 : d->rank == 64 ? 6 : 7;
+        a.most = adapter_most(d->n_tokens, d->n_adapter, d->rank);
+        a.flags = reinterpret_cast<uint64_t *>(static_cast<char *>(d->workspace) + adapter_t_bytes(d->n_tokens, d->rank));
         CUtensorMap x;
-        if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows) ||
-            launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
+        if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows))
+            return LATENT_ERR_CUDA;
+        cudaError_t err;
+        if (d->n_tokens <= adapter::kRows && launch_adapter_decode(a, &x, sms, s, &err))
+            return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+        const bool wide = d->y_type == d->type && d->n_tokens > 256;
+        if (launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
             (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, s)) != cudaSuccess)
             return LATENT_ERR_CUDA;
         return LATENT_OK;

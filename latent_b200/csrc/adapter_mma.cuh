@@ -19,12 +19,29 @@ namespace latent {
 
 struct AdapterArgs {
     latent_adapter_desc d;
-    float *t;        // [T][rank] scale * x.A (fp32)
+    float *t;        // [T][rank] x.A (fp32)
     int tile_rows;   // rows per tile: 128, fewer rounded up to 16
     int log2r;       // rank = 1 << log2r
+    // k_ad_skinny's one-launch form
+    uint64_t *flags; // [blocks][tiles of stacked rank columns][cluster]
+    uint64_t nonce;  // what a flag holds once its partial sums are there
+    int most;        // tiles of stacked rank columns at most
 };
 
+// Workspace: t, then the flags of the one-launch form, which serves one tile of rows.
+constexpr int kMaxCluster = 16, kMaxBlocks = 256;
+inline size_t adapter_t_bytes(int64_t T, int rank) { return (T * rank * 4 + 255) / 256 * 256; }
+inline int adapter_most(int64_t T, int n_adapter, int rank) {
+    return (int)(((int64_t)(n_adapter < T ? n_adapter : T) * rank + 127) / 128);
+}
+inline size_t adapter_flag_bytes(int64_t T, int n_adapter, int rank) {
+    return T <= 128 ? (size_t)kMaxBlocks * kMaxCluster * 8 * adapter_most(T, n_adapter, rank) : 0;
+}
+
+
 // x_map: the CUtensorMap of x with a box of tile_rows rows.
+// One launch for both steps; false where it does not serve the call (*err then untouched).
+bool launch_adapter_decode(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s, cudaError_t *err);
 cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
 cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
 cudaError_t launch_adapter_wide(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
@@ -181,9 +198,10 @@ constexpr int kExt = 32;
 // 128B-swizzled tiles: t where the row's own segment lies, zeros elsewhere.  A
 // 128-byte row holds two parts of the 32 values (a third goes to a second
 // tile, tile_bytes further); what a part that is not finite leaves is zero.
+// `t`: the row's x.A, taken times scale.
 template <bool BF, int PARTS>
 __device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t tile_bytes, int row, int seg, int rank, int log2r,
-                                            const float *t, int r0) {
+                                            const float *t, float scale, int r0) {
     float4 v[8];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {  // all loads first: one trip to L2
@@ -192,6 +210,13 @@ __device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t tile_bytes, 
         const float4 *p = reinterpret_cast<const float4 *>(t + (r & (rank - 1)));
         v[2 * c] = mine ? __ldcg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
         v[2 * c + 1] = mine ? __ldcg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i].x *= scale;
+        v[i].y *= scale;
+        v[i].z *= scale;
+        v[i].w *= scale;
     }
 #pragma unroll
     for (int p = 0; p < PARTS; ++p)
@@ -221,20 +246,23 @@ __device__ __forceinline__ uint32_t t_offset(int p, int kk, uint32_t tile_bytes)
 
 // fp16 parts reach 65504.  A row whose t goes further (or is not a number)
 // enters the tile as zeros and is finished in fp32 by the epilogue.
-__device__ __forceinline__ bool beyond_f16(const float *t, int rank) {
+__device__ __forceinline__ bool beyond_f16(const float *t, float scale, int rank) {
     bool in = true;
     for (int r = 0; r < rank; r += 4) {
         const float4 u = __ldcg(reinterpret_cast<const float4 *>(t + r));
-        in = in && fabsf(u.x) <= 65504.f && fabsf(u.y) <= 65504.f && fabsf(u.z) <= 65504.f && fabsf(u.w) <= 65504.f;
+        in = in && fabsf(u.x * scale) <= 65504.f && fabsf(u.y * scale) <= 65504.f && fabsf(u.z * scale) <= 65504.f &&
+             fabsf(u.w * scale) <= 65504.f;
     }
     return !in;
 }
 
+// The adapter's part of y in column n, in fp32.
 template <bool BF>
 __device__ __forceinline__ float adapter_dot(const latent_adapter_desc &d, const float *t, int a, int n) {
     float s = 0.f;
+    const float scale = __ldg(d.scale + a);
     const int64_t row = (int64_t)a * d.rank;
-    for (int r = 0; r < d.rank; ++r) s = fmaf(__ldcg(t + r), load16<BF>(d.b, (row + r) * d.ldb + n), s);
+    for (int r = 0; r < d.rank; ++r) s = fmaf(__ldcg(t + r) * scale, load16<BF>(d.b, (row + r) * d.ldb + n), s);
     return s;
 }
 

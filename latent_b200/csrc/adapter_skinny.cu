@@ -15,7 +15,11 @@
 // only before the extension blocks.
 #include <cuda.h>
 
+#include <atomic>
+#include <chrono>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "adapter_mma.cuh"
 
@@ -30,7 +34,7 @@ constexpr int kMaxStages = 12;
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2], t_full[2], t_empty[2], seg;
+    uint64_t acc_full[2], acc_empty[2], t_full[2], t_empty[2], seg, sent;
     uint32_t tmem;
     volatile int abort;
     uint8_t wide[kRows];   // fp16: rows finished in fp32
@@ -43,6 +47,7 @@ struct Plan {
     int rows;       // N of the MMA: rows of x per tile, a multiple of 16
     int stages;
     int chunk;      // blocks per accumulator (k_ad_skinny)
+    int shrink_col; // x.A's accumulator behind the product's (one-launch form)
     uint32_t cols;  // TMEM columns
     size_t smem;
 };
@@ -79,7 +84,7 @@ __device__ __forceinline__ void drain() {
 // Barriers by warp 0, which goes on at once (its first loads wait for nobody),
 // TMEM by warp 2, which then lets a dependent kernel start.
 template <bool DEPENDENTS>
-__device__ __forceinline__ void setup(Shared &sh, const Plan &p, int warp, int lane) {
+__device__ __forceinline__ void setup(Shared &sh, const Plan &p, int cluster, int warp, int lane) {
     if (warp == 0) {
         if (lane == 0) {
             for (int s = 0; s < p.stages; ++s) {
@@ -93,6 +98,7 @@ __device__ __forceinline__ void setup(Shared &sh, const Plan &p, int warp, int l
                 mbar_init(sh.t_empty + b, 1);
             }
             mbar_init(&sh.seg, 128);
+            mbar_init(&sh.sent, (uint32_t)cluster * 4u);  // the four epilogue warps of every rank
             sh.abort = 0;
             fence_barrier_init();
         }
@@ -138,6 +144,11 @@ __device__ __forceinline__ void set_dest(Shared &sh, const float *recv, int r, i
     sh.dest[r] = r < nt ? map_rank(smem_addr(recv) + (uint32_t)(q * per + r % per) * row_bytes, r / per) : kNoRow;
 }
 
+__device__ __forceinline__ void arrive_rank(uint64_t *bar, int rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_addr(bar), rank))
+                 : "memory");
+}
+
 // x.A.  Block (cluster rank, slot, row tile); the stacked rank columns of the
 // tile's adapters in tiles of 128: slot, slot + gridDim.y, ...  Rank q of the
 // cluster sums K blocks of its share; every block sends the t of a row to the
@@ -166,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         const int r = threadIdx.x - 128;
         a = row_adapter(d, t0 + r, r < nt, q == 0 && blockIdx.y == 0);
     }
-    setup<true>(sh, p, warp, lane);
+    setup<true>(sh, p, CS, warp, lane);
     const uint32_t tmem = warp ? sh.tmem : 0u, read = (uint32_t)(p.rows + 31) & ~31u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
@@ -254,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     if (warp < 4) cluster_wait();
     cluster_arrive();
     cluster_wait();
-    // this block's rows: t[row][j] = scale * sum over the cluster, in rank order
+    // this block's rows: t[row][j] = sum over the cluster, in rank order
     const int r0 = q * per, r1 = min(nt, r0 + per);
     for (int i = threadIdx.x; i < (r1 - r0) << log2r; i += kThreads) {
         const int r = i >> log2r, s = sh.segs.row[r0 + r];
@@ -262,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         if (s < 0 || ((uint32_t)(s << log2r) / 128u) % gridDim.y != blockIdx.y) continue;
         float v = 0.f;
         for (int c = 0; c < CS; ++c) v += recv[((c * per) << log2r) + i];
-        g.t[((int64_t)(t0 + r0) << log2r) + i] = v * __ldg(d.scale + sh.segs.id[s]);
+        g.t[((int64_t)(t0 + r0) << log2r) + i] = v;
     }
     tc_fence_before();
     __syncthreads();
@@ -270,11 +281,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     if (warp == 2) tmem_dealloc(tmem, p.cols);
 }
 
+__device__ __forceinline__ void st_release(uint64_t *p, uint64_t v) {
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint64_t ld_acquire(const uint64_t *p) {
+    uint64_t v;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+    return v;
+}
+
 // The product.  Block (cluster rank, 128 output columns, row tile).
-template <bool BF, bool KN, int PARTS, typename Y>
+//
+// ONE (one launch for both steps, one tile of rows, a cooperative launch):
+// the x.A tiles of 128 stacked rank columns are dealt to the clusters, which
+// make theirs before they turn to W (sums over the ranks' parts of K by the
+// rows' owners, as above).  A block that has stored its rows of a tile sets a
+// flag for every block of the grid (its own copy: [reader][tile][rank]); a
+// reader waits for all
+// flags of the call and clears them, so that the words are ready for the next
+// replay of a captured launch.  A flag is set to the call's nonce, 64 bits that
+// no call before it used: whatever the workspace holds at first, nothing has to
+// be cleared by a launch of its own.
+template <bool BF, bool KN, int PARTS, typename Y, bool ONE>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant__ CUtensorMap mW,
                                                            const __grid_constant__ CUtensorMap mB,
-                                                           const __grid_constant__ CUtensorMap mX, AdapterArgs g,
+                                                           const __grid_constant__ CUtensorMap mX,
+                                                           const __grid_constant__ CUtensorMap mA, AdapterArgs g,
                                                            Plan p) {
     constexpr uint32_t kTiles = (PARTS + 1) / 2;
     extern __shared__ uint8_t raw[];
@@ -294,21 +326,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         prefetch_tensormap(&mW);
         prefetch_tensormap(&mX);
         prefetch_tensormap(&mB);
+        if (ONE) prefetch_tensormap(&mA);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
-        a = row_adapter(d, t0 + r, r < nt, false);
+        a = row_adapter(d, t0 + r, r < nt, ONE && q == 0 && blockIdx.y == 0);
     }
-    setup<false>(sh, p, warp, lane);
+    setup<false>(sh, p, CS, warp, lane);
     const uint32_t tmem = warp ? sh.tmem : 0u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
+    const int slot = blockIdx.y, slots = gridDim.y;
+    const bool shrinks = ONE && slot < g.most;  // this cluster may have tiles of x.A
     bool ok = true;
     if (warp == 0) {
         Ring at;
-        for (int k = k0; k < k1 && ok; ++k, at.next(p.stages)) {
+        // the ring's next slot, free; all lanes or none
+        auto next_slot = [&]() {
             if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
-            if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+            return ok = __all_sync(0xffffffffu, ok);
+        };
+        if (shrinks) {
+            ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
+            const int total = ok ? sh.segs.n * rank : 0;
+            for (int m = slot * 128; m < total && ok; m += slots * 128) {
+                const int cols = min(128, total - m), boxes = cols >> log2r;
+                int row = 0;
+                if (lane < boxes) row = sh.segs.id[(m >> log2r) + lane] << log2r;
+                for (int k = k0; k < k1 && next_slot(); ++k, at.next(p.stages)) {
+                    uint8_t *st = ring + at.s * stage;
+                    if (lane == 31) {
+                        mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(cols + p.rows) * 128u);
+                        tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
+                    }
+                    if (lane < boxes) tma_load_2d(st + ((uint32_t)lane << log2r) * 128u, &mA, k * kBK, row, sh.full + at.s);
+                }
+            }
+        }
+        for (int k = k0; ok && k < k1 && next_slot(); ++k, at.next(p.stages)) {
             uint8_t *st = ring + at.s * stage;
             if (lane == 0) {
                 mbar_arrive_expect_tx(sh.full + at.s, stage);
@@ -324,9 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         if (ok) {
             const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
             const int e1 = (int)((int64_t)ne * (q + 1) / CS), box = min(rank, kExt);
-            for (int e = (int)((int64_t)ne * q / CS); e < e1; ++e, at.next(p.stages)) {
-                if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
-                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+            for (int e = (int)((int64_t)ne * q / CS); e < e1 && next_slot(); ++e, at.next(p.stages)) {
                 uint8_t *st = ring + at.s * stage;
                 const int rows = min(kExt, ext - e * kExt), j = (lane >> 1) * box;
                 if (lane == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 256u);
@@ -341,9 +394,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     } else if (warp == 1 && lane == 0) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
         Ring at;
+        if (shrinks) {
+            ok = wait(&sh.seg, 0u);
+            const int total = ok ? sh.segs.n * rank : 0;
+            const uint32_t ids = idesc(BF, p.rows, false, false), acc = tmem + (uint32_t)p.shrink_col;
+            uint32_t n = 0;
+            for (int m = slot * 128; m < total && ok; m += slots * 128, ++n) {
+                if (n >= 1 && !wait(sh.acc_empty + 1, (n - 1u) & 1u)) { ok = false; break; }
+                tc_fence_after();
+                for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+                    if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_f16(acc, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), ids, (k > k0) | kk);
+                    mma_commit(sh.empty + at.s);
+                }
+                if (ok) mma_commit(sh.acc_full + 1);
+            }
+        }
         int in_chunk = 0;
         uint32_t acc = tmem;
-        for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+        for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
             if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
             tc_fence_after();
             const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
@@ -380,6 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 mma_commit(sh.t_empty + b);
             }
         }
+        if (!ok && ONE) mma_commit(sh.acc_full + 1);
         mma_commit(sh.acc_full);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
@@ -387,28 +461,83 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         set_dest(sh, recv, r, nt, per, q, 512u);
         mbar_arrive(&sh.seg);
         ok = wait(&sh.seg, 0u);
-        const int seg = sh.segs.row[r];
         const int ext = ok ? sh.segs.n * rank : 0, ne = (ext + kExt - 1) / kExt;
+        if constexpr (ONE) {
+            // From here to the flags all 128 threads go on or none: the named barrier has no limit of its own.
+            const int tiles = (ext + 127) / 128, own0 = q * per, own = max(0, min(nt, own0 + per) - own0);
+            uint32_t n = 0;
+            cluster_wait();
+            for (int m = slot * 128; m < ext; m += slots * 128, ++n) {
+                ok = ok && wait(sh.acc_full + 1, n & 1u) && !sh.abort;
+                if (!bar_all(1, kRows, ok)) { ok = false; break; }
+                tc_fence_after();
+                const int seg = (m + r) >> log2r;
+                const uint32_t j = (uint32_t)(m + r) & (uint32_t)(rank - 1);
+                for (int c = 0; c < p.rows; c += 32) {
+                    uint32_t v[32], to[32], of[32];
+                    __syncwarp();
+                    tmem_ld32(tmem + (uint32_t)p.shrink_col + ((uint32_t)(r & ~31) << 16) + (uint32_t)c, v);
+                    load32(sh.dest + c, to);
+                    load32(sh.segs.row + c, of);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if ((int)of[i] == seg) st_cluster(to[i] + j * 4u, __uint_as_float(v[i]));
+                }
+                tc_fence_before();
+                mbar_arrive(sh.acc_empty + 1);
+                __syncwarp();
+                if (lane < CS) arrive_rank(&sh.sent, lane);
+                ok = wait<true>(&sh.sent, n & 1u) && !sh.abort;
+                if (!bar_all(1, kRows, ok)) { ok = false; break; }
+                for (int i = r; i < own << log2r; i += kRows) {
+                    const int row = i >> log2r, s = sh.segs.row[own0 + row];
+                    if (s < 0 || (s << log2r) < m || (s << log2r) >= m + 128) continue;
+                    float v = 0.f;
+                    for (int c = 0; c < CS; ++c) v += recv[(c * per + row) * 128 + (i & (rank - 1))];
+                    g.t[((int64_t)(t0 + own0) << log2r) + i] = v;
+                }
+                bar_sync(1, kRows);  // all stores of the block, before the flags that release them
+                for (int i = r; i < slots * CS; i += kRows)
+                    st_release(g.flags + ((int64_t)i * g.most + m / 128) * CS + q, g.nonce);
+            }
+            uint64_t *mine = g.flags + (int64_t)(slot * CS + q) * g.most * CS;
+            const unsigned long long since = global_ns();
+            for (int i = r; i < tiles * CS && ok; i += kRows) {
+                while (ld_acquire(mine + i) != g.nonce) {
+                    if (sh.abort || global_ns() - since > kWaitNs) {
+                        ok = false;
+                        break;
+                    }
+                }
+                if (ok) mine[i] = 0;
+            }
+            ok = bar_all(1, kRows, ok);
+        } else {
+            dependency_wait();
+        }
+        const int seg = ok ? sh.segs.row[r] : -1;
         const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
         const float *t = g.t + ((int64_t)(t0 + r) << log2r);
-        dependency_wait();
-        const bool wide = !BF && seg >= 0 && beyond_f16(t, rank);
+        const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
+        const bool wide = !BF && seg >= 0 && beyond_f16(t, scale, rank);
         sh.wide[r] = wide;
-        for (int e = e0; e < e1; ++e) {
+        for (int e = e0; e < e1 && ok; ++e) {
             const int b = (e - e0) & 1;
             if (e - e0 >= 2 && !wait(sh.t_empty + b, (uint32_t)((e - e0) / 2 - 1) & 1u)) { ok = false; break; }
             if (sh.abort) { ok = false; break; }
             if (r < p.rows)
                 build_t_row<BF, PARTS>(tbuf + (uint32_t)b * kTiles * xbytes, xbytes, r, wide ? -1 : seg, rank, log2r, t,
-                                       e * kExt);
+                                       scale, e * kExt);
             fence_async_shared();
             mbar_arrive(sh.t_full + b);
         }
+        if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
         __syncwarp();
         if (!wait(sh.acc_full, 0u)) ok = false;
         __syncwarp();
         tc_fence_after();
-        cluster_wait();
+        if (!ONE) cluster_wait();
         // column c of the accumulator = row c of x, to its owner
         const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
         for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
@@ -487,21 +616,36 @@ uint32_t tmem_cols(int n) {
     return c;
 }
 
-// Dynamic shared memory of a block beside the static: all of an SM's, or half.  A block's share of the shared memory is at least its share of
-// the 512 TMEM columns, so that whatever blocks an SM holds, of whichever calls
-// and streams, no TMEM allocation waits: blocks of two clusters that wait for
-// each other's columns would never end.
-constexpr size_t kSmemWhole = 227 * 1024 - sizeof(Shared);
-constexpr size_t kSmemHalf = 113 * 1024 - sizeof(Shared);
+// Dynamic shared memory of a block beside the static.  An SM holds one block of
+// these kernels (what the occupancy calculator gives for every kernel here that
+// allocates TMEM, however small).  Should blocks of two calls share an SM all
+// the same, no TMEM allocation may wait: blocks of two clusters that wait for
+// each other's columns would never end.  So a block's share of the shared
+// memory is at least its share of the 512 columns.
+constexpr size_t kSmemMost = 227 * 1024 - sizeof(Shared);
 size_t smem_of(size_t used, uint32_t cols) {
     const size_t share = (size_t)cols * 228 * 1024 / 512 - 1024 - sizeof(Shared);  // of 228 KB; 1 KB goes to the system
     return used < share ? share : used;
 }
 
-cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, int cluster, bool dependent, void **args,
-                           cudaStream_t s) {
-    cudaError_t err = ensure_smem(fn, smem);
+// Clusters of more than 8 blocks, once per kernel and device.
+cudaError_t allow_clusters(const void *fn) {
+    static std::mutex mu;
+    static std::set<std::pair<const void *, int>> done;
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    std::lock_guard<std::mutex> lock(mu);
+    if (done.count({fn, dev})) return cudaSuccess;
+    err = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err == cudaSuccess) done.insert({fn, dev});
+    return err;
+}
+
+enum Launch { kPlain, kDependent, kCooperative };
+cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, Launch how, void **args, cudaStream_t s) {
+    cudaError_t err = ensure_smem(fn, smem);
+    if (err != cudaSuccess || (grid.x > 8 && (err = allow_clusters(fn)) != cudaSuccess)) return err;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
@@ -509,22 +653,28 @@ cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, int cluster, 
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.x = grid.x;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    if (how == kDependent) {
+        at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[1].val.programmaticStreamSerializationAllowed = 1;
+    } else {
+        at[1].id = cudaLaunchAttributeCooperative;
+        at[1].val.cooperative = 1;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = dependent ? 2 : 1;
+    cfg.numAttrs = how == kPlain ? 1 : 2;
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-// Clusters of 1..8 blocks that the device holds at once with one block per SM
-// (a cluster stays within a GPC: 15 of 8, 22 of 6, 33 of 4 on the 148 SMs).
+// Clusters of 1..16 blocks that the device holds at once, one block per SM (a
+// cluster stays within a GPC: 7 of 16, 15 of 9, 22 of 6, 33 of 4 on 148 SMs).
+// More than 8 are not portable to every device; the kernels ask for them.
 const int *cluster_room() {
     struct Table {
         bool set = false;
-        int n[9];
+        int n[kMaxCluster + 1];
     };
     static std::mutex mu;
     static Table tables[64];
@@ -534,12 +684,12 @@ const int *cluster_room() {
     Table &t = tables[dev];
     if (!t.set) {
         const void *fn = (const void *)k_ad_shrink<true>;
-        if (ensure_smem(fn, kSmemWhole) != cudaSuccess) return nullptr;
-        for (int c = 1; c <= 8; ++c) {
+        if (ensure_smem(fn, kSmemMost) != cudaSuccess || allow_clusters(fn) != cudaSuccess) return nullptr;
+        for (int c = 1; c <= kMaxCluster; ++c) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(c, 256);
             cfg.blockDim = dim3(kThreads);
-            cfg.dynamicSmemBytes = kSmemWhole;
+            cfg.dynamicSmemBytes = kSmemMost;
             cudaLaunchAttribute at[1];
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = (unsigned)c;
@@ -554,10 +704,10 @@ const int *cluster_room() {
 }
 
 // Blocks of a cluster for `others` clusters: as many as the contraction has
-// blocks for and as run at once (half: two blocks may share an SM).
-int pick_cluster(int64_t others, int blocks, int sms, const int *room, bool half) {
-    int c = blocks < 8 ? blocks : 8;
-    while (c > 1 && (others * c > sms || others > (half ? 2 : 1) * room[c])) --c;
+// blocks for and as run at once.
+int pick_cluster(int64_t others, int blocks, const int *room) {
+    int c = blocks < kMaxCluster ? blocks : kMaxCluster;
+    while (c > 1 && others > room[c]) --c;
     return c;
 }
 
@@ -566,20 +716,33 @@ size_t recv_bytes(int tile_rows, int cluster, int row) {
     return (size_t)cluster * ((tile_rows + cluster - 1) / cluster) * row;
 }
 
-// Stages beside `other` bytes of shared memory.
-int pick_stages(size_t limit, size_t stage, size_t other) {
-    if (limit < 1024 + other + stage) return 0;
-    const int n = (int)((limit - 1024 - other) / stage);
-    return n < kMaxStages ? n : kMaxStages;
+// Stages beside `other` bytes of shared memory, no more than there are loads.
+int pick_stages(size_t stage, size_t other, int loads) {
+    int n = (int)((kSmemMost - 1024 - other) / stage);
+    if (n > kMaxStages) n = kMaxStages;
+    return n < loads ? n : loads;
 }
 
-template <typename Y>
+template <typename Y, bool ONE>
 const void *skinny_fn(bool bf, bool kn, int parts) {
     if (bf) {
-        if (parts == 3) return kn ? (const void *)k_ad_skinny<true, true, 3, Y> : (const void *)k_ad_skinny<true, false, 3, Y>;
-        return kn ? (const void *)k_ad_skinny<true, true, 2, Y> : (const void *)k_ad_skinny<true, false, 2, Y>;
+        if constexpr (sizeof(Y) == 4)
+            return kn ? (const void *)k_ad_skinny<true, true, 3, Y, ONE> : (const void *)k_ad_skinny<true, false, 3, Y, ONE>;
+        else
+            return kn ? (const void *)k_ad_skinny<true, true, 2, Y, ONE> : (const void *)k_ad_skinny<true, false, 2, Y, ONE>;
     }
-    return kn ? (const void *)k_ad_skinny<false, true, 2, Y> : (const void *)k_ad_skinny<false, false, 2, Y>;
+    return kn ? (const void *)k_ad_skinny<false, true, 2, Y, ONE> : (const void *)k_ad_skinny<false, false, 2, Y, ONE>;
+}
+
+// 64 bits that no call of this process used before.
+uint64_t next_nonce() {
+    static std::atomic<uint64_t> count{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() ^
+                                       (uint64_t)(uintptr_t)&count};
+    uint64_t z = count.fetch_add(0x9E3779B97F4A7C15ull) + 0x9E3779B97F4A7C15ull;  // splitmix64: a bijection of the count
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z ^= z >> 31;
+    return z ? z : 1;
 }
 
 }  // namespace
@@ -607,18 +770,12 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int s
     p.rows = (g.tile_rows + 15) / 16 * 16;
     const int *room = cluster_room();
     if (!room) return cudaErrorInvalidConfiguration;
-    // two blocks per SM where two stages fit into half of its shared memory
     const size_t stage = 16384 + (size_t)p.rows * 128;
-    size_t recv = recv_bytes(g.tile_rows, 8, d.rank * 4);
-    const bool half = pick_stages(kSmemHalf, stage, recv) >= 2;
-    const int cluster = pick_cluster(tiles, nk, sms, room, half);
-    recv = recv_bytes(g.tile_rows, cluster, d.rank * 4);
+    const int cluster = pick_cluster(tiles, nk, room);
+    const size_t recv = recv_bytes(g.tile_rows, cluster, d.rank * 4);
     int slots = sms / (tiles * cluster);  // tiles of stacked rank columns side by side
     slots = slots < 1 ? 1 : slots > most ? most : slots;
-    const int loads = (nk + cluster - 1) / cluster * ((most + slots - 1) / slots);
-    p.stages = pick_stages(half ? kSmemHalf : kSmemWhole, stage, recv);
-    if (p.stages > loads) p.stages = loads;
-    if (p.stages < 1) return cudaErrorInvalidConfiguration;
+    p.stages = pick_stages(stage, recv, (nk + cluster - 1) / cluster * ((most + slots - 1) / slots));
     p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
     p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
     CUtensorMap mA;
@@ -626,10 +783,14 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int s
     AdapterArgs a = g;
     void *args[] = {&mA, const_cast<void *>(x_map), &a, &p};
     return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
-                          dim3(cluster, slots, tiles), p.smem, cluster, false, args, s);
+                          dim3(cluster, slots, tiles), p.smem, kPlain, args, s);
 }
 
-cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
+namespace {
+
+// One launch (one: with x.A in it) of k_ad_skinny; false, with nothing launched, where a cooperative
+// launch would not fit the device.
+bool launch_skinny(const AdapterArgs &g, const void *x_map, int sms, bool one, cudaStream_t s, cudaError_t *err) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
     const bool f32 = d.y_type == LATENT_TYPE_F32;
@@ -638,38 +799,56 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
     const int parts = bf && f32 ? 3 : 2;
+    *err = cudaErrorInvalidConfiguration;
     const int *room = cluster_room();
-    if (!room) return cudaErrorInvalidConfiguration;
+    if (!room) return true;
     const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)((parts + 1) / 2) * p.rows * 128;
-    const bool half = pick_stages(kSmemHalf, stage, tb + recv_bytes(g.tile_rows, 8, 512)) >= 2;
-    int cluster = pick_cluster((int64_t)tiles * ntn, nk, sms, room, half);
+    int cluster = pick_cluster((int64_t)tiles * ntn, nk, room);
     // The tensor cores cut a sum off instead of rounding it: a chain over K
     // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
     // fp32 results therefore use an accumulator per 512 of K, added up in
-    // fp32, as far as the 512 TMEM columns go, and clusters long enough.
+    // fp32, as far as the TMEM columns go, and clusters long enough.
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    const int groups = ((half ? 256 : 512) - read) / p.rows + 1;
+    const int groups = (512 - (one ? 2 : 1) * read) / p.rows + 1;
     if (f32)
-        while (cluster < 8 && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
+        while (cluster < kMaxCluster && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
+    if (one && ((int64_t)tiles * ntn * cluster > kMaxBlocks || tiles * ntn > room[cluster])) return false;
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
-    p.cols = tmem_cols(((per + p.chunk - 1) / p.chunk - 1) * p.rows + read);
+    p.shrink_col = ((per + p.chunk - 1) / p.chunk - 1) * p.rows + read;
+    p.cols = tmem_cols(p.shrink_col + (one ? read : 0));
     const size_t recv = recv_bytes(g.tile_rows, cluster, 512);
-    p.stages = pick_stages(half ? kSmemHalf : kSmemWhole, stage, tb + recv);
-    if (p.stages > per + 4) p.stages = per + 4;
-    if (p.stages < 1) return cudaErrorInvalidConfiguration;
+    p.stages = pick_stages(stage, tb + recv, per * (one ? 2 : 1) + 4);
     p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
-    CUtensorMap mW, mB;
+    CUtensorMap mW, mB, mA{};
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
-        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
-                     d.rank < kExt ? d.rank : kExt))
-        return cudaErrorInvalidValue;
-    const void *fn = f32 ? skinny_fn<float>(bf, kn, parts)
-                         : bf ? skinny_fn<__nv_bfloat16>(bf, kn, parts) : skinny_fn<__half>(bf, kn, parts);
+        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, d.rank < kExt ? d.rank : kExt) ||
+        (one && !adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank))) {
+        *err = cudaErrorInvalidValue;
+        return true;
+    }
+    const void *fn = one ? f32 ? skinny_fn<float, true>(bf, kn, parts)
+                               : bf ? skinny_fn<__nv_bfloat16, true>(bf, kn, parts) : skinny_fn<__half, true>(bf, kn, parts)
+                         : f32 ? skinny_fn<float, false>(bf, kn, parts)
+                               : bf ? skinny_fn<__nv_bfloat16, false>(bf, kn, parts) : skinny_fn<__half, false>(bf, kn, parts);
     AdapterArgs a = g;
-    void *args[] = {&mW, &mB, const_cast<void *>(x_map), &a, &p};
-    return launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, cluster, true, args, s);
+    if (one) a.nonce = next_nonce();
+    void *args[] = {&mW, &mB, const_cast<void *>(x_map), &mA, &a, &p};
+    *err = launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, one ? kCooperative : kDependent, args, s);
+    return true;
+}
+
+}  // namespace
+
+cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
+    cudaError_t err;
+    launch_skinny(g, x_map, sms, false, s, &err);
+    return err;
+}
+
+bool launch_adapter_decode(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s, cudaError_t *err) {
+    return launch_skinny(g, x_map, sms, true, s, err);
 }
 
 }  // namespace latent

@@ -348,7 +348,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const int my = a[mine] >= 0 ? sh.first[lead[mine]] : -1;
             const int t = tile.t0 + mine * 128 + tid;
             const float *tp = g.t + (int64_t)t * rank;
-            const bool wide = !BF && my >= 0 && beyond_f16(tp, rank);
+            const float scale = my >= 0 ? __ldg(d.scale + a[mine]) : 0.f;
+            const bool wide = !BF && my >= 0 && beyond_f16(tp, scale, rank);
             seg.row[tid] = (int16_t)my;
             seg.wide[tid] = wide;
             const int ext = seg.n * rank;
@@ -356,7 +357,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             for (int r0 = 0; r0 < ext; r0 += kExt, ++eb) {  // a thread that gives up here is heard at the next tile
                 if (eb >= 2 && !wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
-                build_t_row<BF, kParts>(tbuf + (eb & 1) * kTTile, 0u, tid, wide ? -1 : my, rank, g.log2r, tp, r0);
+                build_t_row<BF, kParts>(tbuf + (eb & 1) * kTTile, 0u, tid, wide ? -1 : my, rank, g.log2r, tp,
+                                        scale, r0);
                 fence_async_shared();
                 arrive_cluster(peer_addr(sh.t_full + (eb & 1), 0));
             }

@@ -104,5 +104,6 @@ def test_adapter_set_layout():
     s = AdapterSet([(a, b, 0.5), (a[:, :3], b[:3])], device="cpu", dtype=torch.float16)
     assert s.rank == 32 and s.a.shape == (2, 32, 16) and s.b.shape == (2, 32, 16) and s.ranks == [17, 3]
     assert torch.equal(s.a[0, :17, :10], a.t().half()) and torch.equal(s.b[1, :3, :13], b[:3].half())
-    assert float(s.a.float().abs().sum()) == float(s.a[0, :17, :10].float().abs().sum() + s.a[1, :3, :10].float().abs().sum())
+    live = s.a[0, :17, :10].double().abs().sum() + s.a[1, :3, :10].double().abs().sum()
+    assert float((s.a.double().abs().sum() - live).abs()) <= 1e-9 * float(live)
     assert s.scale.tolist() == [0.5, 1.0]
