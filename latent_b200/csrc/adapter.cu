@@ -177,11 +177,11 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows))
             return LATENT_ERR_CUDA;
         cudaError_t err;
-        if (d->n_tokens <= adapter::kRows && launch_adapter_decode(a, &x, sms, s, &err))
+        if (d->n_tokens <= adapter::kRows && launch_adapter_decode(a, &x, s, &err))
             return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
         const bool wide = d->y_type == d->type && d->n_tokens > 256;
         if (launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
-            (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, s)) != cudaSuccess)
+            (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, s)) != cudaSuccess)
             return LATENT_ERR_CUDA;
         return LATENT_OK;
     }

@@ -41,9 +41,9 @@ inline size_t adapter_flag_bytes(int64_t T, int n_adapter, int rank) {
 
 // x_map: the CUtensorMap of x with a box of tile_rows rows.
 // One launch for both steps; false where it does not serve the call (*err then untouched).
-bool launch_adapter_decode(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s, cudaError_t *err);
+bool launch_adapter_decode(const AdapterArgs &a, const void *x_map, cudaStream_t s, cudaError_t *err);
 cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
-cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
+cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, cudaStream_t s);
 cudaError_t launch_adapter_wide(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
 
 namespace adapter {
@@ -198,19 +198,21 @@ constexpr int kExt = 32;
 // 128B-swizzled tiles: t where the row's own segment lies, zeros elsewhere.  A
 // 128-byte row holds two parts of the 32 values (a third goes to a second
 // tile, tile_bytes further); what a part that is not finite leaves is zero.
-// `t`: the row's x.A, taken times scale.
-template <bool BF, int PARTS>
-__device__ __forceinline__ void build_t_row(uint8_t *tile, uint32_t tile_bytes, int row, int seg, int rank, int log2r,
-                                            const float *t, float scale, int r0) {
-    float4 v[8];
+// `t`: the row's x.A, taken times scale.  load_t_row fetches (one trip to L2,
+// which the caller lets run under the block before), store_t_row writes.
+__device__ __forceinline__ void load_t_row(float4 (&v)[8], int seg, int rank, int log2r, const float *t, int r0) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {  // all loads first: one trip to L2
+    for (int c = 0; c < 4; ++c) {
         const int r = r0 + 8 * c;
         const bool mine = seg >= 0 && (r >> log2r) == seg;
         const float4 *p = reinterpret_cast<const float4 *>(t + (r & (rank - 1)));
         v[2 * c] = mine ? __ldcg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
         v[2 * c + 1] = mine ? __ldcg(p + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+}
+
+template <bool BF, int PARTS>
+__device__ __forceinline__ void store_t_row(float4 (&v)[8], uint8_t *tile, uint32_t tile_bytes, int row, float scale) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         v[i].x *= scale;

@@ -31,10 +31,11 @@ using namespace adapter;
 
 constexpr int kThreads = 256;  // warp 0: TMA, 1: MMA, 2: TMEM, 4..7: rows (segments, x.A parts, epilogue)
 constexpr int kMaxStages = 12;
+constexpr int kMaxTBufs = 4;
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2], t_full[2], t_empty[2], seg, sent;
+    uint64_t acc_full[2], acc_empty[2], t_full[kMaxTBufs], t_empty[kMaxTBufs], seg, sent;
     uint32_t tmem;
     volatile int abort;
     uint8_t wide[kRows];   // fp16: rows finished in fp32
@@ -47,6 +48,7 @@ struct Plan {
     int rows;       // N of the MMA: rows of x per tile, a multiple of 16
     int stages;
     int chunk;      // blocks per accumulator (k_ad_skinny)
+    int tbufs;      // tiles of x.A parts
     int shrink_col; // x.A's accumulator behind the product's (one-launch form)
     uint32_t cols;  // TMEM columns
     size_t smem;
@@ -94,6 +96,8 @@ __device__ __forceinline__ void setup(Shared &sh, const Plan &p, int cluster, in
             for (int b = 0; b < 2; ++b) {
                 mbar_init(sh.acc_full + b, 1);
                 mbar_init(sh.acc_empty + b, 128);
+            }
+            for (int b = 0; b < kMaxTBufs; ++b) {
                 mbar_init(sh.t_full + b, 128);
                 mbar_init(sh.t_empty + b, 1);
             }
@@ -292,7 +296,12 @@ __device__ __forceinline__ uint64_t ld_acquire(const uint64_t *p) {
 
 // The product.  Block (cluster rank, 128 output columns, row tile).
 //
-// ONE (one launch for both steps, one tile of rows, a cooperative launch):
+// kSelf (one launch, one tile of rows): every cluster makes all of x.A itself,
+// behind its W loads, and the owner of a row adds x.A.B for its 128 columns on
+// the CUDA cores: no trip of x.A through global memory, at the price of every
+// cluster loading the adapters' A.
+//
+// kOne (one launch for both steps, one tile of rows, a cooperative launch):
 // the x.A tiles of 128 stacked rank columns are dealt to the clusters, which
 // make theirs before they turn to W (sums over the ranks' parts of K by the
 // rows' owners, as above).  A block that has stored its rows of a tile sets a
@@ -302,42 +311,47 @@ __device__ __forceinline__ uint64_t ld_acquire(const uint64_t *p) {
 // replay of a captured launch.  A flag is set to the call's nonce, 64 bits that
 // no call before it used: whatever the workspace holds at first, nothing has to
 // be cleared by a launch of its own.
-template <bool BF, bool KN, int PARTS, typename Y, bool ONE>
+enum Mode { kTwo, kOne, kSelf };
+
+template <bool BF, bool KN, int PARTS, typename Y, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant__ CUtensorMap mW,
                                                            const __grid_constant__ CUtensorMap mB,
                                                            const __grid_constant__ CUtensorMap mX,
                                                            const __grid_constant__ CUtensorMap mA, AdapterArgs g,
                                                            Plan p) {
     constexpr uint32_t kTiles = (PARTS + 1) / 2;
+    constexpr bool ONE = MODE == kOne, SELF = MODE == kSelf;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = align1024(raw);
     const uint32_t xbytes = (uint32_t)p.rows * 128u, stage = 16384u + xbytes;
-    uint8_t *tbuf = ring + p.stages * stage;                                      // 2 x kTiles x [rows][128 bytes]
-    float *recv = reinterpret_cast<float *>(tbuf + 2 * kTiles * xbytes);          // [cluster][rows of a rank][128]
+    uint8_t *tbuf = ring + p.stages * stage;                                      // tbufs x kTiles x [rows][128 bytes]
+    // [cluster][rows of a rank][128 sums, kSelf: and those of x.A]
+    float *recv = reinterpret_cast<float *>(tbuf + p.tbufs * kTiles * xbytes);
     __shared__ Shared sh;
     const int q = blockIdx.x, CS = gridDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int n0 = blockIdx.y * 128, t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
     const int rank = d.rank, log2r = g.log2r;
+    const int pitch = SELF ? 128 + rank : 128;
     cluster_arrive();
     int a = -1;
     if (warp == 0 && lane == 0) {
         prefetch_tensormap(&mW);
         prefetch_tensormap(&mX);
         prefetch_tensormap(&mB);
-        if (ONE) prefetch_tensormap(&mA);
+        if (MODE != kTwo) prefetch_tensormap(&mA);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
-        a = row_adapter(d, t0 + r, r < nt, ONE && q == 0 && blockIdx.y == 0);
+        a = row_adapter(d, t0 + r, r < nt, MODE != kTwo && q == 0 && blockIdx.y == 0);
     }
     setup<false>(sh, p, CS, warp, lane);
     const uint32_t tmem = warp ? sh.tmem : 0u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
-    const int slot = blockIdx.y, slots = gridDim.y;
-    const bool shrinks = ONE && slot < g.most;  // this cluster may have tiles of x.A
+    const int slot = SELF ? 0 : blockIdx.y, slots = SELF ? 1 : gridDim.y;
+    const bool shrinks = SELF || (ONE && slot < g.most);  // this cluster may have tiles of x.A
     bool ok = true;
     if (warp == 0) {
         Ring at;
@@ -346,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
             return ok = __all_sync(0xffffffffu, ok);
         };
-        if (shrinks) {
+        auto load_a = [&]() {  // lane i loads the i-th adapter's run of stacked columns, the last one x
             ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
             const int total = ok ? sh.segs.n * rank : 0;
             for (int m = slot * 128; m < total && ok; m += slots * 128) {
@@ -362,7 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                     if (lane < boxes) tma_load_2d(st + ((uint32_t)lane << log2r) * 128u, &mA, k * kBK, row, sh.full + at.s);
                 }
             }
-        }
+        };
+        if (ONE && shrinks) load_a();
         for (int k = k0; ok && k < k1 && next_slot(); ++k, at.next(p.stages)) {
             uint8_t *st = ring + at.s * stage;
             if (lane == 0) {
@@ -375,8 +390,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
             }
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
-        if (ok) {
+        if (SELF && ok) load_a();
+        if (!SELF && ok) ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
+        if (!SELF && ok) {
             const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
             const int e1 = (int)((int64_t)ne * (q + 1) / CS), box = min(rank, kExt);
             for (int e = (int)((int64_t)ne * q / CS); e < e1 && next_slot(); ++e, at.next(p.stages)) {
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     } else if (warp == 1 && lane == 0) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
         Ring at;
-        if (shrinks) {
+        auto multiply_a = [&]() {
             ok = wait(&sh.seg, 0u);
             const int total = ok ? sh.segs.n * rank : 0;
             const uint32_t ids = idesc(BF, p.rows, false, false), acc = tmem + (uint32_t)p.shrink_col;
@@ -413,7 +429,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 }
                 if (ok) mma_commit(sh.acc_full + 1);
             }
-        }
+        };
+        if (ONE && shrinks) multiply_a();
         int in_chunk = 0;
         uint32_t acc = tmem;
         for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
@@ -431,13 +448,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             ++in_chunk;
             mma_commit(sh.empty + at.s);
         }
-        if (ok) ok = wait(&sh.seg, 0u);
-        if (ok) {
+        if (SELF) {
+            if (ok) mma_commit(sh.acc_full);
+            if (ok) multiply_a();
+        } else if (ok) {
+            ok = wait(&sh.seg, 0u);
+        }
+        if (!SELF && ok) {
             const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
             const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
-            for (int e = e0; e < e1; ++e, at.next(p.stages)) {
-                const int b = (e - e0) & 1;
-                if (!wait(sh.full + at.s, at.phase) || !wait(sh.t_full + b, (uint32_t)((e - e0) >> 1) & 1u) || sh.abort) {
+            Ring tb;
+            for (int e = e0; e < e1; ++e, at.next(p.stages), tb.next(p.tbufs)) {
+                const int b = tb.s;
+                if (!wait(sh.full + at.s, at.phase) || !wait(sh.t_full + b, tb.phase) || sh.abort) {
                     ok = false;
                     break;
                 }
@@ -453,15 +476,66 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 mma_commit(sh.t_empty + b);
             }
         }
-        if (!ok && ONE) mma_commit(sh.acc_full + 1);
-        mma_commit(sh.acc_full);
+        if (!ok && MODE != kTwo) mma_commit(sh.acc_full + 1);
+        if (!SELF || !ok) mma_commit(sh.acc_full);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
         build_segments(sh.segs, a, nt, r, 1);
-        set_dest(sh, recv, r, nt, per, q, 512u);
+        set_dest(sh, recv, r, nt, per, q, (uint32_t)pitch * 4u);
         mbar_arrive(&sh.seg);
         ok = wait(&sh.seg, 0u);
         const int ext = ok ? sh.segs.n * rank : 0, ne = (ext + kExt - 1) / kExt;
+        // x.A of the tile at stacked column m, column j of this lane's adapter, to the rows' owners, `off` bytes into a row
+        auto send_a = [&](int m, uint32_t off) {
+            const int seg = (m + r) >> log2r;
+            const uint32_t j = (uint32_t)(m + r) & (uint32_t)(rank - 1);
+            for (int c = 0; c < p.rows; c += 32) {
+                uint32_t v[32], to[32], of[32];
+                __syncwarp();
+                tmem_ld32(tmem + (uint32_t)p.shrink_col + ((uint32_t)(r & ~31) << 16) + (uint32_t)c, v);
+                load32(sh.dest + c, to);
+                load32(sh.segs.row + c, of);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if ((int)of[i] == seg) st_cluster(to[i] + off + j * 4u, __uint_as_float(v[i]));
+            }
+            tc_fence_before();
+            mbar_arrive(sh.acc_empty + 1);
+        };
+        // column c of the accumulator = row c of x, to its owner
+        auto send_product = [&]() {
+            const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
+            for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
+                float s[32];
+                uint32_t to[32];
+                load32(sh.dest + c, to);
+                for (int gr = 0; gr < groups; ++gr) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld32(tmem + ((uint32_t)(r & ~31) << 16) + (uint32_t)(gr * p.rows + c), v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) s[j] = gr ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (to[j] != kNoRow) st_cluster(to[j] + (uint32_t)r * 4u, s[j]);
+            }
+            tc_fence_before();
+        };
+        if constexpr (SELF) {
+            ok = __all_sync(0xffffffffu, wait(sh.acc_full, 0u) && !sh.abort);
+            tc_fence_after();
+            cluster_wait();
+            if (ok) send_product();
+            uint32_t n = 0;
+            for (int m = 0; m < ext && ok; m += 128, ++n) {
+                ok = __all_sync(0xffffffffu, wait(sh.acc_full + 1, n & 1u) && !sh.abort);
+                tc_fence_after();
+                if (ok) send_a(m, 512u);
+            }
+        }
         if constexpr (ONE) {
             // From here to the flags all 128 threads go on or none: the named barrier has no limit of its own.
             const int tiles = (ext + 127) / 128, own0 = q * per, own = max(0, min(nt, own0 + per) - own0);
@@ -471,21 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 ok = ok && wait(sh.acc_full + 1, n & 1u) && !sh.abort;
                 if (!bar_all(1, kRows, ok)) { ok = false; break; }
                 tc_fence_after();
-                const int seg = (m + r) >> log2r;
-                const uint32_t j = (uint32_t)(m + r) & (uint32_t)(rank - 1);
-                for (int c = 0; c < p.rows; c += 32) {
-                    uint32_t v[32], to[32], of[32];
-                    __syncwarp();
-                    tmem_ld32(tmem + (uint32_t)p.shrink_col + ((uint32_t)(r & ~31) << 16) + (uint32_t)c, v);
-                    load32(sh.dest + c, to);
-                    load32(sh.segs.row + c, of);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if ((int)of[i] == seg) st_cluster(to[i] + j * 4u, __uint_as_float(v[i]));
-                }
-                tc_fence_before();
-                mbar_arrive(sh.acc_empty + 1);
+                send_a(m, 0u);
                 __syncwarp();
                 if (lane < CS) arrive_rank(&sh.sent, lane);
                 ok = wait<true>(&sh.sent, n & 1u) && !sh.abort;
@@ -513,24 +573,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 if (ok) mine[i] = 0;
             }
             ok = bar_all(1, kRows, ok);
-        } else {
-            dependency_wait();
         }
+        if constexpr (!SELF) {
+        if (!ONE) dependency_wait();
         const int seg = ok ? sh.segs.row[r] : -1;
         const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
         const float *t = g.t + ((int64_t)(t0 + r) << log2r);
         const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
         const bool wide = !BF && seg >= 0 && beyond_f16(t, scale, rank);
         sh.wide[r] = wide;
-        for (int e = e0; e < e1 && ok; ++e) {
-            const int b = (e - e0) & 1;
-            if (e - e0 >= 2 && !wait(sh.t_empty + b, (uint32_t)((e - e0) / 2 - 1) & 1u)) { ok = false; break; }
+        const int live = wide ? -1 : seg;
+        float4 v[8];
+        if (e0 < e1) load_t_row(v, live, rank, log2r, t, e0 * kExt);
+        Ring tb;
+        for (int e = e0; e < e1 && ok; ++e, tb.next(p.tbufs)) {
+            const int b = tb.s;
+            if (tb.wrapped && !wait(sh.t_empty + b, tb.phase ^ 1u)) { ok = false; break; }
             if (sh.abort) { ok = false; break; }
-            if (r < p.rows)
-                build_t_row<BF, PARTS>(tbuf + (uint32_t)b * kTiles * xbytes, xbytes, r, wide ? -1 : seg, rank, log2r, t,
-                                       scale, e * kExt);
+            if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)b * kTiles * xbytes, xbytes, r, scale);
             fence_async_shared();
             mbar_arrive(sh.t_full + b);
+            if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
         }
         if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
         __syncwarp();
@@ -538,25 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         __syncwarp();
         tc_fence_after();
         if (!ONE) cluster_wait();
-        // column c of the accumulator = row c of x, to its owner
-        const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
-        for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
-            float s[32];
-            uint32_t to[32];
-            load32(sh.dest + c, to);
-            for (int gr = 0; gr < groups; ++gr) {
-                uint32_t v[32];
-                __syncwarp();
-                tmem_ld32(tmem + ((uint32_t)(r & ~31) << 16) + (uint32_t)(gr * p.rows + c), v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 32; ++j) s[j] = gr ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (to[j] != kNoRow) st_cluster(to[j] + (uint32_t)r * 4u, s[j]);
+        send_product();
         }
-        tc_fence_before();
     }
     if (!ok) {
         give_up(sh, d.err);
@@ -568,15 +614,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     cluster_wait();
     // this block's rows, two columns per thread: the cluster's parts in rank order
     const int r0 = q * per, r1 = min(nt, r0 + per);
+    float *own_t = reinterpret_cast<float *>(ring);  // kSelf: [row][rank] scale * x.A (the ring's loads have all been used)
+    if constexpr (SELF) {
+        for (int i = threadIdx.x; i < max(0, r1 - r0) << log2r; i += kThreads) {
+            const int row = i >> log2r, s = sh.segs.row[r0 + row];
+            float v = 0.f;
+            if (s >= 0) {
+                for (int c = 0; c < CS; ++c) v += recv[(c * per + row) * pitch + 128 + (i & (rank - 1))];
+                v *= __ldg(d.scale + sh.segs.id[s]);
+            }
+            own_t[i] = v;
+        }
+        __syncthreads();
+    }
     const int n = n0 + 2 * (threadIdx.x & 63);
     for (int r = r0 + (threadIdx.x >> 6); r < r1 && n < d.n_out; r += kThreads / 64) {
         float2 v = make_float2(0.f, 0.f);
         for (int c = 0; c < CS; ++c) {
-            const float2 u = *reinterpret_cast<const float2 *>(recv + (c * per + r - r0) * 128 + 2 * (threadIdx.x & 63));
+            const float2 u = *reinterpret_cast<const float2 *>(recv + (c * per + r - r0) * pitch + 2 * (threadIdx.x & 63));
             v.x += u.x;
             v.y += u.y;
         }
-        if (!BF && sh.wide[r]) {
+        if constexpr (SELF) {
+            const int s = sh.segs.row[r];
+            if (s >= 0) {
+                const uint16_t *b = static_cast<const uint16_t *>(d.b) + (((int64_t)sh.segs.id[s] << log2r) * d.ldb + n);
+                const float *t = own_t + ((r - r0) << log2r);
+#pragma unroll 16
+                for (int j = 0; j < rank; ++j) {
+                    const float2 u = unpack2<BF>(__ldg(reinterpret_cast<const uint32_t *>(b + j * d.ldb)));
+                    v.x = fmaf(t[j], u.x, v.x);
+                    v.y = fmaf(t[j], u.y, v.y);
+                }
+            }
+        } else if (!BF && sh.wide[r]) {
             const float *t = g.t + ((int64_t)(t0 + r) << log2r);
             const int ad = sh.segs.id[sh.segs.row[r]];
             v.x += adapter_dot<BF>(d, t, ad, n);
@@ -641,6 +712,8 @@ cudaError_t allow_clusters(const void *fn) {
     if (err == cudaSuccess) done.insert({fn, dev});
     return err;
 }
+
+constexpr int kSelfTiles = 1;  // x.A tiles at most that every cluster makes itself
 
 enum Launch { kPlain, kDependent, kCooperative };
 cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, Launch how, void **args, cudaStream_t s) {
@@ -723,15 +796,16 @@ int pick_stages(size_t stage, size_t other, int loads) {
     return n < loads ? n : loads;
 }
 
-template <typename Y, bool ONE>
-const void *skinny_fn(bool bf, bool kn, int parts) {
-    if (bf) {
-        if constexpr (sizeof(Y) == 4)
-            return kn ? (const void *)k_ad_skinny<true, true, 3, Y, ONE> : (const void *)k_ad_skinny<true, false, 3, Y, ONE>;
-        else
-            return kn ? (const void *)k_ad_skinny<true, true, 2, Y, ONE> : (const void *)k_ad_skinny<true, false, 2, Y, ONE>;
-    }
-    return kn ? (const void *)k_ad_skinny<false, true, 2, Y, ONE> : (const void *)k_ad_skinny<false, false, 2, Y, ONE>;
+template <typename Y, Mode MODE>
+const void *skinny_fn(bool bf, bool kn) {
+    constexpr int P = sizeof(Y) == 4 ? 3 : 2;
+    if (bf) return kn ? (const void *)k_ad_skinny<true, true, P, Y, MODE> : (const void *)k_ad_skinny<true, false, P, Y, MODE>;
+    return kn ? (const void *)k_ad_skinny<false, true, 2, Y, MODE> : (const void *)k_ad_skinny<false, false, 2, Y, MODE>;
+}
+template <Mode MODE>
+const void *skinny_fn(bool bf, bool kn, bool f32) {
+    if (f32) return skinny_fn<float, MODE>(bf, kn);
+    return bf ? skinny_fn<__nv_bfloat16, MODE>(bf, kn) : skinny_fn<__half, MODE>(bf, kn);
 }
 
 // 64 bits that no call of this process used before.
@@ -788,12 +862,11 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int s
 
 namespace {
 
-// One launch (one: with x.A in it) of k_ad_skinny; false, with nothing launched, where a cooperative
-// launch would not fit the device.
-bool launch_skinny(const AdapterArgs &g, const void *x_map, int sms, bool one, cudaStream_t s, cudaError_t *err) {
+// One launch of k_ad_skinny; false, with nothing launched, where a cooperative launch (kOne) would not fit the device.
+bool launch_skinny(const AdapterArgs &g, const void *x_map, Mode mode, cudaStream_t s, cudaError_t *err) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
-    const bool f32 = d.y_type == LATENT_TYPE_F32;
+    const bool f32 = d.y_type == LATENT_TYPE_F32, shrinks = mode != kTwo;
     const int tiles = (d.n_tokens + g.tile_rows - 1) / g.tile_rows, ntn = (d.n_out + 127) / 128;
     const int nk = (d.n_in + kBK - 1) / kBK;
     Plan p{};
@@ -802,53 +875,54 @@ bool launch_skinny(const AdapterArgs &g, const void *x_map, int sms, bool one, c
     *err = cudaErrorInvalidConfiguration;
     const int *room = cluster_room();
     if (!room) return true;
-    const size_t stage = 16384 + (size_t)p.rows * 128, tb = 2 * (size_t)((parts + 1) / 2) * p.rows * 128;
+    // as far as the ring still holds the loads of a trip to DRAM
+    p.tbufs = mode == kSelf ? 0 : p.rows <= 64 ? kMaxTBufs : 2;
+    const size_t stage = 16384 + (size_t)p.rows * 128, tb = (size_t)p.tbufs * ((parts + 1) / 2) * p.rows * 128;
     int cluster = pick_cluster((int64_t)tiles * ntn, nk, room);
     // The tensor cores cut a sum off instead of rounding it: a chain over K
     // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
     // fp32 results therefore use an accumulator per 512 of K, added up in
     // fp32, as far as the TMEM columns go, and clusters long enough.
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    const int groups = (512 - (one ? 2 : 1) * read) / p.rows + 1;
+    const int groups = (512 - (shrinks ? 2 : 1) * read) / p.rows + 1;
     if (f32)
         while (cluster < kMaxCluster && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
-    if (one && ((int64_t)tiles * ntn * cluster > kMaxBlocks || tiles * ntn > room[cluster])) return false;
+    if (mode == kOne && ((int64_t)tiles * ntn * cluster > kMaxBlocks || tiles * ntn > room[cluster])) return false;
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
     p.shrink_col = ((per + p.chunk - 1) / p.chunk - 1) * p.rows + read;
-    p.cols = tmem_cols(p.shrink_col + (one ? read : 0));
-    const size_t recv = recv_bytes(g.tile_rows, cluster, 512);
-    p.stages = pick_stages(stage, tb + recv, per * (one ? 2 : 1) + 4);
+    p.cols = tmem_cols(p.shrink_col + (shrinks ? read : 0));
+    const size_t recv = recv_bytes(g.tile_rows, cluster, mode == kSelf ? 512 + d.rank * 4 : 512);
+    p.stages = pick_stages(stage, tb + recv, per * (shrinks ? 2 : 1) + 4);
     p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
     CUtensorMap mW, mB, mA{};
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, d.rank < kExt ? d.rank : kExt) ||
-        (one && !adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank))) {
+        (shrinks && !adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank))) {
         *err = cudaErrorInvalidValue;
         return true;
     }
-    const void *fn = one ? f32 ? skinny_fn<float, true>(bf, kn, parts)
-                               : bf ? skinny_fn<__nv_bfloat16, true>(bf, kn, parts) : skinny_fn<__half, true>(bf, kn, parts)
-                         : f32 ? skinny_fn<float, false>(bf, kn, parts)
-                               : bf ? skinny_fn<__nv_bfloat16, false>(bf, kn, parts) : skinny_fn<__half, false>(bf, kn, parts);
+    const void *fn = mode == kOne ? skinny_fn<kOne>(bf, kn, f32)
+                     : mode == kSelf ? skinny_fn<kSelf>(bf, kn, f32) : skinny_fn<kTwo>(bf, kn, f32);
     AdapterArgs a = g;
-    if (one) a.nonce = next_nonce();
+    if (mode == kOne) a.nonce = next_nonce();
     void *args[] = {&mW, &mB, const_cast<void *>(x_map), &mA, &a, &p};
-    *err = launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, one ? kCooperative : kDependent, args, s);
+    *err = launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem,
+                          mode == kOne ? kCooperative : mode == kTwo ? kDependent : kPlain, args, s);
     return true;
 }
 
 }  // namespace
 
-cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
+cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, cudaStream_t s) {
     cudaError_t err;
-    launch_skinny(g, x_map, sms, false, s, &err);
+    launch_skinny(g, x_map, kTwo, s, &err);
     return err;
 }
 
-bool launch_adapter_decode(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s, cudaError_t *err) {
-    return launch_skinny(g, x_map, sms, true, s, err);
+bool launch_adapter_decode(const AdapterArgs &g, const void *x_map, cudaStream_t s, cudaError_t *err) {
+    return launch_skinny(g, x_map, g.most <= kSelfTiles ? kSelf : kOne, s, err);
 }
 
 }  // namespace latent

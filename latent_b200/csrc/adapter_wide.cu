@@ -354,11 +354,14 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             seg.wide[tid] = wide;
             const int ext = seg.n * rank;
             mbar_arrive(sh.seg_full + (tl & 1));
+            const int live = wide ? -1 : my;
+            float4 v[8];
+            if (ext) load_t_row(v, live, rank, g.log2r, tp, 0);
             for (int r0 = 0; r0 < ext; r0 += kExt, ++eb) {  // a thread that gives up here is heard at the next tile
                 if (eb >= 2 && !wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
-                build_t_row<BF, kParts>(tbuf + (eb & 1) * kTTile, 0u, tid, wide ? -1 : my, rank, g.log2r, tp,
-                                        scale, r0);
+                store_t_row<BF, kParts>(v, tbuf + (eb & 1) * kTTile, 0u, tid, scale);
+                if (r0 + kExt < ext) load_t_row(v, live, rank, g.log2r, tp, r0 + kExt);
                 fence_async_shared();
                 arrive_cluster(peer_addr(sh.t_full + (eb & 1), 0));
             }

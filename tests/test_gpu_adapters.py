@@ -67,6 +67,7 @@ SHAPES = [
     (2, 8, 16, [3, 1, 2]),
     (7, 1024, 704, [16, 5, 16]),
     (16, 256, 136, [64]),
+    (20, 1024, 2048, [32] * 9),
     (33, 2048, 1408, [16] * 40),
     (64, 1024, 256, [8, 16, 3]),
     (128, 512, 384, [33, 64]),
@@ -163,17 +164,18 @@ def test_a_row_that_is_not_finite_stays_alone(cuda, T):
     assert not bool(torch.isfinite(got[3]).any()) and not bool(torch.isfinite(got[7]).any())
 
 
-@pytest.mark.parametrize("T", [9, 300])
-def test_fp16_intermediate_beyond_the_fp16_range(cuda, T):
+@pytest.mark.parametrize("T,n,out", [(9, 2, HF), (9, 2, F32), (20, 12, HF), (20, 12, F32), (128, 12, HF), (300, 2, HF),
+                                     (300, 2, F32)])
+def test_fp16_intermediate_beyond_the_fp16_range(cuda, T, n, out):
     """x.A of some rows passes 65504 while the result does not: B is small."""
     K, N = 512, 256
-    x, w, ads, i = make(T, K, N, [16, 16], HF, seed=9, ids="packed")
+    x, w, ads, i = make(T, K, N, [16] * n, HF, seed=9, ids="packed")
     x[1::3] *= 400.0
-    ads = [((a.float() * 200).to(HF), (b.float() * 1e-4).to(HF), s) for a, b, s in ads]
+    ads = [((a.float() * 200).to(HF), (b.float() * 1e-4).to(HF), 1.0 + 0.5 * (k % 2)) for k, (a, b, _) in enumerate(ads)]
     y, S = reference(x, w, ads, i)
-    t = x[i == 1].double() @ ads[1][0].double()
+    t = torch.cat([x[i == k].double() @ ads[k][0].double() for k in range(n)])
     assert float(t.abs().max()) > 65504 and float(y.abs().max()) < 60000
-    assert_close(adapter_project(x, w, AdapterSet(ads), i), y, S, K, 16)
+    assert_close(adapter_project(x, w, AdapterSet(ads), i, out_dtype=out), y, S, K, 16)
 
 
 def test_factor_pair_as_the_shared_projection(cuda):
