@@ -103,6 +103,48 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
     }
 }
 
+// The loads and MMAs take their addresses and coordinates from uniform
+// registers.  Issued under `lane == 0`, or with operands that the compiler
+// cannot prove equal over the warp, each of them is wrapped in a loop over the
+// lanes' values: about 100 cycles an instruction more (measured: a one-warp
+// load loop at 315 cycles a turn against 194).  So their loops are run by whole
+// warps, on values and conditions that are uniform by construction (block
+// indexes, votes, shuffles from a constant lane), and only the instructions
+// themselves by one elected lane, always the same.
+constexpr uint32_t kAll = 0xffffffffu;
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kAll, v, 0); }
+__device__ __forceinline__ int warp_index() { return uniform((int)threadIdx.x >> 5); }
+
+// By a whole warp, with one result for all lanes; false as well once *abort is set.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    const bool done = wait<CLUSTER>(bar, parity) && !*abort;
+    return __all_sync(kAll, done);
+}
+
+// Position in a ring: slot and the parity of its current phase.
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    bool wrapped = false;
+    __device__ __forceinline__ void next(int slots) {
+        if (++s == slots) {
+            s = 0;
+            phase ^= 1u;
+            wrapped = true;
+        }
+    }
+};
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -54,20 +54,6 @@ struct Plan {
     size_t smem;
 };
 
-// Position in the ring of stages: slot and the parity of its current phase.
-struct Ring {
-    int s = 0;
-    uint32_t phase = 0;
-    bool wrapped = false;
-    __device__ __forceinline__ void next(int stages) {
-        if (++s == stages) {
-            s = 0;
-            phase ^= 1u;
-            wrapped = true;
-        }
-    }
-};
-
 __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
     return reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
 }
@@ -153,6 +139,47 @@ __device__ __forceinline__ void arrive_rank(uint64_t *bar, int rank) {
                  : "memory");
 }
 
+// By the load warp: the K blocks [k0, k1) of stacked rank columns m .. m + 127 (rows of A) and of x.
+template <bool BF>
+__device__ __forceinline__ bool load_stacked(Shared &sh, const Plan &p, Ring &at, uint8_t *ring, uint32_t stage,
+                                             const CUtensorMap *mA, const CUtensorMap *mX, int m, int total, int k0,
+                                             int k1, int t0, int rank, int log2r) {
+    const int cols = min(128, total - m), boxes = cols >> log2r, lane = threadIdx.x & 31;
+    const int row = lane < boxes ? sh.segs.id[(m >> log2r) + lane] << log2r : 0;  // of the lane-th adapter
+    int rows[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(kAll, row, i);
+    for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+        if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) return false;
+        if (elect()) {
+            uint8_t *st = ring + at.s * stage;
+            mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(cols + p.rows) * 128u);
+            tma_load_2d(st + 16384, mX, k * kBK, t0, sh.full + at.s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < boxes) tma_load_2d(st + ((uint32_t)i << log2r) * 128u, mA, k * kBK, rows[i], sh.full + at.s);
+        }
+    }
+    return true;
+}
+
+// By the MMA warp: their product into acc.
+__device__ __forceinline__ bool multiply_stacked(Shared &sh, const Plan &p, Ring &at, uint8_t *ring, uint32_t stage,
+                                                 uint32_t acc, uint32_t id, int k0, int k1) {
+    for (int k = k0; k < k1; ++k, at.next(p.stages)) {
+        if (!wait_warp(sh.full + at.s, at.phase, &sh.abort)) return false;
+        tc_fence_after();
+        if (elect()) {
+            const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                mma_f16(acc, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), id, (k > k0) | kk);
+            mma_commit(sh.empty + at.s);
+        }
+    }
+    return true;
+}
+
 // x.A.  Block (cluster rank, slot, row tile); the stacked rank columns of the
 // tile's adapters in tiles of 128: slot, slot + gridDim.y, ...  Rank q of the
 // cluster sums K blocks of its share; every block sends the t of a row to the
@@ -168,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     float *recv = reinterpret_cast<float *>(ring + p.stages * stage);  // [cluster][rows of a rank][rank]
     __shared__ Shared sh;
     const int q = blockIdx.x, CS = gridDim.x;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
     const int rank = d.rank, log2r = g.log2r;
@@ -192,47 +219,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         set_dest(sh, recv, threadIdx.x - 128, nt, per, q, (uint32_t)rank * 4u);
         mbar_arrive(&sh.seg);
     }
-    ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
-    const int total = ok ? sh.segs.n * rank : 0;  // stacked rank columns
+    ok = wait_warp(&sh.seg, 0u, &sh.abort);
+    const int total = ok ? uniform(sh.segs.n) * rank : 0;  // stacked rank columns
     if (warp == 0) {
-        // lane i loads the i-th run of stacked columns of a stage; the last one loads x
         Ring at;
-        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128) {
-            const int cols = min(128, total - m), boxes = cols >> log2r;
-            int row = 0;
-            if (lane < boxes) row = sh.segs.id[(m >> log2r) + lane] << log2r;
-            for (int k = k0; k < k1; ++k, at.next(p.stages)) {
-                if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
-                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
-                uint8_t *st = ring + at.s * stage;
-                if (lane == 31) {
-                    mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(cols + p.rows) * 128u);
-                    tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
-                }
-                if (lane < boxes) tma_load_2d(st + ((uint32_t)lane << log2r) * 128u, &mA, k * kBK, row, sh.full + at.s);
-            }
-        }
-    } else if (warp == 1 && lane == 0) {
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128)
+            ok = load_stacked<BF>(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
+    } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, false, false);
         Ring at;
         uint32_t n = 0;
         for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128, ++n) {
             const uint32_t b = n & 1u;
-            if (n >= 2 && !wait(sh.acc_empty + b, ((n >> 1) - 1u) & 1u)) { ok = false; break; }
+            if (n >= 2 && !wait_warp(sh.acc_empty + b, ((n >> 1) - 1u) & 1u, &sh.abort)) { ok = false; break; }
             tc_fence_after();
-            for (int k = k0; k < k1; ++k, at.next(p.stages)) {
-                if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    mma_f16(tmem + b * read, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), id,
-                            (k > k0) | kk);
-                mma_commit(sh.empty + at.s);
-            }
-            if (ok) mma_commit(sh.acc_full + b);
+            ok = multiply_stacked(sh, p, at, ring, stage, tmem + b * read, id, k0, k1);
+            if (ok && elect()) mma_commit(sh.acc_full + b);
         }
-        if (!ok) {
+        if (!ok && elect()) {
             mma_commit(sh.acc_full);
             mma_commit(sh.acc_full + 1);
         }
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     float *recv = reinterpret_cast<float *>(tbuf + p.tbufs * kTiles * xbytes);
     __shared__ Shared sh;
     const int q = blockIdx.x, CS = gridDim.x;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int n0 = blockIdx.y * 128, t0 = blockIdx.z * g.tile_rows, nt = min(g.tile_rows, d.n_tokens - t0);
     const int rank = d.rank, log2r = g.log2r;
@@ -355,129 +359,116 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     bool ok = true;
     if (warp == 0) {
         Ring at;
-        // the ring's next slot, free; all lanes or none
-        auto next_slot = [&]() {
-            if ((at.wrapped && !wait(sh.empty + at.s, at.phase ^ 1u)) || sh.abort) ok = false;
-            return ok = __all_sync(0xffffffffu, ok);
-        };
-        auto load_a = [&]() {  // lane i loads the i-th adapter's run of stacked columns, the last one x
-            ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
-            const int total = ok ? sh.segs.n * rank : 0;
-            for (int m = slot * 128; m < total && ok; m += slots * 128) {
-                const int cols = min(128, total - m), boxes = cols >> log2r;
-                int row = 0;
-                if (lane < boxes) row = sh.segs.id[(m >> log2r) + lane] << log2r;
-                for (int k = k0; k < k1 && next_slot(); ++k, at.next(p.stages)) {
-                    uint8_t *st = ring + at.s * stage;
-                    if (lane == 31) {
-                        mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(cols + p.rows) * 128u);
-                        tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
-                    }
-                    if (lane < boxes) tma_load_2d(st + ((uint32_t)lane << log2r) * 128u, &mA, k * kBK, row, sh.full + at.s);
-                }
-            }
+        auto load_a = [&]() {
+            ok = wait_warp(&sh.seg, 0u, &sh.abort);
+            const int total = ok ? uniform(sh.segs.n) * rank : 0;
+            for (int m = slot * 128; m < total && ok; m += slots * 128)
+                ok = load_stacked<BF>(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
         };
         if (ONE && shrinks) load_a();
-        for (int k = k0; ok && k < k1 && next_slot(); ++k, at.next(p.stages)) {
-            uint8_t *st = ring + at.s * stage;
-            if (lane == 0) {
+        for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
+            if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
+            if (elect()) {
+                uint8_t *st = ring + at.s * stage;
                 mbar_arrive_expect_tx(sh.full + at.s, stage);
-                if (KN) tma_load_2d(st, &mW, n0, k * kBK, sh.full + at.s);
-                else tma_load_2d(st, &mW, k * kBK, n0, sh.full + at.s);
-            } else if (lane == 1) {
-                if (KN) tma_load_2d(st + 8192, &mW, n0 + 64, k * kBK, sh.full + at.s);
-            } else if (lane == 2) {
+                if (KN) {
+                    tma_load_2d(st, &mW, n0, k * kBK, sh.full + at.s);
+                    tma_load_2d(st + 8192, &mW, n0 + 64, k * kBK, sh.full + at.s);
+                } else {
+                    tma_load_2d(st, &mW, k * kBK, n0, sh.full + at.s);
+                }
                 tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
             }
         }
         if (SELF && ok) load_a();
-        if (!SELF && ok) ok = __all_sync(0xffffffffu, wait(&sh.seg, 0u));
+        if (!SELF && ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
         if (!SELF && ok) {
-            const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
+            const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
             const int e1 = (int)((int64_t)ne * (q + 1) / CS), box = min(rank, kExt);
-            for (int e = (int)((int64_t)ne * q / CS); e < e1 && next_slot(); ++e, at.next(p.stages)) {
-                uint8_t *st = ring + at.s * stage;
-                const int rows = min(kExt, ext - e * kExt), j = (lane >> 1) * box;
-                if (lane == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 256u);
-                __syncwarp();
-                if (j < rows) {
-                    const int r = e * kExt + j;
-                    tma_load_2d(st + (lane & 1) * 8192 + j * 128, &mB, n0 + (lane & 1) * 64,
-                                (sh.segs.id[r >> log2r] << log2r) + (r & (rank - 1)), sh.full + at.s);
+            for (int e = (int)((int64_t)ne * q / CS); e < e1; ++e, at.next(p.stages)) {
+                if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
+                const int rows = min(kExt, ext - e * kExt), r = e * kExt + lane * box;  // one box of 32 rows or two of 16
+                const int src = lane * box < rows ? (sh.segs.id[r >> log2r] << log2r) + (r & (rank - 1)) : 0;
+                const int src0 = __shfl_sync(kAll, src, 0), src1 = __shfl_sync(kAll, src, 1);
+                if (elect()) {
+                    uint8_t *st = ring + at.s * stage;
+                    mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 256u);
+                    tma_load_2d(st, &mB, n0, src0, sh.full + at.s);
+                    tma_load_2d(st + 8192, &mB, n0 + 64, src0, sh.full + at.s);
+                    if (box < rows) {
+                        tma_load_2d(st + 2048, &mB, n0, src1, sh.full + at.s);
+                        tma_load_2d(st + 8192 + 2048, &mB, n0 + 64, src1, sh.full + at.s);
+                    }
                 }
             }
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
         Ring at;
         auto multiply_a = [&]() {
-            ok = wait(&sh.seg, 0u);
-            const int total = ok ? sh.segs.n * rank : 0;
-            const uint32_t ids = idesc(BF, p.rows, false, false), acc = tmem + (uint32_t)p.shrink_col;
+            ok = wait_warp(&sh.seg, 0u, &sh.abort);
+            const int total = ok ? uniform(sh.segs.n) * rank : 0;
             uint32_t n = 0;
             for (int m = slot * 128; m < total && ok; m += slots * 128, ++n) {
-                if (n >= 1 && !wait(sh.acc_empty + 1, (n - 1u) & 1u)) { ok = false; break; }
+                if (n >= 1 && !wait_warp(sh.acc_empty + 1, (n - 1u) & 1u, &sh.abort)) { ok = false; break; }
                 tc_fence_after();
-                for (int k = k0; k < k1; ++k, at.next(p.stages)) {
-                    if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_f16(acc, desc_kmajor_sw128(w + kk * 32), desc_kmajor_sw128(x + kk * 32), ids, (k > k0) | kk);
-                    mma_commit(sh.empty + at.s);
-                }
-                if (ok) mma_commit(sh.acc_full + 1);
+                ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
+                if (ok && elect()) mma_commit(sh.acc_full + 1);
             }
         };
         if (ONE && shrinks) multiply_a();
         int in_chunk = 0;
         uint32_t acc = tmem;
         for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
-            if (!wait(sh.full + at.s, at.phase) || sh.abort) { ok = false; break; }
+            if (!wait_warp(sh.full + at.s, at.phase, &sh.abort)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
             if (in_chunk == p.chunk) {
                 in_chunk = 0;
                 acc += (uint32_t)p.rows;
             }
+            if (elect()) {
+                const uint32_t w = smem_addr(ring + at.s * stage), x = w + 16384u;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                mma_f16(acc, KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32),
-                        desc_kmajor_sw128(x + kk * 32), id, in_chunk | kk);
+                for (int kk = 0; kk < 4; ++kk)
+                    mma_f16(acc, KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32),
+                            desc_kmajor_sw128(x + kk * 32), id, in_chunk | kk);
+                mma_commit(sh.empty + at.s);
+            }
             ++in_chunk;
-            mma_commit(sh.empty + at.s);
         }
         if (SELF) {
-            if (ok) mma_commit(sh.acc_full);
+            if (ok && elect()) mma_commit(sh.acc_full);
             if (ok) multiply_a();
         } else if (ok) {
-            ok = wait(&sh.seg, 0u);
+            ok = wait_warp(&sh.seg, 0u, &sh.abort);
         }
         if (!SELF && ok) {
-            const int ext = sh.segs.n * rank, ne = (ext + kExt - 1) / kExt;
+            const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
             const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
             Ring tb;
             for (int e = e0; e < e1; ++e, at.next(p.stages), tb.next(p.tbufs)) {
-                const int b = tb.s;
-                if (!wait(sh.full + at.s, at.phase) || !wait(sh.t_full + b, tb.phase) || sh.abort) {
+                if (!wait_warp(sh.full + at.s, at.phase, &sh.abort) || !wait_warp(sh.t_full + tb.s, tb.phase, &sh.abort)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t w = smem_addr(ring + at.s * stage), t = smem_addr(tbuf) + (uint32_t)b * kTiles * xbytes;
-                const int steps = min(kExt / 16, (ext - e * kExt) / 16);
-                for (int kk = 0; kk < steps; ++kk)
+                if (elect()) {
+                    const uint32_t w = smem_addr(ring + at.s * stage), t = smem_addr(tbuf) + (uint32_t)tb.s * kTiles * xbytes;
+                    const int steps = min(kExt / 16, (ext - e * kExt) / 16);
+                    for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
-                    for (int w2 = 0; w2 < PARTS; ++w2)
-                        mma_f16(acc, desc_mnmajor_sw128(w + kk * 2048), desc_kmajor_sw128(t + t_offset(w2, kk, xbytes)),
-                                idx, 1);
-                mma_commit(sh.empty + at.s);
-                mma_commit(sh.t_empty + b);
+                        for (int w2 = 0; w2 < PARTS; ++w2)
+                            mma_f16(acc, desc_mnmajor_sw128(w + kk * 2048), desc_kmajor_sw128(t + t_offset(w2, kk, xbytes)),
+                                    idx, 1);
+                    mma_commit(sh.empty + at.s);
+                    mma_commit(sh.t_empty + tb.s);
+                }
             }
         }
-        if (!ok && MODE != kTwo) mma_commit(sh.acc_full + 1);
-        if (!SELF || !ok) mma_commit(sh.acc_full);
+        if (elect()) {
+            if (!ok && MODE != kTwo) mma_commit(sh.acc_full + 1);
+            if (!SELF || !ok) mma_commit(sh.acc_full);
+        }
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
         build_segments(sh.segs, a, nt, r, 1);

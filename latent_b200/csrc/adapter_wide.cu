@@ -115,8 +115,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     uint8_t *tbuf = ring + kStages * kStage;
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t cta = cluster.block_rank();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cta = blockIdx.x & 1;  // its rank in the cluster
+    const int warp = warp_index(), lane = threadIdx.x & 31;
     const latent_adapter_desc &d = g.d;
     const int rank = d.rank;
     const int tm = (d.n_tokens + kPairRows - 1) / kPairRows, tn = (d.n_out + kPairCols - 1) / kPairCols;
@@ -152,27 +152,20 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     const uint32_t tmem = sh.tmem;
     bool ok = true;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         // ---------------- loads ----------------
-        int it = 0, tl = 0;
+        Ring at;
+        int tl = 0;
+        const uint32_t full0 = peer_addr(sh.full, 0);
         for (int i = pair; i < tiles && ok; i += pairs, ++tl) {
             const Tile tile = tile_at(i, tm, tn);
-            const int row = tile.t0 + (int)cta * 128, col = tile.n0 + (int)cta * 128;
-            int ext = 0;
-            const PairSegments &seg = sh.seg[tl & 1];
-            for (int k = 0;; ++k, ++it) {
-                if (k == nk) {
-                    if (!wait(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
-                    ext = seg.n * rank;
-                }
-                if (k >= nk && (k - nk) * kExt >= ext) break;
-                const int s = it % kStages;
-                if (it >= kStages && !wait(sh.empty + s, (uint32_t)(it / kStages - 1) & 1u)) { ok = false; break; }
-                if (sh.abort) { ok = false; break; }
-                uint8_t *st = ring + s * kStage;
-                const uint32_t bar = peer_addr(sh.full + s, 0);
-                if (k < nk) {
-                    if (cta == 0) mbar_arrive_expect_tx(sh.full + s, 2 * kStage);
+            const int row = tile.t0 + cta * 128, col = tile.n0 + cta * 128;
+            for (int k = 0; k < nk; ++k, at.next(kStages)) {
+                if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
+                if (elect()) {
+                    uint8_t *st = ring + at.s * kStage;
+                    const uint32_t bar = full0 + at.s * 8;
+                    if (cta == 0) mbar_arrive_expect_tx(sh.full + at.s, 2 * kStage);
                     load_pair(st, &mX, k * kBK, row, bar);
                     if (KN) {
                         load_pair(st + 16384, &mW, col, k * kBK, bar);
@@ -180,66 +173,79 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                     } else {
                         load_pair(st + 16384, &mW, k * kBK, col, bar);
                     }
-                } else {
-                    const int r0 = (k - nk) * kExt, box = min(rank, kExt), rows = min(kExt, ext - r0);
-                    if (cta == 0) mbar_arrive_expect_tx(sh.full + s, (uint32_t)rows * 512u);
-                    for (int j = 0; j < rows; j += box) {
-                        const int src = (seg.id[(r0 + j) >> g.log2r] << g.log2r) + ((r0 + j) & (rank - 1));
-                        load_pair(st + 16384 + j * 128, &mB, col, src, bar);
-                        load_pair(st + 16384 + 8192 + j * 128, &mB, col + 64, src, bar);
+                }
+            }
+            if (!ok || !wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
+            const PairSegments &seg = sh.seg[tl & 1];
+            const int ext = uniform(seg.n) * rank, box = min(rank, kExt);
+            for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages)) {
+                if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
+                const int rows = min(kExt, ext - r0), r = r0 + lane * box;  // one box of 32 rows or two of 16
+                const int src = lane * box < rows ? (seg.id[r >> g.log2r] << g.log2r) + (r & (rank - 1)) : 0;
+                const int src0 = __shfl_sync(kAll, src, 0), src1 = __shfl_sync(kAll, src, 1);
+                if (elect()) {
+                    uint8_t *st = ring + at.s * kStage + 16384;
+                    const uint32_t bar = full0 + at.s * 8;
+                    if (cta == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 512u);
+                    load_pair(st, &mB, col, src0, bar);
+                    load_pair(st + 8192, &mB, col + 64, src0, bar);
+                    if (box < rows) {
+                        load_pair(st + 2048, &mB, col, src1, bar);
+                        load_pair(st + 8192 + 2048, &mB, col + 64, src1, bar);
                     }
                 }
             }
-            if (ok) mbar_arrive(sh.seg_empty + (tl & 1));
+            if (ok && lane == 0) mbar_arrive(sh.seg_empty + (tl & 1));
         }
-    } else if (warp == 1 && lane == 0) {
-        // ---------------- MMAs (the leader's thread, for both blocks) ----------------
-        int it = 0, tl = 0, eb = 0;
+    } else if (warp == 1) {
+        // ---------------- MMAs (the leader's warp, for both blocks) ----------------
+        Ring at, tb;
+        int tl = 0;
         constexpr uint32_t id = idesc_pair(BF, KN), idx = idesc_pair(BF, true);
         for (int i = pair; i < tiles && ok; i += pairs, ++tl) {
             const int b = tl & 1;
+            const uint32_t acc = tmem + (uint32_t)b * 256u;
             if (cta == 0) {
-                if (tl >= 2 && !wait<true>(sh.acc_empty + b, (uint32_t)((tl >> 1) - 1) & 1u)) { ok = false; break; }
+                if (tl >= 2 && !wait_warp<true>(sh.acc_empty + b, (uint32_t)((tl >> 1) - 1) & 1u, &sh.abort)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t acc = tmem + (uint32_t)b * 256u;
-                for (int k = 0; k < nk; ++k, ++it) {
-                    const int s = it % kStages;
-                    if (!wait(sh.full + s, (uint32_t)(it / kStages) & 1u) || sh.abort) { ok = false; break; }
+                for (int k = 0; k < nk; ++k, at.next(kStages)) {
+                    if (!wait_warp(sh.full + at.s, at.phase, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t x = smem_addr(ring + s * kStage), w = x + 16384u;
+                    if (elect()) {
+                        const uint32_t x = smem_addr(ring + at.s * kStage), w = x + 16384u;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_pair(acc, desc_kmajor_sw128(x + kk * 32),
-                                 KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32), id, k | kk);
-                    commit_pair(sh.empty + s);
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_pair(acc, desc_kmajor_sw128(x + kk * 32),
+                                     KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32), id, k | kk);
+                        commit_pair(sh.empty + at.s);
+                    }
                 }
                 if (!ok) break;
             }
-            if (!wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u)) { ok = false; break; }
-            const int ext = sh.seg[b].n * rank;
+            if (!wait_warp(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
+            const int ext = uniform(sh.seg[b].n) * rank;
             if (cta == 0) {
-                const uint32_t acc = tmem + (uint32_t)b * 256u;
-                for (int r0 = 0; r0 < ext; r0 += kExt, ++it, ++eb) {
-                    const int s = it % kStages;
-                    if (!wait(sh.full + s, (uint32_t)(it / kStages) & 1u) ||
-                        !wait<true>(sh.t_full + (eb & 1), (uint32_t)(eb >> 1) & 1u) || sh.abort) { ok = false; break; }
+                for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages), tb.next(2)) {
+                    if (!wait_warp(sh.full + at.s, at.phase, &sh.abort) ||
+                        !wait_warp<true>(sh.t_full + tb.s, tb.phase, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t w = smem_addr(ring + s * kStage) + 16384u, t = smem_addr(tbuf + (eb & 1) * kTTile);
-                    const int steps = min(kExt / 16, (ext - r0) / 16);
-                    for (int kk = 0; kk < steps; ++kk)
+                    if (elect()) {
+                        const uint32_t w = smem_addr(ring + at.s * kStage) + 16384u, t = smem_addr(tbuf + tb.s * kTTile);
+                        const int steps = min(kExt / 16, (ext - r0) / 16);
+                        for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
-                        for (int q = 0; q < kParts; ++q)
-                            mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 0u)),
-                                     desc_mnmajor_sw128(w + kk * 2048), idx, 1);
-                    commit_pair(sh.empty + s);
-                    commit_pair(sh.t_empty + (eb & 1));
+                            for (int q = 0; q < kParts; ++q)
+                                mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 0u)), desc_mnmajor_sw128(w + kk * 2048), idx, 1);
+                        commit_pair(sh.empty + at.s);
+                        commit_pair(sh.t_empty + tb.s);
+                    }
                 }
                 if (!ok) break;
-                commit_pair(sh.acc_full + b);
+                if (elect()) commit_pair(sh.acc_full + b);
             }
-            mbar_arrive(sh.seg_empty + b);
+            if (lane == 0) mbar_arrive(sh.seg_empty + b);
         }
-        if (!ok && cta == 0) {
+        if (!ok && cta == 0 && elect()) {
             commit_pair(sh.acc_full);  // lets the waiting epilogues go on to the abort flag
             commit_pair(sh.acc_full + 1);
         }
@@ -253,7 +259,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             if (!wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u) ||
                 !wait(sh.acc_full + b, (uint32_t)(tl >> 1) & 1u) || sh.abort) { ok = false; break; }
             tc_fence_after();
-            const int t = tile.t0 + (int)cta * 128 + r;
+            const int t = tile.t0 + cta * 128 + r;
             const bool live = t < d.n_tokens;
             const bool wide = !BF && sh.seg[b].wide[r];
             const int a = wide ? sh.seg[b].id[sh.seg[b].row[r]] : 0;
@@ -344,7 +350,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                 seg.n = n;
             }
             bar_sync(1, 128);
-            const int mine = (int)cta;
+            const int mine = cta;
             const int my = a[mine] >= 0 ? sh.first[lead[mine]] : -1;
             const int t = tile.t0 + mine * 128 + tid;
             const float *tp = g.t + (int64_t)t * rank;
