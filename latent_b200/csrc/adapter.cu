@@ -179,7 +179,7 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         cudaError_t err;
         if (d->n_tokens <= adapter::kRows && launch_adapter_decode(a, &x, s, &err))
             return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
-        const bool wide = d->y_type == d->type && d->n_tokens > 256;
+        const bool wide = d->n_tokens > 256;
         if (launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
             (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, s)) != cudaSuccess)
             return LATENT_ERR_CUDA;

@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         a = row_adapter(d, t0 + r, r < nt, q == 0 && blockIdx.y == 0);
     }
     setup<true>(sh, p, CS, warp, lane);
-    const uint32_t tmem = warp ? sh.tmem : 0u, read = (uint32_t)(p.rows + 31) & ~31u;
+    const uint32_t tmem = warp ? (uint32_t)uniform((int)sh.tmem) : 0u, read = (uint32_t)(p.rows + 31) & ~31u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         a = row_adapter(d, t0 + r, r < nt, MODE != kTwo && q == 0 && blockIdx.y == 0);
     }
     setup<false>(sh, p, CS, warp, lane);
-    const uint32_t tmem = warp ? sh.tmem : 0u;
+    const uint32_t tmem = warp ? (uint32_t)uniform((int)sh.tmem) : 0u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
@@ -812,17 +812,29 @@ uint64_t next_nonce() {
 
 }  // namespace
 
-bool adapter_map(void *map, bool bf16, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+namespace {
+bool encode(void *map, CUtensorMapDataType type, int size, const void *base, uint64_t rows, uint64_t cols, uint64_t ld,
+            uint32_t box_rows) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)adapter::kBK, box_rows};
+    cuuint64_t strides[1] = {ld * size};
+    cuuint32_t box[2] = {128u / size, box_rows};
     cuuint32_t es[2] = {1, 1};
-    return fn(static_cast<CUtensorMap *>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-              2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-           CUDA_SUCCESS;
+    return fn(static_cast<CUtensorMap *>(map), type, 2, const_cast<void *>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace
+
+bool adapter_map(void *map, bool bf16, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, rows, cols, ld,
+                  box_rows);
+}
+
+bool adapter_out_map(void *map, int y_type, void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+    if (y_type == LATENT_TYPE_F32) return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_rows);
+    return adapter_map(map, y_type == LATENT_TYPE_BF16, base, rows, cols, ld, box_rows);
 }
 
 cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {

@@ -1,18 +1,24 @@
 // The adapters' product for prompt-sized batches: y = x.W + the adapters'
-// part, tiles of 256 rows x 256 columns on pairs of SMs (tcgen05 cta_group::2).
+// part, tiles of 256 rows x 256 columns (fp32 results: 128) on pairs of SMs
+// (tcgen05 cta_group::2).
 //
 // Persistent, one cluster of two blocks per tile at a time.  Each block holds
-// 128 rows of x and 128 columns of W per stage (32 KB, a ring of 5) and the
-// 128 x 256 half of the accumulator in TMEM, twice, so that the epilogue of
-// one tile runs under the MMAs of the next.  Per block: warp 0 loads (TMA,
-// plain per-block loads that complete on the leader's barrier), warp 1 of the
-// leader issues the pair's MMAs, warps 4..7 drain accumulators, warps 8..11
-// list the adapters of the tile's 256 rows and build the x.A parts of the
-// extension blocks (32 stacked B rows each: both parts side by side in one
-// 128-byte row).
+// 128 rows of x and half the tile's columns of W per stage (a ring of 5) and
+// its 128 rows of the accumulator in TMEM, twice, so that the epilogue of one
+// tile runs under the MMAs of the next.  Per block: warp 0 loads (TMA, plain
+// per-block loads that complete on the leader's barrier), warp 1 of the leader
+// issues the pair's MMAs, warps 4..7 drain accumulators (through shared memory
+// to TMA stores, which also clip the ragged edges), warps 8..11 list the
+// adapters of the tile's 256 rows and build the x.A parts of the extension
+// blocks (32 stacked B rows each).
 //
-// A pair tile costs 512 cycles of MMA per 64 of K against 64 KB of loads: half
-// the L2 traffic per operation of one block working alone.
+// A pair tile of 256 columns costs 512 cycles of MMA per 64 of K against 64 KB
+// of loads: half the L2 traffic per operation of one block working alone.
+//
+// fp32 results: the tensor cores cut a sum off instead of rounding it (a chain
+// over K = 7168 is off by 8e-6 of the result, one over 512 by 5e-7), so the two
+// accumulators take turns every 512 of K and the epilogue adds them up in fp32
+// registers, 128 a thread, hence the narrower tile.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -26,17 +32,26 @@ namespace cg = cooperative_groups;
 using namespace adapter;
 
 constexpr int kThreads = 384;
-constexpr int kStages = 5;
-constexpr int kPairRows = 256, kPairCols = 256;
-constexpr uint32_t kStage = 32768;             // 16 KB of x, 16 KB of W
-constexpr uint32_t kTTile = 16384;             // 128 rows x (2 parts x 32) of x.A
-constexpr int kParts = 2;
-constexpr int kGroupM = 8;                     // row tiles that share a sweep over the columns (L2 reuse)
-// All of an SM's shared memory, more than the ring needs: the block takes all
+constexpr int kPairRows = 256;
+constexpr int kGroupM = 8;       // row tiles that share a sweep over the columns (L2 reuse)
+constexpr uint32_t kXBytes = 16384;
+constexpr uint32_t kOut = 4096;  // a warp's staging: 32 rows of 128 bytes
+// All of an SM's shared memory, more than the kernel needs: the block takes all
 // TMEM columns, and no other block that wants some may start beside it.
 constexpr size_t kStatic = 6144;
 constexpr size_t kSmem = 227 * 1024 - kStatic;
-static_assert(1024 + kStages * kStage + 2 * kTTile <= kSmem, "ring and x.A tiles");
+
+template <bool BF, bool F32>
+struct Cfg {
+    static constexpr int kCols = F32 ? 128 : 256;                    // of a pair's tile
+    static constexpr int kStages = 5;
+    static constexpr uint32_t kStage = kXBytes + kCols / 2 * 128;    // x, W
+    static constexpr int kParts = BF && F32 ? 3 : 2;
+    static constexpr uint32_t kTTile = 16384u * ((kParts + 1) / 2);  // 128 rows x (2 parts x 32) of x.A, and the third part
+    static constexpr int kChunk = F32 ? 8 : 1 << 30;                 // K blocks per accumulator
+    static constexpr int kOutBufs = F32 ? 1 : 1;
+    static_assert(1024 + kStages * kStage + 2 * kTTile + 4 * kOutBufs * kOut <= kSmem, "shared memory");
+};
 
 struct PairSegments {
     int n;
@@ -46,7 +61,7 @@ struct PairSegments {
 };
 
 struct Shared {
-    uint64_t full[kStages], empty[kStages];
+    uint64_t full[5], empty[5];
     uint64_t acc_full[2], acc_empty[2], t_full[2], t_empty[2], seg_full[2], seg_empty[2];
     uint32_t tmem;
     volatile int abort;
@@ -90,29 +105,56 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar) {
         : "memory");
 }
 
+__device__ __forceinline__ void store_box(const CUtensorMap *map, int c0, int c1, const void *src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1),
+                 "r"(smem_addr(src))
+                 : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// 32 lanes x 16 columns of 32-bit TMEM words into 16 registers per thread.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 struct Tile {
     int t0, n0;
 };
 // Tiles in sweeps of kGroupM row tiles: all columns of one sweep before the next.
+template <int COLS>
 __device__ __forceinline__ Tile tile_at(int i, int tm, int tn) {
     const int per = kGroupM * tn, g = i / per, first = g * kGroupM;
     const int rows = min(kGroupM, tm - first), j = i - g * per;
-    return {(first + j % rows) * kPairRows, (j / rows) * kPairCols};
+    return {(first + j % rows) * kPairRows, (j / rows) * COLS};
 }
 
 // M = 256 over the pair.
-__host__ __device__ constexpr uint32_t idesc_pair(bool bf16, bool b_mn) {
+__host__ __device__ constexpr uint32_t idesc_pair(bool bf16, int cols, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
-           ((uint32_t)(kPairCols >> 3) << 17) | ((uint32_t)(kPairRows >> 4) << 24);
+           ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kPairRows >> 4) << 24);
 }
 
-template <bool BF, bool KN>
+template <bool BF, bool KN, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtensorMap mW,
-          const __grid_constant__ CUtensorMap mB, AdapterArgs g) {
+          const __grid_constant__ CUtensorMap mB, const __grid_constant__ CUtensorMap mY, AdapterArgs g) {
+    using C = Cfg<BF, F32>;
+    constexpr int kStages = C::kStages, kPairCols = C::kCols, kHalf = kPairCols / 2;
+    constexpr uint32_t kStage = C::kStage;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t *tbuf = ring + kStages * kStage;
+    uint8_t *obuf = tbuf + 2 * C::kTTile;
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int cta = blockIdx.x & 1;  // its rank in the cluster
@@ -121,7 +163,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     const int rank = d.rank;
     const int tm = (d.n_tokens + kPairRows - 1) / kPairRows, tn = (d.n_out + kPairCols - 1) / kPairCols;
     const int tiles = tm * tn, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int nk = (d.n_in + kBK - 1) / kBK;
+    const int nk = (d.n_in + kBK - 1) / kBK, chunks = (nk - 1) / C::kChunk + 1;  // of K per tile
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -149,7 +191,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     __syncthreads();
     cluster.sync();  // both blocks' barriers exist before either arrives on the other's
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
     bool ok = true;
 
     if (warp == 0) {
@@ -158,8 +200,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         int tl = 0;
         const uint32_t full0 = peer_addr(sh.full, 0);
         for (int i = pair; i < tiles && ok; i += pairs, ++tl) {
-            const Tile tile = tile_at(i, tm, tn);
-            const int row = tile.t0 + cta * 128, col = tile.n0 + cta * 128;
+            const Tile tile = tile_at<kPairCols>(i, tm, tn);
+            const int row = tile.t0 + cta * 128, col = tile.n0 + cta * kHalf;
             for (int k = 0; k < nk; ++k, at.next(kStages)) {
                 if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
                 if (elect()) {
@@ -168,10 +210,10 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                     if (cta == 0) mbar_arrive_expect_tx(sh.full + at.s, 2 * kStage);
                     load_pair(st, &mX, k * kBK, row, bar);
                     if (KN) {
-                        load_pair(st + 16384, &mW, col, k * kBK, bar);
-                        load_pair(st + 16384 + 8192, &mW, col + 64, k * kBK, bar);
+                        load_pair(st + kXBytes, &mW, col, k * kBK, bar);
+                        if (kHalf > 64) load_pair(st + kXBytes + 8192, &mW, col + 64, k * kBK, bar);
                     } else {
-                        load_pair(st + 16384, &mW, k * kBK, col, bar);
+                        load_pair(st + kXBytes, &mW, k * kBK, col, bar);
                     }
                 }
             }
@@ -184,14 +226,14 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                 const int src = lane * box < rows ? (seg.id[r >> g.log2r] << g.log2r) + (r & (rank - 1)) : 0;
                 const int src0 = __shfl_sync(kAll, src, 0), src1 = __shfl_sync(kAll, src, 1);
                 if (elect()) {
-                    uint8_t *st = ring + at.s * kStage + 16384;
+                    uint8_t *st = ring + at.s * kStage + kXBytes;
                     const uint32_t bar = full0 + at.s * 8;
-                    if (cta == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)rows * 512u);
+                    if (cta == 0) mbar_arrive_expect_tx(sh.full + at.s, (uint32_t)(rows * kPairCols * 2));
                     load_pair(st, &mB, col, src0, bar);
-                    load_pair(st + 8192, &mB, col + 64, src0, bar);
+                    if (kHalf > 64) load_pair(st + 8192, &mB, col + 64, src0, bar);
                     if (box < rows) {
                         load_pair(st + 2048, &mB, col, src1, bar);
-                        load_pair(st + 8192 + 2048, &mB, col + 64, src1, bar);
+                        if (kHalf > 64) load_pair(st + 8192 + 2048, &mB, col + 64, src1, bar);
                     }
                 }
             }
@@ -200,50 +242,61 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     } else if (warp == 1) {
         // ---------------- MMAs (the leader's warp, for both blocks) ----------------
         Ring at, tb;
-        int tl = 0;
-        constexpr uint32_t id = idesc_pair(BF, KN), idx = idesc_pair(BF, true);
+        int tl = 0, cc = 0;  // tiles, accumulators
+        constexpr uint32_t id = idesc_pair(BF, kPairCols, KN), idx = idesc_pair(BF, kPairCols, true);
         for (int i = pair; i < tiles && ok; i += pairs, ++tl) {
-            const int b = tl & 1;
-            const uint32_t acc = tmem + (uint32_t)b * 256u;
+            uint32_t acc = 0;
             if (cta == 0) {
-                if (tl >= 2 && !wait_warp<true>(sh.acc_empty + b, (uint32_t)((tl >> 1) - 1) & 1u, &sh.abort)) { ok = false; break; }
-                tc_fence_after();
+                int left = 0;  // blocks until the next accumulator
                 for (int k = 0; k < nk; ++k, at.next(kStages)) {
+                    if (left == 0) {
+                        if (k && elect()) commit_pair(sh.acc_full + ((cc - 1) & 1));
+                        if (cc >= 2 && !wait_warp<true>(sh.acc_empty + (cc & 1), (uint32_t)((cc >> 1) - 1) & 1u, &sh.abort)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        acc = tmem + (uint32_t)(cc & 1) * (uint32_t)kPairCols;
+                        left = min(C::kChunk, nk - k);
+                        ++cc;
+                    }
                     if (!wait_warp(sh.full + at.s, at.phase, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
                     if (elect()) {
-                        const uint32_t x = smem_addr(ring + at.s * kStage), w = x + 16384u;
+                        const uint32_t x = smem_addr(ring + at.s * kStage), w = x + kXBytes;
+                        const uint32_t more = left != min(C::kChunk, nk - k / C::kChunk * C::kChunk);  // not the first of its accumulator
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             mma_pair(acc, desc_kmajor_sw128(x + kk * 32),
-                                     KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32), id, k | kk);
+                                     KN ? desc_mnmajor_sw128(w + kk * 2048) : desc_kmajor_sw128(w + kk * 32), id, more | kk);
                         commit_pair(sh.empty + at.s);
                     }
+                    --left;
                 }
                 if (!ok) break;
             }
-            if (!wait_warp(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
-            const int ext = uniform(sh.seg[b].n) * rank;
-            if (cta == 0) {
+            if (!wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
+            const int ext = uniform(sh.seg[tl & 1].n) * rank;
+            if (cta == 0) {  // the adapters' part goes to the last accumulator
                 for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages), tb.next(2)) {
                     if (!wait_warp(sh.full + at.s, at.phase, &sh.abort) ||
                         !wait_warp<true>(sh.t_full + tb.s, tb.phase, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
                     if (elect()) {
-                        const uint32_t w = smem_addr(ring + at.s * kStage) + 16384u, t = smem_addr(tbuf + tb.s * kTTile);
+                        const uint32_t w = smem_addr(ring + at.s * kStage) + kXBytes, t = smem_addr(tbuf + tb.s * C::kTTile);
                         const int steps = min(kExt / 16, (ext - r0) / 16);
                         for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
-                            for (int q = 0; q < kParts; ++q)
-                                mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 0u)), desc_mnmajor_sw128(w + kk * 2048), idx, 1);
+                            for (int q = 0; q < C::kParts; ++q)
+                                mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 16384u)), desc_mnmajor_sw128(w + kk * 2048), idx, 1);
                         commit_pair(sh.empty + at.s);
                         commit_pair(sh.t_empty + tb.s);
                     }
                 }
                 if (!ok) break;
-                if (elect()) commit_pair(sh.acc_full + b);
+                if (elect()) commit_pair(sh.acc_full + ((cc - 1) & 1));
             }
-            if (lane == 0) mbar_arrive(sh.seg_empty + b);
+            if (lane == 0) mbar_arrive(sh.seg_empty + (tl & 1));
         }
         if (!ok && cta == 0 && elect()) {
             commit_pair(sh.acc_full);  // lets the waiting epilogues go on to the abort flag
@@ -251,56 +304,107 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         }
     } else if (warp >= 4 && warp < 8) {
         // ---------------- epilogue: lane = row ----------------
-        const int r = threadIdx.x - 128;
-        int tl = 0;
+        const int r = threadIdx.x - 128, w = warp - 4;
+        uint8_t *out = obuf + w * C::kOutBufs * kOut;
+        const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
+        int tl = 0, cc = 0;
         for (int i = pair; i < tiles; i += pairs, ++tl) {
-            const int b = tl & 1;
-            const Tile tile = tile_at(i, tm, tn);
-            if (!wait(sh.seg_full + b, (uint32_t)(tl >> 1) & 1u) ||
-                !wait(sh.acc_full + b, (uint32_t)(tl >> 1) & 1u) || sh.abort) { ok = false; break; }
-            tc_fence_after();
-            const int t = tile.t0 + cta * 128 + r;
-            const bool live = t < d.n_tokens;
-            const bool wide = !BF && sh.seg[b].wide[r];
-            const int a = wide ? sh.seg[b].id[sh.seg[b].row[r]] : 0;
-            const uint32_t acc = tmem + (uint32_t)b * 256u + ((uint32_t)(r & ~31) << 16);
-            uint16_t *y = static_cast<uint16_t *>(d.y) + (int64_t)t * d.ldy + tile.n0;
-#pragma unroll 1
-            for (int c = 0; c < kPairCols; c += 32) {
-                uint32_t v[32];
-                __syncwarp();
-                tmem_ld32(acc + (uint32_t)c, v);
-                tmem_ld_wait();
-                if (live) {
-                    if (!BF && wide) {
+            const Tile tile = tile_at<kPairCols>(i, tm, tn);
+            if (!wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
+            const PairSegments &seg = sh.seg[tl & 1];
+            const int t = tile.t0 + cta * 128 + r, row0 = tile.t0 + cta * 128 + w * 32;
+            const bool wide = !BF && t < d.n_tokens && seg.wide[r];
+            const int a = wide ? seg.id[seg.row[r]] : 0;
+            const uint32_t wide_rows = BF ? 0u : __ballot_sync(kAll, wide);
+            float v[F32 ? kPairCols : 64];
+            if constexpr (F32) {
+                for (int c = 0; c < chunks; ++c, ++cc) {
+                    if (!wait_warp(sh.acc_full + (cc & 1), (uint32_t)(cc >> 1) & 1u, &sh.abort)) { ok = false; break; }
+                    tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (tile.n0 + c + j < d.n_out)
-                                v[j] = __float_as_uint(__uint_as_float(v[j]) +
-                                                       adapter_dot<BF>(d, g.t + (int64_t)t * rank, a, tile.n0 + c + j));
+                    for (int n = 0; n < kPairCols; n += 16) {
+                        uint32_t u[16];
+                        tmem_ld16(lanes + (uint32_t)((cc & 1) * kPairCols + n), u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[n + j] = c ? v[n + j] + __uint_as_float(u[j]) : __uint_as_float(u[j]);
                     }
+                    tc_fence_before();
+                    arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
+                }
+                if (!ok) break;
+            } else {
+                if (!wait_warp(sh.acc_full + (cc & 1), (uint32_t)(cc >> 1) & 1u, &sh.abort)) { ok = false; break; }
+                tc_fence_after();
+            }
+            // 128 bytes of a row at a time: registers, swizzled shared memory, one TMA store per warp
+            constexpr int kRun = F32 ? 32 : 64;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 o;
-                        o.x = pack2<BF>(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
-                        o.y = pack2<BF>(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
-                        o.z = pack2<BF>(__uint_as_float(v[j + 4]), __uint_as_float(v[j + 5]));
-                        o.w = pack2<BF>(__uint_as_float(v[j + 6]), __uint_as_float(v[j + 7]));
-                        if (tile.n0 + c + j < d.n_out) *reinterpret_cast<uint4 *>(y + c + j) = o;
+            for (int c = 0; c < kPairCols; c += kRun) {
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int h = 0; h < 64; h += 32) {
+                        uint32_t u[32];
+                        tmem_ld32(lanes + (uint32_t)((cc & 1) * kPairCols + c + h), u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[h + j] = __uint_as_float(u[j]);
                     }
                 }
+                float *x = v + (F32 ? c : 0);
+                if constexpr (!BF) {  // rows whose x.A fp16 cannot hold: the warp makes a row's part, its lane takes it
+                    for (uint32_t rest = wide_rows; rest; rest &= rest - 1) {
+                        const int b = __ffs(rest) - 1, ad = __shfl_sync(kAll, a, b);
+                        const float *tb = g.t + (int64_t)(row0 + b) * rank;
+                        const int n = tile.n0 + c + lane * (kRun / 32);
+                        float p0 = 0.f, p1 = 0.f;
+                        if (n < d.n_out) p0 = adapter_dot<BF>(d, tb, ad, n);
+                        if (kRun > 32 && n + 1 < d.n_out) p1 = adapter_dot<BF>(d, tb, ad, n + 1);
+#pragma unroll
+                        for (int j = 0; j < kRun; ++j) {
+                            const float p = kRun > 32 ? __shfl_sync(kAll, j & 1 ? p1 : p0, j >> 1) : __shfl_sync(kAll, p0, j);
+                            if (lane == b) x[j] += p;
+                        }
+                    }
+                }
+                __syncwarp();
+                if (elect()) store_wait_read<0>();  // the store before has left the buffer
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint4 o;
+                    if constexpr (F32) {
+                        o = make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]),
+                                       __float_as_uint(x[4 * j + 3]));
+                    } else {
+                        o = make_uint4(pack2<BF>(x[8 * j], x[8 * j + 1]), pack2<BF>(x[8 * j + 2], x[8 * j + 3]),
+                                       pack2<BF>(x[8 * j + 4], x[8 * j + 5]), pack2<BF>(x[8 * j + 6], x[8 * j + 7]));
+                    }
+                    *reinterpret_cast<uint4 *>(out + lane * 128 + ((j ^ (lane & 7)) * 16)) = o;
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (row0 < d.n_tokens && tile.n0 + c < d.n_out && elect()) {
+                    store_box(&mY, tile.n0 + c, row0, out);
+                    store_commit();
+                }
             }
-            tc_fence_before();
-            arrive_cluster(peer_addr(sh.acc_empty + b, 0));
-            mbar_arrive(sh.seg_empty + b);
+            if constexpr (!F32) {
+                tc_fence_before();
+                arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
+                ++cc;
+            }
+            mbar_arrive(sh.seg_empty + (tl & 1));
         }
+        __syncwarp();
+        if (elect()) store_wait();
     } else if (warp >= 8) {
         // ---------------- adapters of the tile, x.A parts ----------------
         const int tid = threadIdx.x - 256;
         int tl = 0, eb = 0;
         dependency_wait();
         for (int i = pair; i < tiles; i += pairs, ++tl) {
-            const Tile tile = tile_at(i, tm, tn);
+            const Tile tile = tile_at<kPairCols>(i, tm, tn);
             if (tl >= 2 && ok) ok = wait(sh.seg_empty + (tl & 1), (uint32_t)((tl >> 1) - 1) & 1u);
             // all 128 go on or none: the named barriers below have no limit of their own
             if (!bar_all(2, 128, ok && !sh.abort)) { ok = false; break; }
@@ -366,7 +470,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             for (int r0 = 0; r0 < ext; r0 += kExt, ++eb) {  // a thread that gives up here is heard at the next tile
                 if (eb >= 2 && !wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
-                store_t_row<BF, kParts>(v, tbuf + (eb & 1) * kTTile, 0u, tid, scale);
+                store_t_row<BF, C::kParts>(v, tbuf + (eb & 1) * C::kTTile, 16384u, tid, scale);
                 if (r0 + kExt < ext) load_t_row(v, live, rank, g.log2r, tp, r0 + kExt);
                 fence_async_shared();
                 arrive_cluster(peer_addr(sh.t_full + (eb & 1), 0));
@@ -393,16 +497,21 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
 cudaError_t launch_adapter_wide(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
-    CUtensorMap mW, mB;
-    if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
-        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb,
-                     d.rank < kExt ? d.rank : kExt))
+    const bool f32 = d.y_type == LATENT_TYPE_F32;
+    const int cols = f32 ? Cfg<true, true>::kCols : Cfg<true, false>::kCols;
+    CUtensorMap mW, mB, mY;
+    if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK)
+             : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, cols / 2)) ||
+        !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, d.rank < kExt ? d.rank : kExt) ||
+        !adapter_out_map(&mY, d.y_type, d.y, d.n_tokens, d.n_out, d.ldy, 32))
         return cudaErrorInvalidValue;
-    const void *fn = bf ? kn ? (const void *)k_ad_wide<true, true> : (const void *)k_ad_wide<true, false>
-                        : kn ? (const void *)k_ad_wide<false, true> : (const void *)k_ad_wide<false, false>;
+    const void *fn = f32 ? bf ? kn ? (const void *)k_ad_wide<true, true, true> : (const void *)k_ad_wide<true, false, true>
+                              : kn ? (const void *)k_ad_wide<false, true, true> : (const void *)k_ad_wide<false, false, true>
+                     : bf ? kn ? (const void *)k_ad_wide<true, true, false> : (const void *)k_ad_wide<true, false, false>
+                          : kn ? (const void *)k_ad_wide<false, true, false> : (const void *)k_ad_wide<false, false, false>;
     cudaError_t err = ensure_smem(fn, kSmem);
     if (err != cudaSuccess) return err;
-    const int64_t tiles = ((int64_t)d.n_tokens + kPairRows - 1) / kPairRows * ((d.n_out + kPairCols - 1) / kPairCols);
+    const int64_t tiles = ((int64_t)d.n_tokens + kPairRows - 1) / kPairRows * ((d.n_out + cols - 1) / cols);
     const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * pairs);
@@ -415,7 +524,7 @@ cudaError_t launch_adapter_wide(const AdapterArgs &g, const void *x_map, int sms
     cfg.attrs = at;
     cfg.numAttrs = 1;
     AdapterArgs a = g;
-    void *args[] = {const_cast<void *>(x_map), &mW, &mB, &a};
+    void *args[] = {const_cast<void *>(x_map), &mW, &mB, &mY, &a};
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
