@@ -128,6 +128,44 @@ bool ad_tensor_cores(const latent_adapter_desc *d) {
            ad_aligned(d->a, 16) && ad_aligned(d->b, 16) && ad_aligned(d->y, 16);
 }
 
+enum AdapterPath { kPathSelf, kPathSkinny, kPathWide };
+
+int tile_rows(int n, AdapterPath path) { return path == kPathWide || n >= adapter::kRows ? adapter::kRows : (n + 15) / 16 * 16; }
+
+// Which kernels serve a call, by what they cost in measured steps (B200,
+// bf16): k_ad_skinny takes 0.5 us per 64 of a block's share of K at 128 rows
+// (as many bytes less at fewer), k_ad_wide 0.23 us (fp32 results 0.26) per 64
+// of K and 3 us more to start where the batch is too small to hide it.  An
+// extension block of 32 stacked rank columns, of which a batch of single
+// tokens may need one per adapter and 32 ranks, costs 0.5 us of one of a
+// cluster's blocks against 0.8 us of the pair.  E.g. 1024 rows of 2048 x 2048
+// (rank 16): 25.6 us skinny, 18.0 wide; 1024 rows of 7168 x 512: 24.4 and 39.8.
+// Up to 64 rows whose adapters fit one tile of 128 stacked rank columns, with
+// at most 8 steps of K per block, k_ad_skinny makes x.A itself (one row of
+// 1024 x 4096: 8.5 us against 10.3 in two launches, of 7168 x 2048: 15.7
+// against 11.5).
+AdapterPath pick_path(const AdapterArgs &g, int sms) {
+    const latent_adapter_desc &d = g.d;
+    AdapterArgs a = g;
+    a.tile_rows = tile_rows(d.n_tokens, kPathSkinny);
+    const int64_t nk = (d.n_in + 63) / 64;
+    const int64_t stacked = (int64_t)(d.n_adapter < d.n_tokens ? d.n_adapter : d.n_tokens) * d.rank;
+    if (d.n_tokens <= 64 && stacked <= 128) {
+        const int c = adapter_self_cluster(a);
+        if ((nk + c - 1) / c <= 8) return kPathSelf;
+    }
+    if (d.n_tokens <= 96) return kPathSkinny;
+    const int64_t ext = d.n_tokens <= 256 ? (stacked + 31) / 32 : 0;  // longer batches: packed prompts, few adapters a tile
+    const int c = adapter_skinny_cluster(a, sms);
+    const int64_t clusters = ((int64_t)d.n_tokens + 127) / 128 * ((d.n_out + 127) / 128);
+    const int64_t skinny = adapter_waves(clusters, c) * ((nk + c - 1) / c + (ext + c - 1) / c) * 50;
+    const int cols = d.y_type == LATENT_TYPE_F32 ? 128 : 256;
+    const int64_t tiles = ((int64_t)d.n_tokens + 255) / 256 * ((d.n_out + cols - 1) / cols);
+    const int64_t wide = (tiles + sms / 2 - 1) / (sms / 2) * (nk * (cols == 128 ? 26 : 23) + ext * 80) +
+                         (d.n_tokens <= 256 ? 300 : 0);
+    return wide < skinny ? kPathWide : kPathSkinny;
+}
+
 }  // namespace
 
 }  // namespace latent
@@ -136,7 +174,7 @@ extern "C" LATENT_API int latent_adapter_workspace_size(const latent_adapter_des
     const int st = latent::ad_validate(d);
     if (st) return st;
     if (!bytes) return LATENT_ERR_INVALID;
-    *bytes = latent::adapter_t_bytes(d->n_tokens, d->rank) + latent::adapter_flag_bytes(d->n_tokens, d->n_adapter, d->rank) + 256;
+    *bytes = ((size_t)d->n_tokens * d->rank * 4 + 511) / 256 * 256;
     return LATENT_OK;
 }
 
@@ -169,20 +207,17 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         AdapterArgs a{};
         a.d = *d;
         a.t = tt;
-        a.tile_rows = d->n_tokens < adapter::kRows ? (d->n_tokens + 15) / 16 * 16 : adapter::kRows;
         a.log2r = d->rank == 16 ? 4 : d->rank == 32 ? 5 : d->rank == 64 ? 6 : 7;
-        a.most = adapter_most(d->n_tokens, d->n_adapter, d->rank);
-        a.flags = reinterpret_cast<uint64_t *>(static_cast<char *>(d->workspace) + adapter_t_bytes(d->n_tokens, d->rank));
+        const AdapterPath path = pick_path(a, sms);
+        a.tile_rows = tile_rows(d->n_tokens, path);
         CUtensorMap x;
         if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows))
             return LATENT_ERR_CUDA;
-        cudaError_t err;
-        if (d->n_tokens <= adapter::kRows && launch_adapter_decode(a, &x, s, &err))
-            return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
-        const bool wide = d->n_tokens > 256;
-        if (launch_adapter_shrink(a, &x, sms, s) != cudaSuccess ||
-            (wide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, s)) != cudaSuccess)
-            return LATENT_ERR_CUDA;
+        cudaError_t err = cudaSuccess;
+        if (path != kPathSelf) err = launch_adapter_shrink(a, &x, sms, s);
+        if (err == cudaSuccess)
+            err = path == kPathWide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, path == kPathSelf, s);
+        if (err != cudaSuccess) return LATENT_ERR_CUDA;
         return LATENT_OK;
     }
     const dim3 gs((unsigned)d->n_tokens, (unsigned)d->rank / kShrinkWarps);

@@ -22,29 +22,20 @@ struct AdapterArgs {
     float *t;        // [T][rank] x.A (fp32)
     int tile_rows;   // rows per tile: 128, fewer rounded up to 16
     int log2r;       // rank = 1 << log2r
-    // k_ad_skinny's one-launch form
-    uint64_t *flags; // [blocks][tiles of stacked rank columns][cluster]
-    uint64_t nonce;  // what a flag holds once its partial sums are there
-    int most;        // tiles of stacked rank columns at most
 };
 
-// Workspace: t, then the flags of the one-launch form, which serves one tile of rows.
-constexpr int kMaxCluster = 16, kMaxBlocks = 256;
-inline size_t adapter_t_bytes(int64_t T, int rank) { return (T * rank * 4 + 255) / 256 * 256; }
-inline int adapter_most(int64_t T, int n_adapter, int rank) {
-    return (int)(((int64_t)(n_adapter < T ? n_adapter : T) * rank + 127) / 128);
-}
-inline size_t adapter_flag_bytes(int64_t T, int n_adapter, int rank) {
-    return T <= 128 ? (size_t)kMaxBlocks * kMaxCluster * 8 * adapter_most(T, n_adapter, rank) : 0;
-}
-
+constexpr int kMaxCluster = 16;
 
 // x_map: the CUtensorMap of x with a box of tile_rows rows.
-// One launch for both steps; false where it does not serve the call (*err then untouched).
-bool launch_adapter_decode(const AdapterArgs &a, const void *x_map, cudaStream_t s, cudaError_t *err);
 cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
-cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, cudaStream_t s);
+// self: with x.A in the same launch (one tile of rows).
+cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, int sms, bool self, cudaStream_t s);
 cudaError_t launch_adapter_wide(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
+// What the choice between them goes by: blocks that split K (with x.A in a launch of its own, and in the same), and
+// how often that many clusters have to take turns.
+int adapter_skinny_cluster(const AdapterArgs &a, int sms);
+int adapter_self_cluster(const AdapterArgs &a);
+int adapter_waves(int64_t clusters, int cluster);
 
 namespace adapter {
 

@@ -10,13 +10,12 @@
 // partial tiles are added up in rank order through distributed shared memory,
 // so results do not depend on timing.
 //
-// k_ad_skinny is launched as a programmatic dependent of k_ad_shrink: it
+// k_ad_skinny is launched as a programmatic dependent of k_ad_shrink (unless it
+// makes x.A itself): it
 // streams W while x.A is still being made and waits for it (griddepcontrol)
 // only before the extension blocks.
 #include <cuda.h>
 
-#include <atomic>
-#include <chrono>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -35,7 +34,7 @@ constexpr int kMaxTBufs = 4;
 
 struct Shared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2], t_full[kMaxTBufs], t_empty[kMaxTBufs], seg, sent;
+    uint64_t acc_full[2], acc_empty[2], t_full[kMaxTBufs], t_empty[kMaxTBufs], seg;
     uint32_t tmem;
     volatile int abort;
     uint8_t wide[kRows];   // fp16: rows finished in fp32
@@ -49,7 +48,7 @@ struct Plan {
     int stages;
     int chunk;      // blocks per accumulator (k_ad_skinny)
     int tbufs;      // tiles of x.A parts
-    int shrink_col; // x.A's accumulator behind the product's (one-launch form)
+    int shrink_col; // x.A's accumulator behind the product's (SELF)
     uint32_t cols;  // TMEM columns
     size_t smem;
 };
@@ -72,7 +71,7 @@ __device__ __forceinline__ void drain() {
 // Barriers by warp 0, which goes on at once (its first loads wait for nobody),
 // TMEM by warp 2, which then lets a dependent kernel start.
 template <bool DEPENDENTS>
-__device__ __forceinline__ void setup(Shared &sh, const Plan &p, int cluster, int warp, int lane) {
+__device__ __forceinline__ void setup(Shared &sh, const Plan &p, int warp, int lane) {
     if (warp == 0) {
         if (lane == 0) {
             for (int s = 0; s < p.stages; ++s) {
@@ -88,7 +87,6 @@ __device__ __forceinline__ void setup(Shared &sh, const Plan &p, int cluster, in
                 mbar_init(sh.t_empty + b, 1);
             }
             mbar_init(&sh.seg, 128);
-            mbar_init(&sh.sent, (uint32_t)cluster * 4u);  // the four epilogue warps of every rank
             sh.abort = 0;
             fence_barrier_init();
         }
@@ -134,13 +132,7 @@ __device__ __forceinline__ void set_dest(Shared &sh, const float *recv, int r, i
     sh.dest[r] = r < nt ? map_rank(smem_addr(recv) + (uint32_t)(q * per + r % per) * row_bytes, r / per) : kNoRow;
 }
 
-__device__ __forceinline__ void arrive_rank(uint64_t *bar, int rank) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_addr(bar), rank))
-                 : "memory");
-}
-
 // By the load warp: the K blocks [k0, k1) of stacked rank columns m .. m + 127 (rows of A) and of x.
-template <bool BF>
 __device__ __forceinline__ bool load_stacked(Shared &sh, const Plan &p, Ring &at, uint8_t *ring, uint32_t stage,
                                              const CUtensorMap *mA, const CUtensorMap *mX, int m, int total, int k0,
                                              int k1, int t0, int rank, int log2r) {
@@ -180,6 +172,25 @@ __device__ __forceinline__ bool multiply_stacked(Shared &sh, const Plan &p, Ring
     return true;
 }
 
+// By the epilogue warps: x.A of the tile at stacked column m (acc: lane = stacked column, column = row of x) to the
+// rows' owners, `off` bytes into a row's place.
+__device__ __forceinline__ void send_stacked(const Shared &sh, const Plan &p, uint32_t acc, int m, int rank, int log2r,
+                                             int tid, uint32_t off) {
+    const int seg = (m + tid) >> log2r;
+    off += ((uint32_t)(m + tid) & (uint32_t)(rank - 1)) * 4u;
+    for (int c = 0; c < p.rows; c += 32) {
+        uint32_t v[32], to[32], of[32];
+        __syncwarp();
+        tmem_ld32(acc + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
+        load32(sh.dest + c, to);
+        load32(sh.segs.row + c, of);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if ((int)of[i] == seg) st_cluster(to[i] + off, __uint_as_float(v[i]));
+    }
+}
+
 // x.A.  Block (cluster rank, slot, row tile); the stacked rank columns of the
 // tile's adapters in tiles of 128: slot, slot + gridDim.y, ...  Rank q of the
 // cluster sums K blocks of its share; every block sends the t of a row to the
@@ -208,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         const int r = threadIdx.x - 128;
         a = row_adapter(d, t0 + r, r < nt, q == 0 && blockIdx.y == 0);
     }
-    setup<true>(sh, p, CS, warp, lane);
+    setup<true>(sh, p, warp, lane);
     const uint32_t tmem = warp ? (uint32_t)uniform((int)sh.tmem) : 0u, read = (uint32_t)(p.rows + 31) & ~31u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
@@ -224,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     if (warp == 0) {
         Ring at;
         for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128)
-            ok = load_stacked<BF>(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
+            ok = load_stacked(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
     } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, false, false);
         Ring at;
@@ -249,18 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
             if (!wait(sh.acc_full + b, (n >> 1) & 1u) || sh.abort) ok = false;
             if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
             tc_fence_after();
-            const int seg = (m + tid) >> log2r, j = (m + tid) & (rank - 1);
-            for (int c = 0; c < p.rows; c += 32) {
-                uint32_t v[32], to[32], of[32];
-                __syncwarp();
-                tmem_ld32(tmem + b * read + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
-                load32(sh.dest + c, to);
-                load32(sh.segs.row + c, of);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if ((int)of[i] == seg) st_cluster(to[i] + (uint32_t)j * 4u, __uint_as_float(v[i]));
-            }
+            send_stacked(sh, p, tmem + b * read, m, rank, log2r, tid, 0u);
             tc_fence_before();
             mbar_arrive(sh.acc_empty + b);
         }
@@ -289,47 +289,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     if (warp == 2) tmem_dealloc(tmem, p.cols);
 }
 
-__device__ __forceinline__ void st_release(uint64_t *p, uint64_t v) {
-    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-__device__ __forceinline__ uint64_t ld_acquire(const uint64_t *p) {
-    uint64_t v;
-    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-    return v;
-}
-
 // The product.  Block (cluster rank, 128 output columns, row tile).
 //
-// kSelf (one launch, one tile of rows): every cluster makes all of x.A itself,
+// SELF (one launch, one tile of rows): every cluster makes all of x.A itself,
 // behind its W loads, and the owner of a row adds x.A.B for its 128 columns on
 // the CUDA cores: no trip of x.A through global memory, at the price of every
 // cluster loading the adapters' A.
-//
-// kOne (one launch for both steps, one tile of rows, a cooperative launch):
-// the x.A tiles of 128 stacked rank columns are dealt to the clusters, which
-// make theirs before they turn to W (sums over the ranks' parts of K by the
-// rows' owners, as above).  A block that has stored its rows of a tile sets a
-// flag for every block of the grid (its own copy: [reader][tile][rank]); a
-// reader waits for all
-// flags of the call and clears them, so that the words are ready for the next
-// replay of a captured launch.  A flag is set to the call's nonce, 64 bits that
-// no call before it used: whatever the workspace holds at first, nothing has to
-// be cleared by a launch of its own.
-enum Mode { kTwo, kOne, kSelf };
-
-template <bool BF, bool KN, int PARTS, typename Y, Mode MODE>
+template <bool BF, bool KN, int PARTS, typename Y, bool SELF>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant__ CUtensorMap mW,
                                                            const __grid_constant__ CUtensorMap mB,
                                                            const __grid_constant__ CUtensorMap mX,
                                                            const __grid_constant__ CUtensorMap mA, AdapterArgs g,
                                                            Plan p) {
     constexpr uint32_t kTiles = (PARTS + 1) / 2;
-    constexpr bool ONE = MODE == kOne, SELF = MODE == kSelf;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = align1024(raw);
     const uint32_t xbytes = (uint32_t)p.rows * 128u, stage = 16384u + xbytes;
     uint8_t *tbuf = ring + p.stages * stage;                                      // tbufs x kTiles x [rows][128 bytes]
-    // [cluster][rows of a rank][128 sums, kSelf: and those of x.A]
+    // [cluster][rows of a rank][128 sums, SELF: and those of x.A]
     float *recv = reinterpret_cast<float *>(tbuf + p.tbufs * kTiles * xbytes);
     __shared__ Shared sh;
     const int q = blockIdx.x, CS = gridDim.x;
@@ -344,28 +321,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         prefetch_tensormap(&mW);
         prefetch_tensormap(&mX);
         prefetch_tensormap(&mB);
-        if (MODE != kTwo) prefetch_tensormap(&mA);
+        if (SELF) prefetch_tensormap(&mA);
     } else if (warp >= 4) {
         const int r = threadIdx.x - 128;
-        a = row_adapter(d, t0 + r, r < nt, MODE != kTwo && q == 0 && blockIdx.y == 0);
+        a = row_adapter(d, t0 + r, r < nt, SELF && q == 0 && blockIdx.y == 0);
     }
-    setup<false>(sh, p, CS, warp, lane);
+    setup<false>(sh, p, warp, lane);
     const uint32_t tmem = warp ? (uint32_t)uniform((int)sh.tmem) : 0u;
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
-    const int slot = SELF ? 0 : blockIdx.y, slots = SELF ? 1 : gridDim.y;
-    const bool shrinks = SELF || (ONE && slot < g.most);  // this cluster may have tiles of x.A
     bool ok = true;
     if (warp == 0) {
         Ring at;
-        auto load_a = [&]() {
-            ok = wait_warp(&sh.seg, 0u, &sh.abort);
-            const int total = ok ? uniform(sh.segs.n) * rank : 0;
-            for (int m = slot * 128; m < total && ok; m += slots * 128)
-                ok = load_stacked<BF>(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
-        };
-        if (ONE && shrinks) load_a();
         for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
             if (at.wrapped && !wait_warp(sh.empty + at.s, at.phase ^ 1u, &sh.abort)) { ok = false; break; }
             if (elect()) {
@@ -380,8 +348,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 tma_load_2d(st + 16384, &mX, k * kBK, t0, sh.full + at.s);
             }
         }
-        if (SELF && ok) load_a();
-        if (!SELF && ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
+        if (ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
+        if (SELF && ok) {
+            const int total = uniform(sh.segs.n) * rank;
+            for (int m = 0; m < total && ok; m += 128)
+                ok = load_stacked(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
+        }
         if (!SELF && ok) {
             const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
             const int e1 = (int)((int64_t)ne * (q + 1) / CS), box = min(rank, kExt);
@@ -405,18 +377,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
         Ring at;
-        auto multiply_a = [&]() {
-            ok = wait_warp(&sh.seg, 0u, &sh.abort);
-            const int total = ok ? uniform(sh.segs.n) * rank : 0;
-            uint32_t n = 0;
-            for (int m = slot * 128; m < total && ok; m += slots * 128, ++n) {
-                if (n >= 1 && !wait_warp(sh.acc_empty + 1, (n - 1u) & 1u, &sh.abort)) { ok = false; break; }
-                tc_fence_after();
-                ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
-                if (ok && elect()) mma_commit(sh.acc_full + 1);
-            }
-        };
-        if (ONE && shrinks) multiply_a();
         int in_chunk = 0;
         uint32_t acc = tmem;
         for (int k = k0; ok && k < k1; ++k, at.next(p.stages)) {
@@ -436,11 +396,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             }
             ++in_chunk;
         }
-        if (SELF) {
-            if (ok && elect()) mma_commit(sh.acc_full);
-            if (ok) multiply_a();
-        } else if (ok) {
-            ok = wait_warp(&sh.seg, 0u, &sh.abort);
+        if (SELF && ok && elect()) mma_commit(sh.acc_full);
+        if (ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
+        if (SELF && ok) {
+            const int total = uniform(sh.segs.n) * rank;
+            uint32_t n = 0;
+            for (int m = 0; m < total; m += 128, ++n) {
+                if (n >= 1 && !wait_warp(sh.acc_empty + 1, (n - 1u) & 1u, &sh.abort)) { ok = false; break; }
+                tc_fence_after();
+                ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
+                if (!ok) break;
+                if (elect()) mma_commit(sh.acc_full + 1);
+            }
         }
         if (!SELF && ok) {
             const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
@@ -466,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             }
         }
         if (elect()) {
-            if (!ok && MODE != kTwo) mma_commit(sh.acc_full + 1);
+            if (!ok && SELF) mma_commit(sh.acc_full + 1);
             if (!SELF || !ok) mma_commit(sh.acc_full);
         }
     } else if (warp >= 4) {
@@ -475,25 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         set_dest(sh, recv, r, nt, per, q, (uint32_t)pitch * 4u);
         mbar_arrive(&sh.seg);
         ok = wait(&sh.seg, 0u);
-        const int ext = ok ? sh.segs.n * rank : 0, ne = (ext + kExt - 1) / kExt;
-        // x.A of the tile at stacked column m, column j of this lane's adapter, to the rows' owners, `off` bytes into a row
-        auto send_a = [&](int m, uint32_t off) {
-            const int seg = (m + r) >> log2r;
-            const uint32_t j = (uint32_t)(m + r) & (uint32_t)(rank - 1);
-            for (int c = 0; c < p.rows; c += 32) {
-                uint32_t v[32], to[32], of[32];
-                __syncwarp();
-                tmem_ld32(tmem + (uint32_t)p.shrink_col + ((uint32_t)(r & ~31) << 16) + (uint32_t)c, v);
-                load32(sh.dest + c, to);
-                load32(sh.segs.row + c, of);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if ((int)of[i] == seg) st_cluster(to[i] + off + j * 4u, __uint_as_float(v[i]));
-            }
-            tc_fence_before();
-            mbar_arrive(sh.acc_empty + 1);
-        };
+        const int ext = ok ? sh.segs.n * rank : 0;
         // column c of the accumulator = row c of x, to its owner
         auto send_product = [&]() {
             const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
@@ -524,75 +473,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             for (int m = 0; m < ext && ok; m += 128, ++n) {
                 ok = __all_sync(0xffffffffu, wait(sh.acc_full + 1, n & 1u) && !sh.abort);
                 tc_fence_after();
-                if (ok) send_a(m, 512u);
+                if (ok) send_stacked(sh, p, tmem + (uint32_t)p.shrink_col, m, rank, log2r, r, 512u);
+                tc_fence_before();
+                mbar_arrive(sh.acc_empty + 1);
             }
-        }
-        if constexpr (ONE) {
-            // From here to the flags all 128 threads go on or none: the named barrier has no limit of its own.
-            const int tiles = (ext + 127) / 128, own0 = q * per, own = max(0, min(nt, own0 + per) - own0);
-            uint32_t n = 0;
-            cluster_wait();
-            for (int m = slot * 128; m < ext; m += slots * 128, ++n) {
-                ok = ok && wait(sh.acc_full + 1, n & 1u) && !sh.abort;
-                if (!bar_all(1, kRows, ok)) { ok = false; break; }
-                tc_fence_after();
-                send_a(m, 0u);
-                __syncwarp();
-                if (lane < CS) arrive_rank(&sh.sent, lane);
-                ok = wait<true>(&sh.sent, n & 1u) && !sh.abort;
-                if (!bar_all(1, kRows, ok)) { ok = false; break; }
-                for (int i = r; i < own << log2r; i += kRows) {
-                    const int row = i >> log2r, s = sh.segs.row[own0 + row];
-                    if (s < 0 || (s << log2r) < m || (s << log2r) >= m + 128) continue;
-                    float v = 0.f;
-                    for (int c = 0; c < CS; ++c) v += recv[(c * per + row) * 128 + (i & (rank - 1))];
-                    g.t[((int64_t)(t0 + own0) << log2r) + i] = v;
-                }
-                bar_sync(1, kRows);  // all stores of the block, before the flags that release them
-                for (int i = r; i < slots * CS; i += kRows)
-                    st_release(g.flags + ((int64_t)i * g.most + m / 128) * CS + q, g.nonce);
-            }
-            uint64_t *mine = g.flags + (int64_t)(slot * CS + q) * g.most * CS;
-            const unsigned long long since = global_ns();
-            for (int i = r; i < tiles * CS && ok; i += kRows) {
-                while (ld_acquire(mine + i) != g.nonce) {
-                    if (sh.abort || global_ns() - since > kWaitNs) {
-                        ok = false;
-                        break;
-                    }
-                }
-                if (ok) mine[i] = 0;
-            }
-            ok = bar_all(1, kRows, ok);
         }
         if constexpr (!SELF) {
-        if (!ONE) dependency_wait();
-        const int seg = ok ? sh.segs.row[r] : -1;
-        const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
-        const float *t = g.t + ((int64_t)(t0 + r) << log2r);
-        const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
-        const bool wide = !BF && seg >= 0 && beyond_f16(t, scale, rank);
-        sh.wide[r] = wide;
-        const int live = wide ? -1 : seg;
-        float4 v[8];
-        if (e0 < e1) load_t_row(v, live, rank, log2r, t, e0 * kExt);
-        Ring tb;
-        for (int e = e0; e < e1 && ok; ++e, tb.next(p.tbufs)) {
-            const int b = tb.s;
-            if (tb.wrapped && !wait(sh.t_empty + b, tb.phase ^ 1u)) { ok = false; break; }
-            if (sh.abort) { ok = false; break; }
-            if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)b * kTiles * xbytes, xbytes, r, scale);
-            fence_async_shared();
-            mbar_arrive(sh.t_full + b);
-            if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
-        }
-        if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
-        __syncwarp();
-        if (!wait(sh.acc_full, 0u)) ok = false;
-        __syncwarp();
-        tc_fence_after();
-        if (!ONE) cluster_wait();
-        send_product();
+            const int seg = ok ? sh.segs.row[r] : -1;
+            const int ne = (ext + kExt - 1) / kExt;
+            const int e0 = (int)((int64_t)ne * q / CS), e1 = (int)((int64_t)ne * (q + 1) / CS);
+            const float *t = g.t + ((int64_t)(t0 + r) << log2r);
+            const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
+            dependency_wait();
+            const bool wide = !BF && seg >= 0 && beyond_f16(t, scale, rank);
+            sh.wide[r] = wide;
+            const int live = wide ? -1 : seg;
+            float4 v[8];
+            if (e0 < e1) load_t_row(v, live, rank, log2r, t, e0 * kExt);
+            Ring tb;
+            for (int e = e0; e < e1 && ok; ++e, tb.next(p.tbufs)) {
+                if (tb.wrapped && !wait(sh.t_empty + tb.s, tb.phase ^ 1u)) { ok = false; break; }
+                if (sh.abort) { ok = false; break; }
+                if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)tb.s * kTiles * xbytes, xbytes, r, scale);
+                fence_async_shared();
+                mbar_arrive(sh.t_full + tb.s);
+                if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
+            }
+            if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
+            __syncwarp();
+            if (!wait(sh.acc_full, 0u)) ok = false;
+            __syncwarp();
+            tc_fence_after();
+            cluster_wait();
+            send_product();
         }
     }
     if (!ok) {
@@ -605,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
     cluster_wait();
     // this block's rows, two columns per thread: the cluster's parts in rank order
     const int r0 = q * per, r1 = min(nt, r0 + per);
-    float *own_t = reinterpret_cast<float *>(ring);  // kSelf: [row][rank] scale * x.A (the ring's loads have all been used)
+    float *own_t = reinterpret_cast<float *>(ring);  // SELF: [row][rank] scale * x.A (the ring's loads have all been used)
     if constexpr (SELF) {
         for (int i = threadIdx.x; i < max(0, r1 - r0) << log2r; i += kThreads) {
             const int row = i >> log2r, s = sh.segs.row[r0 + row];
@@ -704,10 +617,7 @@ cudaError_t allow_clusters(const void *fn) {
     return err;
 }
 
-constexpr int kSelfTiles = 1;  // x.A tiles at most that every cluster makes itself
-
-enum Launch { kPlain, kDependent, kCooperative };
-cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, Launch how, void **args, cudaStream_t s) {
+cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, bool dependent, void **args, cudaStream_t s) {
     cudaError_t err = ensure_smem(fn, smem);
     if (err != cudaSuccess || (grid.x > 8 && (err = allow_clusters(fn)) != cudaSuccess)) return err;
     cudaLaunchConfig_t cfg{};
@@ -720,15 +630,10 @@ cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, Launch how, v
     at[0].val.clusterDim.x = grid.x;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
-    if (how == kDependent) {
-        at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[1].val.programmaticStreamSerializationAllowed = 1;
-    } else {
-        at[1].id = cudaLaunchAttributeCooperative;
-        at[1].val.cooperative = 1;
-    }
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = how == kPlain ? 1 : 2;
+    cfg.numAttrs = dependent ? 2 : 1;
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
@@ -787,27 +692,16 @@ int pick_stages(size_t stage, size_t other, int loads) {
     return n < loads ? n : loads;
 }
 
-template <typename Y, Mode MODE>
+template <typename Y, bool SELF>
 const void *skinny_fn(bool bf, bool kn) {
     constexpr int P = sizeof(Y) == 4 ? 3 : 2;
-    if (bf) return kn ? (const void *)k_ad_skinny<true, true, P, Y, MODE> : (const void *)k_ad_skinny<true, false, P, Y, MODE>;
-    return kn ? (const void *)k_ad_skinny<false, true, 2, Y, MODE> : (const void *)k_ad_skinny<false, false, 2, Y, MODE>;
+    if (bf) return kn ? (const void *)k_ad_skinny<true, true, P, Y, SELF> : (const void *)k_ad_skinny<true, false, P, Y, SELF>;
+    return kn ? (const void *)k_ad_skinny<false, true, 2, Y, SELF> : (const void *)k_ad_skinny<false, false, 2, Y, SELF>;
 }
-template <Mode MODE>
+template <bool SELF>
 const void *skinny_fn(bool bf, bool kn, bool f32) {
-    if (f32) return skinny_fn<float, MODE>(bf, kn);
-    return bf ? skinny_fn<__nv_bfloat16, MODE>(bf, kn) : skinny_fn<__half, MODE>(bf, kn);
-}
-
-// 64 bits that no call of this process used before.
-uint64_t next_nonce() {
-    static std::atomic<uint64_t> count{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() ^
-                                       (uint64_t)(uintptr_t)&count};
-    uint64_t z = count.fetch_add(0x9E3779B97F4A7C15ull) + 0x9E3779B97F4A7C15ull;  // splitmix64: a bijection of the count
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    z ^= z >> 31;
-    return z ? z : 1;
+    if (f32) return skinny_fn<float, SELF>(bf, kn);
+    return bf ? skinny_fn<__nv_bfloat16, SELF>(bf, kn) : skinny_fn<__half, SELF>(bf, kn);
 }
 
 }  // namespace
@@ -837,95 +731,120 @@ bool adapter_out_map(void *map, int y_type, void *base, uint64_t rows, uint64_t 
     return adapter_map(map, y_type == LATENT_TYPE_BF16, base, rows, cols, ld, box_rows);
 }
 
+namespace {
+
+struct ShrinkPlan {
+    Plan p;
+    int cluster, slots, tiles;
+};
+ShrinkPlan plan_shrink(const AdapterArgs &g, int sms, const int *room) {
+    const latent_adapter_desc &d = g.d;
+    ShrinkPlan r{};
+    Plan &p = r.p;
+    r.tiles = (d.n_tokens + g.tile_rows - 1) / g.tile_rows;
+    const int most = ((d.n_adapter < g.tile_rows ? d.n_adapter : g.tile_rows) * d.rank + 127) / 128;
+    const int nk = (d.n_in + kBK - 1) / kBK;
+    p.rows = (g.tile_rows + 15) / 16 * 16;
+    const size_t stage = 16384 + (size_t)p.rows * 128;
+    r.cluster = pick_cluster(r.tiles, nk, room);
+    const size_t recv = recv_bytes(g.tile_rows, r.cluster, d.rank * 4);
+    r.slots = sms / (r.tiles * r.cluster);  // tiles of stacked rank columns side by side
+    r.slots = r.slots < 1 ? 1 : r.slots > most ? most : r.slots;
+    p.stages = pick_stages(stage, recv, (nk + r.cluster - 1) / r.cluster * ((most + r.slots - 1) / r.slots));
+    p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
+    p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
+    return r;
+}
+
+// Blocks of a cluster of k_ad_skinny.  Where both kernels are small, its
+// clusters start beside the shrink's blocks and stream W meanwhile, so those
+// SMs are not counted on (4096 columns, one row: 10.3 us with, 8.8 without).
+int plan_skinny(const AdapterArgs &g, int sms, const int *room, int beside) {
+    const latent_adapter_desc &d = g.d;
+    const int64_t others = ((int64_t)d.n_tokens + g.tile_rows - 1) / g.tile_rows * ((d.n_out + 127) / 128);
+    const int nk = (d.n_in + kBK - 1) / kBK;
+    int c = pick_cluster(others, nk, room);
+    while (beside && c > 1 && others * c > sms - beside) --c;
+    return c;
+}
+
+}  // namespace
+
 cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16;
-    const int tiles = (d.n_tokens + g.tile_rows - 1) / g.tile_rows;
-    const int most = ((d.n_adapter < g.tile_rows ? d.n_adapter : g.tile_rows) * d.rank + 127) / 128;
-    const int nk = (d.n_in + kBK - 1) / kBK;
-    Plan p{};
-    p.rows = (g.tile_rows + 15) / 16 * 16;
     const int *room = cluster_room();
     if (!room) return cudaErrorInvalidConfiguration;
-    const size_t stage = 16384 + (size_t)p.rows * 128;
-    const int cluster = pick_cluster(tiles, nk, room);
-    const size_t recv = recv_bytes(g.tile_rows, cluster, d.rank * 4);
-    int slots = sms / (tiles * cluster);  // tiles of stacked rank columns side by side
-    slots = slots < 1 ? 1 : slots > most ? most : slots;
-    p.stages = pick_stages(stage, recv, (nk + cluster - 1) / cluster * ((most + slots - 1) / slots));
-    p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
-    p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
+    ShrinkPlan r = plan_shrink(g, sms, room);
+    if (r.p.stages < 1) return cudaErrorInvalidConfiguration;
     CUtensorMap mA;
     if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank)) return cudaErrorInvalidValue;
     AdapterArgs a = g;
-    void *args[] = {&mA, const_cast<void *>(x_map), &a, &p};
+    void *args[] = {&mA, const_cast<void *>(x_map), &a, &r.p};
     return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
-                          dim3(cluster, slots, tiles), p.smem, kPlain, args, s);
+                          dim3(r.cluster, r.slots, r.tiles), r.p.smem, false, args, s);
 }
 
-namespace {
-
-// One launch of k_ad_skinny; false, with nothing launched, where a cooperative launch (kOne) would not fit the device.
-bool launch_skinny(const AdapterArgs &g, const void *x_map, Mode mode, cudaStream_t s, cudaError_t *err) {
+cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, bool self, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16, kn = !(d.flags & LATENT_ADAPTER_W_TRANSPOSED);
-    const bool f32 = d.y_type == LATENT_TYPE_F32, shrinks = mode != kTwo;
+    const bool f32 = d.y_type == LATENT_TYPE_F32;
     const int tiles = (d.n_tokens + g.tile_rows - 1) / g.tile_rows, ntn = (d.n_out + 127) / 128;
     const int nk = (d.n_in + kBK - 1) / kBK;
+    const int *room = cluster_room();
+    if (!room) return cudaErrorInvalidConfiguration;
     Plan p{};
     p.rows = (g.tile_rows + 15) / 16 * 16;
     const int parts = bf && f32 ? 3 : 2;
-    *err = cudaErrorInvalidConfiguration;
-    const int *room = cluster_room();
-    if (!room) return true;
     // as far as the ring still holds the loads of a trip to DRAM
-    p.tbufs = mode == kSelf ? 0 : p.rows <= 64 ? kMaxTBufs : 2;
+    p.tbufs = self ? 0 : p.rows <= 64 ? kMaxTBufs : 2;
     const size_t stage = 16384 + (size_t)p.rows * 128, tb = (size_t)p.tbufs * ((parts + 1) / 2) * p.rows * 128;
-    int cluster = pick_cluster((int64_t)tiles * ntn, nk, room);
+    int cluster = self ? pick_cluster((int64_t)tiles * ntn, nk, room) : adapter_skinny_cluster(g, sms);
     // The tensor cores cut a sum off instead of rounding it: a chain over K
     // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
     // fp32 results therefore use an accumulator per 512 of K, added up in
     // fp32, as far as the TMEM columns go, and clusters long enough.
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    const int groups = (512 - (shrinks ? 2 : 1) * read) / p.rows + 1;
+    const int groups = (512 - (self ? 2 : 1) * read) / p.rows + 1;
     if (f32)
         while (cluster < kMaxCluster && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
-    if (mode == kOne && ((int64_t)tiles * ntn * cluster > kMaxBlocks || tiles * ntn > room[cluster])) return false;
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
     p.shrink_col = ((per + p.chunk - 1) / p.chunk - 1) * p.rows + read;
-    p.cols = tmem_cols(p.shrink_col + (shrinks ? read : 0));
-    const size_t recv = recv_bytes(g.tile_rows, cluster, mode == kSelf ? 512 + d.rank * 4 : 512);
-    p.stages = pick_stages(stage, tb + recv, per * (shrinks ? 2 : 1) + 4);
+    p.cols = tmem_cols(p.shrink_col + (self ? read : 0));
+    const size_t recv = recv_bytes(g.tile_rows, cluster, self ? 512 + d.rank * 4 : 512);
+    p.stages = pick_stages(stage, tb + recv, per * (self ? 2 : 1) + 4);
+    if (p.stages < 1) return cudaErrorInvalidConfiguration;
     p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
     CUtensorMap mW, mB, mA{};
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, d.rank < kExt ? d.rank : kExt) ||
-        (shrinks && !adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank))) {
-        *err = cudaErrorInvalidValue;
-        return true;
-    }
-    const void *fn = mode == kOne ? skinny_fn<kOne>(bf, kn, f32)
-                     : mode == kSelf ? skinny_fn<kSelf>(bf, kn, f32) : skinny_fn<kTwo>(bf, kn, f32);
+        (self && !adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank)))
+        return cudaErrorInvalidValue;
+    const void *fn = self ? skinny_fn<true>(bf, kn, f32) : skinny_fn<false>(bf, kn, f32);
     AdapterArgs a = g;
-    if (mode == kOne) a.nonce = next_nonce();
     void *args[] = {&mW, &mB, const_cast<void *>(x_map), &mA, &a, &p};
-    *err = launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem,
-                          mode == kOne ? kCooperative : mode == kTwo ? kDependent : kPlain, args, s);
-    return true;
+    return launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, !self, args, s);
 }
 
-}  // namespace
-
-cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, cudaStream_t s) {
-    cudaError_t err;
-    launch_skinny(g, x_map, kTwo, s, &err);
-    return err;
+int adapter_skinny_cluster(const AdapterArgs &g, int sms) {
+    const int *room = cluster_room();
+    if (!room) return 1;
+    const ShrinkPlan r = plan_shrink(g, sms, room);
+    const int shrink = r.cluster * r.slots * r.tiles;
+    return plan_skinny(g, sms, room, shrink <= sms / 3 ? shrink : 0);
 }
 
-bool launch_adapter_decode(const AdapterArgs &g, const void *x_map, cudaStream_t s, cudaError_t *err) {
-    return launch_skinny(g, x_map, g.most <= kSelfTiles ? kSelf : kOne, s, err);
+int adapter_waves(int64_t clusters, int cluster) {
+    const int *room = cluster_room();
+    return room ? (int)((clusters + room[cluster] - 1) / room[cluster]) : 1;
+}
+
+int adapter_self_cluster(const AdapterArgs &g) {
+    const int *room = cluster_room();
+    const latent_adapter_desc &d = g.d;
+    return room ? pick_cluster((d.n_out + 127) / 128, (d.n_in + kBK - 1) / kBK, room) : 1;
 }
 
 }  // namespace latent

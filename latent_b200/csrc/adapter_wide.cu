@@ -49,8 +49,8 @@ struct Cfg {
     static constexpr int kParts = BF && F32 ? 3 : 2;
     static constexpr uint32_t kTTile = 16384u * ((kParts + 1) / 2);  // 128 rows x (2 parts x 32) of x.A, and the third part
     static constexpr int kChunk = F32 ? 8 : 1 << 30;                 // K blocks per accumulator
-    static constexpr int kOutBufs = F32 ? 1 : 1;
-    static_assert(1024 + kStages * kStage + 2 * kTTile + 4 * kOutBufs * kOut <= kSmem, "shared memory");
+    static constexpr int kTBufs = 2;
+    static_assert(1024 + kStages * kStage + kTBufs * kTTile + 4 * kOut <= kSmem, "shared memory");
 };
 
 struct PairSegments {
@@ -154,7 +154,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t *tbuf = ring + kStages * kStage;
-    uint8_t *obuf = tbuf + 2 * C::kTTile;
+    uint8_t *obuf = tbuf + C::kTBufs * C::kTTile;
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int cta = blockIdx.x & 1;  // its rank in the cluster
@@ -278,7 +278,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             if (!wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
             const int ext = uniform(sh.seg[tl & 1].n) * rank;
             if (cta == 0) {  // the adapters' part goes to the last accumulator
-                for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages), tb.next(2)) {
+                for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages), tb.next(C::kTBufs)) {
                     if (!wait_warp(sh.full + at.s, at.phase, &sh.abort) ||
                         !wait_warp<true>(sh.t_full + tb.s, tb.phase, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
@@ -305,7 +305,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     } else if (warp >= 4 && warp < 8) {
         // ---------------- epilogue: lane = row ----------------
         const int r = threadIdx.x - 128, w = warp - 4;
-        uint8_t *out = obuf + w * C::kOutBufs * kOut;
+        uint8_t *out = obuf + w * kOut;
         const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
         int tl = 0, cc = 0;
         for (int i = pair; i < tiles; i += pairs, ++tl) {
@@ -401,7 +401,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     } else if (warp >= 8) {
         // ---------------- adapters of the tile, x.A parts ----------------
         const int tid = threadIdx.x - 256;
-        int tl = 0, eb = 0;
+        int tl = 0;
+        Ring tb;
         dependency_wait();
         for (int i = pair; i < tiles; i += pairs, ++tl) {
             const Tile tile = tile_at<kPairCols>(i, tm, tn);
@@ -467,13 +468,13 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const int live = wide ? -1 : my;
             float4 v[8];
             if (ext) load_t_row(v, live, rank, g.log2r, tp, 0);
-            for (int r0 = 0; r0 < ext; r0 += kExt, ++eb) {  // a thread that gives up here is heard at the next tile
-                if (eb >= 2 && !wait(sh.t_empty + (eb & 1), (uint32_t)((eb >> 1) - 1) & 1u)) { ok = false; break; }
+            for (int r0 = 0; r0 < ext; r0 += kExt, tb.next(C::kTBufs)) {  // a thread that gives up here is heard at the next tile
+                if (tb.wrapped && !wait(sh.t_empty + tb.s, tb.phase ^ 1u)) { ok = false; break; }
                 if (sh.abort) { ok = false; break; }
-                store_t_row<BF, C::kParts>(v, tbuf + (eb & 1) * C::kTTile, 16384u, tid, scale);
+                store_t_row<BF, C::kParts>(v, tbuf + tb.s * C::kTTile, 16384u, tid, scale);
                 if (r0 + kExt < ext) load_t_row(v, live, rank, g.log2r, tp, r0 + kExt);
                 fence_async_shared();
-                arrive_cluster(peer_addr(sh.t_full + (eb & 1), 0));
+                arrive_cluster(peer_addr(sh.t_full + tb.s, 0));
             }
         }
     }
