@@ -461,9 +461,19 @@ LATENT_API int latent_router_route(const float *scores, int32_t n_tokens, int32_
  * dropped slots.  LATENT_ERR_UNSUPPORTED beyond 1024 experts or top_k 32.
  * Stream-ordered, allocates nothing; repeated calls agree bit for bit. */
 enum { LATENT_ROUTER_ACCUMULATE = 1u << 2 };
-LATENT_API int latent_router_grad(const void *scores, int32_t type, const int32_t *ids, const float *d_weights,
-                                  int32_t n_tokens, int32_t n_expert, int32_t top_k, uint32_t flags, void *d_scores,
-                                  struct CUstream_st *stream);
+typedef struct latent_router_grad_desc {
+    int32_t n_tokens;        /* T */
+    int32_t n_expert;        /* E */
+    int32_t top_k;           /* k */
+    int32_t type;            /* latent_type of scores and d_scores */
+    uint32_t flags;          /* LATENT_ROUTER_* */
+    int32_t reserved;        /* 0 */
+    const void *scores;      /* [T][E] */
+    const int32_t *ids;      /* [T][k] */
+    const float *d_weights;  /* [T][k] */
+    void *d_scores;          /* [T][E] */
+} latent_router_grad_desc;
+LATENT_API int latent_router_grad(const latent_router_grad_desc *desc, struct CUstream_st *stream);
 
 /* Load-balance and z losses of a router over packed sequences, the expert
  * counts, and the loss's gradient (no counterpart in the reference).

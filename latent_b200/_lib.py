@@ -194,10 +194,27 @@ class BalanceDesc(C.Structure):
     ]
 
 
-# The two descriptors' fields in order, for callers that pack one per call (a third of the Structure's time).
+class RouterGradDesc(C.Structure):
+    _fields_ = [
+        ("n_tokens", C.c_int32),
+        ("n_expert", C.c_int32),
+        ("top_k", C.c_int32),
+        ("type", C.c_int32),
+        ("flags", C.c_uint32),
+        ("reserved", C.c_int32),
+        ("scores", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("d_weights", C.c_void_p),
+        ("d_scores", C.c_void_p),
+    ]
+
+
+# These descriptors' fields in order, for callers that pack one per call (a third of the Structure's time).
 ADAPTER_DESC = struct.Struct("=8i15q")
 BALANCE_DESC = struct.Struct("=6i2f10q")
+ROUTER_GRAD_DESC = struct.Struct("=6i4q")
 assert ADAPTER_DESC.size == C.sizeof(AdapterDesc) and BALANCE_DESC.size == C.sizeof(BalanceDesc)
+assert ROUTER_GRAD_DESC.size == C.sizeof(RouterGradDesc)
 
 EXPORTS.update({
     "latent_adapter_workspace_size": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
@@ -205,8 +222,7 @@ EXPORTS.update({
     "latent_adapter_check": (C.c_int, [C.c_void_p, C.c_void_p]),
     "latent_balance_workspace_size": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
     "latent_balance_loss": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "latent_router_grad": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
-                                     C.c_uint32, C.c_void_p, C.c_void_p]),
+    "latent_router_grad": (C.c_int, [C.c_void_p, C.c_void_p]),
     "latent_ep_workspace_size": (C.c_int, [C.POINTER(EpDesc), C.POINTER(C.c_size_t)]),
     "latent_ep_dispatch": (C.c_int, [C.POINTER(EpDesc), C.c_void_p]),
     "latent_ep_combine": (C.c_int, [C.POINTER(EpDesc), C.c_void_p]),

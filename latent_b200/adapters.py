@@ -28,7 +28,6 @@ from .runtime import FactorPair, project
 __all__ = ["AdapterSet", "adapter_project"]
 
 _TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
-_Y_TYPES = {**_TYPES, torch.float32: _lib.TYPE_F32}
 
 
 def _tensor(a, device, dtype) -> torch.Tensor:
@@ -89,6 +88,7 @@ class AdapterSet:
         # a, lda, b, ldb, scale as a call's descriptor takes them
         self._factors = (self.a.data_ptr(), self.a.shape[2], self.b.data_ptr(), self.b.shape[2], self.scale.data_ptr())
         self._err_ptr = self.err.data_ptr()
+        self._type = _TYPES[dtype]
         self._ws = {}
 
     def workspace_bytes(self, n_tokens: int) -> int:
@@ -125,15 +125,16 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     """
     s = adapters
     dev, dt, K, N = s.device, s.dtype, s.n_in, s.n_out
-    if x.dim() != 2 or x.shape[1] != K:
-        raise ValueError(f"x must be [T, {K}], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != K:
+        raise ValueError(f"x must be [T, {K}], got {tuple(shape)}")
     if x.dtype != dt:
         raise ValueError(f"x must be {dt} like the adapters, got {x.dtype}")
-    T = x.shape[0]
-    if ids.dim() != 1 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
+    T = shape[0]
+    if ids.shape != (T,) or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"ids must be contiguous int32 [{T}]")
     pair = isinstance(weight, FactorPair)
-    if not pair and (weight.dim() != 2 or weight.shape[0] != K or weight.shape[1] != N or weight.dtype != dt):
+    if not pair and (weight.shape != (K, N) or weight.dtype != dt):
         raise ValueError(f"weight must be {dt} [{K}, {N}]")
     if x.device != dev or ids.device != dev or (not pair and weight.device != dev) or \
             (out is not None and out.device != dev):
@@ -147,9 +148,11 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
         out_dtype = out.dtype
         if tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{T}, {N}] with contiguous rows")
-    elif out_dtype is None:
-        out_dtype = dt
-    if out_dtype != dt and out_dtype != torch.float32:
+    if out_dtype is None or out_dtype == dt:
+        out_dtype, y_type = dt, s._type
+    elif out_dtype == torch.float32:
+        y_type = _lib.TYPE_F32
+    else:
         raise ValueError(f"out_dtype {out_dtype} unsupported ({dt} or float32)")
     if T == 0:
         return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=dev)
@@ -174,10 +177,12 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
             raise ValueError("weight must be row-major or the transposed view of a row-major matrix")
         w_ptr = weight.data_ptr()
         y = out if out is not None else torch.empty(T, N, dtype=out_dtype, device=dev)
-    n = s.workspace_bytes(T)
+    if pair:
+        y_type = _lib.TYPE_F32
+    n = s._ws.get(T) or s.workspace_bytes(T)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    d = _lib.ADAPTER_DESC.pack(s.n_adapter, s.rank, K, N, T, _TYPES[dt], _Y_TYPES[y.dtype], flags, x.data_ptr(), ldx,
-                               w_ptr, ldw, *s._factors, ids.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
+    d = _lib.ADAPTER_DESC.pack(s.n_adapter, s.rank, K, N, T, s._type, y_type, flags, x.data_ptr(), ldx, w_ptr, ldw,
+                               *s._factors, ids.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
                                s._err_ptr, ws.data_ptr(), n)
     _lib.check(_on(dev, _lib.lib().latent_adapter_project, d), "latent_adapter_project")
     if pair:

@@ -619,17 +619,20 @@ int launch_kept(const T *scores, const int32_t *ids, const float *dw, int n, int
 }
 
 template <typename T>
-int launch_router_grad(const void *scores, const int32_t *ids, const float *dw, int n, int E, int k, uint32_t flags,
-                       void *out, cudaStream_t s) {
-    const T *sc = static_cast<const T *>(scores);
-    T *o = static_cast<T *>(out);
+int launch_router_grad(const latent_router_grad_desc &d, cudaStream_t s) {
+    const T *sc = static_cast<const T *>(d.scores);
+    T *o = static_cast<T *>(d.d_scores);
+    const int32_t *ids = d.ids;
+    const float *dw = d.d_weights;
+    const int n = d.n_tokens, E = d.n_expert, k = d.top_k;
+    const uint32_t flags = d.flags;
     const bool softmax = flags & LATENT_ROUTER_SOFTMAX, renorm = flags & LATENT_ROUTER_RENORMALIZE;
     const bool accum = flags & LATENT_ROUTER_ACCUMULATE;
     if (softmax && renorm) return launch_kept<T, true, true>(sc, ids, dw, n, E, k, accum, o, s);
     if (renorm) return launch_kept<T, false, true>(sc, ids, dw, n, E, k, accum, o, s);
     if (!softmax) return launch_kept<T, false, false>(sc, ids, dw, n, E, k, accum, o, s);
     const unsigned g = (unsigned)((n + kRowWarps - 1) / kRowWarps);
-    return with_row<T>(E, is_aligned(scores, 16) && is_aligned(out, 16), [&](auto pl, auto v) {
+    return with_row<T>(E, is_aligned(sc, 16) && is_aligned(o, 16), [&](auto pl, auto v) {
         constexpr int PL = decltype(pl)::value, V = decltype(v)::value;
         if (accum) k_router_grad_raw<T, PL, V, true><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
         else k_router_grad_raw<T, PL, V, false><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
@@ -691,25 +694,26 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
     }
 }
 
-extern "C" LATENT_API int latent_router_grad(const void *scores, int32_t type, const int32_t *ids,
-                                             const float *d_weights, int32_t n_tokens, int32_t n_expert, int32_t top_k,
-                                             uint32_t flags, void *d_scores, CUstream_st *stream) {
+extern "C" LATENT_API int latent_router_grad(const latent_router_grad_desc *d, CUstream_st *stream) {
     using namespace latent;
-    const int st = train_shape(n_tokens, n_expert, top_k);
+    if (!d) return LATENT_ERR_INVALID;
+    const int st = train_shape(d->n_tokens, d->n_expert, d->top_k);
     if (st) return st;
-    if (flags & ~(uint32_t)(LATENT_ROUTER_RENORMALIZE | LATENT_ROUTER_SOFTMAX | LATENT_ROUTER_ACCUMULATE))
+    if (d->reserved ||
+        (d->flags & ~(uint32_t)(LATENT_ROUTER_RENORMALIZE | LATENT_ROUTER_SOFTMAX | LATENT_ROUTER_ACCUMULATE)))
         return LATENT_ERR_INVALID;
-    if (!float_type(type)) return LATENT_ERR_DTYPE;
-    if (top_k > kMaxTrainTopK) return LATENT_ERR_UNSUPPORTED;
-    if (n_tokens == 0) return LATENT_OK;
-    if (!scores || !ids || !d_weights || !d_scores) return LATENT_ERR_INVALID;
-    const size_t es = type_size(type);
-    if (!is_aligned(scores, es) || !is_aligned(d_scores, es) || !is_aligned(ids, 4) || !is_aligned(d_weights, 4))
+    if (!float_type(d->type)) return LATENT_ERR_DTYPE;
+    if (d->top_k > kMaxTrainTopK) return LATENT_ERR_UNSUPPORTED;
+    if (d->n_tokens == 0) return LATENT_OK;
+    if (!d->scores || !d->ids || !d->d_weights || !d->d_scores) return LATENT_ERR_INVALID;
+    const size_t es = type_size(d->type);
+    if (!is_aligned(d->scores, es) || !is_aligned(d->d_scores, es) || !is_aligned(d->ids, 4) ||
+        !is_aligned(d->d_weights, 4))
         return LATENT_ERR_ALIGN;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    switch (type) {
-        case LATENT_TYPE_F32: return launch_router_grad<float>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
-        case LATENT_TYPE_F16: return launch_router_grad<__half>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
-        default: return launch_router_grad<__nv_bfloat16>(scores, ids, d_weights, n_tokens, n_expert, top_k, flags, d_scores, s);
+    switch (d->type) {
+        case LATENT_TYPE_F32: return launch_router_grad<float>(*d, s);
+        case LATENT_TYPE_F16: return launch_router_grad<__half>(*d, s);
+        default: return launch_router_grad<__nv_bfloat16>(*d, s);
     }
 }

@@ -63,17 +63,20 @@ def _workspace_bytes(n_seq: int, n_expert: int) -> int:
 
 
 def _router_inputs(logits: torch.Tensor, ids: torch.Tensor, name: str):
+    """(logits, ids) contiguous, T, E, k, latent_type; raises ValueError on anything else than [T, E] and int32 [T, k]."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError(f"{name} must be [T, E], got {tuple(logits.shape)}")
-    if logits.dtype not in _X_TYPES:
+    shape, slots = logits.shape, ids.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{name} must be [T, E], got {tuple(shape)}")
+    kind = _X_TYPES.get(logits.dtype)
+    if kind is None:
         raise ValueError(f"{name} dtype {logits.dtype} unsupported")
-    if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or ids.shape[1] < 1 or ids.dtype != torch.int32:
+    if len(slots) != 2 or slots[0] != shape[0] or slots[1] < 1 or ids.dtype != torch.int32:
         raise ValueError("ids must be int32 [T, k]")
-    if ids.device != logits.device:
+    if ids.get_device() != logits.get_device():
         raise ValueError(f"ids must be on {logits.device}")
-    return logits.contiguous(), ids.contiguous()
+    return logits.contiguous(), ids.contiguous(), shape[0], shape[1], slots[1], kind
 
 
 def _no_capture(what: str) -> None:
@@ -88,7 +91,7 @@ def _no_capture(what: str) -> None:
 def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradient):
     T, E = logits.shape
     dev = logits.device
-    n = _workspace_bytes(n_seq, E)
+    n = _WS_BYTES.get((n_seq, E)) or _workspace_bytes(n_seq, E)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     losses = torch.empty(3, dtype=torch.float32, device=dev)
     # [E] when the rows are one sequence without borders
@@ -147,17 +150,16 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 
     underflows: scale the two coefficients up.  Without it, logits that
     require a gradient make ``loss`` differentiable by autograd.
     """
-    flat, ids = _router_inputs(logits, ids, "logits")
-    T = flat.shape[0]
+    flat, ids, T = _router_inputs(logits, ids, "logits")[:3]
     n_seq = 1
     if cu_seqlens is not None:
-        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2 or cu_seqlens.dtype != torch.int32 or \
-                cu_seqlens.device != flat.device:
+        n_seq = cu_seqlens.numel() - 1
+        if cu_seqlens.dim() != 1 or n_seq < 1 or cu_seqlens.dtype != torch.int32 or \
+                cu_seqlens.get_device() != flat.get_device():
             raise ValueError(f"cu_seqlens must be int32 [S + 1] on {flat.device}")
         cu_seqlens = cu_seqlens.contiguous()
-        n_seq = cu_seqlens.shape[0] - 1
     if valid is not None:
-        if tuple(valid.shape) != (T,) or valid.dtype != torch.bool or valid.device != flat.device:
+        if tuple(valid.shape) != (T,) or valid.dtype != torch.bool or valid.get_device() != flat.get_device():
             raise ValueError(f"valid must be bool [{T}] on {flat.device}")
         valid = valid.contiguous()
     balance_coef, z_coef = float(balance_coef), float(z_coef)
@@ -180,8 +182,8 @@ def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.T
     fixed.  ``out``: a contiguous tensor of the scores' shape and dtype that
     the gradient is added into (for instance ``balance_loss(...).grad``).
     """
-    flat, ids = _router_inputs(scores, ids, "scores")
-    if d_weights.shape != ids.shape or d_weights.dtype != torch.float32 or d_weights.device != flat.device:
+    flat, ids, T, E, k, kind = _router_inputs(scores, ids, "scores")
+    if d_weights.shape != ids.shape or d_weights.dtype != torch.float32 or d_weights.get_device() != flat.get_device():
         raise ValueError(f"d_weights must be float32 {tuple(ids.shape)} on {flat.device}")
     flags = (_lib.ROUTER_RENORMALIZE if renormalize else 0) | (_lib.ROUTER_SOFTMAX if logits else 0)
     if out is None:
@@ -196,10 +198,9 @@ def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.T
         flags |= _lib.ROUTER_ACCUMULATE
         g = out
     d_weights = d_weights.contiguous()
-    T, E = flat.shape
-    _lib.check(_on(flat.device, _lib.lib().latent_router_grad, flat.data_ptr(), _X_TYPES[flat.dtype], ids.data_ptr(),
-                   d_weights.data_ptr(), T, E, ids.shape[1], flags, g.data_ptr()),
-               "latent_router_grad")
+    d = _lib.ROUTER_GRAD_DESC.pack(T, E, k, kind, flags, 0, flat.data_ptr(), ids.data_ptr(), d_weights.data_ptr(),
+                                   g.data_ptr())
+    _lib.check(_on(flat.device, _lib.lib().latent_router_grad, d), "latent_router_grad")
     return g
 
 

@@ -17,18 +17,19 @@ def lib():
 
 
 def test_router_grad_validates_on_the_host(lib):
-    f = lib.latent_router_grad
-    assert f(None, 0, None, None, 4, 0, 2, 0, None, None) == 2            # no experts
-    assert f(None, 0, None, None, -1, 8, 2, 0, None, None) == 2
-    assert f(None, 0, None, None, 4, 8, 0, 0, None, None) == 2
-    assert f(None, 0, None, None, 1 << 28, 8, 32, 0, None, None) == 2     # too many slots
-    assert f(None, 0, None, None, 4, 8, 2, 8, None, None) == 1            # unknown flag
-    assert f(None, 7, None, None, 4, 8, 2, 0, None, None) == 3
-    assert f(None, 0, None, None, 4, 2048, 2, 0, None, None) == 9
-    assert f(None, 0, None, None, 4, 64, 33, 0, None, None) == 9
-    assert f(None, 0, None, None, 0, 8, 2, 0, None, None) == 0            # empty batch
-    assert f(None, 0, None, None, 4, 8, 2, 0, None, None) == 1            # missing buffers
-    assert f(64, 0, 64, 64, 4, 8, 2, 0, 66, None) == 4                    # unaligned gradient
+    def f(**kw):
+        d = dict(n_tokens=4, n_expert=8, top_k=2, scores=64, ids=64, d_weights=64, d_scores=64)
+        return lib.latent_router_grad(C.byref(_lib.RouterGradDesc(**{**d, **kw})), None)
+
+    assert lib.latent_router_grad(None, None) == 1
+    assert f(n_expert=0) == 2 and f(n_tokens=-1) == 2 and f(top_k=0) == 2
+    assert f(n_tokens=1 << 28, top_k=32) == 2                             # too many slots
+    assert f(flags=8) == 1 and f(reserved=1) == 1 and f(type=7) == 3
+    assert f(n_expert=2048) == 9 and f(n_expert=64, top_k=33) == 9
+    assert f(n_tokens=0, scores=None) == 0                                # empty batch
+    for name in ("scores", "ids", "d_weights", "d_scores"):
+        assert f(**{name: None}) == 1, name
+        assert f(**{name: 66}) == 4, name
 
 
 def test_balance_loss_validates_on_the_host(lib):
