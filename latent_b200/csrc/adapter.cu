@@ -214,7 +214,7 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         if (!adapter_map(&x, d->type == LATENT_TYPE_BF16, d->x, d->n_tokens, d->n_in, d->ldx, a.tile_rows))
             return LATENT_ERR_CUDA;
         cudaError_t err = cudaSuccess;
-        if (path != kPathSelf) err = launch_adapter_shrink(a, &x, sms, s);
+        if (path != kPathSelf) err = launch_adapter_shrink(a, &x, s);
         if (err == cudaSuccess)
             err = path == kPathWide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, path == kPathSelf, s);
         if (err != cudaSuccess) return LATENT_ERR_CUDA;

@@ -27,7 +27,7 @@ struct AdapterArgs {
 constexpr int kMaxCluster = 16;
 
 // x_map: the CUtensorMap of x with a box of tile_rows rows.
-cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);
+cudaError_t launch_adapter_shrink(const AdapterArgs &a, const void *x_map, cudaStream_t s);
 // self: with x.A in the same launch (one tile of rows).
 cudaError_t launch_adapter_skinny(const AdapterArgs &a, const void *x_map, int sms, bool self, cudaStream_t s);
 cudaError_t launch_adapter_wide(const AdapterArgs &a, const void *x_map, int sms, cudaStream_t s);

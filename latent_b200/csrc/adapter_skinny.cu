@@ -737,7 +737,7 @@ struct ShrinkPlan {
     Plan p;
     int cluster, slots, tiles;
 };
-ShrinkPlan plan_shrink(const AdapterArgs &g, int sms, const int *room) {
+ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
     const latent_adapter_desc &d = g.d;
     ShrinkPlan r{};
     Plan &p = r.p;
@@ -746,10 +746,22 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, int sms, const int *room) {
     const int nk = (d.n_in + kBK - 1) / kBK;
     p.rows = (g.tile_rows + 15) / 16 * 16;
     const size_t stage = 16384 + (size_t)p.rows * 128;
-    r.cluster = pick_cluster(r.tiles, nk, room);
+    // Clusters, and tiles of stacked rank columns side by side: the fewest K blocks one after the other.  A batch of
+    // one row tile may use every adapter; longer ones are packed prompts with few to a tile.
+    const int expect = r.tiles == 1 ? most : 1;
+    int64_t best = INT64_MAX;
+    for (int c = 1; c <= kMaxCluster && c <= nk; ++c) {
+        int slots = room[c] / r.tiles;
+        slots = slots < 1 ? 1 : slots > most ? most : slots;
+        const int64_t turns = ((int64_t)r.tiles * slots + room[c] - 1) / room[c];
+        const int64_t cost = turns * ((expect + slots - 1) / slots) * ((nk + c - 1) / c);
+        if (cost < best) {
+            best = cost;
+            r.cluster = c;
+            r.slots = slots;
+        }
+    }
     const size_t recv = recv_bytes(g.tile_rows, r.cluster, d.rank * 4);
-    r.slots = sms / (r.tiles * r.cluster);  // tiles of stacked rank columns side by side
-    r.slots = r.slots < 1 ? 1 : r.slots > most ? most : r.slots;
     p.stages = pick_stages(stage, recv, (nk + r.cluster - 1) / r.cluster * ((most + r.slots - 1) / r.slots));
     p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
     p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
@@ -770,12 +782,12 @@ int plan_skinny(const AdapterArgs &g, int sms, const int *room, int beside) {
 
 }  // namespace
 
-cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, int sms, cudaStream_t s) {
+cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, cudaStream_t s) {
     const latent_adapter_desc &d = g.d;
     const bool bf = d.type == LATENT_TYPE_BF16;
     const int *room = cluster_room();
     if (!room) return cudaErrorInvalidConfiguration;
-    ShrinkPlan r = plan_shrink(g, sms, room);
+    ShrinkPlan r = plan_shrink(g, room);
     if (r.p.stages < 1) return cudaErrorInvalidConfiguration;
     CUtensorMap mA;
     if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank)) return cudaErrorInvalidValue;
@@ -831,7 +843,7 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
 int adapter_skinny_cluster(const AdapterArgs &g, int sms) {
     const int *room = cluster_room();
     if (!room) return 1;
-    const ShrinkPlan r = plan_shrink(g, sms, room);
+    const ShrinkPlan r = plan_shrink(g, room);
     const int shrink = r.cluster * r.slots * r.tiles;
     return plan_skinny(g, sms, room, shrink <= sms / 3 ? shrink : 0);
 }
