@@ -89,6 +89,7 @@ class AdapterSet:
         self._factors = (self.a.data_ptr(), self.a.shape[2], self.b.data_ptr(), self.b.shape[2], self.scale.data_ptr())
         self._err_ptr = self.err.data_ptr()
         self._type = _TYPES[dtype]
+        self._keep = (self.a, self.b, self.scale, self.err)
         self._ws = {}
 
     def workspace_bytes(self, n_tokens: int) -> int:

@@ -178,7 +178,7 @@ extern "C" LATENT_API int latent_adapter_workspace_size(const latent_adapter_des
     return LATENT_OK;
 }
 
-extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, CUstream_st *stream) {
+extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, CUstream_st *stream) try {
     using namespace latent;
     const int st = ad_validate(d);
     if (st) return st;
@@ -217,7 +217,10 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         if (path != kPathSelf) err = launch_adapter_shrink(a, &x, s);
         if (err == cudaSuccess)
             err = path == kPathWide ? launch_adapter_wide(a, &x, sms, s) : launch_adapter_skinny(a, &x, sms, path == kPathSelf, s);
-        if (err != cudaSuccess) return LATENT_ERR_CUDA;
+        if (err != cudaSuccess) {
+            cudaGetLastError();  // not left for the caller's next check
+            return LATENT_ERR_CUDA;
+        }
         return LATENT_OK;
     }
     const dim3 gs((unsigned)d->n_tokens, (unsigned)d->rank / kShrinkWarps);
@@ -230,6 +233,8 @@ extern "C" LATENT_API int latent_adapter_project(const latent_adapter_desc *d, C
         k_ad_any<__nv_bfloat16><<<gp, 256, 0, s>>>(*d, tt);
     }
     return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+} catch (...) {  // the tables of kernel attributes allocate on the host
+    return LATENT_ERR_CUDA;
 }
 
 extern "C" LATENT_API int latent_adapter_check(uint32_t *err, CUstream_st *stream) {

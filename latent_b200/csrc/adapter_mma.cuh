@@ -136,6 +136,17 @@ struct Ring {
     }
 };
 
+// By the load warp, behind its last load: until the MMAs have handed every slot
+// back.  Their arrivals are made by the tensor core on its own; none may reach a
+// block that has gone.
+__device__ __forceinline__ bool ring_drained(const Ring &at, uint64_t *empty, int slots, volatile int *abort) {
+    for (int s = 0; s < slots; ++s) {
+        if (!at.wrapped && s >= at.s) break;
+        if (!wait_warp(empty + s, s < at.s ? at.phase : at.phase ^ 1u, abort)) return false;
+    }
+    return true;
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

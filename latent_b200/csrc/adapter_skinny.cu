@@ -50,7 +50,6 @@ struct Plan {
     int tbufs;      // tiles of x.A parts
     int shrink_col; // x.A's accumulator behind the product's (SELF)
     uint32_t cols;  // TMEM columns
-    size_t smem;
 };
 
 __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
@@ -236,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         Ring at;
         for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128)
             ok = load_stacked(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
+        if (ok) ok = ring_drained(at, sh.empty, p.stages, &sh.abort);
     } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, false, false);
         Ring at;
@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 }
             }
         }
+        if (ok) ok = ring_drained(at, sh.empty, p.stages, &sh.abort);
     } else if (warp == 1) {
         const uint32_t id = idesc(BF, p.rows, KN, false), idx = idesc(BF, p.rows, true, false);
         Ring at;
@@ -499,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 mbar_arrive(sh.t_full + tb.s);
                 if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
             }
+            if (warp == 4 && __all_sync(kAll, ok)) ok = ring_drained(tb, sh.t_empty, p.tbufs, &sh.abort);
             if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
             __syncwarp();
             if (!wait(sh.acc_full, 0u)) ok = false;
@@ -591,17 +593,11 @@ uint32_t tmem_cols(int n) {
     return c;
 }
 
-// Dynamic shared memory of a block beside the static.  An SM holds one block of
-// these kernels (what the occupancy calculator gives for every kernel here that
-// allocates TMEM, however small).  Should blocks of two calls share an SM all
-// the same, no TMEM allocation may wait: blocks of two clusters that wait for
-// each other's columns would never end.  So a block's share of the shared
-// memory is at least its share of the 512 columns.
-constexpr size_t kSmemMost = 227 * 1024 - sizeof(Shared);
-size_t smem_of(size_t used, uint32_t cols) {
-    const size_t share = (size_t)cols * 228 * 1024 / 512 - 1024 - sizeof(Shared);  // of 228 KB; 1 KB goes to the system
-    return used < share ? share : used;
-}
+// Dynamic shared memory of a block beside the static: all of an SM's, whatever
+// the ring needs, so that no block of another kernel that wants TMEM starts
+// beside it: clusters whose blocks wait for columns that the other's hold would
+// wait for each other.
+constexpr size_t kSmem = 227 * 1024 - sizeof(Shared);
 
 // Clusters of more than 8 blocks, once per kernel and device.
 cudaError_t allow_clusters(const void *fn) {
@@ -617,13 +613,13 @@ cudaError_t allow_clusters(const void *fn) {
     return err;
 }
 
-cudaError_t launch_cluster(const void *fn, dim3 grid, size_t smem, bool dependent, void **args, cudaStream_t s) {
-    cudaError_t err = ensure_smem(fn, smem);
+cudaError_t launch_cluster(const void *fn, dim3 grid, bool dependent, void **args, cudaStream_t s) {
+    cudaError_t err = ensure_smem(fn, kSmem);
     if (err != cudaSuccess || (grid.x > 8 && (err = allow_clusters(fn)) != cudaSuccess)) return err;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -653,12 +649,12 @@ const int *cluster_room() {
     Table &t = tables[dev];
     if (!t.set) {
         const void *fn = (const void *)k_ad_shrink<true>;
-        if (ensure_smem(fn, kSmemMost) != cudaSuccess || allow_clusters(fn) != cudaSuccess) return nullptr;
+        if (ensure_smem(fn, kSmem) != cudaSuccess || allow_clusters(fn) != cudaSuccess) return nullptr;
         for (int c = 1; c <= kMaxCluster; ++c) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(c, 256);
             cfg.blockDim = dim3(kThreads);
-            cfg.dynamicSmemBytes = kSmemMost;
+            cfg.dynamicSmemBytes = kSmem;
             cudaLaunchAttribute at[1];
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = (unsigned)c;
@@ -687,7 +683,7 @@ size_t recv_bytes(int tile_rows, int cluster, int row) {
 
 // Stages beside `other` bytes of shared memory, no more than there are loads.
 int pick_stages(size_t stage, size_t other, int loads) {
-    int n = (int)((kSmemMost - 1024 - other) / stage);
+    int n = (int)((kSmem - 1024 - other) / stage);
     if (n > kMaxStages) n = kMaxStages;
     return n < loads ? n : loads;
 }
@@ -751,6 +747,7 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
     const int expect = r.tiles == 1 ? most : 1;
     int64_t best = INT64_MAX;
     for (int c = 1; c <= kMaxCluster && c <= nk; ++c) {
+        if (room[c] < 1) continue;
         int slots = room[c] / r.tiles;
         slots = slots < 1 ? 1 : slots > most ? most : slots;
         const int64_t turns = ((int64_t)r.tiles * slots + room[c] - 1) / room[c];
@@ -764,7 +761,6 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
     const size_t recv = recv_bytes(g.tile_rows, r.cluster, d.rank * 4);
     p.stages = pick_stages(stage, recv, (nk + r.cluster - 1) / r.cluster * ((most + r.slots - 1) / r.slots));
     p.cols = tmem_cols(2 * ((p.rows + 31) / 32 * 32));
-    p.smem = smem_of(1024 + p.stages * stage + recv, p.cols);
     return r;
 }
 
@@ -794,7 +790,7 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, cudaS
     AdapterArgs a = g;
     void *args[] = {&mA, const_cast<void *>(x_map), &a, &r.p};
     return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
-                          dim3(r.cluster, r.slots, r.tiles), r.p.smem, false, args, s);
+                          dim3(r.cluster, r.slots, r.tiles), false, args, s);
 }
 
 cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, bool self, cudaStream_t s) {
@@ -819,7 +815,7 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
     const int groups = (512 - (self ? 2 : 1) * read) / p.rows + 1;
     if (f32)
-        while (cluster < kMaxCluster && cluster < nk && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
+        while (cluster < kMaxCluster && cluster < nk && room[cluster + 1] > 0 && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
@@ -828,7 +824,6 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     const size_t recv = recv_bytes(g.tile_rows, cluster, self ? 512 + d.rank * 4 : 512);
     p.stages = pick_stages(stage, tb + recv, per * (self ? 2 : 1) + 4);
     if (p.stages < 1) return cudaErrorInvalidConfiguration;
-    p.smem = smem_of(1024 + p.stages * stage + tb + recv, p.cols);
     CUtensorMap mW, mB, mA{};
     if (!(kn ? adapter_map(&mW, bf, d.w, d.n_in, d.n_out, d.ldw, kBK) : adapter_map(&mW, bf, d.w, d.n_out, d.n_in, d.ldw, 128)) ||
         !adapter_map(&mB, bf, d.b, (uint64_t)d.n_adapter * d.rank, d.n_out, d.ldb, d.rank < kExt ? d.rank : kExt) ||
@@ -837,7 +832,7 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     const void *fn = self ? skinny_fn<true>(bf, kn, f32) : skinny_fn<false>(bf, kn, f32);
     AdapterArgs a = g;
     void *args[] = {&mW, &mB, const_cast<void *>(x_map), &mA, &a, &p};
-    return launch_cluster(fn, dim3(cluster, ntn, tiles), p.smem, !self, args, s);
+    return launch_cluster(fn, dim3(cluster, ntn, tiles), !self, args, s);
 }
 
 int adapter_skinny_cluster(const AdapterArgs &g, int sms) {
@@ -850,7 +845,7 @@ int adapter_skinny_cluster(const AdapterArgs &g, int sms) {
 
 int adapter_waves(int64_t clusters, int cluster) {
     const int *room = cluster_room();
-    return room ? (int)((clusters + room[cluster] - 1) / room[cluster]) : 1;
+    return room && room[cluster] > 0 ? (int)((clusters + room[cluster] - 1) / room[cluster]) : 1;
 }
 
 int adapter_self_cluster(const AdapterArgs &g) {

@@ -36,8 +36,9 @@ constexpr int kPairRows = 256;
 constexpr int kGroupM = 8;       // row tiles that share a sweep over the columns (L2 reuse)
 constexpr uint32_t kXBytes = 16384;
 constexpr uint32_t kOut = 4096;  // a warp's staging: 32 rows of 128 bytes
-// All of an SM's shared memory, more than the kernel needs: the block takes all
-// TMEM columns, and no other block that wants some may start beside it.
+// All of an SM's shared memory, more than the kernel needs, so that no block of
+// another kernel that wants TMEM starts beside it: clusters whose blocks wait
+// for columns that the other's hold would wait for each other.
 constexpr size_t kStatic = 6144;
 constexpr size_t kSmem = 227 * 1024 - kStatic;
 
@@ -193,6 +194,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
     bool ok = true;
+    Ring tb_last;  // the builders' x.A tiles
 
     if (warp == 0) {
         // ---------------- loads ----------------
@@ -239,6 +241,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             }
             if (ok && lane == 0) mbar_arrive(sh.seg_empty + (tl & 1));
         }
+        if (ok) ok = ring_drained(at, sh.empty, kStages, &sh.abort);
     } else if (warp == 1) {
         // ---------------- MMAs (the leader's warp, for both blocks) ----------------
         Ring at, tb;
@@ -402,7 +405,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         // ---------------- adapters of the tile, x.A parts ----------------
         const int tid = threadIdx.x - 256;
         int tl = 0;
-        Ring tb;
+        Ring &tb = tb_last;
         dependency_wait();
         for (int i = pair; i < tiles; i += pairs, ++tl) {
             const Tile tile = tile_at<kPairCols>(i, tm, tn);
@@ -478,6 +481,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             }
         }
     }
+    if (warp == 8 && __all_sync(kAll, ok)) ok = ring_drained(tb_last, sh.t_empty, C::kTBufs, &sh.abort);
     if (!ok) {
         atomicOr(d.err, kErrTimeout);
         sh.abort = 1;

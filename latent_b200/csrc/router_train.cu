@@ -598,7 +598,9 @@ int launch_balance(const BalanceArgs &a, int sms, cudaStream_t s) {
     else if (a.E <= 256) err = launch_balance_rows<T, 32, 8>(a, vec, sms, s);
     else if (a.E <= 512) err = launch_balance_rows<T, 32, 16>(a, vec, sms, s);
     else err = launch_balance_rows<T, 32, 32>(a, vec, sms, s);
-    return err == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+    if (err == cudaSuccess) return LATENT_OK;
+    cudaGetLastError();  // not left for the caller's next check
+    return LATENT_ERR_CUDA;
 }
 
 template <typename T, bool SOFTMAX, bool RENORM>

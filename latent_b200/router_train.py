@@ -116,7 +116,7 @@ class _BalanceLossFn(torch.autograd.Function):
         ctx.save_for_backward(flat, ids, valid, cu)
         ctx.args = (balance_coef, z_coef, n_seq)
         loss, balance, z = losses.unbind()
-        loss, balance, z = loss.clone(), balance.clone(), z.clone()
+        loss = loss.clone()  # a tensor of its own: users add to it in place
         ctx.mark_non_differentiable(balance, z, counts)
         return loss, balance, z, counts
 

@@ -232,6 +232,64 @@ def test_streams_graphs_and_repeats(cuda, T):
     s.check()
 
 
+def test_calls_of_all_kinds_on_two_streams_at_once(cuda):
+    """Blocks of several calls share the GPU: every result is the one of the call alone."""
+    calls = []
+    for T, K, N, n in ((1, 1024, 2048, 2), (48, 2048, 1408, 40), (200, 1024, 640, 6), (700, 512, 1024, 3), (64, 7168, 256, 16)):
+        for out in (None, F32):
+            x, w, ads, i = make(T, K, N, [16] * n, BF, seed=T)
+            s = AdapterSet(ads)
+            calls.append((x, w, s, i, out, adapter_project(x, w, s, i, out_dtype=out)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for rep in range(6):
+        got = []
+        for k, (x, w, s, i, out, _) in enumerate(calls):
+            with torch.cuda.stream(streams[(k + rep) % 3]):
+                got.append(adapter_project(x, w, s, i, out_dtype=out))
+        torch.cuda.synchronize()
+        for g, c in zip(got, calls):
+            assert torch.equal(g, c[5])
+    for c in calls:
+        c[2].check()
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from latent_b200 import AdapterSet, adapter_project, balance_loss, router_topk_grad
+g = torch.Generator("cuda").manual_seed(0)
+rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
+w, l = rand(256, 512), torch.randn((100, 64), device="cuda")
+s = AdapterSet([(rand(256, 16), rand(16, 512), 1.0) for _ in range(12)])
+xs = [rand(T, 256) for T in (1, 40, 700)]
+ids = [torch.zeros(x.shape[0], dtype=torch.int32, device="cuda") for x in xs]
+slots = torch.randint(0, 64, (100, 4), device="cuda").to(torch.int32)
+dw = torch.randn((100, 4), device="cuda")
+
+def step():
+    r = balance_loss(l, slots, 0.1, 0.1, gradient=True)
+    return [adapter_project(x, w, s, i) for x, i in zip(xs, ids)] + [r.loss, router_topk_grad(l, slots, dw, logits=True, out=r.grad)]
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, step()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(cuda):
+    import subprocess
+    import sys
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=ROOT, capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_refusals(cuda):
     x, w, ads, i = make(4, 64, 32, [16], BF)
     s = AdapterSet(ads)

@@ -296,7 +296,9 @@ def test_autograd_matches_the_explicit_gradients(cuda):
     dw = torch.randn(w.shape, device="cuda")
     r = balance_loss(leaf, ids, 0.02, 0.001)
     assert r.grad is None and torch.equal(r.counts, counts)
-    (3.0 * r.loss + (w * dw).sum()).backward()
+    total = r.loss
+    total *= 3.0                                      # a tensor of its own, not a view of the kernel's results
+    (total + (w * dw).sum()).backward()
     g = balance_loss(l, ids, 0.06, 0.003, gradient=True).grad
     g = g.double() + router_topk_grad(l, ids, dw, logits=True).double()
     # two fp32 gradients, each within a few steps of the other form's, and their sum
