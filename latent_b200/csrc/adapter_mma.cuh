@@ -136,15 +136,12 @@ struct Ring {
     }
 };
 
-// By the load warp, behind its last load: until the MMAs have handed every slot
-// back.  Their arrivals are made by the tensor core on its own; none may reach a
-// block that has gone.
+// By a whole warp, behind its last use of a ring: until the MMAs have handed
+// the last slot back (commits arrive in their order).  These arrivals are made
+// by the tensor core on its own; none may reach a block that has gone.
 __device__ __forceinline__ bool ring_drained(const Ring &at, uint64_t *empty, int slots, volatile int *abort) {
-    for (int s = 0; s < slots; ++s) {
-        if (!at.wrapped && s >= at.s) break;
-        if (!wait_warp(empty + s, s < at.s ? at.phase : at.phase ^ 1u, abort)) return false;
-    }
-    return true;
+    if (!at.wrapped && at.s == 0) return true;
+    return at.s ? wait_warp(empty + at.s - 1, at.phase, abort) : wait_warp(empty + slots - 1, at.phase ^ 1u, abort);
 }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
