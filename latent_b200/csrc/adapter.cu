@@ -138,7 +138,7 @@ int tile_rows(int n, AdapterPath path) { return path == kPathWide || n >= adapte
 // of K and 3 us more to start where the batch is too small to hide it.  An
 // extension block of 32 stacked rank columns, of which a batch of single
 // tokens may need one per adapter and 32 ranks, costs 0.5 us of one of a
-// cluster's blocks against 0.8 us of the pair.  E.g. 1024 rows of 2048 x 2048
+// cluster's blocks against 0.55 us of the pair.  E.g. 1024 rows of 2048 x 2048
 // (rank 16): 25.6 us skinny, 18.0 wide; 1024 rows of 7168 x 512: 24.4 and 39.8.
 // Up to 64 rows whose adapters fit one tile of 128 stacked rank columns, with
 // at most 8 steps of K per block, k_ad_skinny makes x.A itself (one row of
@@ -161,7 +161,7 @@ AdapterPath pick_path(const AdapterArgs &g, int sms) {
     const int64_t skinny = adapter_waves(clusters, c) * ((nk + c - 1) / c + (ext + c - 1) / c) * 50;
     const int cols = d.y_type == LATENT_TYPE_F32 ? 128 : 256;
     const int64_t tiles = ((int64_t)d.n_tokens + 255) / 256 * ((d.n_out + cols - 1) / cols);
-    const int64_t wide = (tiles + sms / 2 - 1) / (sms / 2) * (nk * (cols == 128 ? 26 : 23) + ext * 80) +
+    const int64_t wide = (tiles + sms / 2 - 1) / (sms / 2) * (nk * (cols == 128 ? 26 : 23) + ext * 55) +
                          (d.n_tokens <= 256 ? 300 : 0);
     return wide < skinny ? kPathWide : kPathSkinny;
 }

@@ -82,7 +82,7 @@ __device__ __forceinline__ void setup(Shared &sh, const Plan &p, int warp, int l
                 mbar_init(sh.acc_empty + b, 128);
             }
             for (int b = 0; b < kMaxTBufs; ++b) {
-                mbar_init(sh.t_full + b, 128);
+                mbar_init(sh.t_full + b, 4);  // the builders' warps
                 mbar_init(sh.t_empty + b, 1);
             }
             mbar_init(&sh.seg, 128);
@@ -492,12 +492,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             float4 v[8];
             if (e0 < e1) load_t_row(v, live, rank, log2r, t, e0 * kExt);
             Ring tb;
-            for (int e = e0; e < e1 && ok; ++e, tb.next(p.tbufs)) {
-                if (tb.wrapped && !wait(sh.t_empty + tb.s, tb.phase ^ 1u)) { ok = false; break; }
-                if (sh.abort) { ok = false; break; }
+            for (int e = e0; e < e1; ++e, tb.next(p.tbufs)) {
+                if (tb.wrapped && !wait_warp(sh.t_empty + tb.s, tb.phase ^ 1u, &sh.abort)) { ok = false; break; }
                 if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)tb.s * kTiles * xbytes, xbytes, r, scale);
                 fence_async_shared();
-                mbar_arrive(sh.t_full + tb.s);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.t_full + tb.s);
                 if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
             }
             if (warp == 4 && __all_sync(kAll, ok)) ok = ring_drained(tb, sh.t_empty, p.tbufs, &sh.abort);

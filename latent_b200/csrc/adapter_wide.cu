@@ -79,8 +79,11 @@ __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
     return r;
 }
+// What the arrival stands for is ordered before it already: shared memory that
+// the tensor core reads by the proxy fence, TMEM reads by their wait.  A release
+// at cluster scope on top cost 0.8 us an arrival.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(
@@ -173,11 +176,11 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(sh.acc_full + b, 1);
-            mbar_init(sh.acc_empty + b, 256);  // the epilogue threads of both blocks
-            mbar_init(sh.t_full + b, 256);     // the builders of both
+            mbar_init(sh.acc_empty + b, 8);    // the epilogue warps of both blocks
+            mbar_init(sh.t_full + b, 8);       // the builders' warps of both
             mbar_init(sh.t_empty + b, 1);
             mbar_init(sh.seg_full + b, 128);
-            mbar_init(sh.seg_empty + b, 130);  // loader, MMA warp and epilogue threads of this block
+            mbar_init(sh.seg_empty + b, 6);    // loader, MMA warp and epilogue warps of this block
         }
         sh.abort = 0;
         fence_barrier_init();
@@ -333,7 +336,8 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                         for (int j = 0; j < 16; ++j) v[n + j] = c ? v[n + j] + __uint_as_float(u[j]) : __uint_as_float(u[j]);
                     }
                     tc_fence_before();
-                    arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
+                    __syncwarp();
+                    if (lane == 0) arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
                 }
                 if (!ok) break;
             } else {
@@ -394,10 +398,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             }
             if constexpr (!F32) {
                 tc_fence_before();
-                arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
+                __syncwarp();
+                if (lane == 0) arrive_cluster(peer_addr(sh.acc_empty + (cc & 1), 0));
                 ++cc;
             }
-            mbar_arrive(sh.seg_empty + (tl & 1));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sh.seg_empty + (tl & 1));
         }
         __syncwarp();
         if (elect()) store_wait();
@@ -472,12 +478,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             float4 v[8];
             if (ext) load_t_row(v, live, rank, g.log2r, tp, 0);
             for (int r0 = 0; r0 < ext; r0 += kExt, tb.next(C::kTBufs)) {  // a thread that gives up here is heard at the next tile
-                if (tb.wrapped && !wait(sh.t_empty + tb.s, tb.phase ^ 1u)) { ok = false; break; }
-                if (sh.abort) { ok = false; break; }
+                if (tb.wrapped && !wait_warp(sh.t_empty + tb.s, tb.phase ^ 1u, &sh.abort)) { ok = false; break; }
                 store_t_row<BF, C::kParts>(v, tbuf + tb.s * C::kTTile, 16384u, tid, scale);
                 if (r0 + kExt < ext) load_t_row(v, live, rank, g.log2r, tp, r0 + kExt);
                 fence_async_shared();
-                arrive_cluster(peer_addr(sh.t_full + tb.s, 0));
+                __syncwarp();
+                if (lane == 0) arrive_cluster(peer_addr(sh.t_full + tb.s, 0));
             }
         }
     }
