@@ -133,13 +133,15 @@ enum AdapterPath { kPathSelf, kPathSkinny, kPathWide };
 int tile_rows(int n, AdapterPath path) { return path == kPathWide || n >= adapter::kRows ? adapter::kRows : (n + 15) / 16 * 16; }
 
 // Which kernels serve a call, by what they cost in measured steps (B200,
-// bf16): k_ad_skinny takes 0.5 us per 64 of a block's share of K at 128 rows
-// (as many bytes less at fewer), k_ad_wide 0.23 us (fp32 results 0.26) per 64
-// of K and 3 us more to start where the batch is too small to hide it.  An
-// extension block of 32 stacked rank columns, of which a batch of single
-// tokens may need one per adapter and 32 ranks, costs 0.5 us of one of a
-// cluster's blocks against 0.55 us of the pair.  E.g. 1024 rows of 2048 x 2048
-// (rank 16): 25.6 us skinny, 18.0 wide; 1024 rows of 7168 x 512: 24.4 and 39.8.
+// bf16): k_ad_skinny takes 2 us per wave and 0.45 us (fp32 results 0.5) per 64
+// of a block's share of K at 128 rows (as many bytes less at fewer), k_ad_wide
+// 3 us and 0.23 us (fp32 results 0.26) per 64 of K.  An extension block of 32
+// stacked rank columns, of which a batch of single tokens may need one per
+// adapter and 32 ranks, costs 0.5 us (fp32 results 0.6) of one of a cluster's
+// blocks, or of the pair.  E.g. skinny and wide, rank 16: 320 rows of
+// 2048 x 2048 16.1 and 18.9 us, 1024 rows 26.9 and 18.3, 1024 rows of
+// 7168 x 512 25.1 and 39.6; 24 adapters of rank 64 in 200 rows of
+// 1024 x 14336, fp32 results: 105.0 and 87.9.
 // Up to 64 rows whose adapters fit one tile of 128 stacked rank columns, with
 // at most 8 steps of K per block, k_ad_skinny makes x.A itself (one row of
 // 1024 x 4096: 8.5 us against 10.3 in two launches, of 7168 x 2048: 15.7
@@ -158,11 +160,12 @@ AdapterPath pick_path(const AdapterArgs &g, int sms) {
     const int64_t ext = d.n_tokens <= 256 ? (stacked + 31) / 32 : 0;  // longer batches: packed prompts, few adapters a tile
     const int c = adapter_skinny_cluster(a, sms);
     const int64_t clusters = ((int64_t)d.n_tokens + 127) / 128 * ((d.n_out + 127) / 128);
-    const int64_t skinny = adapter_waves(clusters, c) * ((nk + c - 1) / c + (ext + c - 1) / c) * 50;
-    const int cols = d.y_type == LATENT_TYPE_F32 ? 128 : 256;
+    const bool f32 = d.y_type == LATENT_TYPE_F32;
+    const int step = f32 ? 60 : 50;  // of an extension block; all in 10 ns
+    const int64_t skinny = adapter_waves(clusters, c) * ((nk + c - 1) / c * (f32 ? 50 : 45) + (ext + c - 1) / c * step + 200);
+    const int cols = f32 ? 128 : 256;
     const int64_t tiles = ((int64_t)d.n_tokens + 255) / 256 * ((d.n_out + cols - 1) / cols);
-    const int64_t wide = (tiles + sms / 2 - 1) / (sms / 2) * (nk * (cols == 128 ? 26 : 23) + ext * 55) +
-                         (d.n_tokens <= 256 ? 300 : 0);
+    const int64_t wide = (tiles + sms / 2 - 1) / (sms / 2) * (nk * (f32 ? 26 : 23) + ext * step) + 300;
     return wide < skinny ? kPathWide : kPathSkinny;
 }
 

@@ -6,7 +6,7 @@
 // of the stacked adapters' rank columns, fill the 128 TMEM lanes) and up to
 // 128 rows of x on the N side, so that a batch of one row costs a 16-column
 // MMA and the kernel is a stream of W (bytes bound).  K is split over a
-// cluster of up to 8 blocks so that a narrow W still reaches most SMs; the
+// cluster of up to 16 blocks so that a narrow W still reaches most SMs; the
 // partial tiles are added up in rank order through distributed shared memory,
 // so results do not depend on timing.
 //
@@ -764,15 +764,31 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
     return r;
 }
 
+// Accumulators of `rows` columns in k_ad_skinny's TMEM.  The tensor cores cut a
+// sum off instead of rounding it: a chain over K = 7168 is off by 8e-6 of the
+// result, one over 512 by 5e-7 (measured).  fp32 results therefore use an
+// accumulator per 512 of K, added up in fp32, as far as the TMEM columns go,
+// and clusters long enough.
+int accumulators(int rows, bool self) {
+    const int read = (rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
+    return (512 - (self ? 2 : 1) * read) / rows + 1;
+}
+
 // Blocks of a cluster of k_ad_skinny.  Where both kernels are small, its
 // clusters start beside the shrink's blocks and stream W meanwhile, so those
-// SMs are not counted on (4096 columns, one row: 10.3 us with, 8.8 without).
-int plan_skinny(const AdapterArgs &g, int sms, const int *room, int beside) {
+// SMs are not counted on as long as two blocks per cluster are left (8 rows of
+// 4096 x 4096 with 8 of 64 adapters of rank 16: 13.0 us, 14.7 with all SMs; of
+// 4096 x 8192, where one block of two would be left: 24.7 us, 17.8 with all).
+int plan_skinny(const AdapterArgs &g, const int *room, int beside, int sms) {
     const latent_adapter_desc &d = g.d;
     const int64_t others = ((int64_t)d.n_tokens + g.tile_rows - 1) / g.tile_rows * ((d.n_out + 127) / 128);
     const int nk = (d.n_in + kBK - 1) / kBK;
     int c = pick_cluster(others, nk, room);
-    while (beside && c > 1 && others * c > sms - beside) --c;
+    while (beside && c > 2 && others * c > sms - beside) --c;
+    if (d.y_type == LATENT_TYPE_F32) {
+        const int groups = accumulators((g.tile_rows + 15) / 16 * 16, false);
+        while (c < kMaxCluster && c < nk && room[c + 1] > 0 && (nk + c - 1) / c > 8 * groups) ++c;
+    }
     return c;
 }
 
@@ -807,15 +823,8 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     // as far as the ring still holds the loads of a trip to DRAM
     p.tbufs = self ? 0 : p.rows <= 64 ? kMaxTBufs : 2;
     const size_t stage = 16384 + (size_t)p.rows * 128, tb = (size_t)p.tbufs * ((parts + 1) / 2) * p.rows * 128;
-    int cluster = self ? pick_cluster((int64_t)tiles * ntn, nk, room) : adapter_skinny_cluster(g, sms);
-    // The tensor cores cut a sum off instead of rounding it: a chain over K
-    // = 7168 is off by 8e-6 of the result, one over 512 by 5e-7 (measured).
-    // fp32 results therefore use an accumulator per 512 of K, added up in
-    // fp32, as far as the TMEM columns go, and clusters long enough.
-    const int read = (p.rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    const int groups = (512 - (self ? 2 : 1) * read) / p.rows + 1;
-    if (f32)
-        while (cluster < kMaxCluster && cluster < nk && room[cluster + 1] > 0 && (nk + cluster - 1) / cluster > 8 * groups) ++cluster;
+    const int cluster = self ? adapter_self_cluster(g) : adapter_skinny_cluster(g, sms);
+    const int read = (p.rows + 31) / 32 * 32, groups = accumulators(p.rows, self);
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
@@ -840,7 +849,7 @@ int adapter_skinny_cluster(const AdapterArgs &g, int sms) {
     if (!room) return 1;
     const ShrinkPlan r = plan_shrink(g, room);
     const int shrink = r.cluster * r.slots * r.tiles;
-    return plan_skinny(g, sms, room, shrink <= sms / 3 ? shrink : 0);
+    return plan_skinny(g, room, shrink <= sms / 3 ? shrink : 0, sms);
 }
 
 int adapter_waves(int64_t clusters, int cluster) {
