@@ -488,8 +488,9 @@ LATENT_API int latent_router_grad(const latent_router_grad_desc *desc, struct CU
  *   losses[2] = mean over counted rows of logsumexp(logits)^2
  *   losses[0] = balance_coef losses[1] + z_coef losses[2]
  * and grad (optional) = *d_loss dlosses[0]/dlogits in the logits' type, with f
- * held fixed (d_loss: the device scalar that comes from behind, NULL: 1).  A row whose logits are all -inf has no distribution: it counts as a
- * row, adds nothing and has a zero gradient.  Workspace: 256-byte aligned,
+ * held fixed (d_loss: the device scalar that comes from behind, NULL: 1).  A
+ * row whose logits are all -inf has no distribution: it counts as a row, adds
+ * nothing and has a zero gradient.  Workspace: 256-byte aligned,
  * latent_balance_workspace_size() bytes.  LATENT_ERR_UNSUPPORTED beyond 1024
  * experts.  Stream-ordered; repeated calls agree bit for bit. */
 typedef struct latent_balance_desc {
@@ -528,8 +529,11 @@ LATENT_API int latent_balance_loss(const latent_balance_desc *desc, struct CUstr
  * y += the adapters' part.  An id >= n_adapter counts as none and is recorded
  * in *err (latent_adapter_check).  Adapter factors must be finite: a
  * tile of rows multiplies by the factors of every adapter that one of them
- * uses, zero times the others' (0 x inf would not stay out).  Workspace:
- * 256-byte aligned, latent_adapter_workspace_size() bytes. */
+ * uses, zero times the others' (0 x inf would not stay out).  y must not share
+ * memory with the inputs.  Workspace: 256-byte aligned,
+ * latent_adapter_workspace_size() bytes.  At most 2^30 for n_in and n_out and
+ * 4194240 rows (LATENT_ERR_SHAPE).  Stream-ordered, allocates nothing on the
+ * device; repeated calls agree bit for bit. */
 enum { LATENT_ADAPTER_W_TRANSPOSED = 1u << 0 };
 typedef struct latent_adapter_desc {
     int32_t n_adapter;

@@ -82,9 +82,10 @@ class AdapterSet:
         self.b.view(n * rank, -1)[live, :N] = torch.cat([_tensor(ad[1], dev, dtype) for ad in adapters], 0)
         scales = [float(ad[2]) if len(ad) > 2 else 1.0 for ad in adapters]
         self.scale = torch.tensor(scales, dtype=torch.float32, device=dev)
+        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+        # (reads the result: a set can be used on any stream from here on)
         if not np.isfinite(scales).all() or not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
             raise ValueError(f"adapter factors and scales must be finite in {dtype}")
-        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         # a, lda, b, ldb, scale as a call's descriptor takes them
         self._factors = (self.a.data_ptr(), self.a.shape[2], self.b.data_ptr(), self.b.shape[2], self.scale.data_ptr())
         self._err_ptr = self.err.data_ptr()
@@ -122,7 +123,8 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     with the adapters' part in fp32); ids int32 [T], negative: no adapter,
     >= n_adapter: none either, and ``adapters.check()`` reports it.  Returns
     [T, N] in ``out_dtype`` (x's dtype or float32; x's by default), fp32 sums
-    rounded once, or fills ``out`` (rows may be strided).
+    rounded once, or fills ``out`` (rows may be strided; it must not share
+    memory with the inputs).
     """
     s = adapters
     dev, dt, K, N = s.device, s.dtype, s.n_in, s.n_out

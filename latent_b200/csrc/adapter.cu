@@ -1,8 +1,8 @@
 // Low-rank adapters of many requests beside one shared projection
 // (latent_adapter_project): y[t] = x[t].W + s_a (x[t].A_a).B_a, a = ids[t].
 //
-// Two steps: t[t] = s_a x[t].A_a (fp32, [T][rank] in the workspace), then a
-// product kernel that adds t.B_a to x.W.  This file has the entry points and
+// Two steps: t = x[t].A_a (fp32, [T][rank] in the workspace), then a product
+// kernel that adds s_a t.B_a to x.W.  This file has the entry points and
 // both steps on the CUDA cores (k_ad_shrink_any, k_ad_any), for what the
 // tensor-core kernels cannot read: sizes or strides that are not multiples of
 // 8, unaligned rows, and the adapters' part alone (no dense W).
@@ -114,6 +114,7 @@ bool ad_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 int ad_validate(const latent_adapter_desc *d) {
     if (!d) return LATENT_ERR_INVALID;
     if (d->n_adapter < 0 || d->n_in < 1 || d->n_out < 1 || d->n_tokens < 0) return LATENT_ERR_SHAPE;
+    if (d->n_in > 1 << 30 || d->n_out > 1 << 30) return LATENT_ERR_SHAPE;  // tiles reach past the end in 32 bits
     if (d->rank != 16 && d->rank != 32 && d->rank != 64 && d->rank != 128) return LATENT_ERR_UNSUPPORTED;
     if (d->type != LATENT_TYPE_F16 && d->type != LATENT_TYPE_BF16) return LATENT_ERR_DTYPE;
     if (d->y_type != d->type && d->y_type != LATENT_TYPE_F32) return LATENT_ERR_DTYPE;
@@ -121,9 +122,10 @@ int ad_validate(const latent_adapter_desc *d) {
     return LATENT_OK;
 }
 
-// What TMA and 16-byte stores need: rows of multiples of 16 bytes from 16-byte boundaries.
+// What TMA and 16-byte stores need: rows of multiples of 16 bytes from 16-byte boundaries, coordinates of 32 bits,
+// and a grid over the columns.
 bool ad_tensor_cores(const latent_adapter_desc *d) {
-    return d->w && d->n_adapter > 0 && (d->n_in | d->n_out) % 8 == 0 &&
+    return d->w && d->n_adapter > 0 && (int64_t)d->n_adapter * d->rank <= INT32_MAX && d->n_out <= 65535 * 128 && (d->n_in | d->n_out) % 8 == 0 &&
            (d->ldx | d->ldw | d->lda | d->ldb | d->ldy) % 8 == 0 && ad_aligned(d->x, 16) && ad_aligned(d->w, 16) &&
            ad_aligned(d->a, 16) && ad_aligned(d->b, 16) && ad_aligned(d->y, 16);
 }

@@ -311,9 +311,9 @@ __device__ __forceinline__ float adapter_dot(const latent_adapter_desc &d, const
 
 }  // namespace adapter
 
-// A row-major 16-bit matrix as a 2-D TMA map with a {64, box_rows} box, 128B swizzle.
-// The output matrix, a box of 128-byte rows.
+// The output matrix as a 2-D TMA map, a box of 128-byte rows, 128B swizzle.
 bool adapter_out_map(void *map, int y_type, void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
+// A row-major 16-bit matrix, likewise: a {64, box_rows} box.
 bool adapter_map(void *map, bool bf16, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
 
 }  // namespace latent

@@ -11,9 +11,8 @@
 // so results do not depend on timing.
 //
 // k_ad_skinny is launched as a programmatic dependent of k_ad_shrink (unless it
-// makes x.A itself): it
-// streams W while x.A is still being made and waits for it (griddepcontrol)
-// only before the extension blocks.
+// makes x.A itself): it streams W while x.A is still being made and waits for
+// it (griddepcontrol) only before the extension blocks.
 #include <cuda.h>
 
 #include <mutex>
@@ -350,9 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         }
         if (ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
         if (SELF && ok) {
-            const int total = uniform(sh.segs.n) * rank;
-            for (int m = 0; m < total && ok; m += 128)
-                ok = load_stacked(sh, p, at, ring, stage, &mA, &mX, m, total, k0, k1, t0, rank, log2r);
+            const int total = uniform(sh.segs.n) * rank;  // 128 at most
+            if (total) ok = load_stacked(sh, p, at, ring, stage, &mA, &mX, 0, total, k0, k1, t0, rank, log2r);
         }
         if (!SELF && ok) {
             const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
@@ -399,16 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         }
         if (SELF && ok && elect()) mma_commit(sh.acc_full);
         if (ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
-        if (SELF && ok) {
-            const int total = uniform(sh.segs.n) * rank;
-            uint32_t n = 0;
-            for (int m = 0; m < total; m += 128, ++n) {
-                if (n >= 1 && !wait_warp(sh.acc_empty + 1, (n - 1u) & 1u, &sh.abort)) { ok = false; break; }
-                tc_fence_after();
-                ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
-                if (!ok) break;
-                if (elect()) mma_commit(sh.acc_full + 1);
-            }
+        if (SELF && ok && uniform(sh.segs.n)) {
+            ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
+            if (ok && elect()) mma_commit(sh.acc_full + 1);
         }
         if (!SELF && ok) {
             const int ext = uniform(sh.segs.n) * rank, ne = (ext + kExt - 1) / kExt;
@@ -470,13 +461,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             tc_fence_after();
             cluster_wait();
             if (ok) send_product();
-            uint32_t n = 0;
-            for (int m = 0; m < ext && ok; m += 128, ++n) {
-                ok = __all_sync(0xffffffffu, wait(sh.acc_full + 1, n & 1u) && !sh.abort);
+            if (ext && ok) {
+                ok = __all_sync(0xffffffffu, wait(sh.acc_full + 1, 0u) && !sh.abort);
                 tc_fence_after();
-                if (ok) send_stacked(sh, p, tmem + (uint32_t)p.shrink_col, m, rank, log2r, r, 512u);
+                if (ok) send_stacked(sh, p, tmem + (uint32_t)p.shrink_col, 0, rank, log2r, r, 512u);
                 tc_fence_before();
-                mbar_arrive(sh.acc_empty + 1);
             }
         }
         if constexpr (!SELF) {

@@ -6,9 +6,9 @@ experts (its per-slot rows give d_weights = <d_out, y_slot>),
 ``router_topk_grad`` carries that back to the logits and ``balance_loss``
 adds the load-balance and z losses.  The reference has no training code.
 Both kernels return explicit gradients, which add up in one buffer
-(``out=``) and can be captured into a CUDA graph; where autograd is on and
-the logits require a gradient, ``balance_loss`` and ``router_topk`` are
-differentiable through it as well (outside graph capture).
+(``out=``) and can be captured into a CUDA graph.  Where autograd is on and
+the logits require a gradient, ``balance_loss`` and, when asked,
+``router_topk`` are differentiable through it as well (outside graph capture).
 """
 
 from __future__ import annotations
@@ -205,7 +205,7 @@ def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.T
 
 
 class RouterTopK(torch.autograd.Function):
-    """``router_topk`` with weights that autograd can differentiate."""
+    """``router_topk(..., differentiable=True)``: weights that autograd can differentiate."""
 
     @staticmethod
     def forward(ctx, scores, top_k, threshold, renormalize, logits, expert_counts):

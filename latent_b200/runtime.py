@@ -359,7 +359,7 @@ _OPS: Dict[int, ExpertFFN] = {}
 
 
 def router_topk(scores: torch.Tensor, top_k: int, threshold: float = 0.95, renormalize: bool = True,
-                logits: bool = False, expert_counts: bool = False):
+                logits: bool = False, expert_counts: bool = False, differentiable: bool = False):
     """Adaptive top-k routing on the device (latent_router_topk).
 
     scores: [T, E] fp32 router scores on a CUDA device.  Returns (ids [T, k]
@@ -371,8 +371,9 @@ def router_topk(scores: torch.Tensor, top_k: int, threshold: float = 0.95, renor
     With ``logits`` the scores are router logits and the softmax runs in the
     same kernel (latent_router_route); with ``expert_counts`` a fourth
     result holds the kept slots per expert [E] int32.
-    When autograd is on and ``scores`` requires a gradient, the weights carry
-    one (latent_b200.router_topk_grad; the kept set is held fixed).
+    With ``differentiable``, where autograd is on and ``scores`` requires a
+    gradient, the weights carry one (latent_b200.router_topk_grad; the kept
+    set is held fixed); not inside a graph capture.
     Raises ValueError where the reference does (threshold outside (0, 1],
     top_k > n_experts, scores not 2-D)."""
     if not torch.is_tensor(scores) or scores.device.type != "cuda":
@@ -386,7 +387,7 @@ def router_topk(scores: torch.Tensor, top_k: int, threshold: float = 0.95, renor
         raise ValueError(f"top_k must be positive, got {top_k}")
     if not 0.0 < threshold <= 1.0:
         raise ValueError(f"threshold must be in (0, 1], got {threshold}")
-    if scores.requires_grad and torch.is_grad_enabled():
+    if differentiable and scores.requires_grad and torch.is_grad_enabled():
         from .router_train import RouterTopK
         ids, w, n_kept, counts = RouterTopK.apply(scores, top_k, threshold, renormalize, logits, expert_counts)
         return (ids, w, n_kept, counts) if expert_counts else (ids, w, n_kept)

@@ -287,12 +287,13 @@ def test_router_grad_against_differences(cuda):
 def test_autograd_matches_the_explicit_gradients(cuda):
     l, _ = inputs(200, 64, 6, F32, seed=4)
     leaf = l.clone().requires_grad_(True)
-    ids, w, nk, counts = router_topk(leaf, 6, 0.9, logits=True, expert_counts=True)
+    ids, w, nk, counts = router_topk(leaf, 6, 0.9, logits=True, expert_counts=True, differentiable=True)
     with torch.no_grad():
         plain = router_topk(l, 6, 0.9, logits=True, expert_counts=True)
     for a, b in zip((ids, w, nk, counts), plain):
         assert torch.equal(a, b) and not b.requires_grad
     assert w.requires_grad and not ids.requires_grad
+    assert not any(t.requires_grad for t in router_topk(leaf, 6, 0.9, logits=True))  # only when asked
     dw = torch.randn(w.shape, device="cuda")
     r = balance_loss(leaf, ids, 0.02, 0.001)
     assert r.grad is None and torch.equal(r.counts, counts)
@@ -304,7 +305,7 @@ def test_autograd_matches_the_explicit_gradients(cuda):
     # two fp32 gradients, each within a few steps of the other form's, and their sum
     assert float((leaf.grad.double() - g).abs().max()) <= 8 * 2.0 ** -24 * float(g.abs().max())
     leaf16 = l.to(BF).requires_grad_(True)
-    ids, w, _ = router_topk(leaf16, 6, 0.9, logits=True, renormalize=False)
+    ids, w, _ = router_topk(leaf16, 6, 0.9, logits=True, renormalize=False, differentiable=True)
     w.sum().backward()
     assert leaf16.grad.dtype == BF
     assert torch.equal(leaf16.grad, router_topk_grad(leaf16.detach(), ids, torch.ones_like(w), False, True))
@@ -356,7 +357,7 @@ def test_streams_and_graphs(cuda):
             with pytest.raises(RuntimeError, match="capture"):
                 balance_loss(leaf, ids)
             with pytest.raises(RuntimeError, match="capture"):
-                router_topk(leaf, 4, logits=True)
+                router_topk(leaf, 4, logits=True, differentiable=True)
         finally:
             g.capture_end()
     torch.cuda.synchronize()

@@ -70,7 +70,7 @@ def test_adapter_project_validates_on_the_host(lib):
     f = lib.latent_adapter_project
     assert f(None, None) == 1
     for bad in ({"n_adapter": -1}, {"n_in": 0}, {"n_out": 0}, {"n_tokens": -1}, {"ldx": 63}, {"ldw": 31}, {"lda": 63},
-                {"ldb": 31}, {"ldy": 31}, {"flags": 1, "ldw": 63}):
+                {"ldb": 31}, {"ldy": 31}, {"flags": 1, "ldw": 63}, {"n_in": (1 << 30) + 1}, {"n_out": 0x7fffffff}):
         assert f(_desc(**bad), None) == 2, bad
     for bad in ({"rank": 8}, {"rank": 48}, {"rank": 256}):
         assert f(_desc(**bad), None) == 9, bad
