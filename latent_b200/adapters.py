@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .router_train import _on
+from .router_train import _on, _with_workspace
 from .runtime import FactorPair, project
 
 __all__ = ["AdapterSet", "adapter_project"]
@@ -182,12 +182,10 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
         y = out if out is not None else torch.empty(T, N, dtype=out_dtype, device=dev)
     if pair:
         y_type = _lib.TYPE_F32
-    n = s._ws.get(T) or s.workspace_bytes(T)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    d = _lib.ADAPTER_DESC.pack(s.n_adapter, s.rank, K, N, T, s._type, y_type, flags, x.data_ptr(), ldx, w_ptr, ldw,
-                               *s._factors, ids.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
-                               s._err_ptr, ws.data_ptr(), n)
-    _lib.check(_on(dev, _lib.lib().latent_adapter_project, d), "latent_adapter_project")
+    _with_workspace(dev, s._ws.get(T) or s.workspace_bytes(T), _lib.lib().latent_adapter_project,
+                    "latent_adapter_project", _lib.ADAPTER_DESC,
+                    (s.n_adapter, s.rank, K, N, T, s._type, y_type, flags, x.data_ptr(), ldx, w_ptr, ldw, *s._factors,
+                     ids.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N, s._err_ptr))
     if pair:
         return y.to(out_dtype) if out is None else out.copy_(y)
     return y

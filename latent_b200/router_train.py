@@ -47,6 +47,23 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _with_workspace(device: torch.device, size: int, fn, what: str, desc, fields) -> None:
+    """Calls ``fn`` on the descriptor ``fields`` + (workspace, size), with ``device`` current, on its current stream.
+
+    The workspace is the caching allocator's memory of that stream, as a tensor's would be (a captured call's comes
+    from its graph's pool), given back behind the call; without a tensor around it, which costs 1 us of a call's 9."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(device):
+            return _with_workspace(device, size, fn, what, desc, fields)
+    stream = _raw_stream(index)
+    ws = torch._C._cuda_cudaCachingAllocator_raw_alloc(size, stream)
+    try:
+        _lib.check(fn(desc.pack(*fields, ws, size), stream), what)
+    finally:
+        torch._C._cuda_cudaCachingAllocator_raw_delete(ws)
+
+
 _WS_BYTES = {}    # workspace size by (sequences, experts)
 
 
@@ -92,18 +109,16 @@ def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradie
     T, E = logits.shape
     dev = logits.device
     n = _WS_BYTES.get((n_seq, E)) or _workspace_bytes(n_seq, E)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     losses = torch.empty(3, dtype=torch.float32, device=dev)
     # [E] when the rows are one sequence without borders
     counts = torch.empty(E, dtype=torch.int32, device=dev) if cu is None else \
         torch.empty(n_seq, E, dtype=torch.int32, device=dev)
     grad = torch.empty_like(logits) if gradient else None
-    d = _lib.BALANCE_DESC.pack(T, E, ids.shape[1], n_seq, _X_TYPES[logits.dtype], 0, balance_coef, z_coef,
-                               logits.data_ptr(), ids.data_ptr(), 0 if valid is None else valid.data_ptr(),
-                               0 if cu is None else cu.data_ptr(), 0 if d_loss is None else d_loss.data_ptr(),
-                               losses.data_ptr(), counts.data_ptr(), 0 if grad is None else grad.data_ptr(),
-                               ws.data_ptr(), n)
-    _lib.check(_on(dev, _lib.lib().latent_balance_loss, d), "latent_balance_loss")
+    _with_workspace(dev, n, _lib.lib().latent_balance_loss, "latent_balance_loss", _lib.BALANCE_DESC,
+                    (T, E, ids.shape[1], n_seq, _X_TYPES[logits.dtype], 0, balance_coef, z_coef, logits.data_ptr(),
+                     ids.data_ptr(), 0 if valid is None else valid.data_ptr(), 0 if cu is None else cu.data_ptr(),
+                     0 if d_loss is None else d_loss.data_ptr(), losses.data_ptr(), counts.data_ptr(),
+                     0 if grad is None else grad.data_ptr()))
     return losses, counts, grad
 
 
