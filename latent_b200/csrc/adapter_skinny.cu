@@ -194,6 +194,10 @@ __device__ __forceinline__ void send_stacked(const Shared &sh, const Plan &p, ui
 // cluster sums K blocks of its share; every block sends the t of a row to the
 // row's owner (rows are dealt to the cluster in runs), which adds them up in
 // rank order.
+// Measured: 64 rows of K = 7168 with 24 adapters of rank 64 10.4 us (22 MB of A,
+// 2.2 TB/s); 2047 rows of K = 4096 with one adapter of rank 64 11.5 us, without
+// any 4.8 (start, adapter list, the cluster's barriers): in between the blocks
+// fetch 27 MB of x and A, 4 TB/s.
 template <bool BF>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant__ CUtensorMap mA,
                                                            const __grid_constant__ CUtensorMap mX, AdapterArgs g,
@@ -294,6 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
 // behind its W loads, and the owner of a row adds x.A.B for its 128 columns on
 // the CUDA cores: no trip of x.A through global memory, at the price of every
 // cluster loading the adapters' A.
+//
+// Measured: one row of 2048 x 2048, rank 16, SELF: 8.3 us against 1.3 for its 8.5
+// MB: start, one trip to DRAM, two cluster barriers and the end of the grid are
+// what is left.  64 rows of 7168 x 2048, 24 adapters of rank 64: 15.1 us for 36
+// MB of W and B (2.4 TB/s; the extension blocks wait for x.A).
 template <bool BF, bool KN, int PARTS, typename Y, bool SELF>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant__ CUtensorMap mW,
                                                            const __grid_constant__ CUtensorMap mB,

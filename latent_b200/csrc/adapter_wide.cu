@@ -14,6 +14,10 @@
 //
 // A pair tile of 256 columns costs 512 cycles of MMA per 64 of K against 64 KB
 // of loads: half the L2 traffic per operation of one block working alone.
+// Measured: 8192 rows of 4096 x 14336, bf16: 602 us, 1.60 PFLOP/s, tensor pipe
+// 93% active (power bound in a long run: 650 us).  2047 rows of 4096 x 4096: 51
+// us without adapters (128 tiles on 74 pairs: two turns, the second of 54), 56
+// with five packed prompts of rank 64, 65 with six adapters mixed over all rows.
 //
 // fp32 results: the tensor cores cut a sum off instead of rounding it (a chain
 // over K = 7168 is off by 8e-6 of the result, one over 512 by 5e-7), so the two
@@ -80,8 +84,9 @@ __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     return r;
 }
 // What the arrival stands for is ordered before it already: shared memory that
-// the tensor core reads by the proxy fence, TMEM reads by their wait.  A release
-// at cluster scope on top cost 0.8 us an arrival.
+// the tensor core reads by the proxy fence, TMEM reads by their wait.  With a
+// release at cluster scope on top an extension block took its builders 1.3 us
+// instead of 0.5.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
