@@ -254,6 +254,45 @@ def test_calls_of_all_kinds_on_two_streams_at_once(cuda):
         c[2].check()
 
 
+def test_calls_from_two_threads(cuda):
+    from concurrent.futures import ThreadPoolExecutor
+    calls = []
+    for T, K, N, n in ((1, 1024, 2048, 2), (40, 2048, 704, 30), (300, 512, 1024, 3), (9, 100, 37, 2)):
+        x, w, ads, i = make(T, K, N, [16] * n, BF, seed=T + 1)
+        s = AdapterSet(ads)
+        calls.append((x, w, s, i, adapter_project(x, w, s, i)))
+    torch.cuda.synchronize()
+
+    def run(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [[adapter_project(*c[:4]) for c in calls[k:] + calls[:k]] for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(g, c[4]) for r in got for g, c in zip(r, calls[k:] + calls[:k]))
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(run, (0, 2)))
+
+
+@pytest.mark.parametrize("T,K,N", [(160000, 64, 14336),   # y beyond 2^31 elements, SM pairs
+                                   (70000, 32768, 64),    # x
+                                   (2, 8192, 270000),     # w
+                                   (20000, 24, 131073)])  # y, CUDA cores
+def test_offsets_beyond_32_bits(cuda, T, K, N):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=BF)  # noqa: E731
+    x, w = rand(T, K), rand(K, N) / K ** 0.5
+    ads = [(rand(K, 16) / K ** 0.5, rand(16, N) * 0.2, 0.5 + 0.25 * i) for i in range(3)]
+    ids = (torch.arange(T, device="cuda") * 4 // T - 1).to(torch.int32)
+    y = adapter_project(x, w, AdapterSet(ads), ids)
+    rows = torch.arange(T, device="cuda")
+    rows = rows[(rows < 2) | (rows >= T - 130)]
+    for lo, hi in ((0, 100), (max(0, N - 1000), N)):
+        want, S = reference(x[rows], w[:, lo:hi], [(a, b[:, lo:hi], s) for a, b, s in ads], ids[rows])
+        assert_close(y[rows, lo:hi], want, S, K, 16)
+    del x, w, y, ads
+    torch.cuda.empty_cache()
+
+
 FIRST_IN_CAPTURE = """
 import torch
 from latent_b200 import AdapterSet, adapter_project, balance_loss, router_topk_grad

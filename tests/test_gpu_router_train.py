@@ -363,6 +363,28 @@ def test_streams_and_graphs(cuda):
     torch.cuda.synchronize()
 
 
+def test_offsets_beyond_32_bits(cuda):
+    T, E, k, n = 2200000, 1000, 2, 64
+    g = torch.Generator("cuda").manual_seed(3)
+    l = torch.randn((T, E), generator=g, device="cuda", dtype=BF)
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda").to(torch.int32)
+    dw = torch.randn((T, k), generator=g, device="cuda")
+    r = balance_loss(l, ids, 1e4, 1e4, gradient=True)
+    assert torch.equal(r.counts.long(), torch.bincount(ids.view(-1).long(), minlength=E))
+    tail = l[-n:].double()
+    p, lse = torch.softmax(tail, 1), torch.logsumexp(tail, 1)[:, None]
+    c = E * r.counts.double() / (k * T) / T
+    d = (p * c).sum(1, keepdim=True)
+    want = 1e4 * p * (c - d + 2 * lse / T)
+    eps, lerr = steps(l[-n:]), lse.abs() * 2.0 ** -22 + 64 * 2.0 ** -24
+    close(r.grad[-n:], want, 1e4 * p * ((c + d) * eps + 2 / T * (lerr + lse.abs() * eps)) + rounding(r.grad, want))
+    del r
+    for renorm in (True, False):
+        got = router_topk_grad(l, ids, dw, renormalize=renorm, logits=True)[-n:].clone()
+        assert torch.equal(got, check_route(l[-n:].contiguous(), ids[-n:], dw[-n:], True, renorm))
+    torch.cuda.empty_cache()
+
+
 def test_refusals(cuda):
     l, ids = inputs(10, 16, 3)
     dw = torch.ones((10, 3), device="cuda")
