@@ -140,8 +140,8 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     if not pair and (weight.shape != (K, N) or weight.dtype != dt):
         raise ValueError(f"weight must be {dt} [{K}, {N}]")
     if x.device != dev or ids.device != dev or (not pair and weight.device != dev) or \
-            (out is not None and out.device != dev):
-        raise ValueError("x, weight, ids and out must be on the adapters' device")
+            (out is not None and out.device != dev) or not x.is_cuda:
+        raise ValueError("x, weight, ids and out must be on the adapters' device, a CUDA device")
     if (x.requires_grad or (not pair and weight.requires_grad) or (out is not None and out.requires_grad)) and \
             torch.is_grad_enabled():
         raise ValueError("adapter_project computes no gradients: call it under torch.no_grad() or on detached tensors")

@@ -293,6 +293,28 @@ def test_offsets_beyond_32_bits(cuda, T, K, N):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("T", [40, 700])
+def test_workspace_of_a_captured_call_stays_the_graphs_own(cuda, T):
+    from latent_b200 import balance_loss
+    x, w, ads, i = make(T, 512, 640, [16] * 12, BF, seed=T)
+    s = AdapterSet(ads)
+    l = torch.randn((T, 64), device="cuda")
+    slots = torch.randint(0, 64, (T, 4), device="cuda").to(torch.int32)
+    want, r = adapter_project(x, w, s, i), balance_loss(l, slots, 0.1, 0.1, gradient=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = adapter_project(x, w, s, i)
+        rg = balance_loss(l, slots, 0.1, 0.1, gradient=True)
+    mine = [torch.full((n,), 7, dtype=torch.uint8, device="cuda")     # would land on it, had it gone back to all
+            for n in (s.workspace_bytes(T), 66560, 70000, 1 << 20) for _ in range(40)]
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(bool((m == 7).all()) for m in mine)
+    assert torch.equal(y, want) and torch.equal(rg.grad, r.grad) and torch.equal(rg.loss, r.loss)
+
+
 FIRST_IN_CAPTURE = """
 import torch
 from latent_b200 import AdapterSet, adapter_project, balance_loss, router_topk_grad

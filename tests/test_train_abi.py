@@ -6,7 +6,7 @@ import ctypes as C
 import pytest
 import torch
 
-from latent_b200 import AdapterSet, _lib, balance_loss, router_topk_grad
+from latent_b200 import AdapterSet, _lib, adapter_project, balance_loss, router_topk_grad
 from latent_b200.build import build
 
 
@@ -91,7 +91,9 @@ def test_adapter_project_validates_on_the_host(lib):
 
 def test_python_refusals_without_a_device():
     l, ids = torch.zeros((4, 8)), torch.zeros((4, 2), dtype=torch.int32)
+    on_host = AdapterSet([(torch.zeros(8, 2), torch.zeros(2, 8))], device="cpu", dtype=torch.float16)
     for bad in (lambda: balance_loss(l, ids), lambda: router_topk_grad(l, ids, torch.zeros((4, 2))),
+                lambda: adapter_project(l.half(), torch.zeros((8, 8), dtype=torch.float16), on_host, ids[:, 0].contiguous()),
                 lambda: AdapterSet([], device="cpu"),
                 lambda: AdapterSet([(torch.zeros(8, 2), torch.zeros(3, 8))], device="cpu"),
                 lambda: AdapterSet([(torch.full((8, 2), float("inf")), torch.zeros(2, 8))], device="cpu")):
