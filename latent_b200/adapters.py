@@ -125,6 +125,10 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     [T, N] in ``out_dtype`` (x's dtype or float32; x's by default), fp32 sums
     rounded once, or fills ``out`` (rows may be strided; it must not share
     memory with the inputs).
+
+    The tensor cores need rows of x and of the weight that start at multiples
+    of 16 bytes (N itself may be odd); others run on the CUDA cores, about ten
+    times slower.
     """
     s = adapters
     dev, dt, K, N = s.device, s.dtype, s.n_in, s.n_out
@@ -164,7 +168,7 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
         x = x.contiguous()
         ldx = K
     if T == 1:
-        ldx = K
+        ldx = (K + 7) // 8 * 8  # no second row: a stride that tensor maps take
     flags, w_ptr, ldw = 0, 0, 0
     if pair:
         y = project(x, weight)

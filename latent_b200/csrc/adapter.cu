@@ -4,7 +4,7 @@
 // Two steps: t = x[t].A_a (fp32, [T][rank] in the workspace), then a product
 // kernel that adds s_a t.B_a to x.W.  This file has the entry points and
 // both steps on the CUDA cores (k_ad_shrink_any, k_ad_any), for what the
-// tensor-core kernels cannot read: sizes or strides that are not multiples of
+// tensor-core kernels cannot read: strides of x or W that are not multiples of
 // 8, unaligned rows, and the adapters' part alone (no dense W).
 #include "adapter_mma.cuh"
 
@@ -122,12 +122,12 @@ int ad_validate(const latent_adapter_desc *d) {
     return LATENT_OK;
 }
 
-// What TMA and 16-byte stores need: rows of multiples of 16 bytes from 16-byte boundaries, coordinates of 32 bits,
-// and a grid over the columns.
+// What TMA loads need: rows from 16-byte boundaries (of any width: a map ends where the matrix does), coordinates of
+// 32 bits, and a grid over the columns.
 bool ad_tensor_cores(const latent_adapter_desc *d) {
-    return d->w && d->n_adapter > 0 && (int64_t)d->n_adapter * d->rank <= INT32_MAX && d->n_out <= 65535 * 128 && (d->n_in | d->n_out) % 8 == 0 &&
-           (d->ldx | d->ldw | d->lda | d->ldb | d->ldy) % 8 == 0 && ad_aligned(d->x, 16) && ad_aligned(d->w, 16) &&
-           ad_aligned(d->a, 16) && ad_aligned(d->b, 16) && ad_aligned(d->y, 16);
+    return d->w && d->n_adapter > 0 && (int64_t)d->n_adapter * d->rank <= INT32_MAX && d->n_out <= 65535 * 128 &&
+           (d->ldx | d->ldw | d->lda | d->ldb) % 8 == 0 && ad_aligned(d->x, 16) && ad_aligned(d->w, 16) &&
+           ad_aligned(d->a, 16) && ad_aligned(d->b, 16);
 }
 
 enum AdapterPath { kPathSelf, kPathSkinny, kPathWide };
@@ -158,7 +158,8 @@ AdapterPath pick_path(const AdapterArgs &g, int sms) {
         const int c = adapter_self_cluster(a);
         if ((nk + c - 1) / c <= 8) return kPathSelf;
     }
-    if (d.n_tokens <= 96) return kPathSkinny;
+    // k_ad_wide stores through TMA, which ends a row at a multiple of 16 bytes, with zeros behind the last column
+    if (d.n_tokens <= 96 || (d.ldy | d.n_out) % 8 || !ad_aligned(d.y, 16)) return kPathSkinny;
     const int64_t ext = d.n_tokens <= 256 ? (stacked + 31) / 32 : 0;  // longer batches: packed prompts, few adapters a tile
     const int c = adapter_skinny_cluster(a, sms);
     const int64_t clusters = ((int64_t)d.n_tokens + 127) / 128 * ((d.n_out + 127) / 128);

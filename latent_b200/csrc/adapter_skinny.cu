@@ -292,6 +292,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     if (warp == 2) tmem_dealloc(tmem, p.cols);
 }
 
+template <typename Y> __device__ __forceinline__ Y to_y(float v);
+template <> __device__ __forceinline__ float to_y<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half to_y<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_y<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
 // The product.  Block (cluster rank, 128 output columns, row tile).
 //
 // SELF (one launch, one tile of rows): every cluster makes all of x.A itself,
@@ -557,10 +562,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             v.x += adapter_dot<BF>(d, t, ad, n);
             v.y += adapter_dot<BF>(d, t, ad, n + 1);
         }
-        if constexpr (sizeof(Y) == 4)
-            *reinterpret_cast<float2 *>(static_cast<float *>(d.y) + (int64_t)(t0 + r) * d.ldy + n) = v;
-        else
-            *reinterpret_cast<uint32_t *>(static_cast<Y *>(d.y) + (int64_t)(t0 + r) * d.ldy + n) = pack2<BF>(v.x, v.y);
+        Y *y = static_cast<Y *>(d.y) + (int64_t)(t0 + r) * d.ldy + n;
+        if (n + 1 < d.n_out && (uintptr_t)y % (2 * sizeof(Y)) == 0) {
+            if constexpr (sizeof(Y) == 4) *reinterpret_cast<float2 *>(y) = v;
+            else *reinterpret_cast<uint32_t *>(y) = pack2<BF>(v.x, v.y);
+        } else {  // rows of y that are not aligned, the last column of an odd width
+            y[0] = to_y<Y>(v.x);
+            if (n + 1 < d.n_out) y[1] = to_y<Y>(v.y);
+        }
     }
     tc_fence_before();
     __syncthreads();

@@ -102,6 +102,41 @@ def test_odd_widths(cuda, T, K, N, layout):
     assert_close(adapter_project(x, w, AdapterSet(ads), i), *reference(x, w, ads, i), K, 32)
 
 
+@pytest.mark.parametrize("T,K,N,ranks", [(1, 2048, 1001, [16]), (1, 72, 1, [3]), (9, 1024, 5003, [16] * 12),
+                                         (40, 512, 37, [64] * 9), (130, 256, 257, [16, 32]), (300, 520, 1999, [16] * 3), (1, 100, 37, [16]),
+                                         (2000, 512, 1001, [16] * 4)])
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (HF, HF), (BF, F32)])
+def test_odd_result_widths(cuda, T, K, N, ranks, dtype, out):
+    """Aligned rows of x and W, results of an odd width: dense, and as columns of a wider matrix that keeps the rest."""
+    x, w, ads, i = make(T, K, N, ranks, dtype, seed=N, layout="nk")
+    s = AdapterSet(ads)
+    y, S = reference(x, w, ads, i)
+    assert_close(adapter_project(x, w, s, i, out_dtype=out), y, S, K, s.rank)
+    for pad in (N + 3, N + 8 - N % 8):
+        big = torch.full((T + 1, pad), 7.0, dtype=out, device="cuda")
+        adapter_project(x, w, s, i, out=big[:T, :N])
+        assert_close(big[:T, :N], y, S, K, s.rank)
+        assert bool((big[T] == 7).all()) and bool((big[:, N:] == 7).all())
+    s.check()
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+@pytest.mark.parametrize("out", [BF, F32])
+def test_odd_contraction_in_padded_rows(cuda, T, out):
+    """A width of x and W that ends inside a 16-byte run: what pads the rows is not read."""
+    K, N = 101, 77
+    x, w, ads, i = make(T, K, N, [16, 5], BF, seed=6, layout="nk")
+    s = AdapterSet(ads)
+    y, S = reference(x, w, ads, i)
+    xp = torch.full((T, 104), float("nan"), dtype=BF, device="cuda")
+    wp = torch.full((N, 104), float("nan"), dtype=BF, device="cuda")
+    xp[:, :K], wp[:, :K] = x, w.t()
+    assert_close(adapter_project(xp[:, :K], wp[:, :K].t(), s, i, out_dtype=out), y, S, K, s.rank)
+    kn = torch.full((K, 80), float("nan"), dtype=BF, device="cuda")
+    kn[:, :N] = w
+    assert_close(adapter_project(xp[:, :K], kn[:, :N], s, i, out_dtype=out), y, S, K, s.rank)
+
+
 @pytest.mark.parametrize("T", [3, 64, 300])
 def test_strided_and_unaligned_rows(cuda, T):
     K, N = 256, 192
