@@ -15,7 +15,7 @@
 // value and gradient need the counts first and then ONE pass over the logits,
 // and no per-expert probability sums.
 //
-// k_balance_count: one cluster of 8 blocks per sequence; each block counts its
+// k_balance_count: one cluster of 1 to 8 blocks per sequence; each block counts its
 // rows' ids in a shared-memory histogram, the blocks add theirs up through
 // distributed shared memory: integers, no global atomics, nothing to zero.  It
 // leaves f as well, in fp32: an integer to float conversion per column and row
@@ -28,8 +28,8 @@
 //
 // Measured, 16384 rows of 256 fp32 experts, top-8, 8 sequences: count 5.1 us,
 // main 11.4 (34 MB read and written, 2.9 TB/s; about half of its blocks' time is
-// waiting on loads and shuffles), 14.7 for both in a graph.  64 rows: 3.1, 4.5
-// and 5.9.
+// waiting on loads and shuffles), 13.8 for both in a graph.  64 rows: 3.1, 4.5
+// and 6.1.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -44,8 +44,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxTrainExperts = 1024;  // 32 logits per lane in registers
 constexpr int kMaxTrainTopK = 32;       // one lane per slot
-constexpr int kCountCluster = 8;
-constexpr int kCountThreads = 512;
+constexpr int kCountThreads = 1024;  // at most
 constexpr int kRowWarps = 8;
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -199,13 +198,14 @@ struct BalanceArgs {
     uint32_t *ticket;
 };
 
-__global__ void __cluster_dims__(kCountCluster, 1, 1) __launch_bounds__(kCountThreads)
+template <int CS>
+__global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(kCountThreads)
 k_balance_count(BalanceArgs a) {
     __shared__ int hist[kMaxTrainExperts];
     __shared__ int tot[2];  // counted rows, kept slots of this block
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank();
-    const int s = blockIdx.x / kCountCluster;
+    const int s = blockIdx.x / CS;
     launch_dependents();
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
     if (threadIdx.x < 2) tot[threadIdx.x] = 0;
@@ -213,7 +213,7 @@ k_balance_count(BalanceArgs a) {
     __syncthreads();
     int lo, hi;
     sequence_rows(a.cu, s, a.T, lo, hi);
-    const int per = (hi - lo + kCountCluster - 1) / kCountCluster;
+    const int per = (hi - lo + CS - 1) / CS;
     const int r0 = min(hi, lo + rank * per), r1 = min(hi, r0 + per);
     int rows = 0, slots = 0;
     const int end = r1 * a.k;
@@ -245,17 +245,17 @@ k_balance_count(BalanceArgs a) {
     }
     cluster.sync();
     // lanes 2q and 2q + 1 have block q's rows and slots: sums over even and over odd lanes
-    int all = (threadIdx.x & 31) < 2 * kCountCluster ? cluster.map_shared_rank(tot, (threadIdx.x & 31) >> 1)[threadIdx.x & 1] : 0;
+    int all = (threadIdx.x & 31) < 2 * CS ? cluster.map_shared_rank(tot, (threadIdx.x & 31) >> 1)[threadIdx.x & 1] : 0;
 #pragma unroll
     for (int o = 16; o > 1; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
     const int counted = __shfl_sync(kFull, all, 0), kept = __shfl_sync(kFull, all, 1);
     const float inv = 1.f / (float)max(1, kept);
-    const int step = (a.E + kCountCluster - 1) / kCountCluster;
+    const int step = (a.E + CS - 1) / CS;
     const int e0 = rank * step, e1 = min(a.E, e0 + step);
     for (int e = e0 + threadIdx.x; e < e1; e += blockDim.x) {
         int c = 0;
 #pragma unroll
-        for (int q = 0; q < kCountCluster; ++q) c += *cluster.map_shared_rank(&hist[e], q);
+        for (int q = 0; q < CS; ++q) c += *cluster.map_shared_rank(&hist[e], q);
         a.counts[(int64_t)s * a.E + e] = c;
         a.share[(int64_t)s * a.share_ld + e] = (float)c * inv;
     }
@@ -677,7 +677,6 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
     int st = train_shape(d->n_tokens, d->n_expert, d->top_k);
     if (st) return st;
     if (d->n_sequences < 1 || (d->n_sequences > 1 && !d->cu_seqlens)) return LATENT_ERR_SHAPE;
-    if ((int64_t)d->n_sequences * kCountCluster > 0x7fffffff) return LATENT_ERR_SHAPE;
     if (!float_type(d->type)) return LATENT_ERR_DTYPE;
     if (d->flags || !d->losses || !d->counts || !d->workspace || (d->n_tokens > 0 && (!d->logits || !d->ids)))
         return LATENT_ERR_INVALID;
@@ -696,7 +695,17 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
                         reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<float *>(ws + L.share), L.share_ld,
                         reinterpret_cast<double *>(ws + L.partial), reinterpret_cast<uint32_t *>(ws + L.ticket)};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    k_balance_count<<<(unsigned)d->n_sequences * kCountCluster, kCountThreads, 0, s>>>(a);
+    // as many blocks for a sequence as run at once (16384 rows of 256 experts, both kernels: 8 sequences 13.6 us with 8
+    // blocks each, 17.1 with one; 1024 sequences 74.0 and 22.8), of 1024 threads where each has many ids (65536 rows of
+    // 128 experts in one sequence 32.3 us, 39.2 with 512; 9001 rows in 37 sequences 12.2 and 10.6)
+    const unsigned S = (unsigned)d->n_sequences;
+    const int share = sms / d->n_sequences;
+    const int cluster = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
+    const int threads = (int64_t)d->n_tokens * d->top_k / S / cluster >= 8 * kCountThreads ? kCountThreads : kCountThreads / 2;
+    if (cluster == 8) k_balance_count<8><<<8 * S, threads, 0, s>>>(a);
+    else if (cluster == 4) k_balance_count<4><<<4 * S, threads, 0, s>>>(a);
+    else if (cluster == 2) k_balance_count<2><<<2 * S, threads, 0, s>>>(a);
+    else k_balance_count<1><<<S, threads, 0, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return LATENT_ERR_CUDA;
     switch (d->type) {
         case LATENT_TYPE_F32: return launch_balance<float>(a, sms, s);

@@ -137,6 +137,18 @@ def test_balance_loss_sequences_and_masks(cuda, cu, masked, dtype):
     assert not bool(r.grad[out].any())
 
 
+@pytest.mark.parametrize("T,S", [(20000, 1), (40000, 2), (3000, 20), (3000, 60), (2000, 200)])
+def test_balance_loss_many_rows_and_many_sequences(cuda, T, S):
+    """Every split of a sequence's counting over blocks and threads."""
+    l, ids = inputs(T, 48, 6, F32, seed=S)
+    g = torch.Generator("cuda").manual_seed(S)
+    cu = torch.sort(torch.randint(0, T + 1, (S + 1,), generator=g, device="cuda")).values.to(torch.int32)
+    if S <= 2:
+        cu[0], cu[-1] = 0, T
+    valid = torch.rand(T, generator=g, device="cuda") < 0.9
+    check_balance(l, ids, valid=valid, cu=cu)
+
+
 def test_balance_loss_masked_experts(cuda):
     """Masked experts (-inf, the type's lowest value), rows with every expert masked, and rows of NaN."""
     T, E, k = 60, 40, 4
