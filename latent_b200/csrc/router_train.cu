@@ -32,8 +32,6 @@
 // and 6.1.
 #include <cooperative_groups.h>
 
-#include <type_traits>
-
 #include "internal.h"
 
 namespace latent {
@@ -478,50 +476,53 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_router_grad_kept(const T *__
     if (kept && lane == __ffs(same) - 1) out[t * E + id] = from_f32<T>(old + g);
 }
 
-// Raw weights of logits: dl_i = p_i (dw_i - c) over the whole row.  One warp
-// per row, lane = slot; the row is written as -c p_i, then the kept columns.
-// Measured: 9001 rows of 160 bf16 experts 5.4 us, 6.2 MB, 1.15 TB/s: bound by the
-// latency of one row's loads and shuffles at this size.
-template <typename T, int PL, int VEC, bool ACCUM>
+// Raw weights of logits: dl_i = p_i (dw_i - c) over the whole row.  LPR lanes
+// per row, as in k_balance_main, and no fewer than top_k: lane = slot; the row
+// is written as -c p_i, then the kept columns.
+// Measured: 9001 rows of 160 bf16 experts 3.7 us, 5.4 with a warp per row; 65536
+// rows of 64 fp32 experts 8.7 (34 MB, 3.9 TB/s) and 23.4; of 256 24.8, 5.4 TB/s.
+template <typename T, int PL, int VEC, int LPR, bool ACCUM>
 __global__ void __launch_bounds__(kRowWarps * 32) k_router_grad_raw(const T *__restrict__ scores,
                                                                     const int32_t *__restrict__ ids,
                                                                     const float *__restrict__ dw, int T_, int E, int k,
                                                                     T *__restrict__ out) {
-    using RW = Row<T, PL, VEC>;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x * kRowWarps + warp;
-    if (t >= T_) return;
-    const T *row = scores + (int64_t)t * E;
-    T *o = out + (int64_t)t * E;
-    const int id = lane < k ? __ldg(ids + (int64_t)t * k + lane) : -1;
+    using RW = Row<T, PL, VEC, LPR>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LPR, sub = lane % LPR;
+    const int64_t t0 = ((int64_t)blockIdx.x * kRowWarps + warp) * (32 / LPR), t = t0 + group;
+    if (t0 >= T_) return;
+    const int cols = t < T_ ? E : 0;
+    const T *row = scores + t * E;
+    T *o = out + t * E;
+    const int id = sub < k && t < T_ ? __ldg(ids + t * k + sub) : -1;
     const bool kept = id >= 0 && id < E;
-    const float d = kept ? __ldg(dw + (int64_t)t * k + lane) : 0.f;
-    const bool any = __any_sync(kFull, kept);
+    const float d = kept ? __ldg(dw + t * k + sub) : 0.f;
+    const unsigned of_row = LPR == 32 ? kFull : ((1u << (LPR & 31)) - 1u) << (group * LPR);
+    const bool any = __ballot_sync(kFull, kept) & of_row;
     const float v = kept ? to_f32(__ldg(row + id)) : 0.f, old = ACCUM && kept ? to_f32(o[id]) : 0.f;
     float x[PL];
-    RW::load(row, E, lane, -INFINITY, x);
+    RW::load(row, cols, sub, -INFINITY, x);
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PL; ++j) m = fmaxf(m, x[j]);
-    m = warp_max(m);
+    m = warp_max<LPR>(m);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
         x[j] = expf(x[j] - m);
         sum += x[j];
     }
-    sum = warp_sum(sum);
+    sum = warp_sum<LPR>(sum);
     const float p = kept ? expf(v - m) / sum : 0.f;
-    const float c = warp_sum(d * p);
+    const float c = warp_sum<LPR>(d * p);
     const float cn = -c / sum;
     float y[PL];
-    if (ACCUM) RW::load_rw(o, E, lane, y);
+    if (ACCUM) RW::load_rw(o, cols, sub, y);
 #pragma unroll
     for (int j = 0; j < PL; ++j) x[j] = (any ? x[j] * cn : 0.f) + (ACCUM ? y[j] : 0.f);
     unsigned same;
-    const float g = same_id_sum(kept ? id : -1 - lane, p * d, same);
+    const float g = same_id_sum(kept ? group * kMaxTrainExperts + id : -1 - lane, p * d, same);
     __syncwarp();
-    RW::store(o, E, lane, x);
+    RW::store(o, cols, sub, x);
     __syncwarp();
     if (kept && lane == __ffs(same) - 1) o[id] = from_f32<T>(old + (g - c * p));  // p (sum of its slots' dw - c)
 }
@@ -553,27 +554,6 @@ BalanceLayout balance_layout(int S, int E) {
     L.ticket = L.partial + (size_t)kMaxBalanceBlocks * 16;
     L.total = L.ticket + 256;
     return L;
-}
-
-// Elements per lane, and whether rows can be moved in vectors of them.
-template <typename T, typename F>
-int with_row(int E, bool vec_ok, F f) {
-    constexpr int MAXV = 16 / (int)sizeof(T);
-    auto pick = [&](auto pl) {
-        constexpr int PL = decltype(pl)::value;
-        constexpr int V = PL < MAXV ? PL : MAXV;
-        if (V > 1 && E % V == 0 && vec_ok)
-            f(std::integral_constant<int, PL>{}, std::integral_constant<int, V>{});
-        else
-            f(std::integral_constant<int, PL>{}, std::integral_constant<int, 1>{});
-    };
-    if (E <= 32) pick(std::integral_constant<int, 1>{});
-    else if (E <= 64) pick(std::integral_constant<int, 2>{});
-    else if (E <= 128) pick(std::integral_constant<int, 4>{});
-    else if (E <= 256) pick(std::integral_constant<int, 8>{});
-    else if (E <= 512) pick(std::integral_constant<int, 16>{});
-    else pick(std::integral_constant<int, 32>{});
-    return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
 
 template <typename T, int PL, int LPR>
@@ -629,6 +609,22 @@ int launch_kept(const T *scores, const int32_t *ids, const float *dw, int n, int
     return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
 }
 
+template <typename T, int PL, int LPR>
+int launch_raw(const latent_router_grad_desc &d, bool vec, cudaStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T), rows = kRowWarps * (32 / LPR);
+    const T *sc = static_cast<const T *>(d.scores);
+    T *o = static_cast<T *>(d.d_scores);
+    const int n = d.n_tokens, E = d.n_expert, k = d.top_k;
+    const unsigned g = (unsigned)((n + rows - 1) / rows);
+    const bool accum = d.flags & LATENT_ROUTER_ACCUMULATE;
+    vec = vec && E % V == 0;
+    if (vec && accum) k_router_grad_raw<T, PL, V, LPR, true><<<g, kRowWarps * 32, 0, s>>>(sc, d.ids, d.d_weights, n, E, k, o);
+    else if (vec) k_router_grad_raw<T, PL, V, LPR, false><<<g, kRowWarps * 32, 0, s>>>(sc, d.ids, d.d_weights, n, E, k, o);
+    else if (accum) k_router_grad_raw<T, PL, 1, LPR, true><<<g, kRowWarps * 32, 0, s>>>(sc, d.ids, d.d_weights, n, E, k, o);
+    else k_router_grad_raw<T, PL, 1, LPR, false><<<g, kRowWarps * 32, 0, s>>>(sc, d.ids, d.d_weights, n, E, k, o);
+    return cudaGetLastError() == cudaSuccess ? LATENT_OK : LATENT_ERR_CUDA;
+}
+
 template <typename T>
 int launch_router_grad(const latent_router_grad_desc &d, cudaStream_t s) {
     const T *sc = static_cast<const T *>(d.scores);
@@ -642,12 +638,16 @@ int launch_router_grad(const latent_router_grad_desc &d, cudaStream_t s) {
     if (softmax && renorm) return launch_kept<T, true, true>(sc, ids, dw, n, E, k, accum, o, s);
     if (renorm) return launch_kept<T, false, true>(sc, ids, dw, n, E, k, accum, o, s);
     if (!softmax) return launch_kept<T, false, false>(sc, ids, dw, n, E, k, accum, o, s);
-    const unsigned g = (unsigned)((n + kRowWarps - 1) / kRowWarps);
-    return with_row<T>(E, is_aligned(sc, 16) && is_aligned(o, 16), [&](auto pl, auto v) {
-        constexpr int PL = decltype(pl)::value, V = decltype(v)::value;
-        if (accum) k_router_grad_raw<T, PL, V, true><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
-        else k_router_grad_raw<T, PL, V, false><<<g, kRowWarps * 32, 0, s>>>(sc, ids, dw, n, E, k, o);
-    });
+    const bool vec = is_aligned(sc, 16) && is_aligned(o, 16);
+    if (k <= 8) {
+        if (E <= 32 && k <= 4) return launch_raw<T, 8, 4>(d, vec, s);
+        if (E <= 64) return launch_raw<T, 8, 8>(d, vec, s);
+        if (E <= 128) return launch_raw<T, 16, 8>(d, vec, s);
+        if (E <= 256) return launch_raw<T, 32, 8>(d, vec, s);
+    }
+    if (E <= 256) return launch_raw<T, 8, 32>(d, vec, s);
+    if (E <= 512 && k <= 16) return launch_raw<T, 32, 16>(d, vec, s);
+    return launch_raw<T, 32, 32>(d, vec, s);
 }
 
 bool float_type(int t) { return t == LATENT_TYPE_F32 || t == LATENT_TYPE_F16 || t == LATENT_TYPE_BF16; }
