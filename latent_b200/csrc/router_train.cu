@@ -262,12 +262,16 @@ k_balance_count(BalanceArgs a) {
 }
 
 constexpr int kBalanceWarps = 4;
+// One turn of resident blocks that loop over the rows: none starts behind the
+// counts' wait and the launch of the others (65536 rows of 64 experts 15.9 us,
+// 20.6 with 16 blocks per SM, 20.0 with 4).
+constexpr int kBalanceBlocksPerSm = 7;
 
 // LPR lanes per row: the sums over a row, its logarithm, its divisions and its
 // place among the sequences cost instructions per group of lanes, so few lanes
 // with up to 32 values each take fewer of them per row than a whole warp.
 template <typename T, int PL, int VEC, int LPR>
-__global__ void __launch_bounds__(kBalanceWarps * 32, 7) k_balance_main(BalanceArgs a) {
+__global__ void __launch_bounds__(kBalanceWarps * 32, kBalanceBlocksPerSm) k_balance_main(BalanceArgs a) {
     using RW = Row<T, PL, VEC, LPR>;
     constexpr int kRows = 32 / LPR;  // rows of a warp
     __shared__ double part[kBalanceWarps][2];
@@ -538,7 +542,6 @@ int sm_count(int *sms) {
     return LATENT_OK;
 }
 
-constexpr int kBalanceBlocksPerSm = 16;
 constexpr int kMaxBalanceBlocks = 4096;  // partial sums in the workspace
 
 struct BalanceLayout {
