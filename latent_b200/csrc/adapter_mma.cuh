@@ -8,8 +8,9 @@
 // where t^s holds t of the rows that use a_s and zero in the others: the same
 // accumulator, no second pass over y.  t (fp32) enters as 2 or 3 parts of the
 // 16-bit operand type that add up to it (each part rounds what the ones
-// before left: 2 parts of bf16 leave 2^-16 of t, of fp16 2^-22, 3 of bf16
-// 2^-24), multiplied by the same B rows.
+// before left: 2 parts of bf16 leave 2^-16 of t, 3 of bf16 2^-24, 2 of fp16
+// 2^-22 or half a step of its subnormals, 2^-25, whichever is more: see
+// beyond_f16), multiplied by the same B rows.
 #pragma once
 
 #include "internal.h"
@@ -287,16 +288,25 @@ __device__ __forceinline__ uint32_t t_offset(int p, int kk, uint32_t tile_bytes)
     return (uint32_t)(p >> 1) * tile_bytes + (uint32_t)(p & 1) * 64u + (uint32_t)kk * 32u;
 }
 
-// fp16 parts reach 65504.  A row whose t goes further (or is not a number)
-// enters the tile as zeros and is finished in fp32 by the epilogue.
+// fp16 parts reach 65504 at one end; at the other they leave up to 2^-25 of
+// each t, however small it is.  A row whose largest t goes further, is not a
+// number, or is so small that 2^-25 is more of it than the results may lose
+// (fp32: 2^-21, what the accumulators' own cuts leave; 16 bits: 2^-16, as two
+// bf16 parts do) enters the tile as zeros and is finished in fp32 by the
+// epilogue.  Without the lower end t of 2^-17 were off by 2^-8 and t below 2^-25
+// were lost.
+template <bool F32>
 __device__ __forceinline__ bool beyond_f16(const float *t, float scale, int rank) {
+    constexpr float kLeast = F32 ? 0x1p-4f : 0x1p-9f;
     bool in = true;
+    float most = 0.f;
     for (int r = 0; r < rank; r += 4) {
         const float4 u = __ldcg(reinterpret_cast<const float4 *>(t + r));
-        in = in && fabsf(u.x * scale) <= 65504.f && fabsf(u.y * scale) <= 65504.f && fabsf(u.z * scale) <= 65504.f &&
-             fabsf(u.w * scale) <= 65504.f;
+        const float x = fabsf(u.x * scale), y = fabsf(u.y * scale), z = fabsf(u.z * scale), w = fabsf(u.w * scale);
+        in = in && x <= 65504.f && y <= 65504.f && z <= 65504.f && w <= 65504.f;
+        most = fmaxf(fmaxf(most, fmaxf(x, y)), fmaxf(z, w));
     }
-    return !in;
+    return !in || (most > 0.f && most < kLeast);
 }
 
 // The adapter's part of y in column n, in fp32.

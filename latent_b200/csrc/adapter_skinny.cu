@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             const float *t = g.t + ((int64_t)(t0 + r) << log2r);
             const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
             dependency_wait();
-            const bool wide = !BF && seg >= 0 && beyond_f16(t, scale, rank);
+            const bool wide = !BF && seg >= 0 && beyond_f16<sizeof(Y) == 4>(t, scale, rank);
             sh.wide[r] = wide;
             const int live = wide ? -1 : seg;
             float4 v[8];

@@ -364,7 +364,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                     }
                 }
                 float *x = v + (F32 ? c : 0);
-                if constexpr (!BF) {  // rows whose x.A fp16 cannot hold: the warp makes a row's part, its lane takes it
+                if constexpr (!BF) {  // rows whose x.A fp16 parts cannot hold: the warp makes a row's part, its lane takes it
                     for (uint32_t rest = wide_rows; rest; rest &= rest - 1) {
                         const int b = __ffs(rest) - 1, ad = __shfl_sync(kAll, a, b);
                         const float *tb = g.t + (int64_t)(row0 + b) * rank;
@@ -474,7 +474,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const int t = tile.t0 + mine * 128 + tid;
             const float *tp = g.t + (int64_t)t * rank;
             const float scale = my >= 0 ? __ldg(d.scale + a[mine]) : 0.f;
-            const bool wide = !BF && my >= 0 && beyond_f16(tp, scale, rank);
+            const bool wide = !BF && my >= 0 && beyond_f16<F32>(tp, scale, rank);
             seg.row[tid] = (int16_t)my;
             seg.wide[tid] = wide;
             const int ext = seg.n * rank;

@@ -1,0 +1,58 @@
+"""How many bits adapter_project keeps, one mechanism at a time: inputs whose products and x.A are exact in fp32, so
+that what a kernel rounds on the way is all that is left.
+
+Sizes and the kernels that serve them (latent_adapter_project's rule): up to 64 rows with at most 128 stacked rank
+columns one launch with x.A inside; up to 96 rows, or narrow results, x.A and then the product with the columns on the
+M side; 2048 rows of 2048 columns x.A and then the product on SM pairs.
+"""
+
+import pytest
+import torch
+
+from latent_b200 import AdapterSet, adapter_project
+
+pytestmark = pytest.mark.gpu
+HF, F32 = torch.float16, torch.float32
+
+
+def signed(g, lo, hi, *shape):
+    """Random signs, magnitudes in [lo, hi)."""
+    u = torch.rand(shape, generator=g, device="cuda") * (hi - lo) + lo
+    return torch.where(torch.rand(shape, generator=g, device="cuda") < 0.5, -u, u)
+
+
+def within(got, y, tol):
+    bad = ~((got.double() - y).abs() <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - y).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("T,K,N,n", [(9, 512, 256, 2), (40, 512, 256, 12), (128, 512, 384, 12), (2048, 512, 2048, 3)])
+@pytest.mark.parametrize("out", [HF, F32])
+@pytest.mark.parametrize("e", [-20, -12, -6, -3, 0, 17])
+def test_fp16_intermediate_of_any_magnitude(cuda, T, K, N, n, out, e):
+    """scale x.A between 2^-28 and 2^19, rows of two magnitudes in every tile, rows that are zero.
+
+    A row of x has one value, so x.A is one product of 11-bit numbers: exact in fp32, and a power of two scales it.  In
+    the tensor cores it is two fp16 parts: off by 2^-22 of itself, or by half a step of the subnormals, 2^-25, which in
+    the rows that go there is at most 2^-21 (fp32 results; fp16: 2^-16) of the row's largest.  Sums of 2 rank terms: 2
+    rank + 8 steps of 2^-24 of the sum of their magnitudes."""
+    g = torch.Generator("cuda").manual_seed(T + e)
+    rank, rows = 16, torch.arange(T, device="cuda")
+    at = torch.randint(0, K, (T,), generator=g, device="cuda")
+    x = torch.zeros((T, K), dtype=HF, device="cuda")
+    x[rows, at] = signed(g, 1, 2, T).to(HF) * torch.where(rows % 2 == 1, 2.0 ** -8, 1.0).to(HF)
+    x[3::7] = 0
+    ads = [(signed(g, 1, 2, K, rank).to(HF), (signed(g, 0.25, 2, rank, N) * 2.0 ** max(-10, min(13, -e))).to(HF), 2.0 ** e)
+           for _ in range(n)]
+    ids = torch.randint(-1, n, (T,), generator=g, device="cuda").to(torch.int32)
+    y = torch.zeros((T, N), dtype=torch.float64, device="cuda")
+    S, most = y.clone(), y.clone()
+    for i, (a, b, s) in enumerate(ads):
+        r = ids == i
+        t = s * (x[r].double() @ a.double())
+        y[r], S[r] = t @ b.double(), t.abs() @ b.double().abs()
+        most[r] = t.abs().max(1, keepdim=True).values * b.double().abs().sum(0)
+    got = adapter_project(x, torch.zeros((K, N), dtype=HF, device="cuda"), AdapterSet(ads), ids, out_dtype=out)
+    tol = (2 * rank + 8) * 2.0 ** -24 * S + (2.0 ** -22 + (2.0 ** -21 if out == F32 else 2.0 ** -16)) * most
+    within(got, y, tol + torch.finfo(out).eps / 2 * y.abs() + (2.0 ** -25 if out == HF else 0.0))
+
