@@ -84,8 +84,8 @@ class AdapterSet:
         self.scale = torch.tensor(scales, dtype=torch.float32, device=dev)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         # (reads the result: a set can be used on any stream from here on)
-        if not np.isfinite(scales).all() or not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
-            raise ValueError(f"adapter factors and scales must be finite in {dtype}")
+        if not bool(torch.isfinite(self.scale).all() & torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
+            raise ValueError(f"adapter factors must be finite in {dtype}, scales in float32")
         # a, lda, b, ldb, scale as a call's descriptor takes them
         self._factors = (self.a.data_ptr(), self.a.shape[2], self.b.data_ptr(), self.b.shape[2], self.scale.data_ptr())
         self._err_ptr = self.err.data_ptr()

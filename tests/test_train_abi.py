@@ -110,3 +110,12 @@ def test_adapter_set_layout():
     live = s.a[0, :17, :10].double().abs().sum() + s.a[1, :3, :10].double().abs().sum()
     assert float((s.a.double().abs().sum() - live).abs()) <= 1e-9 * float(live)
     assert s.scale.tolist() == [0.5, 1.0]
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("inf"), float("nan")])
+def test_scales_are_finite_as_they_are_kept(scale):
+    """A scale that is finite in 64 bits and infinite in the 32 that the device keeps."""
+    good = (torch.ones(8, 2), torch.ones(2, 8), 3e38)
+    assert AdapterSet([good], device="cpu").scale.isfinite().all()
+    with pytest.raises(ValueError, match="finite"):
+        AdapterSet([good, (torch.ones(8, 2), torch.ones(2, 8), scale)], device="cpu")
