@@ -563,8 +563,10 @@ typedef struct latent_adapter_desc {
 
 LATENT_API int latent_adapter_workspace_size(const latent_adapter_desc *desc, size_t *bytes);
 LATENT_API int latent_adapter_project(const latent_adapter_desc *desc, struct CUstream_st *stream);
-/* Synchronises `stream`, reports the error bits in *err (LATENT_ERR_EXPERT_ID:
- * an id >= n_adapter; LATENT_ERR_TIMEOUT) and clears them. */
+/* Synchronises `stream`, reports an error in *err (LATENT_ERR_EXPERT_ID: an id
+ * >= n_adapter; LATENT_ERR_TIMEOUT, which comes first) and clears that one.
+ * Covers the work ordered before it on `stream`; what other streams' work
+ * records meanwhile is reported by this check or kept for the next. */
 LATENT_API int latent_adapter_check(uint32_t *err, struct CUstream_st *stream);
 
 #ifdef __cplusplus

@@ -108,8 +108,9 @@ class AdapterSet:
         return n
 
     def check(self) -> None:
-        """Synchronises and raises if a call since the last check recorded a device-side error
-        (an id >= n_adapter, which counts as no adapter, or a bounded wait that ran out)."""
+        """Synchronises the current stream and raises if a call ordered before on it recorded a device-side error
+        since the last check (an id >= n_adapter, which counts as no adapter, or a bounded wait that ran out).
+        Errors of calls still on their way on other streams are raised now or by the next check, never lost."""
         _lib.check(_on(self.device, _lib.lib().latent_adapter_check, self.err.data_ptr()), "device check")
 
 

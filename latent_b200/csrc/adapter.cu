@@ -109,6 +109,10 @@ __global__ void __launch_bounds__(256) k_ad_any(latent_adapter_desc d, const flo
     }
 }
 
+// Clears the error that is being reported and no other: calls on other streams
+// may record theirs between the read and this.
+__global__ void k_ad_clear(uint32_t *err, uint32_t bit) { atomicAnd(err, ~bit); }
+
 bool ad_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 int ad_validate(const latent_adapter_desc *d) {
@@ -248,10 +252,11 @@ extern "C" LATENT_API int latent_adapter_check(uint32_t *err, CUstream_st *strea
     if (!err) return LATENT_ERR_INVALID;
     uint32_t bits = 0;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (cudaMemcpyAsync(&bits, err, 4, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaMemsetAsync(err, 0, 4, s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
+    if (cudaMemcpyAsync(&bits, err, 4, cudaMemcpyDeviceToHost, s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
         return LATENT_ERR_CUDA;
-    if (bits & kErrTimeout) return LATENT_ERR_TIMEOUT;
-    if (bits & kErrExpertId) return LATENT_ERR_EXPERT_ID;
-    return LATENT_OK;
+    const uint32_t bit = bits & kErrTimeout ? kErrTimeout : bits & kErrExpertId;
+    if (!bit) return LATENT_OK;
+    k_ad_clear<<<1, 1, 0, s>>>(err, bit);
+    if (cudaGetLastError() != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess) return LATENT_ERR_CUDA;
+    return bit == kErrTimeout ? LATENT_ERR_TIMEOUT : LATENT_ERR_EXPERT_ID;
 }
