@@ -83,12 +83,16 @@ __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
     return r;
 }
-// What the arrival stands for is ordered before it already: shared memory that
-// the tensor core reads by the proxy fence, TMEM reads by their wait.  With a
-// release at cluster scope on top an extension block took its builders 1.3 us
-// instead of 0.5.
+// Releases what this thread did and has observed in shared memory to the pair:
+// all that the other block's threads take over from an arrival (the x.A parts;
+// TMEM reads are over before it).  A release of global memory too has an
+// extension block wait for its loads: 1.3 us instead of 0.5 (made by a warp
+// of its own: 0.9).
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void load_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(
