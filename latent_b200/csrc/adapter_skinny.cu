@@ -113,9 +113,10 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-__device__ __forceinline__ void load32(const void *p, uint32_t (&v)[32]) {
+template <int N>
+__device__ __forceinline__ void load_words(const void *p, uint32_t (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
+    for (int i = 0; i < N; i += 4) {
         const uint4 u = reinterpret_cast<const uint4 *>(p)[i / 4];
         v[i] = u.x;
         v[i + 1] = u.y;
@@ -180,12 +181,41 @@ __device__ __forceinline__ void send_stacked(const Shared &sh, const Plan &p, ui
         uint32_t v[32], to[32], of[32];
         __syncwarp();
         tmem_ld32(acc + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
-        load32(sh.dest + c, to);
-        load32(sh.segs.row + c, of);
+        load_words(sh.dest + c, to);
+        load_words(sh.segs.row + c, of);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if ((int)of[i] == seg) st_cluster(to[i] + off, __uint_as_float(v[i]));
+    }
+}
+
+// The same of several accumulators: each into the sums, then these to the owners.
+__device__ __forceinline__ void add_stacked(const Plan &p, uint32_t acc, int tid, float (&sums)[kRows]) {
+#pragma unroll
+    for (int c = 0; c < kRows; c += 16) {
+        if (c >= p.rows) break;
+        uint32_t v[16];
+        __syncwarp();
+        tmem_ld16(acc + ((uint32_t)(tid & ~31) << 16) + (uint32_t)c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[c + i] += __uint_as_float(v[i]);
+    }
+}
+__device__ __forceinline__ void send_sums(const Shared &sh, const Plan &p, const float (&sums)[kRows], int m, int rank,
+                                          int log2r, int tid) {
+    const int seg = (m + tid) >> log2r;
+    const uint32_t off = ((uint32_t)(m + tid) & (uint32_t)(rank - 1)) * 4u;
+#pragma unroll
+    for (int c = 0; c < kRows; c += 16) {
+        if (c >= p.rows) break;
+        uint32_t to[16], of[16];
+        load_words(sh.dest + c, to);
+        load_words(sh.segs.row + c, of);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((int)of[i] == seg) st_cluster(to[i] + off, sums[c + i]);
     }
 }
 
@@ -198,7 +228,13 @@ __device__ __forceinline__ void send_stacked(const Shared &sh, const Plan &p, ui
 // 2.2 TB/s); 2047 rows of K = 4096 with one adapter of rank 64 11.5 us, without
 // any 4.8 (start, adapter list, the cluster's barriers): in between the blocks
 // fetch 27 MB of x and A, 4 TB/s.
-template <bool BF>
+// For fp32 results a block with more than 512 of K has its two accumulators take
+// turns every 512, as the products do, and the epilogue keeps their sums in
+// registers: over K = 7168 x.A is then off by 4.8e-7 (fp16 6.5e-7) instead of
+// 7.9e-6, at 131.1 us instead of 130.5 for 18900 rows with N = 256, 45.6 for
+// 44.0 for 8192 rows of 4096 x 256, nothing for decode batches.  16-bit results
+// keep one chain: x.A enters them in two parts, to 2^-16.
+template <bool BF, bool F32>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant__ CUtensorMap mA,
                                                            const __grid_constant__ CUtensorMap mX, AdapterArgs g,
                                                            Plan p) {
@@ -226,6 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
     const int nk = (d.n_in + kBK - 1) / kBK;
     const int k0 = (int)((int64_t)nk * q / CS), k1 = (int)((int64_t)nk * (q + 1) / CS);
     const int per = (nt + CS - 1) / CS;  // rows of an owner
+    const int chunk = F32 ? 8 : max(1, k1 - k0);  // K blocks per accumulator
     bool ok = true;
     if (warp >= 4) {
         build_segments(sh.segs, a, nt, threadIdx.x - 128, 1);
@@ -243,13 +280,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         const uint32_t id = idesc(BF, p.rows, false, false);
         Ring at;
         uint32_t n = 0;
-        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128, ++n) {
-            const uint32_t b = n & 1u;
-            if (n >= 2 && !wait_warp(sh.acc_empty + b, ((n >> 1) - 1u) & 1u, &sh.abort)) { ok = false; break; }
-            tc_fence_after();
-            ok = multiply_stacked(sh, p, at, ring, stage, tmem + b * read, id, k0, k1);
-            if (ok && elect()) mma_commit(sh.acc_full + b);
-        }
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128)
+            for (int k = k0; k < k1 && ok; k += chunk, ++n) {
+                const uint32_t b = n & 1u;
+                if (n >= 2 && !wait_warp(sh.acc_empty + b, ((n >> 1) - 1u) & 1u, &sh.abort)) { ok = false; break; }
+                tc_fence_after();
+                ok = multiply_stacked(sh, p, at, ring, stage, tmem + b * read, id, k, min(k1, k + chunk));
+                if (ok && elect()) mma_commit(sh.acc_full + b);
+            }
         if (!ok && elect()) {
             mma_commit(sh.acc_full);
             mma_commit(sh.acc_full + 1);
@@ -258,14 +296,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_shrink(const __grid_constant
         const int tid = threadIdx.x - 128;
         cluster_wait();
         uint32_t n = 0;
-        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128, ++n) {
-            const uint32_t b = n & 1u;
-            if (!wait(sh.acc_full + b, (n >> 1) & 1u) || sh.abort) ok = false;
-            if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
-            tc_fence_after();
-            send_stacked(sh, p, tmem + b * read, m, rank, log2r, tid, 0u);
-            tc_fence_before();
-            mbar_arrive(sh.acc_empty + b);
+        for (int m = blockIdx.y * 128; m < total && ok; m += gridDim.y * 128) {
+            float sums[F32 ? kRows : 1] = {};
+            for (int k = k0; k < k1; k += chunk, ++n) {
+                const uint32_t b = n & 1u;
+                if (!wait(sh.acc_full + b, (n >> 1) & 1u) || sh.abort) ok = false;
+                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+                tc_fence_after();
+                const bool all = k1 - k0 <= chunk;
+                if (all) send_stacked(sh, p, tmem + b * read, m, rank, log2r, tid, 0u);
+                if constexpr (F32) {
+                    if (!all) add_stacked(p, tmem + b * read, tid, sums);
+                    if (!all && k + chunk >= k1) send_sums(sh, p, sums, m, rank, log2r, tid);
+                }
+                tc_fence_before();
+                mbar_arrive(sh.acc_empty + b);
+            }
         }
     }
     if (!ok) {
@@ -455,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
                 float s[32];
                 uint32_t to[32];
-                load32(sh.dest + c, to);
+                load_words(sh.dest + c, to);
                 for (int gr = 0; gr < groups; ++gr) {
                     uint32_t v[32];
                     __syncwarp();
@@ -655,7 +701,7 @@ const int *cluster_room() {
     std::lock_guard<std::mutex> lock(mu);
     Table &t = tables[dev];
     if (!t.set) {
-        const void *fn = (const void *)k_ad_shrink<true>;
+        const void *fn = (const void *)k_ad_shrink<true, false>;
         if (ensure_smem(fn, kSmem) != cudaSuccess || allow_clusters(fn) != cudaSuccess) return nullptr;
         for (int c = 1; c <= kMaxCluster; ++c) {
             cudaLaunchConfig_t cfg{};
@@ -772,8 +818,7 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
 }
 
 // Accumulators of `rows` columns in k_ad_skinny's TMEM.  The tensor cores cut a
-// sum off instead of rounding it: a chain over K = 7168 is off by 8e-6 of the
-// result, one over 512 by 5e-7 (measured).  fp32 results therefore use an
+// sum off instead of rounding it (figures at k_ad_wide): fp32 results use an
 // accumulator per 512 of K, added up in fp32, as far as the TMEM columns go,
 // and clusters long enough.
 int accumulators(int rows, bool self) {
@@ -812,8 +857,9 @@ cudaError_t launch_adapter_shrink(const AdapterArgs &g, const void *x_map, cudaS
     if (!adapter_map(&mA, bf, d.a, (uint64_t)d.n_adapter * d.rank, d.n_in, d.lda, d.rank)) return cudaErrorInvalidValue;
     AdapterArgs a = g;
     void *args[] = {&mA, const_cast<void *>(x_map), &a, &r.p};
-    return launch_cluster(bf ? (const void *)k_ad_shrink<true> : (const void *)k_ad_shrink<false>,
-                          dim3(r.cluster, r.slots, r.tiles), false, args, s);
+    const void *fn = d.y_type == LATENT_TYPE_F32 ? bf ? (const void *)k_ad_shrink<true, true> : (const void *)k_ad_shrink<false, true>
+                                                 : bf ? (const void *)k_ad_shrink<true, false> : (const void *)k_ad_shrink<false, false>;
+    return launch_cluster(fn, dim3(r.cluster, r.slots, r.tiles), false, args, s);
 }
 
 cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int sms, bool self, cudaStream_t s) {

@@ -19,10 +19,14 @@
 // us without adapters (128 tiles on 74 pairs: two turns, the second of 54), 56
 // with five packed prompts of rank 64, 65 with six adapters mixed over all rows.
 //
-// fp32 results: the tensor cores cut a sum off instead of rounding it (a chain
-// over K = 7168 is off by 8e-6 of the result, one over 512 by 5e-7), so the two
-// accumulators take turns every 512 of K and the epilogue adds them up in fp32
-// registers, 128 a thread, hence the narrower tile.
+// fp32 results: the tensor cores cut a sum off instead of rounding it, so the
+// two accumulators take turns every 512 of K and the epilogue adds them up in
+// fp32 registers, 128 a thread, hence the narrower tile.  Measured at K = 7168,
+// root mean squares: one chain 7.9e-6 of the result (fp16 8.4e-6; terms of one
+// sign 2.2e-5, fp16 4.4e-5), chains of 512 4.8e-7 (6.5e-7; 2.4e-7, 2.4e-6), a
+// plain fp32 product 8.8e-7 (1.5e-6; 1.2e-6, 1.2e-6).  16-bit results keep the
+// one chain: their rounding is 1.66e-3 (fp16 2.07e-4) with it as without, with
+// terms of one sign 1.29e-3 (fp16 1.67e-4 for 1.61e-4).
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -128,17 +132,6 @@ template <int N> __device__ __forceinline__ void store_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
-// 32 lanes x 16 columns of 32-bit TMEM words into 16 registers per thread.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
-        : "memory");
-}
 
 struct Tile {
     int t0, n0;

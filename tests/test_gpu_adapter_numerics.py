@@ -12,7 +12,7 @@ import torch
 from latent_b200 import AdapterSet, adapter_project
 
 pytestmark = pytest.mark.gpu
-HF, F32 = torch.float16, torch.float32
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 def signed(g, lo, hi, *shape):
@@ -56,3 +56,30 @@ def test_fp16_intermediate_of_any_magnitude(cuda, T, K, N, n, out, e):
     tol = (2 * rank + 8) * 2.0 ** -24 * S + (2.0 ** -22 + (2.0 ** -21 if out == F32 else 2.0 ** -16)) * most
     within(got, y, tol + torch.finfo(out).eps / 2 * y.abs() + (2.0 ** -25 if out == HF else 0.0))
 
+
+# The tensor cores cut the sum of a step (16 terms) off: up to 2^-23 of the partial sum.  Positive terms, chains of 512
+# (32 steps, partial sums that grow evenly): (1 + .. + 32) / 32 = 16.5 steps of 2^-23 at most; then up to 16 such sums
+# are added, half a step of 2^-23 of a growing sum each: 8 more of 2^-24.
+# The terms of a step are aligned to its largest first, two bits below the last of fp32.  A product of bf16 values of
+# [0.5, 1.5) is a multiple of 2^-16 and a partial sum of 512 of them stays below 2^10: its last bit but two is 2^-16 or
+# less and nothing more is cut.  Products of fp16 values reach down to 2^-22: each of the 17 terms loses up to 2^-25 of
+# the partial sum as well, 17 / 4 + 1 steps of 2^-23 in place of one.
+# One chain over 7168 has 14 times as many steps: four (bf16) and 14 / 5.25 times (fp16, as measured) over these bounds.
+CHAIN = {BF: 16.5 * 2.0 ** -23 + 8 * 2.0 ** -24, HF: 16.5 * 5.25 * 2.0 ** -23 + 8 * 2.0 ** -24}
+
+
+@pytest.mark.parametrize("T,N", [(40, 256), (500, 256), (18944, 64)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_fp32_results_of_a_long_intermediate(cuda, T, N, dtype):
+    """x.A over K = 7168, one or a few blocks to a row tile (18944 rows: 148 of them): its sums are cut like x.W's."""
+    K, n = 7168, 12
+    g = torch.Generator("cuda").manual_seed(T)
+    pos = lambda *s: (torch.rand(s, generator=g, device="cuda") + 0.5).to(dtype)  # noqa: E731
+    x = pos(T, K)
+    ads = [(pos(K, 1) * 2.0 ** -8, pos(1, N), 1.0) for _ in range(n)]
+    ids = (torch.arange(T, device="cuda") * n // T).to(torch.int32)
+    y = torch.empty((T, N), dtype=torch.float64, device="cuda")
+    for i, (a, b, _) in enumerate(ads):
+        y[ids == i] = (x[ids == i].double() @ a.double()) @ b.double()
+    got = adapter_project(x, torch.zeros((K, N), dtype=dtype, device="cuda"), AdapterSet(ads), ids, out_dtype=F32)
+    within(got, y, (CHAIN[dtype] + 2.0 ** -22 + 8 * 2.0 ** -24) * y)
