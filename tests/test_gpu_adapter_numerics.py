@@ -57,6 +57,32 @@ def test_fp16_intermediate_of_any_magnitude(cuda, T, K, N, n, out, e):
     within(got, y, tol + torch.finfo(out).eps / 2 * y.abs() + (2.0 ** -25 if out == HF else 0.0))
 
 
+@pytest.mark.parametrize("T,K,N,n", [(9, 512, 256, 2), (40, 512, 256, 12), (128, 512, 384, 12), (2048, 512, 2048, 3)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_fp32_results_keep_the_intermediates_bits(cuda, T, K, N, n, dtype):
+    """fp32 results take x.A in as many 16-bit parts as hold 24 bits (bf16: three) or 22 (fp16: two).
+
+    One rank column, W = 0: y is one product, x.A one (fp16: 22 bits) or two products 2^-8 apart (bf16: 16 bits each, 24
+    in all) that fp32 holds.  Three parts of it, their products and sums: 8 steps of 2^-24.  Two bf16 parts would leave
+    2^-17, one fp16 part 2^-12."""
+    g = torch.Generator("cuda").manual_seed(T)
+    rows = torch.arange(T, device="cuda")
+    at = torch.randint(0, K // 2, (T,), generator=g, device="cuda")
+    x = torch.zeros((T, K), dtype=dtype, device="cuda")
+    x[rows, at] = signed(g, 1, 1.4, T).to(dtype)
+    if dtype == BF:
+        x[rows, K // 2 + at] = signed(g, 1, 1.4, T).to(dtype) * 2.0 ** -8
+    ads = [(signed(g, 1, 1.4, K, 1).to(dtype), signed(g, 0.5, 2, 1, N).to(dtype), 2.0 ** (i % 3)) for i in range(n)]
+    ids = torch.randint(0, n, (T,), generator=g, device="cuda").to(torch.int32)
+    y = torch.zeros((T, N), dtype=torch.float64, device="cuda")
+    for i, (a, b, s) in enumerate(ads):
+        t = x[ids == i].double() @ a.double()
+        assert torch.equal(t, t.float().double())
+        y[ids == i] = s * t @ b.double()
+    got = adapter_project(x, torch.zeros((K, N), dtype=dtype, device="cuda"), AdapterSet(ads), ids, out_dtype=F32)
+    within(got, y, 8 * 2.0 ** -24 * y.abs())
+
+
 # The tensor cores cut the sum of a step (16 terms) off: up to 2^-23 of the partial sum.  Positive terms, chains of 512
 # (32 steps, partial sums that grow evenly): (1 + .. + 32) / 32 = 16.5 steps of 2^-23 at most; then up to 16 such sums
 # are added, half a step of 2^-23 of a growing sum each: 8 more of 2^-24.
@@ -66,6 +92,19 @@ def test_fp16_intermediate_of_any_magnitude(cuda, T, K, N, n, out, e):
 # the partial sum as well, 17 / 4 + 1 steps of 2^-23 in place of one.
 # One chain over 7168 has 14 times as many steps: four (bf16) and 14 / 5.25 times (fp16, as measured) over these bounds.
 CHAIN = {BF: 16.5 * 2.0 ** -23 + 8 * 2.0 ** -24, HF: 16.5 * 5.25 * 2.0 ** -23 + 8 * 2.0 ** -24}
+
+
+@pytest.mark.parametrize("T,N", [(96, 18944), (2048, 2048)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_fp32_results_of_long_sums(cuda, T, N, dtype):
+    K = 7168
+    g = torch.Generator("cuda").manual_seed(T)
+    pos = lambda *s: (torch.rand(s, generator=g, device="cuda") + 0.5).to(dtype)  # noqa: E731
+    x, w = pos(T, K), pos(K, N)
+    s = AdapterSet([(pos(K, 4), pos(4, N), 1.0)])
+    got = adapter_project(x, w, s, torch.full((T,), -1, dtype=torch.int32, device="cuda"), out_dtype=F32)
+    y = x.double() @ w.double()
+    within(got, y, CHAIN[dtype] * y)
 
 
 @pytest.mark.parametrize("T,N", [(40, 256), (500, 256), (18944, 64)])
