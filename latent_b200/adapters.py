@@ -9,7 +9,8 @@ that row's own adapter:
 The shared projection is a dense fp16/bf16 matrix (either memory order) or a
 packed ``FactorPair``.  The rows of a batch may be single tokens of many
 requests or packed prompts, in any order.  An inference operator: inputs that
-require a gradient are refused.  The reference has no adapters; its low-rank
+require a gradient or carry a tangent are refused; a set holds copies of its
+factors, detached.  The reference has no adapters; its low-rank
 projection is loader/latent_runtime.py:35-36.
 """
 
@@ -22,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .router_train import _on, _with_workspace
+from .router_train import _no_tangents, _on, _with_workspace
 from .runtime import FactorPair, project
 
 __all__ = ["AdapterSet", "adapter_project"]
@@ -150,6 +151,7 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     if (x.requires_grad or (not pair and weight.requires_grad) or (out is not None and out.requires_grad)) and \
             torch.is_grad_enabled():
         raise ValueError("adapter_project computes no gradients: call it under torch.no_grad() or on detached tensors")
+    _no_tangents("adapter_project", x, None if pair else weight, out)
     if out is not None:
         if out_dtype not in (None, out.dtype):
             raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")

@@ -9,6 +9,8 @@ Both kernels return explicit gradients, which add up in one buffer
 (``out=``) and can be captured into a CUDA graph.  Where autograd is on and
 the logits require a gradient, ``balance_loss`` and, when asked,
 ``router_topk`` are differentiable through it as well (outside graph capture).
+The explicit gradients are constants to autograd; forward-mode tangents are
+refused.
 """
 
 from __future__ import annotations
@@ -17,6 +19,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .runtime import _X_TYPES
@@ -96,6 +99,13 @@ def _router_inputs(logits: torch.Tensor, ids: torch.Tensor, name: str):
     return logits.contiguous(), ids.contiguous(), shape[0], shape[1], slots[1], kind
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """Raises where one of the tensors carries a forward-mode tangent, which ``what`` would drop."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative: its inputs must not carry tangents")
+
+
 def _no_capture(what: str) -> None:
     # Autograd ties a leaf's gradient to the stream that first used it: a
     # captured backward pass beside an eager one of the same leaves would end
@@ -166,6 +176,7 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 
     require a gradient make ``loss`` differentiable by autograd.
     """
     flat, ids, T = _router_inputs(logits, ids, "logits")[:3]
+    _no_tangents("balance_loss", logits)
     n_seq = 1
     if cu_seqlens is not None:
         n_seq = cu_seqlens.numel() - 1
@@ -195,11 +206,14 @@ def router_topk_grad(scores: torch.Tensor, ids: torch.Tensor, d_weights: torch.T
     ``router_topk``, ``ids`` int32 [T, k] as it returned them, ``d_weights``
     fp32 [T, k].  Returns [T, E] in the scores' dtype; the kept set is held
     fixed.  ``out``: a contiguous tensor of the scores' shape and dtype that
-    the gradient is added into (for instance ``balance_loss(...).grad``).
+    the gradient is added into (for instance ``balance_loss(...).grad``); it
+    shares no memory with the inputs.  The result is a constant to autograd,
+    whether or not ``scores`` or ``d_weights`` require a gradient.
     """
     flat, ids, T, E, k, kind = _router_inputs(scores, ids, "scores")
     if d_weights.shape != ids.shape or d_weights.dtype != torch.float32 or d_weights.get_device() != flat.get_device():
         raise ValueError(f"d_weights must be float32 {tuple(ids.shape)} on {flat.device}")
+    _no_tangents("router_topk_grad", scores, d_weights, out)
     flags = (_lib.ROUTER_RENORMALIZE if renormalize else 0) | (_lib.ROUTER_SOFTMAX if logits else 0)
     if out is None:
         g = torch.empty_like(flat)   # (never carries requires_grad)

@@ -387,8 +387,10 @@ def router_topk(scores: torch.Tensor, top_k: int, threshold: float = 0.95, renor
         raise ValueError(f"top_k must be positive, got {top_k}")
     if not 0.0 < threshold <= 1.0:
         raise ValueError(f"threshold must be in (0, 1], got {threshold}")
+    if differentiable:
+        from .router_train import RouterTopK, _no_tangents
+        _no_tangents("router_topk", scores)
     if differentiable and scores.requires_grad and torch.is_grad_enabled():
-        from .router_train import RouterTopK
         ids, w, n_kept, counts = RouterTopK.apply(scores, top_k, threshold, renormalize, logits, expert_counts)
         return (ids, w, n_kept, counts) if expert_counts else (ids, w, n_kept)
     s = scores.to(torch.float32).contiguous()

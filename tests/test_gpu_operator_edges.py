@@ -2,8 +2,10 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
-from latent_b200 import AdapterSet, _lib, adapter_project
+from latent_b200 import AdapterSet, _lib, adapter_project, balance_loss, router_topk, router_topk_grad
+from test_gpu_router_train import inputs
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -43,3 +45,25 @@ def test_an_error_is_reported_whatever_stream_it_comes_from(cuda):
         seen += raised()
         assert seen
         assert not raised()                               # reported once, then cleared
+
+
+def test_tangents_are_refused(cuda):
+    x, w, s, ids = small_set()
+    l, slots = inputs(10, 16, 3)
+    dw = torch.ones((10, 3), device="cuda")
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: adapter_project(dual(x), w, s, ids), lambda: adapter_project(x, dual(w), s, ids),
+                     lambda: adapter_project(x, dual(w.t().contiguous()).t(), s, ids),
+                     lambda: adapter_project(x, w, s, ids, out=dual(torch.empty((6, 32), dtype=BF, device="cuda"))),
+                     lambda: balance_loss(dual(l), slots), lambda: balance_loss(dual(l), slots, gradient=True),
+                     lambda: router_topk_grad(dual(l), slots, dw), lambda: router_topk_grad(l, slots, dual(dw)),
+                     lambda: router_topk_grad(l, slots, dw, out=dual(torch.zeros_like(l))),
+                     lambda: router_topk(dual(l), 3, differentiable=True)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        # without tangents the calls stand, inside a level as outside
+        router_topk_grad(l, slots, dw)
+        adapter_project(x, w, s, ids)
+        balance_loss(l, slots)
+    router_topk(l, 3, differentiable=True)
