@@ -488,25 +488,26 @@ LATENT_API int latent_router_grad(const latent_router_grad_desc *desc, struct CU
  *   losses[2] = mean over counted rows of logsumexp(logits)^2
  *   losses[0] = balance_coef losses[1] + z_coef losses[2]
  * and grad (optional) = *d_loss dlosses[0]/dlogits in the logits' type, with f
- * held fixed (d_loss: the device scalar that comes from behind, NULL: 1).  A
- * row whose logits are all -inf has no distribution: it counts as a row, adds
+ * held fixed (d_loss: the device scalar that comes from behind, NULL: 1; with
+ * LATENT_BALANCE_D_LOSSES three of them, for losses[0], [1] and [2]).  A row whose logits are all -inf has no distribution: it counts as a row, adds
  * nothing and has a zero gradient.  Workspace: 256-byte aligned,
  * latent_balance_workspace_size() bytes.  LATENT_ERR_UNSUPPORTED beyond 1024
  * experts.  Stream-ordered; repeated calls agree bit for bit. */
+enum { LATENT_BALANCE_D_LOSSES = 1u << 1 };
 typedef struct latent_balance_desc {
     int32_t n_tokens;          /* T */
     int32_t n_expert;          /* E */
     int32_t top_k;             /* k */
     int32_t n_sequences;       /* S */
     int32_t type;              /* latent_type of logits and grad */
-    uint32_t flags;            /* 0 */
+    uint32_t flags;            /* LATENT_BALANCE_* */
     float balance_coef;
     float z_coef;
     const void *logits;        /* [T][E] */
     const int32_t *ids;        /* [T][k] */
     const uint8_t *valid;      /* [T] or NULL */
     const int32_t *cu_seqlens; /* [S + 1], or NULL with S = 1 */
-    const float *d_loss;       /* one device float, or NULL */
+    const float *d_loss;       /* one device float (LATENT_BALANCE_D_LOSSES: three), or NULL */
     float *losses;             /* [3] */
     int32_t *counts;           /* [S][E] */
     void *grad;                /* [T][E] or NULL */

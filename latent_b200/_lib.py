@@ -28,6 +28,7 @@ FLAG_OUT_PER_SLOT = 1 << 1
 ROUTER_RENORMALIZE = 1 << 0
 ROUTER_SOFTMAX = 1 << 1
 ROUTER_ACCUMULATE = 1 << 2
+BALANCE_D_LOSSES = 1 << 1
 ADAPTER_W_TRANSPOSED = 1 << 0
 PATH_AUTO, PATH_DECODE, PATH_PREFILL = 0, 1, 2
 

@@ -186,6 +186,7 @@ struct BalanceArgs {
     int T, E, k, S;
     float b, z;
     const float *d_loss;  // gradient with respect to losses[0]; NULL: 1
+    bool d_losses;        // and behind it those with respect to losses[1] and [2]
     float *losses;
     int32_t *counts;    // [S][E]
     void *grad;
@@ -329,6 +330,10 @@ __global__ void __launch_bounds__(kBalanceWarps * 32, kBalanceBlocksPerSm) k_bal
             const float up = a.d_loss ? __ldg(a.d_loss) : 1.f;
             gb = up * a.b;
             gz = n > 0 ? up * (2.f * a.z / (float)n) : 0.f;
+            if (a.d_losses) {
+                gb += __ldg(a.d_loss + 1);
+                if (n > 0) gz += __ldg(a.d_loss + 2) * (2.f / (float)n);
+            }
         }
         const int rows = __ldcg(a.seq + max(seq, 0));
         const float scale = seq >= 0 ? (float)a.E / ((float)used * (float)rows) : 0.f;  // C = scale * share
@@ -681,7 +686,8 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
     if (st) return st;
     if (d->n_sequences < 1 || (d->n_sequences > 1 && !d->cu_seqlens)) return LATENT_ERR_SHAPE;
     if (!float_type(d->type)) return LATENT_ERR_DTYPE;
-    if (d->flags || !d->losses || !d->counts || !d->workspace || (d->n_tokens > 0 && (!d->logits || !d->ids)))
+    const bool d_losses = d->flags & LATENT_BALANCE_D_LOSSES;
+    if ((d->flags & ~(uint32_t)LATENT_BALANCE_D_LOSSES) || (d_losses && !d->d_loss) || !d->losses || !d->counts || !d->workspace || (d->n_tokens > 0 && (!d->logits || !d->ids)))
         return LATENT_ERR_INVALID;
     const size_t es = type_size(d->type);
     if (!is_aligned(d->logits, es) || !is_aligned(d->grad, es) || !is_aligned(d->ids, 4) ||
@@ -694,7 +700,7 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
     if ((st = sm_count(&sms))) return st;
     char *ws = static_cast<char *>(d->workspace);
     const BalanceArgs a{d->logits, d->ids, d->valid, d->cu_seqlens, d->n_tokens, d->n_expert, d->top_k, d->n_sequences,
-                        d->balance_coef, d->z_coef, d->d_loss, d->losses, d->counts, d->grad,
+                        d->balance_coef, d->z_coef, d->d_loss, d_losses, d->losses, d->counts, d->grad,
                         reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<float *>(ws + L.share), L.share_ld,
                         reinterpret_cast<double *>(ws + L.partial), reinterpret_cast<uint32_t *>(ws + L.ticket)};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -115,7 +115,7 @@ def _no_capture(what: str) -> None:
                            "use the explicit gradient")
 
 
-def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradient):
+def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, gradient, d_losses=None):
     T, E = logits.shape
     dev = logits.device
     n = _WS_BYTES.get((n_seq, E)) or _workspace_bytes(n_seq, E)
@@ -125,9 +125,10 @@ def _balance(logits, ids, balance_coef, z_coef, valid, cu, n_seq, d_loss, gradie
         torch.empty(n_seq, E, dtype=torch.int32, device=dev)
     grad = torch.empty_like(logits) if gradient else None
     _with_workspace(dev, n, _lib.lib().latent_balance_loss, "latent_balance_loss", _lib.BALANCE_DESC,
-                    (T, E, ids.shape[1], n_seq, _X_TYPES[logits.dtype], 0, balance_coef, z_coef, logits.data_ptr(),
+                    (T, E, ids.shape[1], n_seq, _X_TYPES[logits.dtype], 0 if d_losses is None else _lib.BALANCE_D_LOSSES,
+                     balance_coef, z_coef, logits.data_ptr(),
                      ids.data_ptr(), 0 if valid is None else valid.data_ptr(), 0 if cu is None else cu.data_ptr(),
-                     0 if d_loss is None else d_loss.data_ptr(), losses.data_ptr(), counts.data_ptr(),
+                     0 if d_losses is None else d_losses.data_ptr(), losses.data_ptr(), counts.data_ptr(),
                      0 if grad is None else grad.data_ptr()))
     return losses, counts, grad
 
@@ -137,22 +138,20 @@ class _BalanceLossFn(torch.autograd.Function):
     def forward(ctx, logits, ids, balance_coef, z_coef, valid, cu, n_seq):
         _no_capture("balance_loss")
         flat = logits.detach().contiguous()
-        losses, counts, _ = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, None, False)
+        losses, counts, _ = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, False)
         ctx.save_for_backward(flat, ids, valid, cu)
         ctx.args = (balance_coef, z_coef, n_seq)
-        loss, balance, z = losses.unbind()
-        loss = loss.clone()  # a tensor of its own: users add to it in place
-        ctx.mark_non_differentiable(balance, z, counts)
-        return loss, balance, z, counts
+        ctx.mark_non_differentiable(counts)
+        return losses, counts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, *_):
+    def backward(ctx, d_losses, _):
         _no_capture("balance_loss")
         flat, ids, valid, cu = ctx.saved_tensors
         balance_coef, z_coef, n_seq = ctx.args
-        d = d_loss.to(torch.float32).contiguous()
-        grad = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, d, True)[2]
+        d = d_losses.to(torch.float32).contiguous()
+        grad = _balance(flat, ids, balance_coef, z_coef, valid, cu, n_seq, True, d)[2]
         return grad, None, None, None, None, None, None
 
 
@@ -172,8 +171,9 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 
 
     With ``gradient`` the result carries d loss / d logits (the logits'
     dtype), made in the same pass.  An fp16 gradient of a mean over many rows
-    underflows: scale the two coefficients up.  Without it, logits that
-    require a gradient make ``loss`` differentiable by autograd.
+    underflows: scale the two coefficients up.  The losses beside it are constants
+    to autograd.  Without it, logits that require a gradient make ``loss``,
+    ``balance`` and ``z`` differentiable by autograd.
     """
     flat, ids, T = _router_inputs(logits, ids, "logits")[:3]
     _no_tangents("balance_loss", logits)
@@ -190,10 +190,11 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, balance_coef: float = 
         valid = valid.contiguous()
     balance_coef, z_coef = float(balance_coef), float(z_coef)
     if not gradient and logits.requires_grad and torch.is_grad_enabled():
-        loss, balance, z, counts = _BalanceLossFn.apply(logits, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq)
-        grad = None
+        losses, counts = _BalanceLossFn.apply(logits, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq)
+        # one by one: of views made in one call none may be changed in place
+        loss, balance, z, grad = losses[0], losses[1], losses[2], None
     else:
-        losses, counts, grad = _balance(flat, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq, None, gradient)
+        losses, counts, grad = _balance(flat, ids, balance_coef, z_coef, valid, cu_seqlens, n_seq, gradient)
         loss, balance, z = losses.unbind()
     return BalanceLoss(loss, balance, z, counts, grad)
 

@@ -5,10 +5,10 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 from latent_b200 import AdapterSet, _lib, adapter_project, balance_loss, router_topk, router_topk_grad
-from test_gpu_router_train import inputs
+from test_gpu_router_train import close, inputs, loss64, rounding, steps
 
 pytestmark = pytest.mark.gpu
-BF = torch.bfloat16
+F32, BF = torch.float32, torch.bfloat16
 
 
 def small_set(K=64, N=32, n=2):
@@ -67,3 +67,41 @@ def test_tangents_are_refused(cuda):
         adapter_project(x, w, s, ids)
         balance_loss(l, slots)
     router_topk(l, 3, differentiable=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("use", [(1.0, 0.0, 0.0), (0.0, 1.0, 0.0), (0.0, 0.0, 1.0), (0.3, 0.7, 0.2)])
+def test_every_loss_carries_its_gradient(cuda, dtype, use):
+    """loss, balance and z of balance_loss, weighted by the caller, through autograd against 64-bit autograd."""
+    T, E, k, b, z = 300, 72, 6, 2.0, 0.5
+    l, ids = inputs(T, E, k, dtype, seed=8)
+    cu = torch.tensor([0, 100, 101, 290], dtype=torch.int32, device="cuda")
+    leaf = l.clone().requires_grad_(True)
+    r = balance_loss(leaf, ids, b, z, cu_seqlens=cu)
+    parts = [u * v for u, v in zip(use, (r.loss, r.balance, r.z)) if u]
+    assert all(p.requires_grad for p in parts) and not r.counts.requires_grad
+    sum(parts).backward()
+    l64 = l.double().requires_grad_(True)
+    loss, bal, zz, _, coef, enters, n = loss64(l64, ids, b, z, None, cu)
+    (use[0] * loss + use[1] * bal + use[2] * zz).backward()
+    # as balance_loss with the coefficients that the weights amount to, two more roundings of them
+    tb, tz = use[0] * b + use[1], use[0] * z + use[2]
+    lse = torch.where(enters, torch.logsumexp(l64.detach(), 1), 0.0)
+    p, eps = torch.softmax(l64.detach(), 1), steps(l) + 4 * 2.0 ** -24
+    d = (p * coef).sum(1, keepdim=True)
+    lerr = lse.abs() * 2.0 ** -22 + 64 * 2.0 ** -24
+    tol = p * (tb * (coef + d) * eps + 2 * tz / n * (lerr + lse.abs() * eps)[:, None]) + 1e-38
+    assert leaf.grad.dtype == dtype
+    close(leaf.grad, l64.grad, tol + rounding(leaf.grad, l64.grad))
+
+
+def test_losses_may_be_changed_in_place(cuda):
+    l, ids = inputs(20, 16, 3)
+    leaf = l.clone().requires_grad_(True)
+    r = balance_loss(leaf, ids, 0.5, 0.1)
+    want = torch.autograd.grad(2.0 * r.loss + 3.0 * r.z, leaf)[0]
+    r = balance_loss(leaf, ids, 0.5, 0.1)
+    loss, z = r.loss, r.z
+    loss *= 2.0
+    z *= 3.0
+    assert torch.equal(torch.autograd.grad(loss + z, leaf)[0], want)

@@ -119,3 +119,12 @@ def test_scales_are_finite_as_they_are_kept(scale):
     assert AdapterSet([good], device="cpu").scale.isfinite().all()
     with pytest.raises(ValueError, match="finite"):
         AdapterSet([good, (torch.ones(8, 2), torch.ones(2, 8), scale)], device="cpu")
+
+
+def test_balance_loss_gradients_of_all_three_losses_are_given_as_such(lib):
+    d = dict(n_tokens=4, n_expert=8, top_k=2, n_sequences=1, type=0, balance_coef=0.1, logits=256, ids=256, losses=256,
+             counts=256, workspace=256, flags=_lib.BALANCE_D_LOSSES)
+    f = lambda **kw: lib.latent_balance_loss(C.byref(_lib.BalanceDesc(**{**d, **kw})), None)  # noqa: E731
+    assert f() == 1                                                       # the flag without the floats
+    assert f(d_loss=256) == 6                                             # on to the workspace's check
+    assert f(d_loss=256, flags=_lib.BALANCE_D_LOSSES | 4) == 1
