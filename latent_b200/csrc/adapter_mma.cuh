@@ -9,8 +9,11 @@
 // accumulator, no second pass over y.  t (fp32) enters as 2 or 3 parts of the
 // 16-bit operand type that add up to it (each part rounds what the ones
 // before left: 2 parts of bf16 leave 2^-16 of t, 3 of bf16 2^-24, 2 of fp16
-// 2^-22 or half a step of its subnormals, 2^-25, whichever is more: see
-// beyond_f16), multiplied by the same B rows.
+// 2^-22 or half a step of its subnormals, 2^-25, whichever is more), multiplied
+// by the same B rows.  fp16's range is too short for that as it stands: where
+// TMEM has room for another accumulator, the adapters' part goes there, each
+// row's t scaled by a power of two that the epilogue takes back (RowScale);
+// elsewhere the rows that do not fit are made in fp32 (beyond_f16).
 #pragma once
 
 #include "internal.h"
@@ -251,7 +254,7 @@ constexpr int kExt = 32;
 // 128B-swizzled tiles: t where the row's own segment lies, zeros elsewhere.  A
 // 128-byte row holds two parts of the 32 values (a third goes to a second
 // tile, tile_bytes further); what a part that is not finite leaves is zero.
-// `t`: the row's x.A, taken times scale.  load_t_row fetches (one trip to L2,
+// `t`: the row's x.A, taken times scale (and up, a power of two).  load_t_row fetches (one trip to L2,
 // which the caller lets run under the block before), store_t_row writes.
 __device__ __forceinline__ void load_t_row(float4 (&v)[8], int seg, int rank, int log2r, const float *t, int r0) {
 #pragma unroll
@@ -265,13 +268,14 @@ __device__ __forceinline__ void load_t_row(float4 (&v)[8], int seg, int rank, in
 }
 
 template <bool BF, int PARTS>
-__device__ __forceinline__ void store_t_row(float4 (&v)[8], uint8_t *tile, uint32_t tile_bytes, int row, float scale) {
+__device__ __forceinline__ void store_t_row(float4 (&v)[8], uint8_t *tile, uint32_t tile_bytes, int row, float scale,
+                                            float up = 1.f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        v[i].x *= scale;
-        v[i].y *= scale;
-        v[i].z *= scale;
-        v[i].w *= scale;
+        v[i].x = v[i].x * scale * up;
+        v[i].y = v[i].y * scale * up;
+        v[i].z = v[i].z * scale * up;
+        v[i].w = v[i].w * scale * up;
     }
 #pragma unroll
     for (int p = 0; p < PARTS; ++p)
@@ -299,25 +303,43 @@ __device__ __forceinline__ uint32_t t_offset(int p, int kk, uint32_t tile_bytes)
     return (uint32_t)(p >> 1) * tile_bytes + (uint32_t)(p & 1) * 64u + (uint32_t)kk * 32u;
 }
 
-// fp16 parts reach 65504 at one end; at the other they leave up to 2^-25 of
-// each t, however small it is.  A row whose largest t goes further, is not a
-// number, or is so small that 2^-25 is more of it than the results may lose
-// (fp32: 2^-21, what the accumulators' own cuts leave; 16 bits: 2^-16, as two
-// bf16 parts do) enters the tile as zeros and is finished in fp32 by the
-// epilogue.  Without the lower end t of 2^-17 were off by 2^-8 and t below 2^-25
-// were lost.
-template <bool F32>
-__device__ __forceinline__ bool beyond_f16(const float *t, float scale, int rank) {
-    constexpr float kLeast = F32 ? 0x1p-4f : 0x1p-9f;
-    bool in = true;
+// The largest magnitude of a row's t, and whether one is infinite or not a number.
+__device__ __forceinline__ float largest(const float *t, float scale, int rank, bool &finite) {
     float most = 0.f;
+    finite = true;
     for (int r = 0; r < rank; r += 4) {
         const float4 u = __ldcg(reinterpret_cast<const float4 *>(t + r));
         const float x = fabsf(u.x * scale), y = fabsf(u.y * scale), z = fabsf(u.z * scale), w = fabsf(u.w * scale);
-        in = in && x <= 65504.f && y <= 65504.f && z <= 65504.f && w <= 65504.f;
+        finite = finite && isfinite(x) && isfinite(y) && isfinite(z) && isfinite(w);
         most = fmaxf(fmaxf(most, fmaxf(x, y)), fmaxf(z, w));
     }
-    return !in || (most > 0.f && most < kLeast);
+    return most;
+}
+
+// The power of two that takes a row's largest t to 2^14 .. 2^15, and its
+// inverse: what two fp16 parts leave of a t is then 2^-22 of it or 2^-39 of the
+// row's largest.  Rows of zeros, and with values that are not finite: 1.
+struct RowScale {
+    float up = 1.f, down = 1.f;
+    __device__ __forceinline__ void set(const float *t, float scale, int rank) {
+        bool finite;
+        const float most = largest(t, scale, rank, finite);
+        if (!finite || most == 0.f) return;
+        const int e = min(141 - (int)(__float_as_uint(most) >> 23), 126);  // 14 less the exponent
+        up = __uint_as_float((uint32_t)(127 + e) << 23);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+};
+
+// 16-bit results of the pair kernel, whose accumulators fill TMEM: a row whose
+// largest t is beyond fp16's 65504, not finite, or so small that 2^-25 is more
+// than 2^-16 of it (what two bf16 parts leave) enters the tile as zeros and is
+// finished in fp32 by the epilogue (2047 rows of 4096 x 4096, rank 16: 379 us
+// if all rows are, 60 if none is).
+__device__ __forceinline__ bool beyond_f16(const float *t, float scale, int rank) {
+    bool finite;
+    const float most = largest(t, scale, rank, finite);
+    return !finite || most > 65504.f || (most > 0.f && most < 0x1p-9f);
 }
 
 // The adapter's part of y in column n, in fp32.

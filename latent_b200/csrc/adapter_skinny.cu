@@ -36,8 +36,8 @@ struct Shared {
     uint64_t acc_full[2], acc_empty[2], t_full[kMaxTBufs], t_empty[kMaxTBufs], seg;
     uint32_t tmem;
     volatile int abort;
-    uint8_t wide[kRows];   // fp16: rows finished in fp32
     Segments segs;
+    alignas(16) float down[kRows];     // fp16: RowScale's, of the rows' t
     alignas(16) uint32_t dest[kRows];  // where a row's sums go: its owner's shared memory, kNoRow behind the last row
 };
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -47,7 +47,7 @@ struct Plan {
     int stages;
     int chunk;      // blocks per accumulator (k_ad_skinny)
     int tbufs;      // tiles of x.A parts
-    int shrink_col; // x.A's accumulator behind the product's (SELF)
+    int next_col;   // the accumulator behind the product's: x.A's (SELF), else in fp16 the adapters' part's
     uint32_t cols;  // TMEM columns
 };
 
@@ -354,6 +354,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 to_y<__nv_bfloat16>(float v
 // MB: start, one trip to DRAM, two cluster barriers and the end of the grid are
 // what is left.  64 rows of 7168 x 2048, 24 adapters of rank 64: 15.1 us for 36
 // MB of W and B (2.4 TB/s; the extension blocks wait for x.A).
+//
+// fp16: the adapters' part has the accumulator behind x.W's (next_col), its rows
+// scaled (RowScale).
 template <bool BF, bool KN, int PARTS, typename Y, bool SELF>
 __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant__ CUtensorMap mW,
                                                            const __grid_constant__ CUtensorMap mB,
@@ -458,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         if (SELF && ok && elect()) mma_commit(sh.acc_full);
         if (ok) ok = wait_warp(&sh.seg, 0u, &sh.abort);
         if (SELF && ok && uniform(sh.segs.n)) {
-            ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.shrink_col, idesc(BF, p.rows, false, false), k0, k1);
+            ok = multiply_stacked(sh, p, at, ring, stage, tmem + (uint32_t)p.next_col, idesc(BF, p.rows, false, false), k0, k1);
             if (ok && elect()) mma_commit(sh.acc_full + 1);
         }
         if (!SELF && ok) {
@@ -474,11 +477,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                 if (elect()) {
                     const uint32_t w = smem_addr(ring + at.s * stage), t = smem_addr(tbuf) + (uint32_t)tb.s * kTiles * xbytes;
                     const int steps = min(kExt / 16, (ext - e * kExt) / 16);
+                    const uint32_t to = BF ? acc : tmem + (uint32_t)p.next_col, more = BF || e > e0;
                     for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
                         for (int w2 = 0; w2 < PARTS; ++w2)
-                            mma_f16(acc, desc_mnmajor_sw128(w + kk * 2048), desc_kmajor_sw128(t + t_offset(w2, kk, xbytes)),
-                                    idx, 1);
+                            mma_f16(to, desc_mnmajor_sw128(w + kk * 2048), desc_kmajor_sw128(t + t_offset(w2, kk, xbytes)),
+                                    idx, more | kk | w2);
                     mma_commit(sh.empty + at.s);
                     mma_commit(sh.t_empty + tb.s);
                 }
@@ -495,9 +499,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
         mbar_arrive(&sh.seg);
         ok = wait(&sh.seg, 0u);
         const int ext = ok ? sh.segs.n * rank : 0;
-        // column c of the accumulator = row c of x, to its owner
-        auto send_product = [&]() {
-            const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; the extension went to the last
+        // column c of the accumulator = row c of x, to its owner; `part`: with the adapters' part from its own
+        auto send_product = [&](bool part) {
+            const int groups = (k1 - k0 + p.chunk - 1) / p.chunk;  // accumulators in use; bf16: the extension went to the last
             for (int c = 0; c < p.rows; c += 32) {  // columns behind `rows` in the last 32 are allocated and dropped
                 float s[32];
                 uint32_t to[32];
@@ -510,6 +514,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
 #pragma unroll
                     for (int j = 0; j < 32; ++j) s[j] = gr ? s[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
                 }
+                if (!BF && part) {
+                    uint32_t v[32], down[32];
+                    __syncwarp();
+                    tmem_ld32(tmem + ((uint32_t)(r & ~31) << 16) + (uint32_t)(p.next_col + c), v);
+                    load_words(sh.down + c, down);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) s[j] = fmaf(__uint_as_float(v[j]), __uint_as_float(down[j]), s[j]);
+                }
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     if (to[j] != kNoRow) st_cluster(to[j] + (uint32_t)r * 4u, s[j]);
@@ -520,11 +533,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             ok = __all_sync(0xffffffffu, wait(sh.acc_full, 0u) && !sh.abort);
             tc_fence_after();
             cluster_wait();
-            if (ok) send_product();
+            if (ok) send_product(false);
             if (ext && ok) {
                 ok = __all_sync(0xffffffffu, wait(sh.acc_full + 1, 0u) && !sh.abort);
                 tc_fence_after();
-                if (ok) send_stacked(sh, p, tmem + (uint32_t)p.shrink_col, 0, rank, log2r, r, 512u);
+                if (ok) send_stacked(sh, p, tmem + (uint32_t)p.next_col, 0, rank, log2r, r, 512u);
                 tc_fence_before();
             }
         }
@@ -535,19 +548,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             const float *t = g.t + ((int64_t)(t0 + r) << log2r);
             const float scale = seg >= 0 ? __ldg(d.scale + a) : 0.f;
             dependency_wait();
-            const bool wide = !BF && seg >= 0 && beyond_f16<sizeof(Y) == 4>(t, scale, rank);
-            sh.wide[r] = wide;
-            const int live = wide ? -1 : seg;
+            RowScale rs;
+            if constexpr (!BF) {
+                if (seg >= 0 && e0 < e1) rs.set(t, scale, rank);
+                sh.down[r] = rs.down;
+                bar_sync(1, kRows);  // for all of these warps' send_product
+            }
             float4 v[8];
-            if (e0 < e1) load_t_row(v, live, rank, log2r, t, e0 * kExt);
+            if (e0 < e1) load_t_row(v, seg, rank, log2r, t, e0 * kExt);
             Ring tb;
             for (int e = e0; e < e1; ++e, tb.next(p.tbufs)) {
                 if (tb.wrapped && !wait_warp(sh.t_empty + tb.s, tb.phase ^ 1u, &sh.abort)) { ok = false; break; }
-                if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)tb.s * kTiles * xbytes, xbytes, r, scale);
+                if (r < p.rows) store_t_row<BF, PARTS>(v, tbuf + (uint32_t)tb.s * kTiles * xbytes, xbytes, r, scale, rs.up);
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sh.t_full + tb.s);
-                if (e + 1 < e1) load_t_row(v, live, rank, log2r, t, (e + 1) * kExt);
+                if (e + 1 < e1) load_t_row(v, seg, rank, log2r, t, (e + 1) * kExt);
             }
             if (warp == 4 && __all_sync(kAll, ok)) ok = ring_drained(tb, sh.t_empty, p.tbufs, &sh.abort);
             if (!ok) give_up(sh, d.err);  // before the wait below, so that it ends
@@ -556,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
             __syncwarp();
             tc_fence_after();
             cluster_wait();
-            send_product();
+            send_product(e0 < e1);
         }
     }
     if (!ok) {
@@ -602,11 +618,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_ad_skinny(const __grid_constant
                     v.y = fmaf(t[j], u.y, v.y);
                 }
             }
-        } else if (!BF && sh.wide[r]) {
-            const float *t = g.t + ((int64_t)(t0 + r) << log2r);
-            const int ad = sh.segs.id[sh.segs.row[r]];
-            v.x += adapter_dot<BF>(d, t, ad, n);
-            v.y += adapter_dot<BF>(d, t, ad, n + 1);
         }
         Y *y = static_cast<Y *>(d.y) + (int64_t)(t0 + r) * d.ldy + n;
         if (n + 1 < d.n_out && (uintptr_t)y % (2 * sizeof(Y)) == 0) {
@@ -821,9 +832,10 @@ ShrinkPlan plan_shrink(const AdapterArgs &g, const int *room) {
 // sum off instead of rounding it (figures at k_ad_wide): fp32 results use an
 // accumulator per 512 of K, added up in fp32, as far as the TMEM columns go,
 // and clusters long enough.
-int accumulators(int rows, bool self) {
+// `next`: with one more accumulator behind them.
+int accumulators(int rows, bool next) {
     const int read = (rows + 31) / 32 * 32;  // columns the epilogue reads of an accumulator
-    return (512 - (self ? 2 : 1) * read) / rows + 1;
+    return (512 - (next ? 2 : 1) * read) / rows + 1;
 }
 
 // Blocks of a cluster of k_ad_skinny.  Where both kernels are small, its
@@ -838,7 +850,7 @@ int plan_skinny(const AdapterArgs &g, const int *room, int beside, int sms) {
     int c = pick_cluster(others, nk, room);
     while (beside && c > 2 && others * c > sms - beside) --c;
     if (d.y_type == LATENT_TYPE_F32) {
-        const int groups = accumulators((g.tile_rows + 15) / 16 * 16, false);
+        const int groups = accumulators((g.tile_rows + 15) / 16 * 16, d.type == LATENT_TYPE_F16);
         while (c < kMaxCluster && c < nk && room[c + 1] > 0 && (nk + c - 1) / c > 8 * groups) ++c;
     }
     return c;
@@ -877,12 +889,12 @@ cudaError_t launch_adapter_skinny(const AdapterArgs &g, const void *x_map, int s
     p.tbufs = self ? 0 : p.rows <= 64 ? kMaxTBufs : 2;
     const size_t stage = 16384 + (size_t)p.rows * 128, tb = (size_t)p.tbufs * ((parts + 1) / 2) * p.rows * 128;
     const int cluster = self ? adapter_self_cluster(g) : adapter_skinny_cluster(g, sms);
-    const int read = (p.rows + 31) / 32 * 32, groups = accumulators(p.rows, self);
+    const int read = (p.rows + 31) / 32 * 32, groups = accumulators(p.rows, self || !bf);
     const int per = (nk + cluster - 1) / cluster;
     p.chunk = per;
     if (f32) p.chunk = per <= 8 * groups ? 8 : (per + groups - 1) / groups;
-    p.shrink_col = ((per + p.chunk - 1) / p.chunk - 1) * p.rows + read;
-    p.cols = tmem_cols(p.shrink_col + (self ? read : 0));
+    p.next_col = ((per + p.chunk - 1) / p.chunk - 1) * p.rows + read;
+    p.cols = tmem_cols(p.next_col + (self || !bf ? read : 0));
     const size_t recv = recv_bytes(g.tile_rows, cluster, self ? 512 + d.rank * 4 : 512);
     p.stages = pick_stages(stage, tb + recv, per * (self ? 2 : 1) + 4);
     if (p.stages < 1) return cudaErrorInvalidConfiguration;

@@ -27,6 +27,9 @@
 // plain fp32 product 8.8e-7 (1.5e-6; 1.2e-6, 1.2e-6).  16-bit results keep the
 // one chain: their rounding is 1.66e-3 (fp16 2.07e-4) with it as without, with
 // terms of one sign 1.29e-3 (fp16 1.67e-4 for 1.61e-4).
+//
+// fp16 to fp32: the adapters' part takes one more turn of the accumulators, its
+// rows scaled (RowScale).
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -56,6 +59,8 @@ struct Cfg {
     static constexpr int kStages = 5;
     static constexpr uint32_t kStage = kXBytes + kCols / 2 * 128;    // x, W
     static constexpr int kParts = BF && F32 ? 3 : 2;
+    static constexpr bool kScaled = !BF && F32;                      // the adapters' part has an accumulator of its own
+    static constexpr bool kWide = !BF && !F32;                       // rows that fp16 parts cannot hold
     static constexpr uint32_t kTTile = 16384u * ((kParts + 1) / 2);  // 128 rows x (2 parts x 32) of x.A, and the third part
     static constexpr int kChunk = F32 ? 8 : 1 << 30;                 // K blocks per accumulator
     static constexpr int kTBufs = 2;
@@ -66,7 +71,8 @@ struct PairSegments {
     int n;
     int id[kPairRows];
     int16_t row[128];     // of this block's rows
-    uint8_t wide[128];    // fp16: finished in fp32 by the epilogue
+    uint8_t wide[128];    // fp16 results: finished in fp32 by the epilogue
+    float down[128];      // fp16 to fp32: RowScale's, of the rows' t
 };
 
 struct Shared {
@@ -285,7 +291,19 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             }
             if (!wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
             const int ext = uniform(sh.seg[tl & 1].n) * rank;
-            if (cta == 0) {  // the adapters' part goes to the last accumulator
+            if (cta == 0) {  // the adapters' part goes to the last accumulator, or to the next
+                uint32_t more = 1;
+                if (C::kScaled && ext) {
+                    if (elect()) commit_pair(sh.acc_full + ((cc - 1) & 1));
+                    if (cc >= 2 && !wait_warp<true>(sh.acc_empty + (cc & 1), (uint32_t)((cc >> 1) - 1) & 1u, &sh.abort)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    acc = tmem + (uint32_t)(cc & 1) * (uint32_t)kPairCols;
+                    more = 0;
+                    ++cc;
+                }
                 for (int r0 = 0; r0 < ext; r0 += kExt, at.next(kStages), tb.next(C::kTBufs)) {
                     if (!wait_warp(sh.full + at.s, at.phase, &sh.abort) ||
                         !wait_warp<true>(sh.t_full + tb.s, tb.phase, &sh.abort)) { ok = false; break; }
@@ -296,10 +314,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                         for (int kk = 0; kk < steps; ++kk)
 #pragma unroll
                             for (int q = 0; q < C::kParts; ++q)
-                                mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 16384u)), desc_mnmajor_sw128(w + kk * 2048), idx, 1);
+                                mma_pair(acc, desc_kmajor_sw128(t + t_offset(q, kk, 16384u)), desc_mnmajor_sw128(w + kk * 2048), idx,
+                                         more | kk | q);
                         commit_pair(sh.empty + at.s);
                         commit_pair(sh.t_empty + tb.s);
                     }
+                    more = 1;
                 }
                 if (!ok) break;
                 if (elect()) commit_pair(sh.acc_full + ((cc - 1) & 1));
@@ -321,12 +341,14 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             if (!wait_warp(sh.seg_full + (tl & 1), (uint32_t)(tl >> 1) & 1u, &sh.abort)) { ok = false; break; }
             const PairSegments &seg = sh.seg[tl & 1];
             const int t = tile.t0 + cta * 128 + r, row0 = tile.t0 + cta * 128 + w * 32;
-            const bool wide = !BF && t < d.n_tokens && seg.wide[r];
+            const bool wide = C::kWide && t < d.n_tokens && seg.wide[r];
             const int a = wide ? seg.id[seg.row[r]] : 0;
-            const uint32_t wide_rows = BF ? 0u : __ballot_sync(kAll, wide);
+            const uint32_t wide_rows = C::kWide ? __ballot_sync(kAll, wide) : 0u;
             float v[F32 ? kPairCols : 64];
             if constexpr (F32) {
-                for (int c = 0; c < chunks; ++c, ++cc) {
+                const int sums = chunks + (C::kScaled && uniform(seg.n) ? 1 : 0);
+                for (int c = 0; c < sums; ++c, ++cc) {
+                    const float down = C::kScaled && c == chunks ? seg.down[r] : 1.f;
                     if (!wait_warp(sh.acc_full + (cc & 1), (uint32_t)(cc >> 1) & 1u, &sh.abort)) { ok = false; break; }
                     tc_fence_after();
 #pragma unroll
@@ -335,7 +357,10 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                         tmem_ld16(lanes + (uint32_t)((cc & 1) * kPairCols + n), u);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[n + j] = c ? v[n + j] + __uint_as_float(u[j]) : __uint_as_float(u[j]);
+                        for (int j = 0; j < 16; ++j) {
+                            const float p = C::kScaled ? __uint_as_float(u[j]) * down : __uint_as_float(u[j]);
+                            v[n + j] = c ? v[n + j] + p : p;
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -361,7 +386,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
                     }
                 }
                 float *x = v + (F32 ? c : 0);
-                if constexpr (!BF) {  // rows whose x.A fp16 parts cannot hold: the warp makes a row's part, its lane takes it
+                if constexpr (C::kWide) {  // rows whose x.A fp16 parts cannot hold: the warp makes a row's part, its lane takes it
                     for (uint32_t rest = wide_rows; rest; rest &= rest - 1) {
                         const int b = __ffs(rest) - 1, ad = __shfl_sync(kAll, a, b);
                         const float *tb = g.t + (int64_t)(row0 + b) * rank;
@@ -471,9 +496,12 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             const int t = tile.t0 + mine * 128 + tid;
             const float *tp = g.t + (int64_t)t * rank;
             const float scale = my >= 0 ? __ldg(d.scale + a[mine]) : 0.f;
-            const bool wide = !BF && my >= 0 && beyond_f16<F32>(tp, scale, rank);
+            const bool wide = C::kWide && my >= 0 && beyond_f16(tp, scale, rank);
+            RowScale rs;
+            if (C::kScaled && my >= 0) rs.set(tp, scale, rank);
             seg.row[tid] = (int16_t)my;
             seg.wide[tid] = wide;
+            seg.down[tid] = rs.down;
             const int ext = seg.n * rank;
             mbar_arrive(sh.seg_full + (tl & 1));
             const int live = wide ? -1 : my;
@@ -481,7 +509,7 @@ k_ad_wide(const __grid_constant__ CUtensorMap mX, const __grid_constant__ CUtens
             if (ext) load_t_row(v, live, rank, g.log2r, tp, 0);
             for (int r0 = 0; r0 < ext; r0 += kExt, tb.next(C::kTBufs)) {  // a thread that gives up here is heard at the next tile
                 if (tb.wrapped && !wait_warp(sh.t_empty + tb.s, tb.phase ^ 1u, &sh.abort)) { ok = false; break; }
-                store_t_row<BF, C::kParts>(v, tbuf + tb.s * C::kTTile, 16384u, tid, scale);
+                store_t_row<BF, C::kParts>(v, tbuf + tb.s * C::kTTile, 16384u, tid, scale, rs.up);
                 if (r0 + kExt < ext) load_t_row(v, live, rank, g.log2r, tp, r0 + kExt);
                 fence_async_shared();
                 __syncwarp();
