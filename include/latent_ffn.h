@@ -524,8 +524,9 @@ LATENT_API int latent_balance_loss(const latent_balance_desc *desc, struct CUstr
  *   y[t] = x[t].W + scale[a] (x[t].A_a).B_a        (a < 0: x[t].W alone)
  * x, w, a and b have one type, F16 or BF16; y has that type or F32; every sum
  * is fp32 and y is rounded once.  The adapters are stored at one padded rank
- * (16, 32, 64 or 128; zero rows change nothing): a holds A_a transposed,
- * [n_adapter][rank][lda], b holds B_a, [n_adapter][rank][ldb].  w is
+ * (16, 32, 64 or 128; zero rows change nothing in finite rows of x, and make
+ * NaN of an infinite one): a holds A_a transposed, [n_adapter][rank][lda], b
+ * holds B_a, [n_adapter][rank][ldb].  w is
  * [n_in][ldw], or [n_out][ldw] with LATENT_ADAPTER_W_TRANSPOSED; w == NULL:
  * y += the adapters' part.  An id >= n_adapter counts as none and is recorded
  * in *err (latent_adapter_check).  Adapter factors must be finite: a

@@ -39,8 +39,8 @@ class AdapterSet:
     """Device-resident adapters (A [K, r], B [r, N], scale) of one projection.
 
     ``adapters``: one triple per adapter (scale may be left out: 1.0), ranks
-    may differ.  They are stored at one padded rank (16, 32, 64 or 128, zero
-    rows change no result) in ``dtype``: A transposed, so that a rank column
+    may differ.  They are stored at one padded rank (16, 32, 64 or 128; zero
+    rows change no finite result) in ``dtype``: A transposed, so that a rank column
     is contiguous, B as given.  Factors that are not finite in ``dtype`` are
     refused: rows of several adapters share tiles in which a foreign factor
     is multiplied by zero.

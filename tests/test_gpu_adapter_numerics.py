@@ -148,3 +148,21 @@ def test_fp32_results_of_a_long_intermediate(cuda, T, N, dtype):
         y[ids == i] = (x[ids == i].double() @ a.double()) @ b.double()
     got = adapter_project(x, torch.zeros((K, N), dtype=dtype, device="cuda"), AdapterSet(ads), ids, out_dtype=F32)
     within(got, y, (CHAIN[dtype] + 2.0 ** -22 + 8 * 2.0 ** -24) * y)
+
+
+@pytest.mark.parametrize("T,K,N,n", [(12, 256, 256, 2), (40, 256, 256, 12), (300, 256, 256, 3), (2048, 512, 2048, 3)])
+@pytest.mark.parametrize("out", [HF, F32])
+def test_fp16_row_that_is_not_finite_stays_alone(cuda, T, K, N, n, out):
+    """NaN and infinities of a row of x reach no other row, whichever way fp16 rows beyond the parts' range take."""
+    g = torch.Generator("cuda").manual_seed(T)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(HF)  # noqa: E731
+    x, w = rand(T, K), rand(K, N)
+    s = AdapterSet([(rand(K, 16), rand(16, N), 0.5) for _ in range(n)])
+    ids = (torch.arange(T, device="cuda") % (n + 1) - 1).to(torch.int32)
+    want = adapter_project(x, w, s, ids, out_dtype=out)
+    bad = x.clone()
+    bad[3, 5], bad[7, 0], bad[8, 1] = float("nan"), float("inf"), -float("inf")   # adapters 2, 3, none where n = 3
+    got = adapter_project(bad, w, s, ids, out_dtype=out)
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[[3, 7, 8]] = False
+    assert torch.equal(got[rest], want[rest]) and not bool(torch.isfinite(got[~rest]).any())
