@@ -129,7 +129,7 @@ def adapter_project(x: torch.Tensor, weight, adapters: AdapterSet, ids: torch.Te
     memory with the inputs).
 
     The tensor cores need rows of x and of the weight that start at multiples
-    of 16 bytes (N itself may be odd); others run on the CUDA cores, about ten
+    of 16 bytes (N itself may be odd); others run on the CUDA cores, 20 to 70
     times slower.
     """
     s = adapters

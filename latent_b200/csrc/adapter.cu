@@ -147,7 +147,9 @@ int tile_rows(int n, AdapterPath path) { return path == kPathWide || n >= adapte
 // blocks, or of the pair.  E.g. skinny and wide, rank 16: 320 rows of
 // 2048 x 2048 16.1 and 18.9 us, 1024 rows 26.9 and 18.3, 1024 rows of
 // 7168 x 512 25.1 and 39.6; 24 adapters of rank 64 in 200 rows of
-// 1024 x 14336, fp32 results: 105.0 and 87.9.
+// 1024 x 14336, fp32 results: 105.0 and 87.9.  Over 187 shapes of 100 to 2048
+// rows the slower of the two is taken by more than 5% on nine (bf16; 1.19 times
+// at worst) and on three (fp32 results; 1.13).
 // Up to 64 rows whose adapters fit one tile of 128 stacked rank columns, with
 // at most 8 steps of K per block, k_ad_skinny makes x.A itself (one row of
 // 1024 x 4096: 8.5 us against 10.3 in two launches, of 7168 x 2048: 15.7

@@ -11,8 +11,9 @@
 // so results do not depend on timing.
 //
 // k_ad_skinny is launched as a programmatic dependent of k_ad_shrink (unless it
-// makes x.A itself): it streams W while x.A is still being made and waits for
-// it (griddepcontrol) only before the extension blocks.
+// makes x.A itself): on the SMs that the shrink leaves it streams W while x.A is
+// still being made, and it waits for x.A (griddepcontrol) only before the
+// extension blocks.
 #include <cuda.h>
 
 #include <mutex>

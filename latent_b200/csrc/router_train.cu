@@ -26,10 +26,10 @@
 // adds them up in block order, so that a call's results do not depend on the
 // order of execution.
 //
-// Measured, 16384 rows of 256 fp32 experts, top-8, 8 sequences: count 5.1 us,
-// main 11.4 (34 MB read and written, 2.9 TB/s; about half of its blocks' time is
-// waiting on loads and shuffles), 13.8 for both in a graph.  64 rows: 3.1, 4.5
-// and 6.1.
+// Measured, 16384 rows of 256 fp32 experts, top-8, 8 sequences: both kernels in a
+// graph 13.6 us with even loads, 14.4 with skewed ones; under a profiler, caches
+// cold, the count 8.5 and main 15.9 (34 MB read and written; about half of its
+// blocks' time is waiting on loads and shuffles).  64 rows: 6.7 to 7.5 for both.
 #include <cooperative_groups.h>
 
 #include "internal.h"
@@ -704,9 +704,9 @@ extern "C" LATENT_API int latent_balance_loss(const latent_balance_desc *d, CUst
                         reinterpret_cast<int32_t *>(ws + L.seq), reinterpret_cast<float *>(ws + L.share), L.share_ld,
                         reinterpret_cast<double *>(ws + L.partial), reinterpret_cast<uint32_t *>(ws + L.ticket)};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    // as many blocks for a sequence as run at once (16384 rows of 256 experts, both kernels: 8 sequences 13.6 us with 8
-    // blocks each, 17.1 with one; 1024 sequences 74.0 and 22.8), of 1024 threads where each has many ids (65536 rows of
-    // 128 experts in one sequence 32.3 us, 39.2 with 512; 9001 rows in 37 sequences 12.2 and 10.6)
+    // as many blocks for a sequence as run at once (both kernels in a graph: 16384 rows of 256 experts in 8 sequences
+    // 13.5 us with 8 blocks each, 15.1 with one; 16384 of 64 in 1024 sequences 67.8 and 16.7), of 1024 threads where each
+    // has many ids (65536 rows of 128 experts in one sequence 27.2 us, 35.1 with 512; 9001 of 160 in 37 12.0 and 10.8)
     const unsigned S = (unsigned)d->n_sequences;
     const int share = sms / d->n_sequences;
     const int cluster = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
