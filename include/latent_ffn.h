@@ -489,7 +489,8 @@ LATENT_API int latent_router_grad(const latent_router_grad_desc *desc, struct CU
  *   losses[0] = balance_coef losses[1] + z_coef losses[2]
  * and grad (optional) = *d_loss dlosses[0]/dlogits in the logits' type, with f
  * held fixed (d_loss: the device scalar that comes from behind, NULL: 1; with
- * LATENT_BALANCE_D_LOSSES three of them, for losses[0], [1] and [2]).  A row whose logits are all -inf has no distribution: it counts as a row, adds
+ * LATENT_BALANCE_D_LOSSES three of them, for losses[0], [1] and [2]).  A row
+ * whose logits are all -inf has no distribution: it counts as a row, adds
  * nothing and has a zero gradient.  Workspace: 256-byte aligned,
  * latent_balance_workspace_size() bytes.  LATENT_ERR_UNSUPPORTED beyond 1024
  * experts.  Stream-ordered; repeated calls agree bit for bit. */
