@@ -33,9 +33,10 @@ def test_fp16_intermediate_of_any_magnitude(cuda, T, K, N, n, out, e):
     """scale x.A between 2^-68 and 2^19, rows of two magnitudes in every tile, rows that are zero.
 
     A row of x has one value, so x.A is one product of 11-bit numbers: exact in fp32, and a power of two scales it.  In
-    the tensor cores it is two fp16 parts: off by 2^-22 of itself, or by half a step of the subnormals, 2^-25, which in
-    the rows that go there is at most 2^-21 (fp32 results; fp16: 2^-16) of the row's largest.  Sums of 2 rank terms: 2
-    rank + 8 steps of 2^-24 of the sum of their magnitudes."""
+    the tensor cores it is two fp16 parts: off by 2^-22 of itself, or by half a step of the subnormals, 2^-25, which of
+    the row's largest is at most 2^-16 in the rows of 16-bit results on SM pairs that go there as they are, and 2^-39
+    where rows are scaled first (2^-21 allowed for fp32 results).  Sums of 2 rank terms: 2 rank + 8 steps of 2^-24 of
+    the sum of their magnitudes."""
     g = torch.Generator("cuda").manual_seed(T + e)
     rank, rows = 16, torch.arange(T, device="cuda")
     at = torch.randint(0, K, (T,), generator=g, device="cuda")
